@@ -1,5 +1,5 @@
 """Build libcqgdn.so (gfx950 HIP kernels + the C ABI of include/cqgdn.h) and its PyTorch-ROCm
-operator library libcqgdn_torch.so (csrc/torch_ops.cpp, TORCH_LIBRARY(cqgdn)) in-tree.
+operator library libcqgdn_torch.so (csrc/torch_ops.cpp and csrc/attn_ops.cpp, TORCH_LIBRARY(cqgdn)) in-tree.
 
 Usage: python cq-pretrain_amd/build.py [--jobs N]
 
@@ -85,7 +85,7 @@ def build(jobs: int | None = None, extra: list[str] | None = None, verbose: bool
 
 
 def build_ops(verbose: bool = True) -> Path:
-    """csrc/torch_ops.cpp -> cqgdn/libcqgdn_torch.so, linked to libcqgdn.so (rpath $ORIGIN)."""
+    """csrc/torch_ops.cpp and csrc/attn_ops.cpp -> cqgdn/libcqgdn_torch.so, linked to libcqgdn.so (rpath $ORIGIN)."""
     import torch
     from torch.utils import cpp_extension
 
@@ -96,12 +96,12 @@ def build_ops(verbose: bool = True) -> Path:
     tmp = OPS_OUT.with_suffix(".so.tmp")
     cmd = [os.environ.get("CXX", "g++"), "-O2", "-std=c++17", "-shared", "-fPIC", f"-D_GLIBCXX_USE_CXX11_ABI={abi}",
            "-D__HIP_PLATFORM_AMD__=1", "-DUSE_ROCM=1", *(f"-I{p}" for p in includes),
-           str(CSRC / "torch_ops.cpp"), "-o", str(tmp),
+           str(CSRC / "torch_ops.cpp"), str(CSRC / "attn_ops.cpp"), "-o", str(tmp),
            *(f"-L{p}" for p in cpp_extension.library_paths()), "-lc10", "-lc10_hip", "-ltorch_cpu",
            f"-L{OUT.parent}", "-lcqgdn", "-Wl,-rpath,$ORIGIN"]
     proc = subprocess.run(cmd, capture_output=True, text=True)
     if proc.returncode != 0:
-        raise RuntimeError(f"torch_ops.cpp failed to build:\n{proc.stderr}")
+        raise RuntimeError(f"the operator library failed to build:\n{proc.stderr}")
     os.replace(tmp, OPS_OUT)
     if verbose:
         print(f"built {OPS_OUT.relative_to(ROOT)} (TORCH_LIBRARY cqgdn)")

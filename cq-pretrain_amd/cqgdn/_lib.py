@@ -21,6 +21,7 @@ LIB_PATH = Path(__file__).resolve().with_name("libcqgdn.so")
 OPS_PATH = LIB_PATH.with_name("libcqgdn_torch.so")
 
 OK, EINVAL, EUNSUPPORTED, EHIP = 0, 1, 2, 3
+BF16, F16, F32 = 0, 1, 2
 NORMALIZE, TRAINING, PRECISE, NO_OUTPUT, FP16 = 1, 2, 4, 8, 16
 STATIC_WORKSPACE_BYTES = 64 << 20  # CQGDN_STATIC_WORKSPACE_BYTES
 FWD_BUFFERS, BWD_BUFFERS = 9, 8
@@ -62,6 +63,15 @@ SIGNATURES = {
                                     _P, _I64, _P, _I64, _P, _P, _P, _SZ, _P]),
     "cqgdn_layer_decode_workspace_size": (_SZ, [_I, _I]),
     "cqgdn_layer_decode_step": (_I, [_I, _I, _I, _I, _P, _I64, _P, _P, _P, _P, _P, _F, _F, _P, _P, _P, _SZ, _P]),
+    "cqgdn_rotary": (_I, [_P, _I64, _I64, _I, _P, _I64, _I64, _I, _I64, _I, _I, _I, _I, _I, _P, _I, _I64, _I, _P, _P, _P,
+                          _P, _P]),
+    "cqgdn_step_pages": (_I, [_P, _P, _I, _P, _I64, _I, _P, _I, _P, _I, _I64, _P, _P, _P, _P, _P, _P, _P, _P]),
+    "cqgdn_kv4_page_bytes": (_SZ, [_I, _I]),
+    "cqgdn_kv4_write": (_I, [_P, _I64, _I64, _P, _I64, _I64, _I, _P, _I64, _I, _I, _P, _I64, _I, _P]),
+    "cqgdn_kv4_read": (_I, [_P, _I64, _I, _I, _I, _P, _I64, _I, _P, _P, _P]),
+    "cqgdn_kv4_attend_workspace_size": (_SZ, [_I64, _I, _I, _I, _I, _I, _I, _I]),
+    "cqgdn_kv4_attend": (_I, [_P, _I64, _I64, _I, _I64, _I, _I, _P, _I64, _I, _I, _P, _I64, _I, _P, _I, _P, _I, _F, _I,
+                              _P, _P, _P, _SZ, _P]),
     "cqgdn_timer_arm": (_I, [ctypes.c_char_p, _I]),
     "cqgdn_timer_read": (_I, [_P, _I, _P]),
 }
@@ -104,7 +114,7 @@ def lib():
 
 
 def ops():
-    """``torch.ops.cqgdn`` (fwd, bwd, conv1d_fwd, conv1d_bwd, recurrent, layer_decode_step), loaded once; raise if unbuilt."""
+    """``torch.ops.cqgdn`` (the operators of csrc/torch_ops.cpp and csrc/attn_ops.cpp), loaded once; raise if unbuilt."""
     global _OPS
     if _OPS is None:
         lib()  # the operator library links libcqgdn.so: load it (and check it exists) first

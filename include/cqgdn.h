@@ -383,6 +383,86 @@ int cqgdn_chunk_local_cumsum(const float* g, float* out, int64_t T, int H, const
                              int64_t n_chunks, int reverse, void* stream);
 
 /*
+ * Rotary positions with several axes (time, height, width) on q and k, and their gradient.  A head's
+ * first rotary_dim values are pairs, value i with value i + rotary_dim / 2, or 2 i with 2 i + 1 with
+ * `adjacent`; pair i turns by position[axis[i]] * f_i, the other values pass.  `backward` turns the other
+ * way: the gradient of x from that of y.  q [T][q_heads][head_dim] and k with the given strides in
+ * elements (unit stride within a head); the outputs are dense and may not overlap the inputs.
+ *   dtype     : CQGDN_BF16, CQGDN_F16 or CQGDN_F32, of q, k and the outputs; computed in fp32
+ *   positions : [axes][T], int32 (int64 with wide_positions), axes axis_stride elements apart
+ *   turns     : [rotary_dim / 2], f_i / (2 pi) in units of 2^-64 turns a position, so that the angle of
+ *               any integer position is exact to 2^-32 of a turn
+ *   axis      : [rotary_dim / 2], the axis of pair i
+ */
+#define CQGDN_BF16 0
+#define CQGDN_F16 1
+#define CQGDN_F32 2
+int cqgdn_rotary(const void* q, int64_t q_token, int64_t q_head, int q_heads, const void* k, int64_t k_token,
+                 int64_t k_head, int k_heads, int64_t T, int head_dim, int rotary_dim, int adjacent, int backward,
+                 int dtype, const void* positions, int wide_positions, int64_t axis_stride, int axes,
+                 const uint64_t* turns, const int32_t* axis, void* q_out, void* k_out, void* stream);
+
+/*
+ * The pages of one serving step, from request lengths on the device.  All arrays are int32.
+ *   cached, fresh : [N] tokens a request holds, and its tokens of this step (0: none; < 0: it has ended
+ *                   and its pages return to the pool)
+ *   tables        : [N][columns], rows table_stride apart: the pages of each request in order; new ones
+ *                   are written in place
+ *   pool, pool_count : [pool_size] free pages, a stack of *pool_count; returned pages are put on top
+ *   page          : tokens of a page, a power of two from 16 to 65536
+ *   starts [N+1]  : first row of each request among the step's T rows; rows behind the last are padding
+ *   lengths [N]   : tokens each request holds after the step (may be `cached`)
+ *   admitted [N]  : 0 where the pool, the table row or the T rows do not hold the request's new tokens:
+ *                   it keeps what it had, and its rows get slot -1.  Requests take pages in order, and
+ *                   behind one that the pool cannot serve none that needs pages is admitted.
+ *   count [1]     : free pages after the step (may be `pool_count`)
+ *   slots, positions, visible [T] : page * page_size + offset of each row (-1: not to be written), its
+ *                   position in its request, and the positions it sees (itself and those before it; 0 for
+ *                   padding and rows that were not admitted)
+ */
+int cqgdn_step_pages(const int32_t* cached, const int32_t* fresh, int N, int32_t* tables, int64_t table_stride,
+                     int columns, int32_t* pool, int pool_size, const int32_t* pool_count, int page, int64_t T,
+                     int32_t* starts, int32_t* lengths, int32_t* admitted, int32_t* count, int32_t* slots,
+                     int32_t* positions, int32_t* visible, void* stream);
+
+/*
+ * The 4-bit cache of keys and values: data [pages][kv_heads][cqgdn_kv4_page_bytes(page, head_dim)].  A
+ * page of one head holds its key codes [page][head_dim/2], value codes, key scale bytes
+ * [page][head_dim/32] and value scale bytes.  A code is e2m1 (0 .5 1 1.5 2 3 4 6 and a sign), the even
+ * value of a pair in its byte's low half; a scale byte b multiplies 32 neighbouring values by 2^(b - 127),
+ * and 255 makes them NaN.  head_dim is 64, 128 or 256.  cqgdn_kv4_write rounds rows k, v [T][kv_heads]
+ * [head_dim] (bf16 or fp16, strides in elements, multiples of 8) into the slots, to nearest even under
+ * the scale that the block's largest magnitude sets (a block with an infinity or NaN becomes NaN); slots
+ * outside [0, pages * page) are skipped, and no slot may be given twice.  cqgdn_kv4_read returns the values
+ * of slots, dense, zeros for slots outside.
+ */
+size_t cqgdn_kv4_page_bytes(int page, int head_dim);
+int cqgdn_kv4_write(const void* k, int64_t k_token, int64_t k_head, const void* v, int64_t v_token, int64_t v_head,
+                    int dtype, const int32_t* slots, int64_t T, int kv_heads, int head_dim, void* data, int64_t pages,
+                    int page, void* stream);
+int cqgdn_kv4_read(const void* data, int64_t pages, int page, int kv_heads, int head_dim, const int32_t* slots,
+                   int64_t T, int dtype, void* k, void* v, void* stream);
+
+/*
+ * Attention over the 4-bit pages: row t of request r (starts[r] <= t < starts[r+1]) sees the positions
+ * [max(0, visible[t] - window), visible[t]) of its request (window 0: from 0), whose pages are
+ * tables[r][position / page].  out[t][h] = sum_j p_j v_j / sum_j p_j, p_j = exp(scale q k_j), query head h
+ * reading key head h / (heads / kv_heads); rows that see nothing, and rows behind starts[N], are zero.
+ * Positions beyond the table's columns, or whose entry names no page, are not seen.
+ *   q, out      : bf16 or fp16 (dtype) [T][heads][head_dim]; q with strides in elements, multiples of 8
+ *   lse         : NULL, or fp32 [T][heads]: log sum_j exp(scale q k_j), -inf for rows that see nothing
+ *   max_queries : bound of the rows of one request; it sets the launch, and a larger request is served too
+ *   workspace   : >= cqgdn_kv4_attend_workspace_size() bytes (with min(max_queries, T)), 256-byte aligned
+ */
+size_t cqgdn_kv4_attend_workspace_size(int64_t T, int N, int heads, int kv_heads, int head_dim, int max_queries,
+                                       int columns, int page);
+int cqgdn_kv4_attend(const void* q, int64_t q_token, int64_t q_head, int dtype, int64_t T, int heads, int head_dim,
+                     const void* data, int64_t pages, int page, int kv_heads, const int32_t* tables,
+                     int64_t table_stride, int columns, const int32_t* starts, int N, const int32_t* visible,
+                     int window, float scale, int max_queries, void* out, float* lse, void* workspace,
+                     size_t workspace_bytes, void* stream);
+
+/*
  * Instrumentation (no counterpart in the reference; used by the benchmark to
  * price one kernel against its roofline).  cqgdn_timer_arm(name, n) makes the
  * library bracket each of the next n launches of the named kernel with
