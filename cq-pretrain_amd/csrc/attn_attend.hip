@@ -17,13 +17,8 @@ namespace {
 
 constexpr int kWaves = 4;     // of a workgroup; they take its steps in turn
 constexpr int kStep = 32;     // positions of a wave's step
-constexpr float kLazy = 8.f;  // log2 by which scores may pass the running maximum before it moves
 constexpr int kMaxSplits = 64;
-
-// P in [0, 2^(kLazy + bias)]: fp16 keeps 2^-24 at the least, so its P is held 2^7 higher, where the
-// largest is 2^15 and weights down to 2^-31 of the maximum count
-template <class E>
-constexpr float kBias = std::is_same<E, f16>::value ? 7.f : 0.f;
+constexpr int kFewRows = 32;  // of a request and key head: more take the kernel of attn_tile.hip
 
 // The pages of one step's two halves of 16 positions, the codes of its 32 keys and values, and their
 // scale bytes.  Lane (r16, q4) holds key r16 of either half: 16 bytes from each 128 dimensions (8 where
@@ -45,12 +40,6 @@ template <int D>
 __device__ __forceinline__ int value_token(int j, int lane) {
   constexpr int PV = D / 32;  // 16-byte pieces of a row
   return (j * 64 + lane) / PV;
-}
-
-// The entry of the block table that holds position pos, -1 outside the table
-__device__ __forceinline__ int page_of(const AttendArgs& a, int r, int pos) {
-  const int column = pos >> a.page_shift;
-  return column < a.columns ? a.tables[r * a.table_stride + column] : -1;
 }
 
 template <int D>
@@ -121,7 +110,7 @@ __global__ __launch_bounds__(64 * kWaves) void attend_kernel(AttendArgs a, int t
   const int h = b % a.kv_heads;
   b /= a.kv_heads;
   const int tile0 = b % tiles, r = b / tiles, group = a.heads / a.kv_heads, T = (int)a.T;
-  const int from = min(max(a.starts[r], 0), T);
+  const int from = r == 0 ? 0 : min(max(a.starts[r], 0), T);
   const int to = r == a.N ? T : min(max(a.starts[r + 1], from), T);  // request N: the padding behind the last
   const int rows = (to - from) * group;
   const int room = (int)min((int64_t)a.columns << a.page_shift, (int64_t)INT32_MAX - 1024);
@@ -202,21 +191,22 @@ __global__ __launch_bounds__(64 * kWaves) void attend_kernel(AttendArgs a, int t
         float top = sc[0];
 #pragma unroll
         for (int e = 1; e < 8; ++e) top = fmaxf(top, sc[e]);
-        if (__any(top > m + kLazy)) {  // the maximum moves rarely: all lanes of a row agree on the new one
+        if (__any(top > m + kLazy)) {  // the maximum moves rarely, and for each row by itself
           top = fmaxf(top, __shfl_xor(top, 16, 64));
           top = fmaxf(top, __shfl_xor(top, 32, 64));
-          const float to_m = fmaxf(m, top);
-          const float f = m == -INFINITY ? 0.f : exp2f(m - to_m);
-          m = to_m;
-          l *= f;
+          if (top > m + kLazy) {
+            const float f = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m - top);
+            m = top;
+            l *= f;
 #pragma unroll
-          for (int k = 0; k < MT; ++k) o[k] *= f;
+            for (int k = 0; k < MT; ++k) o[k] *= f;
+          }
         }
-        const float base = (m == -INFINITY ? 0.f : m) - kBias<E>;
+        const float base = (m == -INFINITY ? 0.f : m) - kAttendBias<E>;
         float p[8];
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
-          p[e] = exp2f(sc[e] - base);
+          p[e] = __builtin_amdgcn_exp2f(sc[e] - base);
           l += p[e];
         }
         const x8 pf = to8<E>(f32x8{p[0], p[1], p[2], p[3], p[4], p[5], p[6], p[7]});
@@ -295,7 +285,7 @@ __global__ __launch_bounds__(64 * kWaves) void attend_kernel(AttendArgs a, int t
             ml[0] = M;
             ml[1] = L;
           } else if (a.lse) {
-            a.lse[at] = (M - kBias<E> + log2f(L)) * 0.693147180559945309f;
+            a.lse[at] = (M - kAttendBias<E> + log2f(L)) * 0.693147180559945309f;
           }
         }
       }
@@ -327,25 +317,38 @@ __global__ __launch_bounds__(256) void join_kernel(AttendArgs a, int splits) {
 #pragma unroll
   for (int k = 0; k < D / 64; ++k)
     st4(static_cast<E*>(a.out) + at * D + 4 * ((threadIdx.x & 15) + 16 * k), L == 0.f ? zero4() : y[k] * (1.f / L));
-  if (a.lse && (threadIdx.x & 15) == 0) a.lse[at] = (M - kBias<E> + log2f(L)) * 0.693147180559945309f;
+  if (a.lse && (threadIdx.x & 15) == 0) a.lse[at] = (M - kAttendBias<E> + log2f(L)) * 0.693147180559945309f;
 }
 
-// Parts of the positions: as many as bring 1024 workgroups (4 a CU), each of at least 128 positions.
-int attend_splits(int64_t N, int kv_heads, int group, int max_queries, int64_t capacity) {
-  const int64_t blocks = N * kv_heads * (((int64_t)max_queries * group + 15) / 16);
-  const int64_t most = std::min<int64_t>(kMaxSplits, (capacity + 127) / 128);
-  return (int)std::max<int64_t>(1, std::min(most, 1024 / std::max<int64_t>(blocks, 1)));
+// How a call runs: by which kernel, and in how many parts of the positions.
+struct Plan {
+  bool tiles;
+  int splits;
+};
+Plan attend_plan(int64_t N, int kv_heads, int group, int max_queries, int64_t capacity) {
+  const int64_t rows = (int64_t)max_queries * group;
+  if (rows > kFewRows) {
+    const int64_t blocks = N * kv_heads * ((rows + 127) / 128), most = std::min<int64_t>(kMaxSplits, (capacity + 511) / 512);
+    return {true, (int)std::max<int64_t>(1, std::min(most, 512 / std::max<int64_t>(blocks, 1)))};
+  }
+  // as many parts as bring 1024 workgroups (4 a CU), each of at least 128 positions
+  const int64_t blocks = N * kv_heads * ((rows + 15) / 16), most = std::min<int64_t>(kMaxSplits, (capacity + 127) / 128);
+  return {false, (int)std::max<int64_t>(1, std::min(most, 1024 / std::max<int64_t>(blocks, 1)))};
 }
 
 template <class E, int D>
 void launch_dim(const AttendArgs& a, hipStream_t st) {
   const int group = a.heads / a.kv_heads;
-  const int splits = attend_splits(a.N, a.kv_heads, group, a.max_queries, (int64_t)a.columns << a.page_shift);
-  const int64_t each = (int64_t)(a.N + 1) * a.kv_heads * splits;
-  const int tiles = (int)std::max<int64_t>(1, std::min<int64_t>(((int64_t)a.max_queries * group + 15) / 16, (1 << 23) / each));
-  const int64_t blocks = each * tiles;  // a workgroup takes every tiles-th tile: none is left out whatever the bound
-  attend_kernel<E, D><<<(unsigned)blocks, 64 * kWaves, 0, st>>>(a, tiles, splits);
-  if (splits > 1) join_kernel<E, D><<<(unsigned)((a.T * a.heads + 15) / 16), 256, 0, st>>>(a, splits);
+  const Plan p = attend_plan(a.N, a.kv_heads, group, a.max_queries, (int64_t)a.columns << a.page_shift);
+  if (p.tiles) {
+    launch_attend_tiles(a, p.splits, st);
+  } else {
+    const int64_t each = (int64_t)(a.N + 1) * a.kv_heads * p.splits;
+    const int tiles = (int)std::max<int64_t>(1, std::min<int64_t>(((int64_t)a.max_queries * group + 15) / 16, (1 << 23) / each));
+    // a workgroup takes every tiles-th tile: none is left out whatever the bound
+    attend_kernel<E, D><<<(unsigned)(each * tiles), 64 * kWaves, 0, st>>>(a, tiles, p.splits);
+  }
+  if (p.splits > 1) join_kernel<E, D><<<(unsigned)((a.T * a.heads + 15) / 16), 256, 0, st>>>(a, p.splits);
 }
 
 template <class E>
@@ -361,7 +364,7 @@ void by_dim(const AttendArgs& a, hipStream_t st) {
 }  // namespace
 
 size_t attend_workspace_bytes(int64_t T, int64_t N, int heads, int kv_heads, int D, int max_queries, int64_t capacity) {
-  const int splits = attend_splits(N, kv_heads, heads / kv_heads, max_queries, capacity);
+  const int splits = attend_plan(N, kv_heads, heads / kv_heads, max_queries, capacity).splits;
   return splits > 1 ? (size_t)T * heads * splits * (D + 2) * sizeof(float) : 0;
 }
 

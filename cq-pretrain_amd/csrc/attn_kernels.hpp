@@ -87,5 +87,7 @@ struct AttendArgs {
 // bytes of a call's workspace: the parts' O, maxima and sums, where the positions are split
 size_t attend_workspace_bytes(int64_t T, int64_t N, int heads, int kv_heads, int D, int max_queries, int64_t capacity);
 void launch_attend(const AttendArgs& a, hipStream_t st);
+// the kernel for many rows a request (attn_tile.hip); with more than one split its parts are joined by the caller
+void launch_attend_tiles(const AttendArgs& a, int splits, hipStream_t st);
 
 }  // namespace cqgdn

@@ -1,5 +1,6 @@
 // The 4-bit values of the cache as MFMA operands.
 #pragma once
+#include "attn_kernels.hpp"
 #include "gdn_common.hpp"
 
 namespace cqgdn {
@@ -28,6 +29,20 @@ __device__ __forceinline__ f16x8 kv4_values<f16>(uint32_t code, float scale) {
   const auto d = __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(code, scale, 3);
   return __builtin_shufflevector(__builtin_shufflevector(a, b, 0, 1, 2, 3), __builtin_shufflevector(c, d, 0, 1, 2, 3),
                                  0, 1, 2, 3, 4, 5, 6, 7);
+}
+
+// ---- shared by the attention kernels ----------------------------------------------------------------
+constexpr float kLazy = 8.f;  // log2 by which scores may pass the running maximum before it moves
+// P is held 2^bias higher, in [0, 2^(kLazy + bias)], because v_exp_f32 drops results below 2^-126 and fp16
+// keeps 2^-24 at the least: weights down to 2^-134 of the maximum count with bf16 (whose results reach 2^-126),
+// down to 2^-31 with fp16, whose largest P is 2^15.  Values up to 2^110 meet no overflow.
+template <class E>
+constexpr float kAttendBias = std::is_same<E, f16>::value ? 7.f : 8.f;
+
+// The entry of the block table that holds position pos, -1 outside the table
+__device__ __forceinline__ int page_of(const AttendArgs& a, int r, int pos) {
+  const int column = pos >> a.page_shift;
+  return column < a.columns ? a.tables[r * a.table_stride + column] : -1;
 }
 
 }  // namespace cqgdn
