@@ -15,182 +15,237 @@
 namespace cqgdn {
 namespace {
 
-constexpr int kWaves = 4;     // of a workgroup; they take its steps in turn
-constexpr int kStep = 32;     // positions of a wave's step
-constexpr int kMaxSplits = 64;
-constexpr int kFewRows = 32;  // of a request and key head: more take the kernel of attn_tile.hip
+constexpr int kWaves = 4;         // of a workgroup; they take its steps in turn
+constexpr int kStep = 64;         // positions of a wave's step
+constexpr int kMaxSplits = 512;
+constexpr int kBlocks = 1024;     // workgroups of a decode launch, 4 a CU
+constexpr int kFewRows = 32;      // of a request and key head: more take the kernel of attn_tile.hip
 
-// The pages of one step's two halves of 16 positions, the codes of its 32 keys and values, and their
-// scale bytes.  Lane (r16, q4) holds key r16 of either half: 16 bytes from each 128 dimensions (8 where
-// D is 64), which are one block of 32, so an MFMA step's K index (q4, j) stands for dimension
-// 128 x + 32 q4 + 8 kk + j and Q is read likewise.  Values come in rows: 16 bytes (a block) a lane.
-template <int D>
-struct Codes {
-  static constexpr int XK = D > 128 ? D / 128 : 1;  // key loads a half
-  static constexpr int WK = D >= 128 ? 4 : 2;       // words of one
-  static constexpr int NV = D / 64;                 // value loads of the step
-  uint32_t k[2][XK][WK];
-  uint8_t ks[2][XK];
-  u32x4 v[NV];
-  uint8_t vs[NV];
-  bool ok[2];
+// The pages of a step's four 16 positions, the same for all lanes.  An entry that names no page reads as zeros
+// (its buffer has no bytes), and its positions are hidden.
+struct Pages {
+  __amdgpu_buffer_rsrc_t page[4];
+  int shown;  // a bit each
 };
 
+// The codes of a step's keys and their scale bytes.  Lane (r16, q4) holds key r16 of each 16: 16 bytes from
+// every 128 dimensions (8 where D is 64), which are one block of 32, so an MFMA step's K index (q4, j) stands
+// for dimension 128 x + 32 q4 + 8 kk + j and Q is read likewise.
 template <int D>
-__device__ __forceinline__ int value_token(int j, int lane) {
-  constexpr int PV = D / 32;  // 16-byte pieces of a row
-  return (j * 64 + lane) / PV;
-}
-
+struct Keys {
+  static constexpr int XK = D > 128 ? D / 128 : 1;  // loads of 16 keys
+  static constexpr int WK = D >= 128 ? 4 : 2;       // words of one
+  uint32_t w[4][XK][WK];
+  uint8_t s[4][XK];
+};
 template <int D>
-__device__ __forceinline__ void load(const AttendArgs& a, Codes<D>& c, const int (&page)[2], int pos, int h, int lane) {
-  const int r16 = lane & 15, q4 = lane >> 4, size = 1 << a.page_shift;
-  const uint8_t* base[2];
-  int at[2];
+__device__ __forceinline__ void load_keys(Keys<D>& c, const Pages& p, int pos, int size, int lane) {
+  const int r16 = lane & 15, q4 = lane >> 4;
 #pragma unroll
-  for (int half = 0; half < 2; ++half) {
-    c.ok[half] = page[half] >= 0 && page[half] < a.pages;  // an entry that names no page: its positions are hidden
-    base[half] = a.data + ((int64_t)(c.ok[half] ? page[half] : 0) * a.kv_heads + h) * kv4_page_bytes(size, D);
-    at[half] = (pos + 16 * half) & (size - 1);
+  for (int g = 0; g < 4; ++g) {
+    const int at = (pos + 16 * g) & (size - 1), codes = at * (D / 2), scales = size * D + at * (D / 32);
 #pragma unroll
-    for (int x = 0; x < Codes<D>::XK; ++x) {
-      const uint8_t* p = base[half] + (at[half] + r16) * (D / 2);
-      const uint8_t* s = base[half] + size * D + (at[half] + r16) * (D / 32);
+    for (int x = 0; x < Keys<D>::XK; ++x) {
       if constexpr (D >= 128) {
-        const u32x4 w = *reinterpret_cast<const u32x4*>(p + 64 * x + 16 * q4);
+        const u32x4 w = buf_ld16<u32x4>(p.page[g], r16 * (D / 2) + 16 * q4 + 64 * x, codes);
 #pragma unroll
-        for (int i = 0; i < 4; ++i) c.k[half][x][i] = w[i];
-        c.ks[half][x] = s[4 * x + q4];
+        for (int i = 0; i < 4; ++i) c.w[g][x][i] = w[i];
+        c.s[g][x] = __builtin_amdgcn_raw_buffer_load_b8(p.page[g], r16 * (D / 32) + q4 + 4 * x, scales, 0);
       } else {
-        const uint2 w = *reinterpret_cast<const uint2*>(p + 8 * q4);
-        c.k[half][x][0] = w.x;
-        c.k[half][x][1] = w.y;
-        c.ks[half][x] = s[q4 >> 1];
+        const auto w = __builtin_amdgcn_raw_buffer_load_b64(p.page[g], r16 * (D / 2) + 8 * q4, codes, 0);
+        c.w[g][x][0] = w[0];
+        c.w[g][x][1] = w[1];
+        c.s[g][x] = __builtin_amdgcn_raw_buffer_load_b8(p.page[g], r16 * (D / 32) + (q4 >> 1), scales, 0);
       }
     }
   }
-#pragma unroll
-  for (int j = 0; j < Codes<D>::NV; ++j) {
-    constexpr int PV = D / 32;
-    const int tok = value_token<D>(j, lane), piece = lane % PV;
-    const int half = D == 64 ? tok >> 4 : j * 64 / PV / 16;
-    const uint8_t* b = half ? base[1] : base[0];
-    const int row = (half ? at[1] : at[0]) + (tok & 15);
-    c.v[j] = *reinterpret_cast<const u32x4*>(b + size * (D / 2) + row * (D / 2) + 16 * piece);
-    c.vs[j] = b[size * D + size * (D / 32) + row * (D / 32) + piece];
-  }
 }
 
-__device__ __forceinline__ int min16(int x) {
+// Of the values, up to 128 dimensions of 32 positions at a time: PC lanes a position hold 32 of them each.
+template <int D>
+struct Values {
+  static constexpr int DC = D < 128 ? D : 128, PC = DC / 32, J = DC / 64;
+  u32x4 w[D / DC][2][J];
+  uint8_t s[D / DC][2][J];
+  static __device__ __forceinline__ int position(int half, int j, int lane) { return 32 * half + 64 / PC * j + lane / PC; }
+};
+template <int D>
+__device__ __forceinline__ void load_values(Values<D>& c, const Pages& p, int pos, int size, int lane) {
+  typedef Values<D> V;
 #pragma unroll
-  for (int o = 1; o < 16; o <<= 1) x = min(x, __shfl_xor(x, o, 64));
-  return x;
+  for (int half = 0; half < 2; ++half)
+#pragma unroll
+    for (int j = 0; j < V::J; ++j) {
+      const int g = 2 * half + j, at = (pos + 16 * g) & (size - 1);
+      const int codes = size * (D / 2) + at * (D / 2), scales = size * D + size * (D / 32) + at * (D / 32);
+#pragma unroll
+      for (int x = 0; x < D / V::DC; ++x) {
+        if constexpr (D >= 128) {
+          c.w[x][half][j] = buf_ld16<u32x4>(p.page[g], lane / 4 * (D / 2) + lane % 4 * 16 + 64 * x, codes);
+          c.s[x][half][j] = __builtin_amdgcn_raw_buffer_load_b8(p.page[g], lane / 4 * (D / 32) + lane % 4 + 4 * x, scales, 0);
+        } else {
+          // 32 positions a load, which two pages may hold: a lane's offset lies beyond the one that is not its own
+          const int at1 = (pos + 16 * g + 16) & (size - 1), none = 1 << 30;
+          const int lo = lane < 32 ? lane * 16 : none, hi = lane < 32 ? none : (lane - 32) * 16;
+          const int slo = lane < 32 ? lane : none, shi = lane < 32 ? none : lane - 32;
+          c.w[x][half][j] = buf_ld16<u32x4>(p.page[g], lo, codes) |
+                            buf_ld16<u32x4>(p.page[g + 1], hi, size * (D / 2) + at1 * (D / 2));
+          c.s[x][half][j] = __builtin_amdgcn_raw_buffer_load_b8(p.page[g], slo, scales, 0) |
+                            __builtin_amdgcn_raw_buffer_load_b8(p.page[g + 1], shi,
+                                                                size * D + size * (D / 32) + at1 * (D / 32), 0);
+        }
+      }
+    }
+}
+
+// over the 16 rows, by rotations of a row of lanes; the four rows hold the same
+template <int N>
+__device__ __forceinline__ int turned(int x) {
+  return __builtin_amdgcn_mov_dpp(x, 0x120 + N, 0xF, 0xF, true);
+}
+__device__ __forceinline__ int min16(int x) {
+  x = min(x, turned<1>(x));
+  x = min(x, turned<2>(x));
+  x = min(x, turned<4>(x));
+  return __builtin_amdgcn_readfirstlane(min(x, turned<8>(x)));
 }
 __device__ __forceinline__ int max16(int x) {
-#pragma unroll
-  for (int o = 1; o < 16; o <<= 1) x = max(x, __shfl_xor(x, o, 64));
-  return x;
+  x = max(x, turned<1>(x));
+  x = max(x, turned<2>(x));
+  x = max(x, turned<4>(x));
+  return __builtin_amdgcn_readfirstlane(max(x, turned<8>(x)));
 }
 
-// One workgroup: 16 rows of one request and key head, one of `splits` parts of the positions.  The
-// waves' steps interleave, each with its own maximum, sum and O^T, and are joined at the end.
+// One workgroup: 16 rows of one request and key head, one of gridDim.z parts of the positions, `per` steps
+// long (the last parts, which are empty where requests are shorter, come last).  The waves' steps interleave,
+// each with its own maximum, sum and O^T, and are joined at the end.  A step's codes are on their way from the
+// moment those before have been used, in registers.
 template <class E, int D>
-__global__ __launch_bounds__(64 * kWaves) void attend_kernel(AttendArgs a, int tiles, int splits) {
+__global__ __launch_bounds__(64 * kWaves, D == 256 ? 2 : 3) void attend_kernel(AttendArgs a, int tiles, int per) {
   typedef typename Vec<E>::x8 x8;
-  constexpr int LD = D + 16;  // 8 banks further each row: the transposed reads of 8 rows meet no bank twice
+  typedef Values<D> V;
+  constexpr int DC = V::DC, LD = DC + 16;  // 8 banks further each row: the transposed reads of 8 rows meet no bank twice
   constexpr int KQ = D / 32, MT = D / 16;
-  __shared__ __align__(16) E vt[kWaves][kStep * LD];
+  __shared__ __align__(16) E vt[kWaves][32 * LD];
   __shared__ float wm[kWaves][16], wl[kWaves][16];
-  static_assert(kStep * LD * sizeof(E) >= 16 * D * sizeof(float), "the waves' O^T pass through their value tiles");
+  static_assert(32 * LD * sizeof(E) >= 16 * DC * sizeof(float), "the waves' O^T pass through their value tiles");
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int r16 = lane & 15, q4 = lane >> 4;
-  int b = blockIdx.x;
-  const int s = b % splits;
-  b /= splits;
-  const int h = b % a.kv_heads;
-  b /= a.kv_heads;
-  const int tile0 = b % tiles, r = b / tiles, group = a.heads / a.kv_heads, T = (int)a.T;
+  const int s = blockIdx.z, splits = gridDim.z, h = blockIdx.y;
+  const int r = tiles == 1 ? blockIdx.x : blockIdx.x / tiles, tile0 = tiles == 1 ? 0 : blockIdx.x - r * tiles;
+  const int T = (int)a.T, group = a.group.d;
   const int from = r == 0 ? 0 : min(max(a.starts[r], 0), T);
   const int to = r == a.N ? T : min(max(a.starts[r + 1], from), T);  // request N: the padding behind the last
-  const int rows = (to - from) * group;
+  const int rows = (to - from) * group, size = 1 << a.page_shift;
   const int room = (int)min((int64_t)a.columns << a.page_shift, (int64_t)INT32_MAX - 1024);
+  const uint8_t* const head_base = a.data + (int64_t)h * kv4_page_bytes(size, D);
+  const uint64_t stride = (uint64_t)a.kv_heads * kv4_page_bytes(size, D);
+  // the exponent's factor, never 0: a masked score stays -infinity; its sign goes with Q
+  const float c = fmaxf(fabsf(a.scale) * 1.44269504088896341f, 1.17549435e-38f);
 
   for (int tile = tile0; tile * 16 < rows; tile += tiles) {
     const int rho = tile * 16 + r16;
     const bool real = rho < rows;
-    const int t = from + (real ? rho / group : 0), head = h * group + (real ? rho % group : 0);
+    const int row_t = real ? a.group.of(rho) : 0;
+    const int t = from + row_t, head = h * group + (real ? rho - row_t * group : 0);
     const int hi = real && r < a.N ? min(max(a.visible[t], 0), room) : 0;
     const int lo = a.window > 0 ? max(0, hi - a.window) : 0;
     // over the rows that see anything: from the first position any of them sees to the last, and the
     // range that all of them see, where nothing is masked
     const int first = min16(hi > 0 ? lo : INT32_MAX), last = max16(hi);
     const int low = max16(lo), high = min16(real ? hi : INT32_MAX);
+    const int begin = last > 0 ? first & ~(kStep - 1) : 0;
+    const int steps = (last - begin + kStep - 1) / kStep;
+    const int stop = min(steps, (s + 1) * per);
+    if (s > 0 && s * per >= steps) {  // nothing of it here: only the join hears of this part
+      if (tid < 16 && real) {
+        float* ml = a.ws + a.T * a.heads * splits * D + (((int64_t)t * a.heads + head) * splits + s) * 2;
+        ml[0] = -INFINITY;
+        ml[1] = 0.f;
+      }
+      continue;
+    }
 
     x8 qf[KQ];
     {
       const E* q = static_cast<const E*>(a.q) + t * a.q_token + head * a.q_head;
 #pragma unroll
-      for (int i = 0; i < KQ; ++i)
-        qf[i] = real ? ld8(q + (D >= 128 ? 128 * (i / 4) + 32 * q4 + 8 * (i % 4) : 16 * q4 + 8 * i)) : zero8v<E>();
+      for (int k = 0; k < KQ; ++k) {
+        u32x4 w = real ? *reinterpret_cast<const u32x4*>(q + (D >= 128 ? 128 * (k / 4) + 32 * q4 + 8 * (k % 4) : 16 * q4 + 8 * k))
+                       : u32x4{0, 0, 0, 0};
+        if (a.scale < 0.f) w ^= 0x80008000u;
+        qf[k] = __builtin_bit_cast(x8, w);
+      }
     }
     f32x4 o[MT];
 #pragma unroll
     for (int i = 0; i < MT; ++i) o[i] = zero4();
     float m = -INFINITY, l = 0.f;
-
-    const int begin = last > 0 ? first & ~(kStep - 1) : 0;
-    const int steps = (last - begin + kStep - 1) / kStep;
-    const int per = (((steps + splits - 1) / splits) + kWaves - 1) / kWaves * kWaves;
-    const int stop = min(steps, (s + 1) * per);
-    const float c = a.scale * 1.44269504088896341f;
+    uint32_t nan = 0;  // blocks of 32 dimensions in which the row sees a NaN value
     E* const vw = vt[wave];
 
     int i = s * per + wave;
-    if (i < stop) {
-      Codes<D> next;
-      int pg[2];
+    while (i < stop) {
+      // the block table's next 64 entries, an entry a lane: the steps they serve find their pages without a load
+      int pos = begin + i * kStep;
+      const int column0 = pos >> a.page_shift;
+      const int table = column0 + lane < a.columns ? a.tables[r * a.table_stride + column0 + lane] : -1;
+      const int64_t reach = (int64_t)(column0 + 64) << a.page_shift;  // the first position beyond them
+      const int end = (int)min((int64_t)stop, (reach - begin) / kStep);
+      const auto find = [&](int at) {
+        Pages x;
+        x.shown = 0;
+#pragma unroll
+        for (int g = 0; g < 4; ++g) {
+          const uint32_t page = __builtin_amdgcn_readlane(table, ((at + 16 * g) >> a.page_shift) - column0);
+          const bool ok = page < a.page_count;
+          x.page[g] = buf_rsrc(head_base + (ok ? page * stride : 0), ok ? kv4_page_bytes(size, D) : 0);
+          x.shown |= ok ? 1 << g : 0;
+        }
+        return x;
+      };
+      Keys<D> keys;
+      V values;
+      int shown;
       {
-        const int pos = begin + i * kStep;
-        pg[0] = page_of(a, r, pos);
-        pg[1] = page_of(a, r, pos + 16);
-        load<D>(a, next, pg, pos, h, lane);
-        pg[0] = page_of(a, r, pos + kWaves * kStep);
-        pg[1] = page_of(a, r, pos + kWaves * kStep + 16);
+        const Pages p = find(pos);
+        load_keys<D>(keys, p, pos, size, lane);
+        load_values<D>(values, p, pos, size, lane);
+        shown = p.shown;
       }
-      for (; i < stop; i += kWaves) {
-        const Codes<D> now = next;
-        const int pos = begin + i * kStep;
-        if (i + kWaves < stop) {
-          load<D>(a, next, pg, pos + kWaves * kStep, h, lane);
-          pg[0] = page_of(a, r, pos + 2 * kWaves * kStep);
-          pg[1] = page_of(a, r, pos + 2 * kWaves * kStep + 16);
-        }
-        const bool full = pos >= low && pos + kStep <= high && now.ok[0] && now.ok[1];
-        // scores, in units of log2
-        float sc[8];
+      for (; i < end; i += kWaves, pos += kWaves * kStep) {
+        const bool more = i + kWaves < end, full = pos >= low && pos + kStep <= high && shown == 15;
+        f32x4 sc[4];
 #pragma unroll
-        for (int half = 0; half < 2; ++half) {
-          f32x4 acc = zero4();
+        for (int g = 0; g < 4; ++g) {
+          sc[g] = zero4();
 #pragma unroll
-          for (int x = 0; x < Codes<D>::XK; ++x) {
-            const float ks = kv4_scale(now.ks[half][x]);
+          for (int x = 0; x < Keys<D>::XK; ++x) {
+            const float ks = kv4_scale(keys.s[g][x]);
 #pragma unroll
-            for (int w = 0; w < Codes<D>::WK; ++w)
-              acc = mfma(kv4_values<E>(now.k[half][x][w], ks), qf[x * Codes<D>::WK + w], acc);
-          }
-#pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            float y = acc[e] * c;
-            if (!full) {
-              const int p = pos + 16 * half + 4 * q4 + e;
-              if (p < lo || p >= hi || !now.ok[half]) y = -INFINITY;
-            }
-            sc[4 * half + e] = y;
+            for (int w = 0; w < Keys<D>::WK; ++w)
+              sc[g] = mfma(kv4_values<E>(keys.w[g][x][w], ks), qf[x * Keys<D>::WK + w], sc[g]);
           }
         }
-        float top = sc[0];
+        Pages next;
+        if (more) {
+          next = find(pos + kWaves * kStep);
+          load_keys<D>(keys, next, pos + kWaves * kStep, size, lane);
+        }
+        if (!full) {
+          const int at0 = pos + 4 * q4;
 #pragma unroll
-        for (int e = 1; e < 8; ++e) top = fmaxf(top, sc[e]);
+          for (int g = 0; g < 4; ++g)
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+              if (16 * g + e < lo - at0 || 16 * g + e >= hi - at0 || !(shown >> g & 1)) sc[g][e] = -INFINITY;
+        }
+        float top = sc[0][0];
+#pragma unroll
+        for (int g = 0; g < 4; ++g)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) top = fmaxf(top, sc[g][e]);
+        top *= c;
         if (__any(top > m + kLazy)) {  // the maximum moves rarely, and for each row by itself
           top = fmaxf(top, __shfl_xor(top, 16, 64));
           top = fmaxf(top, __shfl_xor(top, 32, 64));
@@ -202,153 +257,217 @@ __global__ __launch_bounds__(64 * kWaves) void attend_kernel(AttendArgs a, int t
             for (int k = 0; k < MT; ++k) o[k] *= f;
           }
         }
-        const float base = (m == -INFINITY ? 0.f : m) - kAttendBias<E>;
-        float p[8];
+        const float base = kAttendBias<E> - (m == -INFINITY ? 0.f : m);
 #pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          p[e] = __builtin_amdgcn_exp2f(sc[e] - base);
-          l += p[e];
-        }
-        const x8 pf = to8<E>(f32x8{p[0], p[1], p[2], p[3], p[4], p[5], p[6], p[7]});
-        // values, row by row; where not every row sees every position, a position that none sees is zero,
-        // and a NaN reaches only the rows that see it
+        for (int half = 0; half < 2; ++half) {
+          f32x8 p;
 #pragma unroll
-        for (int j = 0; j < Codes<D>::NV; ++j) {
-          constexpr int PV = D / 32;
-          const int tok = value_token<D>(j, lane), piece = lane % PV;
-          u32x4 w = now.v[j];
-          uint32_t sb = now.vs[j];
-          if (!full) {
-            const bool any = pos + tok >= first && pos + tok < last && ((tok >> 4) ? now.ok[1] : now.ok[0]);
-            uint64_t bad = __ballot(any && sb == 255);
-            if (!any || sb == 255) {
-              w = u32x4{0, 0, 0, 0};
-              sb = 0;
-            }
-            for (; bad; bad &= bad - 1) {
-              const int n = __builtin_ctzll(bad), at = pos + value_token<D>(j, n);
-              const float add = at >= lo && at < hi ? __builtin_nanf("") : 0.f;
-#pragma unroll
-              for (int k = 0; k < MT; ++k)
-                if (k / 2 == n % PV) o[k] += add;
-            }
+          for (int e = 0; e < 8; ++e) {
+            p[e] = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[2 * half + (e >> 2)][e & 3], c, base));
+            l += p[e];
           }
-          const float vs = kv4_scale(sb);
+          const x8 pf = to8<E>(p);
+          // values: where not every row sees every position, a position that none sees is zero, and a NaN
+          // reaches only the rows that see it
 #pragma unroll
-          for (int e = 0; e < 4; ++e) st8(vw + tok * LD + 32 * piece + 8 * e, kv4_values<E>(w[e], vs));
+          for (int x = 0; x < D / DC; ++x) {
+#pragma unroll
+            for (int j = 0; j < V::J; ++j) {
+              const int tok = V::position(half, j, lane), piece = lane % V::PC;
+              u32x4 w = values.w[x][half][j];
+              uint32_t sb = values.s[x][half][j];
+              if (!full) {
+                const bool any = pos + tok >= first && pos + tok < last;
+                for (uint64_t bad = __ballot(any && sb == 255); bad; bad &= bad - 1) {
+                  const int n = __builtin_ctzll(bad), at = pos + V::position(half, j, n);
+                  nan |= at >= lo && at < hi ? 1u << (V::PC * x + n % V::PC) : 0u;
+                }
+                if (!any || sb == 255) {
+                  w = u32x4{0, 0, 0, 0};
+                  sb = 0;
+                }
+              }
+              const float vs = kv4_scale(sb);
+#pragma unroll
+              for (int e = 0; e < 4; ++e)
+                st8(vw + (tok - 32 * half) * LD + 32 * piece + 8 * e, kv4_values<E>(w[e], vs));
+            }
+#pragma unroll
+            for (int k = 0; k < DC / 16; ++k)
+              o[DC / 16 * x + k] = mfma(ld8_trpv<E>(vw, LD, 0, 16 * k), pf, o[DC / 16 * x + k]);
+          }
         }
-#pragma unroll
-        for (int k = 0; k < MT; ++k) o[k] = mfma(ld8_trpv<E>(vw, LD, 0, 16 * k), pf, o[k]);
+        if (more) {
+          load_values<D>(values, next, pos + kWaves * kStep, size, lane);
+          shown = next.shown;
+        }
       }
     }
     l += __shfl_xor(l, 16, 64);
     l += __shfl_xor(l, 32, 64);
-    // join the waves: O^T rows through LDS, their 16-byte columns XORed with the row against bank conflicts
-    float* const ow = reinterpret_cast<float*>(vw);
+    if (__any(nan != 0)) {
 #pragma unroll
-    for (int k = 0; k < MT; ++k)
-      *reinterpret_cast<f32x4*>(ow + r16 * D + 4 * ((4 * k + q4) ^ r16)) = o[k];
+      for (int k = 0; k < MT; ++k)
+        if (nan >> (k / 2) & 1) o[k] = zero4() + __builtin_nanf("");
+    }
+    // join the waves: O^T rows through LDS, DC dimensions at a time, their 16-byte columns XORed with the row
+    // against bank conflicts
     if (q4 == 0) {
       wm[wave][r16] = m;
       wl[wave][r16] = l;
     }
-    __syncthreads();
-    {
-      const int row = tid >> 4, n = tile * 16 + row;
-      float M = wm[0][row];
+    const int row = tid >> 4, n = tile * 16 + row, n_t = a.group.of(n);
+    const int64_t at = (int64_t)(from + n_t) * a.heads + h * group + n - n_t * group;
+    float M, L = 0.f, f[kWaves];
 #pragma unroll
-      for (int w = 1; w < kWaves; ++w) M = fmaxf(M, wm[w][row]);
-      float f[kWaves], L = 0.f;
+    for (int x = 0; x < D / DC; ++x) {
 #pragma unroll
-      for (int w = 0; w < kWaves; ++w) {
-        f[w] = wm[w][row] == -INFINITY ? 0.f : exp2f(wm[w][row] - M);
-        L += f[w] * wl[w][row];
+      for (int k = 0; k < DC / 16; ++k)
+        *reinterpret_cast<f32x4*>(reinterpret_cast<float*>(vw) + r16 * DC + 4 * ((4 * k + q4) ^ r16)) = o[DC / 16 * x + k];
+      __syncthreads();
+      if (x == 0) {
+        M = wm[0][row];
+#pragma unroll
+        for (int w = 1; w < kWaves; ++w) M = fmaxf(M, wm[w][row]);
+#pragma unroll
+        for (int w = 0; w < kWaves; ++w) {
+          f[w] = wm[w][row] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(wm[w][row] - M);
+          L += f[w] * wl[w][row];
+        }
       }
       if (n < rows) {
-        const int64_t at = (int64_t)(from + n / group) * a.heads + h * group + n % group;
-        const float inv = L == 0.f ? 0.f : 1.f / L;
 #pragma unroll
-        for (int k = 0; k < D / 64; ++k) {
+        for (int k = 0; k < DC / 64; ++k) {
           const int col = (tid & 15) + 16 * k;
           f32x4 y = zero4();
 #pragma unroll
           for (int w = 0; w < kWaves; ++w)
-            y += f[w] * *reinterpret_cast<const f32x4*>(reinterpret_cast<float*>(vt[w]) + row * D + 4 * (col ^ row));
+            y += f[w] * *reinterpret_cast<const f32x4*>(reinterpret_cast<float*>(vt[w]) + row * DC + 4 * (col ^ row));
           if (splits == 1)
-            st4(static_cast<E*>(a.out) + at * D + 4 * col, L == 0.f ? zero4() : y * inv);
+            st4(static_cast<E*>(a.out) + at * D + DC * x + 4 * col, L == 0.f ? zero4() : y * (1.f / L));
           else if (M != -INFINITY || L != 0.f)  // the join reads no part that saw nothing
-            *reinterpret_cast<f32x4*>(a.ws + (at * splits + s) * D + 4 * col) = y;
-        }
-        if ((tid & 15) == 0) {
-          if (splits > 1) {
-            float* ml = a.ws + a.T * a.heads * splits * D + (at * splits + s) * 2;
-            ml[0] = M;
-            ml[1] = L;
-          } else if (a.lse) {
-            a.lse[at] = (M - kAttendBias<E> + log2f(L)) * 0.693147180559945309f;
-          }
+            *reinterpret_cast<f32x4*>(a.ws + (at * splits + s) * D + DC * x + 4 * col) = y;
         }
       }
+      __syncthreads();
     }
-    __syncthreads();
+    if (n < rows && (tid & 15) == 0) {
+      if (splits > 1) {
+        float* ml = a.ws + a.T * a.heads * splits * D + (at * splits + s) * 2;
+        ml[0] = M;
+        ml[1] = L;
+      } else if (a.lse) {
+        a.lse[at] = (M - kAttendBias<E> + log2f(L)) * 0.693147180559945309f;
+      }
+    }
   }
 }
 
-// Joins the parts of a row: 16 rows a workgroup, 16 lanes a row.
+// Joins the parts of a row, a workgroup for 64 dimensions: the parts' weights, then 16 parts at a time.
 template <class E, int D>
 __global__ __launch_bounds__(256) void join_kernel(AttendArgs a, int splits) {
-  const int64_t at = (int64_t)blockIdx.x * 16 + (threadIdx.x >> 4);
-  if (at >= a.T * a.heads) return;
-  const float* ml = a.ws + a.T * a.heads * splits * D + at * splits * 2;
-  float M = -INFINITY;
-  for (int s = 0; s < splits; ++s) M = fmaxf(M, ml[2 * s]);
-  float L = 0.f;
-  f32x4 y[D / 64];
+  constexpr int W = kMaxSplits / 256;
+  __shared__ float weight[kMaxSplits];
+  __shared__ float red[2][4];
+  __shared__ int count[4];
+  __shared__ __align__(16) float part[16][64];
+  const int64_t at = blockIdx.x / (D / 64);
+  const int d0 = blockIdx.x % (D / 64) * 64;
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, col = tid & 15, g = tid >> 4;
+  const float2* ml = reinterpret_cast<const float2*>(a.ws + a.T * a.heads * splits * D) + at * splits;
+  float2 mine[W];
+  float M = -INFINITY, L = 0.f;
+  int n = 0;  // parts up to the last that saw anything; the others wrote no row
 #pragma unroll
-  for (int k = 0; k < D / 64; ++k) y[k] = zero4();
-  for (int s = 0; s < splits; ++s) {
-    if (ml[2 * s] == -INFINITY && ml[2 * s + 1] == 0.f) continue;
-    const float f = exp2f(ml[2 * s] - M);
-    L += f * ml[2 * s + 1];
-#pragma unroll
-    for (int k = 0; k < D / 64; ++k)
-      y[k] += f * *reinterpret_cast<const f32x4*>(a.ws + (at * splits + s) * D + 4 * ((threadIdx.x & 15) + 16 * k));
+  for (int j = 0; j < W; ++j) {
+    const int s = tid + 256 * j;
+    mine[j] = s < splits ? ml[s] : float2{-INFINITY, 0.f};
+    M = fmaxf(M, mine[j].x);
+    if (mine[j].x != -INFINITY || mine[j].y != 0.f) n = s + 1;
   }
 #pragma unroll
-  for (int k = 0; k < D / 64; ++k)
-    st4(static_cast<E*>(a.out) + at * D + 4 * ((threadIdx.x & 15) + 16 * k), L == 0.f ? zero4() : y[k] * (1.f / L));
-  if (a.lse && (threadIdx.x & 15) == 0) a.lse[at] = (M - kAttendBias<E> + log2f(L)) * 0.693147180559945309f;
+  for (int o = 1; o < 64; o <<= 1) {
+    M = fmaxf(M, __shfl_xor(M, o, 64));
+    n = max(n, __shfl_xor(n, o, 64));
+  }
+  if (lane == 0) {
+    red[0][wave] = M;
+    count[wave] = n;
+  }
+  __syncthreads();
+  M = fmaxf(fmaxf(red[0][0], red[0][1]), fmaxf(red[0][2], red[0][3]));
+  n = max(max(count[0], count[1]), max(count[2], count[3]));
+#pragma unroll
+  for (int j = 0; j < W; ++j) {
+    const bool empty = mine[j].x == -INFINITY && mine[j].y == 0.f;
+    const float f = empty ? 0.f : __builtin_amdgcn_exp2f(mine[j].x - M);
+    weight[tid + 256 * j] = empty ? -1.f : f;
+    L += f * mine[j].y;
+  }
+#pragma unroll
+  for (int o = 1; o < 64; o <<= 1) L += __shfl_xor(L, o, 64);
+  if (lane == 0) red[1][wave] = L;
+  __syncthreads();
+  L = (red[1][0] + red[1][1]) + (red[1][2] + red[1][3]);
+  f32x4 y = zero4();
+  const float* rows = a.ws + at * splits * D + d0 + 4 * col;
+#pragma unroll 4
+  for (int s = g; s < n; s += 16) {
+    const f32x4 x = *reinterpret_cast<const f32x4*>(rows + s * D);
+    const float f = weight[s];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) y[e] += f < 0.f ? 0.f : f * x[e];
+  }
+  *reinterpret_cast<f32x4*>(&part[g][4 * col]) = y;
+  __syncthreads();
+  if (tid < 16) {
+#pragma unroll
+    for (int k = 1; k < 16; ++k) y += *reinterpret_cast<const f32x4*>(&part[k][4 * col]);
+    st4(static_cast<E*>(a.out) + at * D + d0 + 4 * col, L == 0.f ? zero4() : y * (1.f / L));
+  }
+  if (a.lse && tid == 0 && d0 == 0) a.lse[at] = (M - kAttendBias<E> + log2f(L)) * 0.693147180559945309f;
 }
 
-// How a call runs: by which kernel, and in how many parts of the positions.
+// How a call runs: by which kernel, and in how many parts of the positions, of `per` steps each (decode).
 struct Plan {
   bool tiles;
-  int splits;
+  int splits, per;
 };
-Plan attend_plan(int64_t N, int kv_heads, int group, int max_queries, int64_t capacity) {
+// `capacity` positions a table row holds; with a window a row sees no more of them than it, and never more parts.
+Plan attend_plan(int64_t N, int kv_heads, int group, int max_queries, int64_t capacity, int window) {
   const int64_t rows = (int64_t)max_queries * group;
+  const int64_t seen = window > 0 ? std::min(capacity, (int64_t)window + max_queries + kStep) : capacity;
   if (rows > kFewRows) {
-    const int64_t blocks = N * kv_heads * ((rows + 127) / 128), most = std::min<int64_t>(kMaxSplits, (capacity + 511) / 512);
-    return {true, (int)std::max<int64_t>(1, std::min(most, 512 / std::max<int64_t>(blocks, 1)))};
+    const int64_t blocks = N * kv_heads * ((rows + 127) / 128), most = std::min<int64_t>(kMaxSplits, (seen + 511) / 512);
+    return {true, (int)std::max<int64_t>(1, std::min(most, 512 / std::max<int64_t>(blocks, 1))), 0};
   }
-  // as many parts as bring 1024 workgroups (4 a CU), each of at least 128 positions
-  const int64_t blocks = N * kv_heads * ((rows + 15) / 16), most = std::min<int64_t>(kMaxSplits, (capacity + 127) / 128);
-  return {false, (int)std::max<int64_t>(1, std::min(most, 1024 / std::max<int64_t>(blocks, 1)))};
+  // parts of the same length, so that ragged requests load the CUs alike: a step a wave at the least, and as
+  // long as keep the launch within kBlocks workgroups, were every request to fill its table row
+  constexpr int64_t kLeast = kWaves * kStep;
+  const auto parts = [](int64_t positions, int64_t most, int64_t& times) {
+    const int64_t least = (positions + kLeast - 1) / kLeast;
+    times = std::max<int64_t>(1, (least + most - 1) / most);
+    return std::max<int64_t>(1, (least + times - 1) / times);
+  };
+  const int64_t blocks = std::max<int64_t>(1, N * kv_heads * ((rows + 15) / 16));
+  int64_t times, splits = parts(capacity, std::min<int64_t>(kMaxSplits, std::max<int64_t>(1, kBlocks / blocks)), times);
+  if (window > 0) splits = parts(seen, splits, times);
+  return {false, (int)splits, (int)(times * kWaves)};
 }
 
 template <class E, int D>
 void launch_dim(const AttendArgs& a, hipStream_t st) {
   const int group = a.heads / a.kv_heads;
-  const Plan p = attend_plan(a.N, a.kv_heads, group, a.max_queries, (int64_t)a.columns << a.page_shift);
+  const Plan p = attend_plan(a.N, a.kv_heads, group, a.max_queries, (int64_t)a.columns << a.page_shift, a.window);
   if (p.tiles) {
     launch_attend_tiles(a, p.splits, st);
   } else {
     const int64_t each = (int64_t)(a.N + 1) * a.kv_heads * p.splits;
     const int tiles = (int)std::max<int64_t>(1, std::min<int64_t>(((int64_t)a.max_queries * group + 15) / 16, (1 << 23) / each));
     // a workgroup takes every tiles-th tile: none is left out whatever the bound
-    attend_kernel<E, D><<<(unsigned)(each * tiles), 64 * kWaves, 0, st>>>(a, tiles, p.splits);
+    attend_kernel<E, D><<<dim3((unsigned)((a.N + 1) * tiles), a.kv_heads, p.splits), 64 * kWaves, 0, st>>>(a, tiles, p.per);
   }
-  if (p.splits > 1) join_kernel<E, D><<<(unsigned)((a.T * a.heads + 15) / 16), 256, 0, st>>>(a, p.splits);
+  if (p.splits > 1) join_kernel<E, D><<<(unsigned)(a.T * a.heads * (D / 64)), 256, 0, st>>>(a, p.splits);
 }
 
 template <class E>
@@ -364,7 +483,7 @@ void by_dim(const AttendArgs& a, hipStream_t st) {
 }  // namespace
 
 size_t attend_workspace_bytes(int64_t T, int64_t N, int heads, int kv_heads, int D, int max_queries, int64_t capacity) {
-  const int splits = attend_plan(N, kv_heads, heads / kv_heads, max_queries, capacity).splits;
+  const int splits = attend_plan(N, kv_heads, heads / kv_heads, max_queries, capacity, 0).splits;
   return splits > 1 ? (size_t)T * heads * splits * (D + 2) * sizeof(float) : 0;
 }
 

@@ -141,7 +141,7 @@ int cqgdn_kv4_attend(const void* q, int64_t q_token, int64_t q_head, int dtype, 
                 "scale=%g", (long long)T, N, columns, (long long)table_stride, heads, kv_heads, window, max_queries,
                 (double)scale);
   if (T == 0) return ok();
-  if (T > (1 << 27) / heads || N >= (1 << 23) / kv_heads)
+  if (T > (1 << 27) / heads || N >= (1 << 23) / kv_heads || kv_heads > 65535)
     return fail(CQGDN_EUNSUPPORTED, "T=%lld rows of %d heads, or N=%d requests, are too many", (long long)T, heads, N);
   if (!q || !out || !visible || !starts || (N > 0 && columns > 0 && !tables) || !aligned(q, 16) || !aligned(out, 16) ||
       q_token % 8 || q_head % 8)
@@ -151,9 +151,9 @@ int cqgdn_kv4_attend(const void* q, int64_t q_token, int64_t q_head, int dtype, 
   const size_t need = attend_workspace_bytes(T, N, heads, kv_heads, head_dim, most, (int64_t)columns * page);
   if (need > 0 && (!workspace || !aligned(workspace, 256) || workspace_bytes < need))
     return fail(CQGDN_EINVAL, "workspace must be 256-byte aligned and >= cqgdn_kv4_attend_workspace_size");
-  const AttendArgs a{q, q_token, q_head, T, heads, kv_heads, head_dim, static_cast<const uint8_t*>(data), pages,
+  const AttendArgs a{q, q_token, q_head, T, heads, kv_heads, head_dim, static_cast<const uint8_t*>(data), (uint32_t)pages,
                      __builtin_ctz(page), tables, table_stride, pages > 0 ? columns : 0, starts, visible, N, window,
-                     scale, dtype == CQGDN_F16, most, out, lse, static_cast<float*>(workspace)};
+                     scale, dtype == CQGDN_F16, most, out, lse, static_cast<float*>(workspace), Divider(heads / kv_heads)};
   launch_attend(a, (hipStream_t)stream);
   return check_launch("cqgdn_kv4_attend");
 }

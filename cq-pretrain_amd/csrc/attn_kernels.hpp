@@ -64,13 +64,25 @@ struct RowsArgs {                 // rows written to, or read from, the cache
 void launch_kv4_write(const RowsArgs& a, hipStream_t st);
 void launch_kv4_read(const RowsArgs& a, hipStream_t st);
 
+// Division of n < 2^31 by d > 0 as a product: m = ceil(2^(31 + s) / d) with 2^s >= d is off by less than
+// 2^s / d / 2^(31 + s) of a unit, n times which stays below 1 / d.
+struct Divider {
+  uint32_t d, m;
+  int s;
+  explicit Divider(uint32_t by) : d(by), m(0), s(0) {
+    while ((1ull << s) < by) ++s;
+    m = (uint32_t)(((1ull << (31 + s)) + by - 1) / by);
+  }
+  __device__ __forceinline__ int of(int n) const { return s == 0 ? n : (int)(__umulhi((uint32_t)n, m) >> (s - 1)); }
+};
+
 struct AttendArgs {
   const void* q;
   int64_t q_token, q_head;
   int64_t T;
   int heads, kv_heads, D;
   const uint8_t* data;
-  int64_t pages;
+  uint32_t page_count;
   int page_shift;
   const int32_t* tables;
   int64_t table_stride;
@@ -83,6 +95,7 @@ struct AttendArgs {
   void* out;
   float* lse;
   float* ws;
+  Divider group;               // heads / kv_heads
 };
 // bytes of a call's workspace: the parts' O, maxima and sums, where the positions are split
 size_t attend_workspace_bytes(int64_t T, int64_t N, int heads, int kv_heads, int D, int max_queries, int64_t capacity);

@@ -54,7 +54,7 @@ template <int D>
 __device__ __forceinline__ Piece fetch(const AttendArgs& a, int page, int pos, int h, int piece) {
   Piece x;
   const int size = 1 << a.page_shift, at = pos & (size - 1);
-  x.ok = page >= 0 && page < a.pages;  // an entry that names no page: its positions are hidden
+  x.ok = page >= 0 && page < (int)a.page_count;  // an entry that names no page: its positions are hidden
   const uint8_t* base = a.data + ((int64_t)(x.ok ? page : 0) * a.kv_heads + h) * kv4_page_bytes(size, D);
   const uint8_t* code = base + at * (D / 2) + 16 * piece;
   const uint8_t* scale = base + size * D + at * (D / 32) + piece;
