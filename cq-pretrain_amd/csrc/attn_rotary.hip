@@ -15,6 +15,7 @@ namespace cqgdn {
 namespace {
 
 constexpr int kThreads = 256;
+constexpr int kTogether = 4;  // heads whose loads are under way at once
 
 __device__ __forceinline__ void turn(uint64_t fraction, float& s, float& c) {
   const int32_t hi = (int32_t)(fraction >> 32);
@@ -30,29 +31,31 @@ __device__ __forceinline__ void turn(uint64_t fraction, float& s, float& c) {
   c = ((quadrant + 1) & 2) ? -b : b;
 }
 
-template <class T, int N>
-struct Pack {
-  T v[N];
-};
-
-// A thread keeps the angles of VEC pairs of one token in registers and takes them through `per` heads,
-// so that a sine and cosine (some 40 operations) are paid once for several heads.
+// A thread keeps the angles of VEC pairs of one token in registers and takes them through `per` heads, so that
+// a sine and cosine (some 40 operations) are paid once for several heads; the loads of kTogether heads go out
+// before the first is turned.
 template <class T, int VEC, bool ADJ>
 __global__ __launch_bounds__(kThreads) void rotary_kernel(RotaryArgs a, int units, int turned, int per) {
   const int64_t t = (int64_t)blockIdx.x * blockDim.y + threadIdx.y;
   if (t >= a.T) return;
-  typedef Pack<T, VEC> P __attribute__((may_alias));
-  const int h0 = blockIdx.y * per, h1 = min(h0 + per, a.heads[0] + a.heads[1]);
+  typedef T P __attribute__((ext_vector_type(VEC)));
+  const int all = a.heads[0] + a.heads[1], h0 = blockIdx.y * per, h1 = min(h0 + per, all);
+  const T* const xq = static_cast<const T*>(a.x[0]) + t * a.token[0];
+  const T* const xk = static_cast<const T*>(a.x[1]) + t * a.token[1];
+  T* const yq = static_cast<T*>(a.y[0]) + t * a.heads[0] * a.D;
+  T* const yk = static_cast<T*>(a.y[1]) + t * a.heads[1] * a.D;
   for (int u = threadIdx.x; u < units; u += blockDim.x) {
     const bool rot = u < turned;
+    // two vectors, one of either half of the values that turn, or of those that pass: lanes side by side in both
+    const int at0 = rot ? u * (ADJ && VEC == 1 ? 2 : VEC) : a.rotary + (u - turned) * VEC;
+    const int at1 = at0 + (rot ? (ADJ && VEC == 1 ? 1 : a.rotary / 2) : (a.D - a.rotary) / 2);
     float s[VEC], c[VEC];
-    int at0, at1;
     if (rot) {
-      at0 = ADJ ? u * 2 * VEC : u * VEC;
-      at1 = ADJ ? at0 + VEC : a.rotary / 2 + u * VEC;
 #pragma unroll
       for (int j = 0; j < VEC; ++j) {
-        const int pair = u * VEC + j;
+        const int pair = !ADJ || VEC == 1 ? u * VEC + j
+                         : j < VEC / 2    ? u * VEC / 2 + j
+                                          : a.rotary / 4 + u * VEC / 2 + j - VEC / 2;
         const int ax = min(max(a.axis[pair], 0), a.axes - 1);
         const int64_t at = ax * a.axis_stride + t;
         const int64_t p = a.wide ? static_cast<const int64_t*>(a.positions)[at]
@@ -60,27 +63,47 @@ __global__ __launch_bounds__(kThreads) void rotary_kernel(RotaryArgs a, int unit
         turn((uint64_t)p * a.turns[pair], s[j], c[j]);
         if (a.back) s[j] = -s[j];
       }
-    } else {
-      at0 = a.rotary + (u - turned) * 2 * VEC;
-      at1 = at0 + VEC;
     }
-    for (int h = h0; h < h1; ++h) {
-      const int w = h >= a.heads[0], g = h - (w ? a.heads[0] : 0);
-      const T* x = static_cast<const T*>(a.x[w]) + t * a.token[w] + g * a.head[w];
-      T* y = static_cast<T*>(a.y[w]) + (t * a.heads[w] + g) * a.D;
-      P p0 = *reinterpret_cast<const P*>(x + at0), p1 = *reinterpret_cast<const P*>(x + at1);
-      if (rot) {
+    for (int h = h0; h < h1; h += kTogether) {
+      P p0[kTogether], p1[kTogether];
 #pragma unroll
-        for (int j = 0; j < VEC; ++j) {
-          T& l = ADJ ? (2 * j < VEC ? p0.v[(2 * j) % VEC] : p1.v[(2 * j) % VEC]) : p0.v[j];
-          T& r = ADJ ? (2 * j + 1 < VEC ? p0.v[(2 * j + 1) % VEC] : p1.v[(2 * j + 1) % VEC]) : p1.v[j];
-          const float fl = (float)l, fr = (float)r;
-          l = (T)(fl * c[j] - fr * s[j]);
-          r = (T)(fr * c[j] + fl * s[j]);
-        }
+      for (int i = 0; i < kTogether; ++i) {
+        const int g = h + i < h1 ? h + i : h1 - 1;  // the last once more rather than a branch between the loads
+        const T* x = g < a.heads[0] ? xq + g * a.head[0] : xk + (g - a.heads[0]) * a.head[1];
+        p0[i] = *reinterpret_cast<const P*>(x + at0);
+        p1[i] = *reinterpret_cast<const P*>(x + at1);
       }
-      *reinterpret_cast<P*>(y + at0) = p0;
-      *reinterpret_cast<P*>(y + at1) = p1;
+#pragma unroll
+      for (int i = 0; i < kTogether; ++i) {
+        const int g = h + i;
+        if (g >= h1) break;
+        if (rot) {
+#pragma unroll
+          for (int j = 0; j < VEC; ++j) {
+            float l, r;
+            if constexpr (!ADJ) {
+              l = (float)p0[i][j];
+              r = (float)p1[i][j];
+              p0[i][j] = (T)(l * c[j] - r * s[j]);
+              p1[i][j] = (T)(r * c[j] + l * s[j]);
+            } else if constexpr (VEC == 1) {
+              l = (float)p0[i][0];
+              r = (float)p1[i][0];
+              p0[i][0] = (T)(l * c[0] - r * s[0]);
+              p1[i][0] = (T)(r * c[0] + l * s[0]);
+            } else {
+              P& p = 2 * j < VEC ? p0[i] : p1[i];
+              l = (float)p[2 * j % VEC];
+              r = (float)p[2 * j % VEC + 1];
+              p[2 * j % VEC] = (T)(l * c[j] - r * s[j]);
+              p[2 * j % VEC + 1] = (T)(r * c[j] + l * s[j]);
+            }
+          }
+        }
+        T* y = g < a.heads[0] ? yq + g * a.D : yk + (g - a.heads[0]) * a.D;
+        *reinterpret_cast<P*>(y + at0) = p0[i];
+        *reinterpret_cast<P*>(y + at1) = p1[i];
+      }
     }
   }
 }
@@ -92,6 +115,8 @@ void launch(const RotaryArgs& a, hipStream_t st) {
   // as many heads a thread as leave 2^18 threads (16 waves a CU)
   int per = min(heads, 16);
   while (per > 1 && a.T * units * ((heads + per - 1) / per) < (1 << 18)) per = (per + 1) / 2;
+  const int groups = (heads + per - 1) / per;  // of about one size, whole loads at once
+  if (per > kTogether) per = ((heads + groups - 1) / groups + kTogether - 1) / kTogether * kTogether;
   const dim3 grid((unsigned)((a.T + by - 1) / by), (heads + per - 1) / per);
   if (a.adjacent)
     rotary_kernel<T, VEC, true><<<grid, dim3(bx, by), 0, st>>>(a, units, turned, per);
