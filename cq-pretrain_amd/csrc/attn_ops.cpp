@@ -12,6 +12,7 @@
 //   kv4_attend(q, data, tables, starts, visible, page, window, scale, max_queries, want_lse) -> (out, lse)
 
 #include <ATen/ATen.h>
+#include <ATen/ops/as_strided_native.h>
 #include <c10/core/DeviceGuard.h>
 #include <c10/hip/HIPStream.h>
 #include <torch/library.h>
@@ -53,6 +54,10 @@ Tensor head_rows(const Tensor& x) {
                    reinterpret_cast<uintptr_t>(x.data_ptr()) % 16 == 0;
   return fit ? x : x.clone(at::MemoryFormat::Contiguous);
 }
+
+// n elements of the vector x from `at` on: a view made without the dispatcher's overhead, which seven narrow()
+// would cost more of than the kernel takes
+Tensor part(const Tensor& x, int64_t at, int64_t n) { return at::native::as_strided_tensorimpl(x, {n}, {1}, at); }
 
 std::tuple<Tensor, Tensor> rotary(const Tensor& q, const Tensor& k, const Tensor& positions, const Tensor& turns,
                                   const Tensor& axis, bool adjacent, bool backward) {
@@ -109,12 +114,12 @@ std::tuple<Tensor, Tensor, Tensor, Tensor, Tensor, Tensor, Tensor> step_pages(co
   // one buffer: starts, admitted, lengths and the count (unless in place), then the three rows' vectors
   const int64_t rows = (tokens + 3) / 4 * 4, heads = (N + 1 + 3) / 4 * 4;
   const Tensor all = at::empty({3 * heads + 4 + 3 * rows}, cached.options());
-  const Tensor starts = all.narrow(0, 0, N + 1), admitted = all.narrow(0, heads, N);
-  const Tensor lengths = in_place ? cached : all.narrow(0, 2 * heads, N);
-  const Tensor left = in_place ? count : all.narrow(0, 3 * heads, 1);
+  const Tensor starts = part(all, 0, N + 1), admitted = part(all, heads, N);
+  const Tensor lengths = in_place ? cached : part(all, 2 * heads, N);
+  const Tensor left = in_place ? count : part(all, 3 * heads, 1);
   const int64_t at = 3 * heads + 4;
-  const Tensor slots = all.narrow(0, at, tokens), positions = all.narrow(0, at + rows, tokens),
-               visible = all.narrow(0, at + 2 * rows, tokens);
+  const Tensor slots = part(all, at, tokens), positions = part(all, at + rows, tokens),
+               visible = part(all, at + 2 * rows, tokens);
   const int columns = (int)tables.size(1);
   check(cqgdn_step_pages(cached.data_ptr<int32_t>(), fresh.data_ptr<int32_t>(), (int)N, tables.data_ptr<int32_t>(),
                          N > 1 ? tables.stride(0) : columns, columns, pool.data_ptr<int32_t>(), (int)pool.numel(),

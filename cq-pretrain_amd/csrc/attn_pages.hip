@@ -6,7 +6,9 @@
 //   ceil(cached / page) pages from the top of the pool, in order; where the pool is too small for it,
 //   it is not admitted (and, its need being counted, neither is a later one that needs pages).
 // One workgroup scans the requests, so the state (pool, tables, counts) has one writer and the result
-// does not depend on timing.
+// does not depend on timing.  A prefix sum gives every page that moves, and every row, its request by a binary
+// search, so that all 1024 threads move them whatever the requests' sizes: what is left is the latency of some
+// six dependent rounds of memory and of the scans.
 #include <hip/hip_runtime.h>
 
 #include "attn_kernels.hpp"
@@ -14,34 +16,51 @@
 namespace cqgdn {
 namespace {
 
-constexpr int kThreads = 1024;
-constexpr int kOneLaunch = 4096;  // tokens that the scanning workgroup writes itself
+constexpr int kThreads = 1024;    // and requests of a round
+constexpr int kOneLaunch = 4096;  // rows that the scanning workgroup writes itself
 
-// exclusive prefix sum over the workgroup; total is the sum over all its threads
-template <class I>
-__device__ __forceinline__ I scan(I x, int64_t* shared, I& total) {
-  I* const part = reinterpret_cast<I*>(shared);
+// exclusive prefix sums over the workgroup of x and y; sx and sy become the sums over all its threads
+struct Parts {
+  int64_t x[kThreads / 64];
+  int y[kThreads / 64];
+};
+__device__ __forceinline__ void scan(int64_t& x, int& y, int64_t& sx, int& sy, Parts& part) {
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  I y = x;
+  const int64_t x0 = x;
+  const int y0 = y;
 #pragma unroll
   for (int o = 1; o < 64; o <<= 1) {
-    const I z = __shfl_up(y, o, 64);
-    if (lane >= o) y += z;
+    const int64_t p = __shfl_up(x, o, 64);
+    const int q = __shfl_up(y, o, 64);
+    if (lane >= o) {
+      x += p;
+      y += q;
+    }
   }
   __syncthreads();  // part is free again
-  if (lane == 63) part[wave] = y;
+  if (lane == 63) {
+    part.x[wave] = x;
+    part.y[wave] = y;
+  }
   __syncthreads();
-  I before = 0;
-  total = 0;
+  sx = 0;
+  sy = 0;
+  int64_t bx = 0;
+  int by = 0;
 #pragma unroll
   for (int w = 0; w < kThreads / 64; ++w) {
-    if (w < wave) before += part[w];
-    total += part[w];
+    if (w < wave) {
+      bx += part.x[w];
+      by += part.y[w];
+    }
+    sx += part.x[w];
+    sy += part.y[w];
   }
-  return before + y - x;
+  x += bx - x0;
+  y += by - y0;
 }
 
-// the last r in 0 .. n - 1 with prefix[r] <= i, for prefix[0] = 0 <= i < prefix[n]
+// the last r in 0 .. n - 1 with prefix[r] <= i, for prefix[0] <= i
 __device__ __forceinline__ int owner(const int32_t* prefix, int n, int i) {
   int lo = 0, hi = n;
   while (hi - lo > 1) {
@@ -54,17 +73,13 @@ __device__ __forceinline__ int owner(const int32_t* prefix, int n, int i) {
   return lo;
 }
 
-__device__ __forceinline__ void token(const PagesArgs& a, int t, int total) {
-  int p = 0, slot = -1;
-  if (t < total) {
-    const int r = owner(a.starts, a.N, t);
-    const bool in = a.admitted[r] != 0;
-    p = a.lengths[r] - (in ? a.fresh[r] : 0) + t - a.starts[r];
-    if (in) {
-      const int entry = a.tables[r * a.table_stride + (p >> a.page_shift)];
-      const int64_t s = ((int64_t)entry << a.page_shift) + (p & ((1 << a.page_shift) - 1));
-      if (entry >= 0 && s <= INT32_MAX) slot = (int)s;
-    }
+// row t, at position p of request r
+__device__ __forceinline__ void row(const PagesArgs& a, int t, int r, int p, bool in) {
+  int slot = -1;
+  if (in) {
+    const int entry = a.tables[r * a.table_stride + (p >> a.page_shift)];
+    const int64_t s = ((int64_t)entry << a.page_shift) + (p & ((1 << a.page_shift) - 1));
+    if (entry >= 0 && s <= INT32_MAX) slot = (int)s;
   }
   a.slots[t] = slot;
   a.positions[t] = p;
@@ -72,60 +87,109 @@ __device__ __forceinline__ void token(const PagesArgs& a, int t, int total) {
 }
 
 __global__ __launch_bounds__(kThreads) void pages_kernel(PagesArgs a) {
-  __shared__ int64_t part[kThreads / 64];
+  __shared__ Parts part;
+  __shared__ int32_t prefix[kThreads], start[kThreads], base[kThreads];
+  __shared__ bool admitted[kThreads];
+  __shared__ int taken;
   const int tid = threadIdx.x, up = (1 << a.page_shift) - 1, sh = a.page_shift;
   const int64_t room = (int64_t)a.columns << sh;
   const int count0 = min(max(*a.pool_count, 0), a.pool_size);
-  int64_t tokens = 0;  // sums over the requests before this chunk; any lengths' sum fits 64 bits
+  const bool once = a.N <= kThreads;  // one round: its values stay in registers and LDS
+  if (tid == 0) taken = 0;
+  int m = 0, c = 0;
+  int64_t first_row = 0, tokens = 0;  // rows before the thread's request, and before the round's; 64 bits hold any
+  const auto request = [&](int r) {
+    m = r < a.N ? a.fresh[r] : 0;
+    c = r < a.N ? max(a.cached[r], 0) : 0;
+  };
   int gone = 0;
   for (int r0 = 0; r0 < a.N; r0 += kThreads) {
-    const int r = r0 + tid;
-    const int m = r < a.N ? a.fresh[r] : 0, c = r < a.N ? max(a.cached[r], 0) : 0;
-    int64_t every;
-    const int64_t s = tokens + scan<int64_t>(max(m, 0), part, every);
-    if (r < a.N) a.starts[r] = (int)min(s, (int64_t)INT32_MAX);
-    tokens += every;
-    int all;
+    const int r = r0 + tid, n = min(kThreads, a.N - r0);
+    request(r);
     const int freed = m < 0 ? (int)min(((int64_t)c + up) >> sh, (int64_t)a.columns) : 0;
-    const int f = scan(freed, part, all);
-    for (int j = 0; j < freed; ++j) {
-      const int at = count0 + gone + f + j;
-      if (at < a.pool_size) a.pool[at] = a.tables[r * a.table_stride + j];
+    int64_t x = max(m, 0), every;
+    int f = freed, all;
+    scan(x, f, every, all, part);
+    first_row = tokens + x;
+    const int clamped = (int)min(first_row, (int64_t)INT32_MAX);
+    prefix[tid] = f;
+    start[tid] = clamped;
+    if (r < a.N) a.starts[r] = clamped;
+    tokens += every;
+    if (all) {
+      __syncthreads();
+      for (int i = tid; i < all; i += kThreads) {
+        const int o = owner(prefix, n, i), at = count0 + gone + i;
+        if (at < a.pool_size) a.pool[at] = a.tables[(r0 + o) * a.table_stride + i - prefix[o]];
+      }
+      gone += all;
     }
-    gone += all;
   }
   if (tid == 0) a.starts[a.N] = (int)min(tokens, (int64_t)INT32_MAX);
   const int count = min(count0 + gone, a.pool_size);
   __syncthreads();  // the pool's new top and the starts are there for every thread
-  int need = 0, taken = 0;
+  int need = 0;
   for (int r0 = 0; r0 < a.N; r0 += kThreads) {
-    const int r = r0 + tid;
-    const int m = r < a.N ? a.fresh[r] : 0, c = r < a.N ? max(a.cached[r], 0) : 0;
-    const bool fits = m > 0 && (int64_t)c + m <= room && (int64_t)a.starts[min(r, a.N)] + m <= a.T;
-    const int first = (int)(((int64_t)c + up) >> sh);
-    const int mine = fits ? (int)(((int64_t)c + m + up) >> sh) - first : 0;
-    int all;
-    const int o = need + scan(mine, part, all);
-    need += all;
-    const bool in = m <= 0 || (fits && (mine == 0 || o + mine <= count));
+    const int r = r0 + tid, n = min(kThreads, a.N - r0);
+    if (!once) {
+      request(r);
+      first_row = r < a.N ? a.starts[r] : 0;
+    }
+    const bool fits = m > 0 && (int64_t)c + m <= room && first_row + m <= a.T;
+    const int held = (int)(((int64_t)c + up) >> sh);
+    const int mine = fits ? (int)(((int64_t)c + m + up) >> sh) - held : 0;
+    int64_t x = 0, none;
+    int o = mine, all;
+    scan(x, o, none, all, part);
+    const bool in = m <= 0 || (fits && (mine == 0 || need + o + mine <= count));
+    // those before the first that finds no pages take all they need
+    if (in && mine > 0) atomicMax(&taken, need + o + mine);
+    prefix[tid] = o;
+    admitted[tid] = in;
+    base[tid] = held;
     if (r < a.N) {
-      if (in)
-        for (int j = 0; j < mine; ++j) a.tables[r * a.table_stride + first + j] = a.pool[count - 1 - o - j];
       a.lengths[r] = m < 0 ? 0 : c + (in ? m : 0);
       a.admitted[r] = in;
     }
-    scan(in ? mine : 0, part, all);
-    taken += all;
+    if (all) {
+      __syncthreads();
+      for (int i = tid; i < all; i += kThreads) {
+        const int w = owner(prefix, n, i);
+        if (admitted[w]) a.tables[(r0 + w) * a.table_stride + base[w] + i - prefix[w]] = a.pool[count - 1 - need - i];
+      }
+      need += all;
+    }
   }
+  __syncthreads();  // the tables and what was taken are there for every thread
   if (tid == 0) *a.count = count - taken;
   if (a.T > kOneLaunch) return;
+  base[tid] = c;
   __syncthreads();
-  for (int t = tid; t < a.T; t += kThreads) token(a, t, (int)min(tokens, (int64_t)a.T));
+  const int total = (int)min(tokens, (int64_t)a.T);
+  for (int t = tid; t < a.T; t += kThreads) {
+    if (t >= total) {
+      row(a, t, 0, 0, false);
+    } else if (once) {
+      const int r = owner(start, a.N, t);
+      row(a, t, r, base[r] + t - start[r], admitted[r]);
+    } else {
+      const int r = owner(a.starts, a.N, t);
+      const bool in = a.admitted[r] != 0;
+      row(a, t, r, a.lengths[r] - (in ? a.fresh[r] : 0) + t - a.starts[r], in);
+    }
+  }
 }
 
 __global__ __launch_bounds__(256) void tokens_kernel(PagesArgs a) {
   const int t = blockIdx.x * 256 + threadIdx.x;
-  if (t < a.T) token(a, t, min(a.starts[a.N], a.T));
+  if (t >= a.T) return;
+  if (t >= min(a.starts[a.N], a.T)) {
+    row(a, t, 0, 0, false);
+    return;
+  }
+  const int r = owner(a.starts, a.N, t);
+  const bool in = a.admitted[r] != 0;
+  row(a, t, r, a.lengths[r] - (in ? a.fresh[r] : 0) + t - a.starts[r], in);
 }
 
 }  // namespace
