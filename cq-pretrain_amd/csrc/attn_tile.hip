@@ -1,8 +1,8 @@
 // Attention of many query rows a request over the 4-bit pages: a prompt's rows share the values of a page.
 //
 // The mathematics is that of attn_attend.hip.  Here a workgroup takes 128 rows of one request and key head,
-// 32 a wave, and kTokens positions a step.  Its threads convert the step's codes once into K and V tiles of E in
-// shared memory, two deep, so that the next step's codes are on their way and being converted while the
+// 32 a wave, and kTokens positions a step.  Its threads convert the step's codes once into K and V tiles of E
+// in shared memory, two deep, so that the next step's codes are on their way and being converted while the
 // waves multiply.  S^T = K Q^T and O^T = V^T P^T run on 32 x 32 x 16 MFMAs with a row a column, so a lane
 // (and its partner 32 lanes on) owns a row: limits, maximum and sum stay in its registers, and S^T's layout
 // is already an operand of O^T.
@@ -16,7 +16,8 @@
 namespace cqgdn {
 namespace {
 
-constexpr int kRows = 128;    // of a workgroup, 32 a wave
+constexpr int kRows = 128;  // of a workgroup, 32 a wave
+constexpr int kEarly = 4;   // MFMA operands read from LDS ahead of their use: a read's latency is that of four MFMAs
 
 typedef float f32x16 __attribute__((ext_vector_type(16)));
 
@@ -27,9 +28,11 @@ __device__ __forceinline__ f32x16 mfma32(f16x8 a, f16x8 b, f32x16 c) {
   return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0);
 }
 
-// Positions a step: 256 threads convert 32 values of K and of V each.
+// Positions a step, of which 256 threads convert kPiece values of K and of V each.
 template <int D>
-constexpr int kTokens = 8192 / D;
+constexpr int kTokens = D == 256 ? 32 : 64;
+template <int D>
+constexpr int kPiece = kTokens<D> * D / 256;
 
 // K rows are 16 bytes longer than their values: read 16 bytes a lane, 16 rows at a time, they meet all 64 banks
 // once.  V is read by quads of rows and 64 bytes of each; its 16-byte column c lies at v_column(row, c), the
@@ -39,40 +42,48 @@ template <int D>
 constexpr int kStrideK = D + 8;
 template <int D>
 __device__ __forceinline__ int v_column(int row, int c) {
-  if constexpr (D == 64) return c ^ (4 * ((row >> 1) & 1)) ^ ((row >> 1) & 3);
+  if constexpr (D == 64) return c ^ (4 * ((row >> 1) & 1)) ^ ((row >> 1) & 1);
   return c ^ (5 * (row & 3)) ^ (D == 256 ? (c >> 4) << 1 : 0);
 }
 
-// what a thread fetches of a step: 32 values of K and of V
-struct Piece {
-  u32x4 k, v;
-  uint32_t ks, vs;
-  bool ok;
-};
-
+// a thread's codes of a step's K or V and their scale byte
 template <int D>
-__device__ __forceinline__ Piece fetch(const AttendArgs& a, int page, int pos, int h, int piece) {
-  Piece x;
-  const int size = 1 << a.page_shift, at = pos & (size - 1);
-  x.ok = page >= 0 && page < (int)a.page_count;  // an entry that names no page: its positions are hidden
-  const uint8_t* base = a.data + ((int64_t)(x.ok ? page : 0) * a.kv_heads + h) * kv4_page_bytes(size, D);
-  const uint8_t* code = base + at * (D / 2) + 16 * piece;
-  const uint8_t* scale = base + size * D + at * (D / 32) + piece;
-  x.k = *reinterpret_cast<const u32x4*>(code);
-  x.v = *reinterpret_cast<const u32x4*>(code + size * (D / 2));
-  x.ks = scale[0];
-  x.vs = scale[size * (D / 32)];
+struct Piece {
+  uint32_t w[kPiece<D> / 8];
+  uint32_t s;
+};
+// from a page's buffer: a lane's offsets and the scalar ones of the step's first position
+template <int D>
+__device__ __forceinline__ Piece<D> fetch(__amdgpu_buffer_rsrc_t page, int code, int code0, int scale, int scale0) {
+  Piece<D> x;
+  if constexpr (D == 64) {
+    const auto w = __builtin_amdgcn_raw_buffer_load_b64(page, code, code0, 0);
+    x.w[0] = w[0];
+    x.w[1] = w[1];
+  } else {
+    const u32x4 w = buf_ld16<u32x4>(page, code, code0);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) x.w[e] = w[e];
+  }
+  x.s = __builtin_amdgcn_raw_buffer_load_b8(page, scale, scale0, 0);
   return x;
 }
 
+// The sum of a step's weights in a lane beyond which the running maximum moves: with bf16 far below where
+// anything overflows, with fp16 where a weight may pass the largest number
+template <class E>
+constexpr float kLimit = std::is_same<E, f16>::value ? 60000.f : 16777216.f;
+
 template <class E, int D>
-__global__ __launch_bounds__(256, 2) void tile_kernel(AttendArgs a, int tiles, int splits) {
+__global__ __launch_bounds__(256, D == 256 ? 1 : 2) void tile_kernel(AttendArgs a, int tiles, int splits) {
   typedef typename Vec<E>::x8 x8;
-  constexpr int TOK = kTokens<D>, PV = D / 32, NS = TOK / 32, KQ = D / 16, MT = D / 32;
+  constexpr int TOK = kTokens<D>, VP = kPiece<D>, PV = D / VP, NS = TOK / 32, KQ = D / 16, MT = D / 32;
+  constexpr int F = NS * KQ, FV = 2 * NS * MT;  // operands of a step: K's and V's
+  constexpr int PARTS = VP / 8, GROUPS = TOK / 16, WAVE_POS = 64 / PV;
   __shared__ __align__(16) E kt[2][TOK * kStrideK<D>];
   __shared__ __align__(16) E vt[2][TOK * D];
-  // of the positions each wave fetched: a bit for every 16 that are hidden, the sign for a NaN among the values
-  __shared__ __align__(16) int marks[2][4];
+  // of the positions each wave converted: whether there is a NaN among the values, and the pieces that have one
+  __shared__ __align__(16) int poison[2][4];
   __shared__ uint64_t bad[2][4];
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int n32 = lane & 31, kg = lane >> 5;
@@ -86,29 +97,31 @@ __global__ __launch_bounds__(256, 2) void tile_kernel(AttendArgs a, int tiles, i
   const int s = b % splits;
   b /= splits;
   const int h = b % a.kv_heads, r = b / a.kv_heads;
-  const int group = a.heads / a.kv_heads, T = (int)a.T;
+  const int group = a.group.d, T = (int)a.T;
   const int from = r == 0 ? 0 : min(max(a.starts[r], 0), T);
   const int to = r == a.N ? T : min(max(a.starts[r + 1], from), T);  // request N: the padding behind the last
-  const int rows = (to - from) * group;
+  const int rows = (to - from) * group, size = 1 << a.page_shift;
   const int room = (int)min((int64_t)a.columns << a.page_shift, (int64_t)INT32_MAX - 1024);
   const int token = tid / PV, piece = tid % PV;  // the thread's part of a step
+  const uint8_t* const head_base = a.data + (int64_t)h * kv4_page_bytes(size, D);
+  const uint64_t stride = (uint64_t)a.kv_heads * kv4_page_bytes(size, D);
   // the exponent's factor, never 0: a masked score stays -infinity; its sign goes with Q
   const float c = fmaxf(fabsf(a.scale) * 1.44269504088896341f, 1.17549435e-38f);
   constexpr float bias = kAttendBias<E>;
   typedef __attribute__((address_space(3))) i16x4 lds_i16x4;
   // the lane's K row of a step, and its piece of V: tokens 4 kg + {0..3, 8..11} at dimension 32 k + n32 come
   // transposed out of quads of lanes
-  const E* const kl = kt[0] + n32 * kStrideK<D> + 8 * kg;
-  const E* vl[MT];
+  const int kl = n32 * kStrideK<D> + 8 * kg;
+  int vl[MT];
 #pragma unroll
   for (int k = 0; k < MT; ++k) {
     const int j = lane & 15, row = 4 * kg + (j >> 2), col = 4 * k + 2 * (lane >> 4 & 1) + (j >> 1 & 1);
-    vl[k] = vt[0] + row * D + 8 * v_column<D>(row, col) + 4 * (j & 1);
+    vl[k] = row * D + 8 * v_column<D>(row, col) + 4 * (j & 1);
   }
 
   for (int tile = tile0; tile * kRows < rows; tile += tiles) {
     const auto limits = [&](int rho, int& lo, int& hi) {
-      hi = rho < rows && r < a.N ? min(max(a.visible[from + rho / group], 0), room) : 0;
+      hi = rho < rows && r < a.N ? min(max(a.visible[from + a.group.of(rho)], 0), room) : 0;
       lo = a.window > 0 ? max(0, hi - a.window) : 0;
     };
     // what the workgroup's rows see together
@@ -128,24 +141,19 @@ __global__ __launch_bounds__(256, 2) void tile_kernel(AttendArgs a, int tiles, i
       last = __builtin_amdgcn_readfirstlane(last);
     }
     const int rho = tile * kRows + 32 * wave + n32;
-    const bool real = rho < rows;
+    const bool real = rho < rows, active = tile * kRows + 32 * wave < rows;
     int lo, hi;
     limits(rho, lo, hi);
-    // the wave's: the range that any of its rows sees, and the one all of them see, where nothing is masked
-    int wfirst = hi > 0 ? lo : INT32_MAX, wlast = hi, low = lo, high = real ? hi : INT32_MAX;
+    // the range that all of the wave's rows see, where nothing is masked
+    int low = lo, high = real ? hi : INT32_MAX;
 #pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-      wfirst = min(wfirst, __shfl_xor(wfirst, o, 64));
-      wlast = max(wlast, __shfl_xor(wlast, o, 64));
-      low = max(low, __shfl_xor(low, o, 64));
-      high = min(high, __shfl_xor(high, o, 64));
+    for (int i = 1; i < 32; i <<= 1) {
+      low = max(low, __shfl_xor(low, i, 64));
+      high = min(high, __shfl_xor(high, i, 64));
     }
-    wfirst = __builtin_amdgcn_readfirstlane(wfirst);
-    wlast = __builtin_amdgcn_readfirstlane(wlast);
     low = __builtin_amdgcn_readfirstlane(low);
     high = __builtin_amdgcn_readfirstlane(high);
-
-    const int t = from + (real ? rho / group : 0), head = h * group + (real ? rho % group : 0);
+    const int row_t = real ? a.group.of(rho) : 0, t = from + row_t, head = h * group + (real ? rho - row_t * group : 0);
     x8 qf[KQ];  // lane (n32, kg): row n32, dimensions 16 i + 8 kg ..
     {
       const E* q = static_cast<const E*>(a.q) + t * a.q_token + head * a.q_head + 8 * kg;
@@ -159,132 +167,192 @@ __global__ __launch_bounds__(256, 2) void tile_kernel(AttendArgs a, int tiles, i
     f32x16 o[MT];
 #pragma unroll
     for (int i = 0; i < MT; ++i) o[i] = f32x16{};
-    float m = -INFINITY, l = 0.f;
+    float m = hi > 0 ? -INFINITY : 0.f, l = 0.f;
+    uint32_t nan = 0;  // blocks of 32 dimensions in which the row sees a NaN value
 
     const int begin = last > 0 ? first & ~(TOK - 1) : 0;
     const int steps = (last - begin + TOK - 1) / TOK, per = (steps + splits - 1) / splits;
-    const int stop = min(steps, (s + 1) * per);
+    const int n = min(steps, (s + 1) * per) - s * per, pos0 = begin + s * per * TOK;
 
-    const auto store = [&](const Piece& x, int buf, int pos) {
-      const int at = pos + token;
-      // a position that no row sees is zero, and so is a NaN value: it goes to the rows that see it below
-      const bool any = x.ok && at >= first && at < last, nan = any && x.vs == 255;
-      const uint64_t hidden = __ballot(!x.ok), nans = __ballot(nan);
-      if (lane == 0) {
-        bad[buf][wave] = nans;
-        marks[buf][wave] = (int)(hidden & 1) | (PV == 2 ? (int)(hidden >> 32 & 1) << 1 : 0) | (nans ? INT32_MIN : 0);
-      }
-      const float ks = kv4_scale(x.ks), vs = any && !nan ? kv4_scale(x.vs) : 0.f;
-      const u32x4 v = any && !nan ? x.v : u32x4{0, 0, 0, 0};
-      E* const kr = kt[buf] + token * kStrideK<D> + 32 * piece;
-      E* const vr = vt[buf] + token * D;
+    // the block table's entries for the 16 positions each of step j, one a lane
+    const auto entries = [&](int j) {
+      const int column = (pos0 + j * TOK + 16 * (lane & (GROUPS - 1))) >> a.page_shift;
+      return j < n && column < a.columns ? a.tables[r * a.table_stride + column] : -1;
+    };
+    Piece<D> kn, vn;
+    const int code = lane / PV * (D / 2) + VP / 2 * piece, scale = lane / PV * (D / 32) + piece * VP / 32;
+    // step j's codes of the wave's positions, which one page holds; one that is hidden reads as zeros.  Returns
+    // which of the step's 16 positions are shown.
+    const auto fetch_step = [&](int table, int j) {
+      const uint32_t page = __builtin_amdgcn_readlane(table, wave * WAVE_POS / 16);
+      const bool ok = page < a.page_count;
+      const __amdgpu_buffer_rsrc_t rs = buf_rsrc(head_base + (ok ? page * stride : 0), ok ? kv4_page_bytes(size, D) : 0);
+      const int at = (pos0 + j * TOK + wave * WAVE_POS) & (size - 1);
+      kn = fetch<D>(rs, code, at * (D / 2), scale, size * D + at * (D / 32));
+      vn = fetch<D>(rs, code, (size + at) * (D / 2), scale, size * D + (size + at) * (D / 32));
+      return (int)__ballot((uint32_t)table < a.page_count) & ((1 << GROUPS) - 1);
+    };
+    // those codes become step j's K and V tiles, PARTS parts of each.  Where the step reaches beyond what the
+    // rows see, a position that no row sees is zero, and so is a NaN value: it goes to the rows that see it by `nan`.
+    float kscale, vscale;
+    E* const kw = kt[0] + token * kStrideK<D> + VP * piece;
+    int vw[PARTS];
 #pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        st8(kr + 8 * e, kv4_values<E>(x.k[e], ks));
-        st8(vr + 8 * v_column<D>(token, 4 * piece + e), kv4_values<E>(v[e], vs));
+    for (int e = 0; e < PARTS; ++e) vw[e] = token * D + 8 * v_column<D>(token, PARTS * piece + e);
+    const auto begin_convert = [&](int j) {
+      uint64_t nans = __ballot(vn.s == 255);
+      const int pos = pos0 + j * TOK;
+      if (nans != 0 || pos < first || pos + TOK > last) {
+        const bool any = pos + token >= first && pos + token < last;
+        nans = __ballot(any && vn.s == 255);
+        if (!any || vn.s == 255) {
+          vn.s = 0;
+#pragma unroll
+          for (int e = 0; e < PARTS; ++e) vn.w[e] = 0;
+        }
+        if (lane == 0) bad[j & 1][wave] = nans;
       }
+      if (lane == 0) poison[j & 1][wave] = nans != 0;
+      kscale = kv4_scale(kn.s);
+      vscale = kv4_scale(vn.s);
+    };
+    const auto convert = [&](int j, int e) {
+      if (e < PARTS)
+        st8(kw + (j & 1) * (TOK * kStrideK<D>) + 8 * e, kv4_values<E>(kn.w[e], kscale));
+      else
+        st8(vt[j & 1] + vw[e - PARTS], kv4_values<E>(vn.w[e - PARTS], vscale));
+    };
+    f32x16 sc[NS];
+    // the weights, two a part, in the order of the scores
+    uint32_t pw[8 * NS];
+    float base, sum;
+    const auto begin_weights = [&]() {
+      base = bias - (m == -INFINITY ? 0.f : m);
+      sum = 0.f;
+    };
+    const auto weights = [&](int i) {
+      typedef float f32x2 __attribute__((ext_vector_type(2)));
+      typedef E x2 __attribute__((ext_vector_type(2)));
+      f32x2 p;
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        p[e] = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[i / 8][2 * (i % 8) + e], c, base));
+        sum += p[e];
+      }
+      pw[i] = __builtin_bit_cast(uint32_t, __builtin_convertvector(p, x2));
     };
 
-    int i = s * per;
-    if (i < stop) {
-      Piece next = fetch<D>(a, page_of(a, r, begin + i * TOK + token), begin + i * TOK + token, h, piece);
-      int pg = page_of(a, r, begin + (i + 1) * TOK + token);
-      store(next, i & 1, begin + i * TOK);
-      if (i + 1 < stop) next = fetch<D>(a, pg, begin + (i + 1) * TOK + token, h, piece);
-      pg = page_of(a, r, begin + (i + 2) * TOK + token);
+    if (n > 0) {
+      int shown = fetch_step(entries(0), 0), shown1 = 0;
+      begin_convert(0);
+#pragma unroll
+      for (int e = 0; e < 2 * PARTS; ++e) convert(0, e);
+      shown1 = fetch_step(entries(1), 1);
+      int table = entries(2);
       __syncthreads();
-      for (; i < stop; ++i) {
-        const int pos = begin + i * TOK, buf = i & 1;
-        if (i + 1 < stop) {
-          store(next, buf ^ 1, pos + TOK);
-          if (i + 2 < stop) next = fetch<D>(a, pg, pos + 2 * TOK + token, h, piece);
-          pg = page_of(a, r, pos + 3 * TOK + token);
-        }
-        if (pos < wlast && pos + TOK > wfirst) {
-          int mark[4];
+#pragma unroll 1
+      for (int j = 0; j < n; ++j) {
+        if (active) {
+          const E* const kp = kt[j & 1] + kl;
+          const E* const vp = vt[j & 1];
+          x8 kf[F], vf[FV];
+          const auto value = [&](int i) {  // positions 16 (i / MT), dimensions 32 (i % MT)
+            const E* p = vp + vl[i % MT] + i / MT * 16 * D;
+            const i16x4 v0 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_i16x4*)p);
+            const i16x4 v1 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_i16x4*)(p + 8 * D));
+            vf[i] = __builtin_bit_cast(x8, __builtin_shufflevector(v0, v1, 0, 1, 2, 3, 4, 5, 6, 7));
+          };
 #pragma unroll
-          for (int w = 0; w < 4; ++w) mark[w] = __builtin_amdgcn_readfirstlane(marks[buf][w]);
-          const bool clean = (mark[0] | mark[1] | mark[2] | mark[3]) == 0;
-          f32x16 sc[NS];
+          for (int i = 0; i < 2 * kEarly; ++i) kf[i] = ld8(kp + i / KQ * 32 * kStrideK<D> + i % KQ * 16);
+          const int4 poisoned = *reinterpret_cast<const int4*>(poison[j & 1]);
+          __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-          for (int u = 0; u < NS; ++u) {
-            sc[u] = f32x16{};
-#pragma unroll
-            for (int k = 0; k < KQ; ++k)
-              sc[u] = mfma32(ld8(kl + buf * (TOK * kStrideK<D>) + 32 * u * kStrideK<D> + 16 * k), qf[k], sc[u]);
+          for (int i = 0; i < F; ++i) {
+            if (i % KQ == 0) sc[i / KQ] = f32x16{};
+            sc[i / KQ] = mfma32(kf[i], qf[i % KQ], sc[i / KQ]);
+            const int k = i + 2 * kEarly;
+            if (k < F) kf[k] = ld8(kp + k / KQ * 32 * kStrideK<D> + k % KQ * 16);
+            __builtin_amdgcn_sched_barrier(0);
           }
-          if (!(clean && pos >= low && pos + TOK <= high)) {
-            const int at0 = pos + 4 * kg;
+          // hidden positions leave the scores
+          const int pos = pos0 + j * TOK;
+          if (shown != (1 << GROUPS) - 1 || pos < low || pos + TOK > high) {
+            const int lo0 = lo - pos - 4 * kg, hi0 = hi - pos - 4 * kg;
 #pragma unroll
             for (int u = 0; u < NS; ++u)
 #pragma unroll
               for (int e = 0; e < 16; ++e) {
-                const int at = 32 * u + 8 * (e >> 2) + (e & 3), g = 2 * u + (e >> 3);
-                const int word = D == 256 ? 2 * g : D == 128 ? g : g >> 1;
-                const bool shown = !(mark[word] >> (D == 64 ? g & 1 : 0) & 1);
-                if (at < lo - at0 || at >= hi - at0 || !shown) sc[u][e] = -INFINITY;
+                const int at = 32 * u + 8 * (e >> 2) + (e & 3);
+                if ((int)(at < lo0) | (int)(at >= hi0) | (int)!(shown >> (2 * u + (e >> 3)) & 1)) sc[u][e] = -INFINITY;
               }
           }
-          float top = sc[0][0];
 #pragma unroll
-          for (int u = 0; u < NS; ++u)
+          for (int i = 0; i < kEarly; ++i) value(i);
+          begin_weights();
 #pragma unroll
-            for (int e = 0; e < 16; ++e) top = fmaxf(top, sc[u][e]);
-          top *= c;
-          if (__any(top > m + kLazy)) {  // the maximum moves rarely, and for each row by itself
-            top = fmaxf(top, __shfl_xor(top, 32, 64));
-            if (top > m + kLazy) {
+          for (int i = 0; i < 8 * NS; ++i) weights(i);
+          // where the weights have grown too large, or are a row's first, its maximum moves and they are made again
+          bool large = sum > kLimit<E> || m == -INFINITY;
+          if (__any(large)) {
+            large = __shfl_xor((int)large, 32, 64) || large;  // the two lanes of a row
+            float top = sc[0][0];
+#pragma unroll
+            for (int u = 0; u < NS; ++u)
+#pragma unroll
+              for (int e = 0; e < 16; ++e) top = fmaxf(top, sc[u][e]);
+            top = fmaxf(top, __shfl_xor(top, 32, 64)) * c;
+            if (large && top > m) {
               const float f = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m - top);
               m = top;
               l *= f;
 #pragma unroll
               for (int k = 0; k < MT; ++k) o[k] *= f;
             }
+            begin_weights();
+#pragma unroll
+            for (int i = 0; i < 8 * NS; ++i) weights(i);
           }
-          const float base = (m == -INFINITY ? 0.f : m) - bias;
-          x8 pf[2 * NS];
+          l += sum;
+          begin_convert(j + 1);  // beyond the last step: of codes that nothing reads
 #pragma unroll
-          for (int u = 0; u < NS; ++u)
+          for (int i = 0; i < FV; ++i) {
+            const int w = i / MT * 4;
+            o[i % MT] = mfma32(vf[i], __builtin_bit_cast(x8, u32x4{pw[w], pw[w + 1], pw[w + 2], pw[w + 3]}), o[i % MT]);
+            if (i + kEarly < FV) value(i + kEarly);
 #pragma unroll
-            for (int e = 0; e < 2; ++e) {
-              f32x8 p;
-#pragma unroll
-              for (int j = 0; j < 8; ++j) {
-                p[j] = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[u][8 * e + j], c, -base));
-                l += p[j];
-              }
-              pf[2 * u + e] = to8<E>(p);
-            }
-          if (!clean) {  // NaN values: to the rows that see them, in their 32 dimensions
+            for (int e = i * 2 * PARTS / FV; e < (i + 1) * 2 * PARTS / FV; ++e) convert(j + 1, e);
+            __builtin_amdgcn_sched_barrier(0);
+          }
+          if (__builtin_amdgcn_readfirstlane(poisoned.x | poisoned.y | poisoned.z | poisoned.w)) {
 #pragma unroll 1
             for (int w = 0; w < 4; ++w)
 #pragma unroll 1
-              for (uint64_t x = bad[buf][w]; x; x &= x - 1) {
-                const int n = 64 * w + __builtin_ctzll(x), at = pos + n / PV;
-                const float add = at >= lo && at < hi ? __builtin_nanf("") : 0.f;
-#pragma unroll
-                for (int k = 0; k < MT; ++k)
-                  if (k == n % PV) o[k] += add;
+              for (uint64_t y = poison[j & 1][w] ? bad[j & 1][w] : 0; y; y &= y - 1) {
+                const int i = 64 * w + __builtin_ctzll(y), at = pos0 + j * TOK + i / PV;
+                nan |= at >= lo && at < hi ? 1u << (i % PV * VP / 32) : 0u;
               }
           }
+        } else {
+          begin_convert(j + 1);
 #pragma unroll
-          for (int k = 0; k < MT; ++k)
-#pragma unroll
-            for (int u = 0; u < 2 * NS; ++u) {
-              const E* p = vl[k] + buf * (TOK * D) + 16 * u * D;
-              const i16x4 v0 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_i16x4*)p);
-              const i16x4 v1 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_i16x4*)(p + 8 * D));
-              o[k] = mfma32(__builtin_bit_cast(x8, __builtin_shufflevector(v0, v1, 0, 1, 2, 3, 4, 5, 6, 7)), pf[u], o[k]);
-            }
+          for (int e = 0; e < 2 * PARTS; ++e) convert(j + 1, e);
         }
+        shown = shown1;
+        shown1 = fetch_step(table, j + 2);
+        table = entries(j + 3);
         __syncthreads();
       }
     }
     l += __shfl_xor(l, 32, 64);
+    if (__any(nan != 0)) {
+#pragma unroll
+      for (int k = 0; k < MT; ++k)
+        if (nan >> k & 1) o[k] = f32x16{} + __builtin_nanf("");
+    }
     if (real) {
       const int64_t at = (int64_t)t * a.heads + head;
       const float inv = l == 0.f ? 0.f : 1.f / l;
-      if (splits == 1 || m != -INFINITY || l != 0.f) {  // the join reads no part that saw nothing
+      if (splits == 1 || l != 0.f) {  // the join reads no part that saw nothing
 #pragma unroll
         for (int k = 0; k < MT; ++k)
 #pragma unroll
@@ -300,7 +368,7 @@ __global__ __launch_bounds__(256, 2) void tile_kernel(AttendArgs a, int tiles, i
       if (kg == 0) {
         if (splits > 1) {
           float* ml = a.ws + a.T * a.heads * splits * D + (at * splits + s) * 2;
-          ml[0] = m;
+          ml[0] = l == 0.f ? -INFINITY : m;
           ml[1] = l;
         } else if (a.lse) {
           a.lse[at] = (m - bias + log2f(l)) * 0.693147180559945309f;
