@@ -24,8 +24,12 @@ constexpr int kFewRows = 32;      // of a request and key head: more take the ke
 // The pages of a step's four 16 positions, the same for all lanes.  An entry that names no page reads as zeros
 // (its buffer has no bytes), and its positions are hidden.
 struct Pages {
-  __amdgpu_buffer_rsrc_t page[4];
+  const uint8_t* base[4];
   int shown;  // a bit each
+  template <int D>
+  __device__ __forceinline__ __amdgpu_buffer_rsrc_t page(int g, int size) const {
+    return buf_rsrc(base[g], shown >> g & 1 ? kv4_page_bytes(size, D) : 0);
+  }
 };
 
 // The codes of a step's keys and their scale bytes.  Lane (r16, q4) holds key r16 of each 16: 16 bytes from
@@ -44,18 +48,19 @@ __device__ __forceinline__ void load_keys(Keys<D>& c, const Pages& p, int pos, i
 #pragma unroll
   for (int g = 0; g < 4; ++g) {
     const int at = (pos + 16 * g) & (size - 1), codes = at * (D / 2), scales = size * D + at * (D / 32);
+    const __amdgpu_buffer_rsrc_t rs = p.template page<D>(g, size);
 #pragma unroll
     for (int x = 0; x < Keys<D>::XK; ++x) {
       if constexpr (D >= 128) {
-        const u32x4 w = buf_ld16<u32x4>(p.page[g], r16 * (D / 2) + 16 * q4 + 64 * x, codes);
+        const u32x4 w = buf_ld16<u32x4>(rs, r16 * (D / 2) + 16 * q4 + 64 * x, codes);
 #pragma unroll
         for (int i = 0; i < 4; ++i) c.w[g][x][i] = w[i];
-        c.s[g][x] = __builtin_amdgcn_raw_buffer_load_b8(p.page[g], r16 * (D / 32) + q4 + 4 * x, scales, 0);
+        c.s[g][x] = __builtin_amdgcn_raw_buffer_load_b8(rs, r16 * (D / 32) + q4 + 4 * x, scales, 0);
       } else {
-        const auto w = __builtin_amdgcn_raw_buffer_load_b64(p.page[g], r16 * (D / 2) + 8 * q4, codes, 0);
+        const auto w = __builtin_amdgcn_raw_buffer_load_b64(rs, r16 * (D / 2) + 8 * q4, codes, 0);
         c.w[g][x][0] = w[0];
         c.w[g][x][1] = w[1];
-        c.s[g][x] = __builtin_amdgcn_raw_buffer_load_b8(p.page[g], r16 * (D / 32) + (q4 >> 1), scales, 0);
+        c.s[g][x] = __builtin_amdgcn_raw_buffer_load_b8(rs, r16 * (D / 32) + (q4 >> 1), scales, 0);
       }
     }
   }
@@ -81,17 +86,17 @@ __device__ __forceinline__ void load_values(Values<D>& c, const Pages& p, int po
 #pragma unroll
       for (int x = 0; x < D / V::DC; ++x) {
         if constexpr (D >= 128) {
-          c.w[x][half][j] = buf_ld16<u32x4>(p.page[g], lane / 4 * (D / 2) + lane % 4 * 16 + 64 * x, codes);
-          c.s[x][half][j] = __builtin_amdgcn_raw_buffer_load_b8(p.page[g], lane / 4 * (D / 32) + lane % 4 + 4 * x, scales, 0);
+          c.w[x][half][j] = buf_ld16<u32x4>(p.template page<D>(g, size), lane / 4 * (D / 2) + lane % 4 * 16 + 64 * x, codes);
+          c.s[x][half][j] = __builtin_amdgcn_raw_buffer_load_b8(p.template page<D>(g, size), lane / 4 * (D / 32) + lane % 4 + 4 * x, scales, 0);
         } else {
           // 32 positions a load, which two pages may hold: a lane's offset lies beyond the one that is not its own
           const int at1 = (pos + 16 * g + 16) & (size - 1), none = 1 << 30;
           const int lo = lane < 32 ? lane * 16 : none, hi = lane < 32 ? none : (lane - 32) * 16;
           const int slo = lane < 32 ? lane : none, shi = lane < 32 ? none : lane - 32;
-          c.w[x][half][j] = buf_ld16<u32x4>(p.page[g], lo, codes) |
-                            buf_ld16<u32x4>(p.page[g + 1], hi, size * (D / 2) + at1 * (D / 2));
-          c.s[x][half][j] = __builtin_amdgcn_raw_buffer_load_b8(p.page[g], slo, scales, 0) |
-                            __builtin_amdgcn_raw_buffer_load_b8(p.page[g + 1], shi,
+          c.w[x][half][j] = buf_ld16<u32x4>(p.template page<D>(g, size), lo, codes) |
+                            buf_ld16<u32x4>(p.template page<D>(g + 1, size), hi, size * (D / 2) + at1 * (D / 2));
+          c.s[x][half][j] = __builtin_amdgcn_raw_buffer_load_b8(p.template page<D>(g, size), slo, scales, 0) |
+                            __builtin_amdgcn_raw_buffer_load_b8(p.template page<D>(g + 1, size), shi,
                                                                 size * D + size * (D / 32) + at1 * (D / 32), 0);
         }
       }
@@ -192,14 +197,14 @@ __global__ __launch_bounds__(64 * kWaves, D == 256 ? 2 : 3) void attend_kernel(A
       const int table = column0 + lane < a.columns ? a.tables[r * a.table_stride + column0 + lane] : -1;
       const int64_t reach = (int64_t)(column0 + 64) << a.page_shift;  // the first position beyond them
       const int end = (int)min((int64_t)stop, (reach - begin) / kStep);
-      const auto find = [&](int at) {
+      const auto find = [&](int at, bool any) {
         Pages x;
         x.shown = 0;
 #pragma unroll
         for (int g = 0; g < 4; ++g) {
-          const uint32_t page = __builtin_amdgcn_readlane(table, ((at + 16 * g) >> a.page_shift) - column0);
-          const bool ok = page < a.page_count;
-          x.page[g] = buf_rsrc(head_base + (ok ? page * stride : 0), ok ? kv4_page_bytes(size, D) : 0);
+          const uint32_t page = __builtin_amdgcn_readlane(table, (((at + 16 * g) >> a.page_shift) - column0) & 63);
+          const bool ok = any && page < a.page_count;
+          x.base[g] = head_base + (ok ? page : 0u) * stride;
           x.shown |= ok ? 1 << g : 0;
         }
         return x;
@@ -208,99 +213,133 @@ __global__ __launch_bounds__(64 * kWaves, D == 256 ? 2 : 3) void attend_kernel(A
       V values;
       int shown;
       {
-        const Pages p = find(pos);
+        const Pages p = find(pos, true);
         load_keys<D>(keys, p, pos, size, lane);
+        __builtin_amdgcn_sched_barrier(0);  // keys before values, so that a wait for them is not one for both
         load_values<D>(values, p, pos, size, lane);
+        __builtin_amdgcn_sched_barrier(0);
         shown = p.shown;
       }
+#pragma unroll 1
       for (; i < end; i += kWaves, pos += kWaves * kStep) {
-        const bool more = i + kWaves < end, full = pos >= low && pos + kStep <= high && shown == 15;
         f32x4 sc[4];
+        float ks[4][Keys<D>::XK];
 #pragma unroll
         for (int g = 0; g < 4; ++g) {
           sc[g] = zero4();
 #pragma unroll
-          for (int x = 0; x < Keys<D>::XK; ++x) {
-            const float ks = kv4_scale(keys.s[g][x]);
+          for (int x = 0; x < Keys<D>::XK; ++x) ks[g][x] = kv4_scale(keys.s[g][x]);
+        }
 #pragma unroll
-            for (int w = 0; w < Keys<D>::WK; ++w)
-              sc[g] = mfma(kv4_values<E>(keys.w[g][x][w], ks), qf[x * Keys<D>::WK + w], sc[g]);
-          }
-        }
-        Pages next;
-        if (more) {
-          next = find(pos + kWaves * kStep);
-          load_keys<D>(keys, next, pos + kWaves * kStep, size, lane);
-        }
-        if (!full) {
-          const int at0 = pos + 4 * q4;
+        for (int x = 0; x < Keys<D>::XK; ++x)
+#pragma unroll
+          for (int w = 0; w < Keys<D>::WK; ++w)
+#pragma unroll
+            for (int g = 0; g < 4; ++g)
+              sc[g] = mfma(kv4_values<E>(keys.w[g][x][w], ks[g][x]), qf[x * Keys<D>::WK + w], sc[g]);
+        // beyond the last step: of no page, which costs no memory traffic
+        const Pages next = find(pos + kWaves * kStep, i + kWaves < end);
+        load_keys<D>(keys, next, pos + kWaves * kStep, size, lane);
+        __builtin_amdgcn_sched_barrier(0);
+        // where not every row sees every position, hidden ones leave the scores, a position that none sees is
+        // zero among the values, and a NaN reaches only the rows that see it
+        if (!(pos >= low && pos + kStep <= high && shown == 15)) {
+          const int lo0 = lo - pos, hi0 = hi - pos;
 #pragma unroll
           for (int g = 0; g < 4; ++g)
 #pragma unroll
-            for (int e = 0; e < 4; ++e)
-              if (16 * g + e < lo - at0 || 16 * g + e >= hi - at0 || !(shown >> g & 1)) sc[g][e] = -INFINITY;
+            for (int e = 0; e < 4; ++e) {
+              const int at = 16 * g + e;  // and 4 q4
+              if ((int)(at < lo0 - 4 * q4) | (int)(at >= hi0 - 4 * q4) | (int)!(shown >> g & 1)) sc[g][e] = -INFINITY;
+            }
+#pragma unroll
+          for (int half = 0; half < 2; ++half)
+#pragma unroll
+            for (int x = 0; x < D / DC; ++x)
+#pragma unroll
+              for (int j = 0; j < V::J; ++j) {
+                const int tok = V::position(half, j, lane);
+                const bool any = pos + tok >= first && pos + tok < last, is_nan = values.s[x][half][j] == 255;
+                for (uint64_t bad = __ballot(any && is_nan); bad; bad &= bad - 1) {
+                  const int n = __builtin_ctzll(bad), at = V::position(half, j, n);
+                  nan |= at >= lo0 && at < hi0 ? 1u << (V::PC * x + n % V::PC) : 0u;
+                }
+                if (!any || is_nan) {
+                  values.w[x][half][j] = u32x4{0, 0, 0, 0};
+                  values.s[x][half][j] = 0;
+                }
+              }
         }
-        float top = sc[0][0];
+        x8 pf[2];
+        float sum;
+        const auto weights = [&] {
+          const float base = kAttendBias<E> - (m == -INFINITY ? 0.f : m);
+          sum = 0.f;
 #pragma unroll
-        for (int g = 0; g < 4; ++g)
+          for (int half = 0; half < 2; ++half) {
+            f32x8 p;
 #pragma unroll
-          for (int e = 0; e < 4; ++e) top = fmaxf(top, sc[g][e]);
-        top *= c;
-        if (__any(top > m + kLazy)) {  // the maximum moves rarely, and for each row by itself
+            for (int e = 0; e < 8; ++e) {
+              p[e] = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[2 * half + (e >> 2)][e & 3], c, base));
+              sum += p[e];
+            }
+            pf[half] = to8<E>(p);
+          }
+        };
+        weights();
+        // where the weights have grown too large, or are a row's first, its maximum moves and they are made again
+        bool large = sum > kAttendLimit<E> || m == -INFINITY;
+        if (__any(large)) {
+          large = __shfl_xor((int)large, 16, 64) || large;  // the four lanes of a row
+          large = __shfl_xor((int)large, 32, 64) || large;
+          float top = sc[0][0];
+#pragma unroll
+          for (int g = 0; g < 4; ++g)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) top = fmaxf(top, sc[g][e]);
           top = fmaxf(top, __shfl_xor(top, 16, 64));
-          top = fmaxf(top, __shfl_xor(top, 32, 64));
-          if (top > m + kLazy) {
+          top = fmaxf(top, __shfl_xor(top, 32, 64)) * c;
+          if (large && top > m) {
             const float f = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m - top);
             m = top;
             l *= f;
 #pragma unroll
             for (int k = 0; k < MT; ++k) o[k] *= f;
           }
+          weights();
         }
-        const float base = kAttendBias<E> - (m == -INFINITY ? 0.f : m);
-#pragma unroll
-        for (int half = 0; half < 2; ++half) {
-          f32x8 p;
-#pragma unroll
-          for (int e = 0; e < 8; ++e) {
-            p[e] = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[2 * half + (e >> 2)][e & 3], c, base));
-            l += p[e];
-          }
-          const x8 pf = to8<E>(p);
-          // values: where not every row sees every position, a position that none sees is zero, and a NaN
-          // reaches only the rows that see it
-#pragma unroll
-          for (int x = 0; x < D / DC; ++x) {
+        l += sum;
+        // values: chunk (half, x) passes through the wave's tile, whose operands are read kEarly MFMAs ahead of
+        // their own (a wave's LDS operations complete in order)
+        constexpr int OPS = DC / 16, ALL = 2 * (D / DC) * OPS, kEarly = 3;
+        x8 vf[ALL];
+        const auto ahead = [&](int i) {
+          const int chunk = i / OPS, half = chunk / (D / DC), x = chunk % (D / DC);
+          if (i % OPS == 0) {
 #pragma unroll
             for (int j = 0; j < V::J; ++j) {
               const int tok = V::position(half, j, lane), piece = lane % V::PC;
-              u32x4 w = values.w[x][half][j];
-              uint32_t sb = values.s[x][half][j];
-              if (!full) {
-                const bool any = pos + tok >= first && pos + tok < last;
-                for (uint64_t bad = __ballot(any && sb == 255); bad; bad &= bad - 1) {
-                  const int n = __builtin_ctzll(bad), at = pos + V::position(half, j, n);
-                  nan |= at >= lo && at < hi ? 1u << (V::PC * x + n % V::PC) : 0u;
-                }
-                if (!any || sb == 255) {
-                  w = u32x4{0, 0, 0, 0};
-                  sb = 0;
-                }
-              }
-              const float vs = kv4_scale(sb);
+              const float vs = kv4_scale(values.s[x][half][j]);
 #pragma unroll
               for (int e = 0; e < 4; ++e)
-                st8(vw + (tok - 32 * half) * LD + 32 * piece + 8 * e, kv4_values<E>(w[e], vs));
+                st8(vw + (tok - 32 * half) * LD + 32 * piece + 8 * e, kv4_values<E>(values.w[x][half][j][e], vs));
             }
-#pragma unroll
-            for (int k = 0; k < DC / 16; ++k)
-              o[DC / 16 * x + k] = mfma(ld8_trpv<E>(vw, LD, 0, 16 * k), pf, o[DC / 16 * x + k]);
           }
+          vf[i] = ld8_trpv<E>(vw, LD, 0, i % OPS * 16);
+        };
+#pragma unroll
+        for (int i = 0; i < kEarly; ++i) ahead(i);
+        __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+        for (int i = 0; i < ALL; ++i) {
+          if (i + kEarly < ALL) ahead(i + kEarly);
+          const int chunk = i / OPS, at = chunk % (D / DC) * OPS + i % OPS;
+          o[at] = mfma(vf[i], pf[chunk / (D / DC)], o[at]);
+          __builtin_amdgcn_sched_barrier(0);
         }
-        if (more) {
-          load_values<D>(values, next, pos + kWaves * kStep, size, lane);
-          shown = next.shown;
-        }
+        load_values<D>(values, next, pos + kWaves * kStep, size, lane);
+        shown = next.shown;
+        __builtin_amdgcn_sched_barrier(0);
       }
     }
     l += __shfl_xor(l, 16, 64);
@@ -312,18 +351,21 @@ __global__ __launch_bounds__(64 * kWaves, D == 256 ? 2 : 3) void attend_kernel(A
     }
     // join the waves: O^T rows through LDS, DC dimensions at a time, their 16-byte columns XORed with the row
     // against bank conflicts
-    if (q4 == 0) {
-      wm[wave][r16] = m;
-      wl[wave][r16] = l;
+    int late = tid;  // what follows is worked out here, not held in registers through the loop
+    asm volatile("" : "+v"(late));
+    const int lr = late & 15, lq = late >> 4 & 3;
+    if (lq == 0) {
+      wm[wave][lr] = m;
+      wl[wave][lr] = l;
     }
-    const int row = tid >> 4, n = tile * 16 + row, n_t = a.group.of(n);
+    const int row = late >> 4, n = tile * 16 + row, n_t = a.group.of(n);
     const int64_t at = (int64_t)(from + n_t) * a.heads + h * group + n - n_t * group;
     float M, L = 0.f, f[kWaves];
 #pragma unroll
     for (int x = 0; x < D / DC; ++x) {
 #pragma unroll
       for (int k = 0; k < DC / 16; ++k)
-        *reinterpret_cast<f32x4*>(reinterpret_cast<float*>(vw) + r16 * DC + 4 * ((4 * k + q4) ^ r16)) = o[DC / 16 * x + k];
+        *reinterpret_cast<f32x4*>(reinterpret_cast<float*>(vw) + lr * DC + 4 * ((4 * k + lq) ^ lr)) = o[DC / 16 * x + k];
       __syncthreads();
       if (x == 0) {
         M = wm[0][row];
@@ -338,7 +380,7 @@ __global__ __launch_bounds__(64 * kWaves, D == 256 ? 2 : 3) void attend_kernel(A
       if (n < rows) {
 #pragma unroll
         for (int k = 0; k < DC / 64; ++k) {
-          const int col = (tid & 15) + 16 * k;
+          const int col = (late & 15) + 16 * k;
           f32x4 y = zero4();
 #pragma unroll
           for (int w = 0; w < kWaves; ++w)
@@ -351,7 +393,7 @@ __global__ __launch_bounds__(64 * kWaves, D == 256 ? 2 : 3) void attend_kernel(A
       }
       __syncthreads();
     }
-    if (n < rows && (tid & 15) == 0) {
+    if (n < rows && (late & 15) == 0) {
       if (splits > 1) {
         float* ml = a.ws + a.T * a.heads * splits * D + (at * splits + s) * 2;
         ml[0] = M;

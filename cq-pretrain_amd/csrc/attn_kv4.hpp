@@ -32,12 +32,16 @@ __device__ __forceinline__ f16x8 kv4_values<f16>(uint32_t code, float scale) {
 }
 
 // ---- shared by the attention kernels ----------------------------------------------------------------
-constexpr float kLazy = 8.f;  // log2 by which scores may pass the running maximum before it moves
-// P is held 2^bias higher, in [0, 2^(kLazy + bias)], because v_exp_f32 drops results below 2^-126 and fp16
-// keeps 2^-24 at the least: weights down to 2^-134 of the maximum count with bf16 (whose results reach 2^-126),
-// down to 2^-31 with fp16, whose largest P is 2^15.  Values up to 2^110 meet no overflow.
+// The maximum of a row's scores that its weights are taken against need not be the exact one.  It is taken from
+// the first positions that the row sees, and moves only where a lane's weights of a step sum to more than
+// kAttendLimit: with fp16 a weight may pass the largest number there (65504), with bf16 nothing is near its
+// end.  P is held 2^bias higher because v_exp_f32 drops results below 2^-126 and fp16 keeps 2^-24 at the least:
+// weights down to 2^-134 of the maximum count with bf16 (whose results reach 2^-126), down to 2^-31 with fp16.
+// Values up to 2^100 meet no overflow.
 template <class E>
 constexpr float kAttendBias = std::is_same<E, f16>::value ? 7.f : 8.f;
+template <class E>
+constexpr float kAttendLimit = std::is_same<E, f16>::value ? 60000.f : 16777216.f;
 
 // The entry of the block table that holds position pos, -1 outside the table
 __device__ __forceinline__ int page_of(const AttendArgs& a, int r, int pos) {

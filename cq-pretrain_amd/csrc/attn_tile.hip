@@ -69,11 +69,6 @@ __device__ __forceinline__ Piece<D> fetch(__amdgpu_buffer_rsrc_t page, int code,
   return x;
 }
 
-// The sum of a step's weights in a lane beyond which the running maximum moves: with bf16 far below where
-// anything overflows, with fp16 where a weight may pass the largest number
-template <class E>
-constexpr float kLimit = std::is_same<E, f16>::value ? 60000.f : 16777216.f;
-
 template <class E, int D>
 __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void tile_kernel(AttendArgs a, int tiles, int splits) {
   typedef typename Vec<E>::x8 x8;
@@ -266,6 +261,7 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void tile_kernel(AttendArgs 
           for (int i = 0; i < 2 * kEarly; ++i) kf[i] = ld8(kp + i / KQ * 32 * kStrideK<D> + i % KQ * 16);
           const int4 poisoned = *reinterpret_cast<const int4*>(poison[j & 1]);
           __builtin_amdgcn_sched_barrier(0);
+          __builtin_amdgcn_s_setprio(1);  // MFMAs first: 8% with short windows, nothing lost elsewhere
 #pragma unroll
           for (int i = 0; i < F; ++i) {
             if (i % KQ == 0) sc[i / KQ] = f32x16{};
@@ -274,6 +270,7 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void tile_kernel(AttendArgs 
             if (k < F) kf[k] = ld8(kp + k / KQ * 32 * kStrideK<D> + k % KQ * 16);
             __builtin_amdgcn_sched_barrier(0);
           }
+          __builtin_amdgcn_s_setprio(0);
           // hidden positions leave the scores
           const int pos = pos0 + j * TOK;
           if (shown != (1 << GROUPS) - 1 || pos < low || pos + TOK > high) {
@@ -292,7 +289,7 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void tile_kernel(AttendArgs 
 #pragma unroll
           for (int i = 0; i < 8 * NS; ++i) weights(i);
           // where the weights have grown too large, or are a row's first, its maximum moves and they are made again
-          bool large = sum > kLimit<E> || m == -INFINITY;
+          bool large = sum > kAttendLimit<E> || m == -INFINITY;
           if (__any(large)) {
             large = __shfl_xor((int)large, 32, 64) || large;  // the two lanes of a row
             float top = sc[0][0];
@@ -313,6 +310,7 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void tile_kernel(AttendArgs 
             for (int i = 0; i < 8 * NS; ++i) weights(i);
           }
           l += sum;
+          __builtin_amdgcn_s_setprio(1);
           begin_convert(j + 1);  // beyond the last step: of codes that nothing reads
 #pragma unroll
           for (int i = 0; i < FV; ++i) {
@@ -323,6 +321,7 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void tile_kernel(AttendArgs 
             for (int e = i * 2 * PARTS / FV; e < (i + 1) * 2 * PARTS / FV; ++e) convert(j + 1, e);
             __builtin_amdgcn_sched_barrier(0);
           }
+          __builtin_amdgcn_s_setprio(0);
           if (__builtin_amdgcn_readfirstlane(poisoned.x | poisoned.y | poisoned.z | poisoned.w)) {
 #pragma unroll 1
             for (int w = 0; w < 4; ++w)
