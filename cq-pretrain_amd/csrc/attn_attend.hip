@@ -153,6 +153,24 @@ __global__ __launch_bounds__(64 * kWaves, D == 256 ? 2 : 3) void attend_kernel(A
     const bool real = rho < rows;
     const int row_t = real ? a.group.of(rho) : 0;
     const int t = from + row_t, head = h * group + (real ? rho - row_t * group : 0);
+    x8 qf[KQ];
+    {
+      const E* q = static_cast<const E*>(a.q) + t * a.q_token + head * a.q_head;
+#pragma unroll
+      for (int k = 0; k < KQ; ++k) {
+        u32x4 w = real ? *reinterpret_cast<const u32x4*>(q + (D >= 128 ? 128 * (k / 4) + 32 * q4 + 8 * (k % 4) : 16 * q4 + 8 * k))
+                       : u32x4{0, 0, 0, 0};
+        if (a.scale < 0.f) w ^= 0x80008000u;
+        qf[k] = __builtin_bit_cast(x8, w);
+      }
+    }
+    // the block table's next 64 entries, an entry a lane, from position `at` on
+    const auto entries = [&](int at) {
+      const int column = (at >> a.page_shift) + lane;
+      return column < a.columns ? a.tables[r * a.table_stride + column] : -1;
+    };
+    // without a window the part's first positions, and with them its pages, are known before the rows' limits
+    const int early = a.window <= 0 && r < a.N ? entries((s * per + wave) * kStep) : -1;
     const int hi = real && r < a.N ? min(max(a.visible[t], 0), room) : 0;
     const int lo = a.window > 0 ? max(0, hi - a.window) : 0;
     // over the rows that see anything: from the first position any of them sees to the last, and the
@@ -171,17 +189,6 @@ __global__ __launch_bounds__(64 * kWaves, D == 256 ? 2 : 3) void attend_kernel(A
       continue;
     }
 
-    x8 qf[KQ];
-    {
-      const E* q = static_cast<const E*>(a.q) + t * a.q_token + head * a.q_head;
-#pragma unroll
-      for (int k = 0; k < KQ; ++k) {
-        u32x4 w = real ? *reinterpret_cast<const u32x4*>(q + (D >= 128 ? 128 * (k / 4) + 32 * q4 + 8 * (k % 4) : 16 * q4 + 8 * k))
-                       : u32x4{0, 0, 0, 0};
-        if (a.scale < 0.f) w ^= 0x80008000u;
-        qf[k] = __builtin_bit_cast(x8, w);
-      }
-    }
     f32x4 o[MT];
 #pragma unroll
     for (int i = 0; i < MT; ++i) o[i] = zero4();
@@ -191,10 +198,10 @@ __global__ __launch_bounds__(64 * kWaves, D == 256 ? 2 : 3) void attend_kernel(A
 
     int i = s * per + wave;
     while (i < stop) {
-      // the block table's next 64 entries, an entry a lane: the steps they serve find their pages without a load
+      // 64 entries: the steps they serve find their pages without a load
       int pos = begin + i * kStep;
       const int column0 = pos >> a.page_shift;
-      const int table = column0 + lane < a.columns ? a.tables[r * a.table_stride + column0 + lane] : -1;
+      const int table = a.window <= 0 && i == s * per + wave ? early : entries(pos);
       const int64_t reach = (int64_t)(column0 + 64) << a.page_shift;  // the first position beyond them
       const int end = (int)min((int64_t)stop, (reach - begin) / kStep);
       const auto find = [&](int at, bool any) {
