@@ -33,7 +33,7 @@ int check_cache(const void* data, int64_t pages, int kv_heads, int D, int page) 
 
 int check_rows(const char* what, int64_t T, int kv_heads, int D) {
   if (T < 0) return fail(CQGDN_EINVAL, "%s: T=%lld", what, (long long)T);
-  if (T > kThreads / (D / 8) / kv_heads)
+  if (T > kThreads / (D / 8) / kv_heads - 16)
     return fail(CQGDN_EUNSUPPORTED, "%s: T=%lld rows of %d heads are too many", what, (long long)T, kv_heads);
   return CQGDN_OK;
 }
@@ -99,8 +99,9 @@ int cqgdn_kv4_write(const void* k, int64_t k_token, int64_t k_head, const void* 
   if (T == 0 || pages == 0) return ok();
   if (!k || !v || !slots || !aligned(k, 16) || !aligned(v, 16) || k_token % 8 || k_head % 8 || v_token % 8 || v_head % 8)
     return fail(CQGDN_EINVAL, "k and v (16-byte aligned, strides multiples of 8 elements) and slots must be non-null");
-  const RowsArgs a{k, v, {k_token, v_token}, {k_head, v_head}, nullptr, nullptr, slots, T, kv_heads, head_dim,
-                   static_cast<uint8_t*>(data), pages, __builtin_ctz(page), dtype == CQGDN_F16};
+  const RowsArgs a{k, v, {k_token, v_token}, {k_head, v_head}, nullptr, nullptr, slots, (int)T, kv_heads,
+                   head_dim, static_cast<uint8_t*>(data), (int)(pages * page), __builtin_ctz(page), dtype == CQGDN_F16,
+                   Divider(kv_heads)};
   launch_kv4_write(a, (hipStream_t)stream);
   return check_launch("cqgdn_kv4_write");
 }
@@ -113,8 +114,9 @@ int cqgdn_kv4_read(const void* data, int64_t pages, int page, int kv_heads, int 
   if (T == 0) return ok();
   if (!k || !v || !slots || !aligned(k, 16) || !aligned(v, 16))
     return fail(CQGDN_EINVAL, "k, v (16-byte aligned) and slots must be non-null");
-  const RowsArgs a{nullptr, nullptr, {0, 0}, {0, 0}, k, v, slots, T, kv_heads, head_dim,
-                   static_cast<uint8_t*>(const_cast<void*>(data)), pages, __builtin_ctz(page), dtype == CQGDN_F16};
+  const RowsArgs a{nullptr, nullptr, {0, 0}, {0, 0}, k, v, slots, (int)T, kv_heads, head_dim,
+                   static_cast<uint8_t*>(const_cast<void*>(data)), (int)(pages * page), __builtin_ctz(page),
+                   dtype == CQGDN_F16, Divider(kv_heads)};
   launch_kv4_read(a, (hipStream_t)stream);
   return check_launch("cqgdn_kv4_read");
 }

@@ -16,6 +16,18 @@ namespace cqgdn {
 // products exact in bf16, and the conversion instructions of gfx950 take codes and scale together.
 __host__ __device__ constexpr int kv4_page_bytes(int page, int D) { return page * (D + D / 16); }
 
+// Division of n < 2^31 by d > 0 as a product: m = ceil(2^(31 + s) / d) with 2^s >= d is off by less than
+// 2^s / d / 2^(31 + s) of a unit, n times which stays below 1 / d.
+struct Divider {
+  uint32_t d, m;
+  int s;
+  explicit Divider(uint32_t by) : d(by), m(0), s(0) {
+    while ((1ull << s) < by) ++s;
+    m = (uint32_t)(((1ull << (31 + s)) + by - 1) / by);
+  }
+  __device__ __forceinline__ int of(int n) const { return s == 0 ? n : (int)(__umulhi((uint32_t)n, m) >> (s - 1)); }
+};
+
 struct RotaryArgs {
   const void* x[2];            // q, k
   void* y[2];
@@ -54,27 +66,14 @@ struct RowsArgs {                 // rows written to, or read from, the cache
   int64_t token[2], head[2];
   void *k_out, *v_out;
   const int32_t* slots;
-  int64_t T;
-  int heads, D;
+  int T, heads, D;
   uint8_t* data;
-  int64_t pages;
-  int page_shift;
+  int slot_count, page_shift;     // pages x page, which 31 bits hold
   bool fp16;
+  Divider by_heads;
 };
 void launch_kv4_write(const RowsArgs& a, hipStream_t st);
 void launch_kv4_read(const RowsArgs& a, hipStream_t st);
-
-// Division of n < 2^31 by d > 0 as a product: m = ceil(2^(31 + s) / d) with 2^s >= d is off by less than
-// 2^s / d / 2^(31 + s) of a unit, n times which stays below 1 / d.
-struct Divider {
-  uint32_t d, m;
-  int s;
-  explicit Divider(uint32_t by) : d(by), m(0), s(0) {
-    while ((1ull << s) < by) ++s;
-    m = (uint32_t)(((1ull << (31 + s)) + by - 1) / by);
-  }
-  __device__ __forceinline__ int of(int n) const { return s == 0 ? n : (int)(__umulhi((uint32_t)n, m) >> (s - 1)); }
-};
 
 struct AttendArgs {
   const void* q;
