@@ -19,7 +19,10 @@ constexpr int kWaves = 4;         // of a workgroup; they take its steps in turn
 constexpr int kStep = 64;         // positions of a wave's step
 constexpr int kMaxSplits = 512;
 constexpr int kBlocks = 1024;     // workgroups of a decode launch, 4 a CU
-constexpr int kFewRows = 32;      // of a request and key head: more take the kernel of attn_tile.hip
+// Rows of a request and key head above which its positions are converted once for all of them (attn_tile.hip)
+// and not once for every 16: over 2000 positions of 64 requests 36 rows take 38 us here and 43 there, 64 rows 49
+// and 46, 128 rows 89 and 58.
+constexpr int kFewRows = 48;
 
 // The pages of a step's four 16 positions, the same for all lanes.  An entry that names no page reads as zeros
 // (its buffer has no bytes), and its positions are hidden.
@@ -412,7 +415,44 @@ __global__ __launch_bounds__(64 * kWaves, D == 256 ? 2 : 3) void attend_kernel(A
   }
 }
 
-// Joins the parts of a row, a workgroup for 64 dimensions: the parts' weights, then 16 parts at a time.
+// Joins the parts of many rows: D / 4 lanes a row, each taking its 4 dimensions through the parts.
+template <class E, int D>
+__global__ __launch_bounds__(256) void join_rows_kernel(AttendArgs a, int splits) {
+  constexpr int L4 = D / 4, UP = 4;  // lanes a row, parts whose loads are under way at once
+  const int64_t at = (int64_t)blockIdx.x * (256 / L4) + threadIdx.x / L4;
+  const int col = threadIdx.x % L4;
+  if (at >= a.T * a.heads) return;
+  const float2* ml = reinterpret_cast<const float2*>(a.ws + a.T * a.heads * splits * D) + at * splits;
+  const float* rows = a.ws + at * splits * D + 4 * col;
+  float M = -INFINITY;
+#pragma unroll 8
+  for (int s = 0; s < splits; ++s) M = fmaxf(M, ml[s].x);
+  f32x4 y = zero4();
+  float L = 0.f;
+  for (int s0 = 0; s0 < splits; s0 += UP) {
+    f32x4 x[UP];
+    float2 part[UP];
+#pragma unroll
+    for (int i = 0; i < UP; ++i) {
+      const int s = min(s0 + i, splits - 1);
+      part[i] = ml[s];
+      x[i] = *reinterpret_cast<const f32x4*>(rows + s * D);
+    }
+#pragma unroll
+    for (int i = 0; i < UP; ++i) {
+      // a part that saw nothing wrote no row
+      const bool none = s0 + i >= splits || (part[i].x == -INFINITY && part[i].y == 0.f);
+      const float f = none ? 0.f : __builtin_amdgcn_exp2f(part[i].x - M);
+      L += f * part[i].y;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) y[e] += none ? 0.f : f * x[i][e];
+    }
+  }
+  st4(static_cast<E*>(a.out) + at * D + 4 * col, L == 0.f ? zero4() : y * (1.f / L));
+  if (a.lse && col == 0) a.lse[at] = (M - kAttendBias<E> + log2f(L)) * 0.693147180559945309f;
+}
+
+// Joins the parts of few rows, a workgroup for 64 dimensions of one: the parts' weights, then 16 parts at a time.
 template <class E, int D>
 __global__ __launch_bounds__(256) void join_kernel(AttendArgs a, int splits) {
   constexpr int W = kMaxSplits / 256;
@@ -483,12 +523,14 @@ struct Plan {
   int splits, per;
 };
 // `capacity` positions a table row holds; with a window a row sees no more of them than it, and never more parts.
-Plan attend_plan(int64_t N, int kv_heads, int group, int max_queries, int64_t capacity, int window) {
+Plan attend_plan(int64_t N, int kv_heads, int group, int D, int max_queries, int64_t capacity, int window) {
   const int64_t rows = (int64_t)max_queries * group;
-  const int64_t seen = window > 0 ? std::min(capacity, (int64_t)window + max_queries + kStep) : capacity;
+  int64_t seen = window > 0 ? std::min(capacity, (int64_t)window + max_queries + kStep) : capacity;
   if (rows > kFewRows) {
-    const int64_t blocks = N * kv_heads * ((rows + 127) / 128), most = std::min<int64_t>(kMaxSplits, (seen + 511) / 512);
-    return {true, (int)std::max<int64_t>(1, std::min(most, 512 / std::max<int64_t>(blocks, 1))), 0};
+    // as many parts as give the CUs the workgroups that their registers hold, each of at least 512 positions
+    const int64_t blocks = N * kv_heads * ((rows + 127) / 128), fit = D == 256 ? 256 : 512;
+    if (window > 0) seen = std::min<int64_t>(capacity, (int64_t)window + 128 / group + 64);
+    return {true, (int)std::max<int64_t>(1, std::min<int64_t>(seen / 512, fit / std::max<int64_t>(blocks, 1))), 0};
   }
   // parts of the same length, so that ragged requests load the CUs alike: a step a wave at the least, and as
   // long as keep the launch within kBlocks workgroups, were every request to fill its table row
@@ -507,7 +549,7 @@ Plan attend_plan(int64_t N, int kv_heads, int group, int max_queries, int64_t ca
 template <class E, int D>
 void launch_dim(const AttendArgs& a, hipStream_t st) {
   const int group = a.heads / a.kv_heads;
-  const Plan p = attend_plan(a.N, a.kv_heads, group, a.max_queries, (int64_t)a.columns << a.page_shift, a.window);
+  const Plan p = attend_plan(a.N, a.kv_heads, group, D, a.max_queries, (int64_t)a.columns << a.page_shift, a.window);
   if (p.tiles) {
     launch_attend_tiles(a, p.splits, st);
   } else {
@@ -516,7 +558,14 @@ void launch_dim(const AttendArgs& a, hipStream_t st) {
     // a workgroup takes every tiles-th tile: none is left out whatever the bound
     attend_kernel<E, D><<<dim3((unsigned)((a.N + 1) * tiles), a.kv_heads, p.splits), 64 * kWaves, 0, st>>>(a, tiles, p.per);
   }
-  if (p.splits > 1) join_kernel<E, D><<<(unsigned)(a.T * a.heads * (D / 64)), 256, 0, st>>>(a, p.splits);
+  if (p.splits > 1) {
+    // 2048 rows of 33 MB in two parts: 60 us by the kernel for few rows; 32 rows in 36 parts: 4 us by it
+    const int64_t groups = (a.T * a.heads * D + 1023) / 1024;
+    if (groups >= 256)
+      join_rows_kernel<E, D><<<(unsigned)groups, 256, 0, st>>>(a, p.splits);
+    else
+      join_kernel<E, D><<<(unsigned)(a.T * a.heads * (D / 64)), 256, 0, st>>>(a, p.splits);
+  }
 }
 
 template <class E>
@@ -532,7 +581,7 @@ void by_dim(const AttendArgs& a, hipStream_t st) {
 }  // namespace
 
 size_t attend_workspace_bytes(int64_t T, int64_t N, int heads, int kv_heads, int D, int max_queries, int64_t capacity) {
-  const int splits = attend_plan(N, kv_heads, heads / kv_heads, max_queries, capacity, 0).splits;
+  const int splits = attend_plan(N, kv_heads, heads / kv_heads, D, max_queries, capacity, 0).splits;
   return splits > 1 ? (size_t)T * heads * splits * (D + 2) * sizeof(float) : 0;
 }
 
