@@ -63,25 +63,6 @@ def plan(rotary_dim, *, theta=10000.0, sections=None, mixed=False, adjacent=Fals
                       bool(adjacent))
 
 
-def _call(q, k, positions, p, backward):
-    CALLS["cqgdn_rotary"] += 1
-    return _lib.ops().rotary(q, k, positions, p.turns, p.axis, p.adjacent, backward)
-
-
-class _Rotate(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, q, k, positions, p):
-        ctx.save_for_backward(positions, p.turns, p.axis)
-        ctx.adjacent = p.adjacent
-        return _call(q, k, positions, p, False)
-
-    @staticmethod
-    def backward(ctx, dq, dk):
-        positions, turns, axis = ctx.saved_tensors
-        dq, dk = _call(dq, dk, positions, RotaryPlan(turns, axis, ctx.adjacent), True)
-        return dq, dk, None, None
-
-
 def rotate(q, k, positions, plan):
     """q [T, Hq, D] and k [T, Hk, D] (bf16, fp16 or fp32, any strides; or [1, T, H, D]) turned by the
     positions of their tokens: int32 or int64 [axes, T], or [T] for one axis.  Values of a head behind
@@ -91,8 +72,6 @@ def rotate(q, k, positions, plan):
         q, k = q[0], k[0]
     if positions.dim() == 1:
         positions = positions[None]
-    if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad):
-        q, k = _Rotate.apply(q, k, positions, plan)
-    else:
-        q, k = _call(q, k, positions, plan, False)
+    CALLS["cqgdn_rotary"] += 1
+    q, k = _lib.ops().rotary(q, k, positions, plan.turns, plan.axis, plan.adjacent, False)
     return (q[None], k[None]) if packed else (q, k)

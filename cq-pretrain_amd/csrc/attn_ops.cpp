@@ -4,7 +4,7 @@
 // contract checks run before any launch and, but for the last ("a ROCm GPU"), for tensors on any device.
 //
 // Schemas:
-//   rotary(q, k, positions, turns, axis, adjacent, backward) -> (q', k')
+//   rotary(q, k, positions, turns, axis, adjacent, backward) -> (q', k'), differentiable in q and k
 //       q [T,Hq,D], k [T,Hk,D] of one type; positions [A,T] int32 or int64
 //   step_pages(cached, new, tables!, free!, free_count, page, tokens, in_place)
 //       -> (starts, lengths, admitted, free_count, slots, positions, visible)
@@ -15,6 +15,7 @@
 #include <ATen/ops/as_strided_native.h>
 #include <c10/core/DeviceGuard.h>
 #include <c10/hip/HIPStream.h>
+#include <torch/csrc/autograd/custom_function.h>
 #include <torch/library.h>
 
 #include "cqgdn.h"
@@ -88,6 +89,48 @@ std::tuple<Tensor, Tensor> rotary(const Tensor& q, const Tensor& k, const Tensor
                      qo.data_ptr(), ko.data_ptr(), stream_of(q)),
         "cqgdn_rotary");
   return {qo, ko};
+}
+
+// The gradient of a turn is the turn back.  In C++ because a Python function and its engine call cost 40 us more
+// than the kernels of a small step.
+struct Rotate : torch::autograd::Function<Rotate> {
+  static torch::autograd::variable_list forward(torch::autograd::AutogradContext* ctx, const Tensor& q, const Tensor& k,
+                                                const Tensor& positions, const Tensor& turns, const Tensor& axis,
+                                                bool adjacent, bool backward) {
+    const at::AutoDispatchBelowADInplaceOrView below;
+    ctx->save_for_backward({positions, turns, axis});
+    ctx->saved_data["adjacent"] = adjacent;
+    ctx->saved_data["backward"] = backward;
+    static const auto op = rotary_op();
+    const auto [y, z] = op.call(q, k, positions, turns, axis, adjacent, backward);
+    return {y, z};
+  }
+  static torch::autograd::variable_list backward(torch::autograd::AutogradContext* ctx,
+                                                 const torch::autograd::variable_list& grad) {
+    static const auto op = rotary_op();
+    const auto saved = ctx->get_saved_variables();
+    const auto [dq, dk] = op.call(grad[0], grad[1], saved[0], saved[1], saved[2], ctx->saved_data["adjacent"].toBool(),
+                                  !ctx->saved_data["backward"].toBool());
+    return {dq, dk, {}, {}, {}, {}, {}};
+  }
+  static c10::TypedOperatorHandle<std::tuple<Tensor, Tensor>(const Tensor&, const Tensor&, const Tensor&, const Tensor&,
+                                                             const Tensor&, bool, bool)>
+  rotary_op() {
+    return c10::Dispatcher::singleton()
+        .findSchemaOrThrow("cqgdn::rotary", "")
+        .typed<std::tuple<Tensor, Tensor>(const Tensor&, const Tensor&, const Tensor&, const Tensor&, const Tensor&, bool,
+                                          bool)>();
+  }
+};
+std::tuple<Tensor, Tensor> rotary_autograd(const Tensor& q, const Tensor& k, const Tensor& positions, const Tensor& turns,
+                                           const Tensor& axis, bool adjacent, bool backward) {
+  if (!at::GradMode::is_enabled() || !(q.requires_grad() || k.requires_grad())) {
+    const at::AutoDispatchBelowADInplaceOrView below;
+    static const auto op = Rotate::rotary_op();
+    return op.call(q, k, positions, turns, axis, adjacent, backward);
+  }
+  const auto out = Rotate::apply(q, k, positions, turns, axis, adjacent, backward);
+  return {out[0], out[1]};
 }
 
 std::tuple<Tensor, Tensor, Tensor, Tensor, Tensor, Tensor, Tensor> step_pages(const Tensor& cached, const Tensor& fresh,
@@ -222,6 +265,8 @@ TORCH_LIBRARY_FRAGMENT(cqgdn, m) {
   m.def("kv4_attend(Tensor q, Tensor data, Tensor tables, Tensor starts, Tensor visible, int page, int window, "
         "float scale, int max_queries, bool want_lse) -> (Tensor, Tensor)");
 }
+
+TORCH_LIBRARY_IMPL(cqgdn, Autograd, m) { m.impl("rotary", &rotary_autograd); }
 
 TORCH_LIBRARY_IMPL(cqgdn, CUDA, m) {
   m.impl("rotary", &rotary);
