@@ -124,12 +124,12 @@ __device__ __forceinline__ int max16(int x) {
   return __builtin_amdgcn_readfirstlane(max(x, turned<8>(x)));
 }
 
-// One workgroup: 16 rows of one request and key head, one of gridDim.z parts of the positions, `per` steps
+// One workgroup: 16 rows of one request and key head, one of gridDim.z parts of the positions, `least` steps
 // long (the last parts, which are empty where requests are shorter, come last).  The waves' steps interleave,
 // each with its own maximum, sum and O^T, and are joined at the end.  A step's codes are on their way from the
 // moment those before have been used, in registers.
 template <class E, int D>
-__global__ __launch_bounds__(64 * kWaves, D == 256 ? 2 : 3) void attend_kernel(AttendArgs a, int tiles, int per) {
+__global__ __launch_bounds__(64 * kWaves, D == 256 ? 2 : 3) void attend_kernel(AttendArgs a, int tiles, int least) {
   typedef typename Vec<E>::x8 x8;
   typedef Values<D> V;
   constexpr int DC = V::DC, LD = DC + 16;  // 8 banks further each row: the transposed reads of 8 rows meet no bank twice
@@ -173,7 +173,7 @@ __global__ __launch_bounds__(64 * kWaves, D == 256 ? 2 : 3) void attend_kernel(A
       return column < a.columns ? a.tables[r * a.table_stride + column] : -1;
     };
     // without a window the part's first positions, and with them its pages, are known before the rows' limits
-    const int early = a.window <= 0 && r < a.N ? entries((s * per + wave) * kStep) : -1;
+    const int early = a.window <= 0 && r < a.N ? entries((s * least + wave) * kStep) : -1;
     const int hi = real && r < a.N ? min(max(a.visible[t], 0), room) : 0;
     const int lo = a.window > 0 ? max(0, hi - a.window) : 0;
     // over the rows that see anything: from the first position any of them sees to the last, and the
@@ -182,6 +182,8 @@ __global__ __launch_bounds__(64 * kWaves, D == 256 ? 2 : 3) void attend_kernel(A
     const int low = max16(lo), high = min16(real ? hi : INT32_MAX);
     const int begin = last > 0 ? first & ~(kStep - 1) : 0;
     const int steps = (last - begin + kStep - 1) / kStep;
+    // with a window the rows' limits may lie further apart than the launch was made for: longer parts then
+    const int per = max(least, ((steps + splits - 1) / splits + kWaves - 1) & ~(kWaves - 1));
     const int stop = min(steps, (s + 1) * per);
     if (s > 0 && s * per >= steps) {  // nothing of it here: only the join hears of this part
       if (tid < 16 && real) {
