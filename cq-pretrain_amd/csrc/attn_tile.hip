@@ -56,7 +56,7 @@ struct Piece {
 template <int D>
 __device__ __forceinline__ Piece<D> fetch(__amdgpu_buffer_rsrc_t page, int code, int code0, int scale, int scale0) {
   Piece<D> x;
-  if constexpr (D == 64) {
+  if constexpr (kPiece<D> == 16) {
     const auto w = __builtin_amdgcn_raw_buffer_load_b64(page, code, code0, 0);
     x.w[0] = w[0];
     x.w[1] = w[1];
@@ -218,23 +218,55 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void tile_kernel(AttendArgs 
         st8(vt[j & 1] + vw[e - PARTS], kv4_values<E>(vn.w[e - PARTS], vscale));
     };
     f32x16 sc[NS];
-    // the weights, two a part, in the order of the scores
-    uint32_t pw[8 * NS];
+    // the weights of 32 positions, two a part, in the order of their scores
+    uint32_t pw[NS][8];
     float base, sum;
     const auto begin_weights = [&]() {
       base = bias - (m == -INFINITY ? 0.f : m);
       sum = 0.f;
     };
-    const auto weights = [&](int i) {
+    const auto weights = [&](int u, int i) {
       typedef float f32x2 __attribute__((ext_vector_type(2)));
       typedef E x2 __attribute__((ext_vector_type(2)));
       f32x2 p;
 #pragma unroll
       for (int e = 0; e < 2; ++e) {
-        p[e] = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[i / 8][2 * (i % 8) + e], c, base));
+        p[e] = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[u][2 * i + e], c, base));
         sum += p[e];
       }
-      pw[i] = __builtin_bit_cast(uint32_t, __builtin_convertvector(p, x2));
+      pw[u][i] = __builtin_bit_cast(uint32_t, __builtin_convertvector(p, x2));
+    };
+    // hidden positions leave the scores
+    const auto mask = [&](int u, int pos, int shown) {
+      if (shown == (1 << GROUPS) - 1 && pos >= low && pos + TOK <= high) return;
+      const int lo0 = lo - pos - 4 * kg, hi0 = hi - pos - 4 * kg;
+#pragma unroll
+      for (int e = 0; e < 16; ++e) {
+        const int at = 32 * u + 8 * (e >> 2) + (e & 3);
+        if ((int)(at < lo0) | (int)(at >= hi0) | (int)!(shown >> (2 * u + (e >> 3)) & 1)) sc[u][e] = -INFINITY;
+      }
+    };
+    // where the weights have grown too large, or are a row's first, its maximum moves and they are made again
+    const auto settle = [&](int u) {
+      bool large = sum > kAttendLimit<E> || m == -INFINITY;
+      if (__any(large)) {
+        large = __shfl_xor((int)large, 32, 64) || large;  // the two lanes of a row
+        float top = sc[u][0];
+#pragma unroll
+        for (int e = 1; e < 16; ++e) top = fmaxf(top, sc[u][e]);
+        top = fmaxf(top, __shfl_xor(top, 32, 64)) * c;
+        if (large && top > m) {
+          const float f = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m - top);
+          m = top;
+          l *= f;
+#pragma unroll
+          for (int k = 0; k < MT; ++k) o[k] *= f;
+        }
+        begin_weights();
+#pragma unroll
+        for (int i = 0; i < 8; ++i) weights(u, i);
+      }
+      l += sum;
     };
 
     if (n > 0) {
@@ -260,68 +292,67 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void tile_kernel(AttendArgs 
 #pragma unroll
           for (int i = 0; i < 2 * kEarly; ++i) kf[i] = ld8(kp + i / KQ * 32 * kStrideK<D> + i % KQ * 16);
           const int4 poisoned = *reinterpret_cast<const int4*>(poison[j & 1]);
-          __builtin_amdgcn_sched_barrier(0);
-          __builtin_amdgcn_s_setprio(1);  // MFMAs first: 8% with short windows, nothing lost elsewhere
-#pragma unroll
-          for (int i = 0; i < F; ++i) {
-            if (i % KQ == 0) sc[i / KQ] = f32x16{};
-            sc[i / KQ] = mfma32(kf[i], qf[i % KQ], sc[i / KQ]);
-            const int k = i + 2 * kEarly;
+          const int pos = pos0 + j * TOK;
+          constexpr int H = FV / NS;  // operands of V for 32 positions
+          const auto score = [&](int u, int i) {
+            if (i == 0) sc[u] = f32x16{};
+            sc[u] = mfma32(kf[u * KQ + i], qf[i], sc[u]);
+            const int k = u * KQ + i + 2 * kEarly;
             if (k < F) kf[k] = ld8(kp + k / KQ * 32 * kStrideK<D> + k % KQ * 16);
+          };
+          const auto gather = [&](int u, int i) {
+            const int w = i / MT * 4;
+            const x8 p = __builtin_bit_cast(x8, u32x4{pw[u][w], pw[u][w + 1], pw[u][w + 2], pw[u][w + 3]});
+            o[i % MT] = mfma32(vf[u * H + i], p, o[i % MT]);
+          };
+          // An MFMA leaves the wave's issue free for about as long as two weights take.  So the first 32
+          // positions' weights stand between the second's scores, the second's between the first's products
+          // with V, and the next step's conversions between the last.
+          __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+          for (int i = 0; i < KQ; ++i) {
+            score(0, i);
             __builtin_amdgcn_sched_barrier(0);
           }
-          __builtin_amdgcn_s_setprio(0);
-          // hidden positions leave the scores
-          const int pos = pos0 + j * TOK;
-          if (shown != (1 << GROUPS) - 1 || pos < low || pos + TOK > high) {
-            const int lo0 = lo - pos - 4 * kg, hi0 = hi - pos - 4 * kg;
-#pragma unroll
-            for (int u = 0; u < NS; ++u)
-#pragma unroll
-              for (int e = 0; e < 16; ++e) {
-                const int at = 32 * u + 8 * (e >> 2) + (e & 3);
-                if ((int)(at < lo0) | (int)(at >= hi0) | (int)!(shown >> (2 * u + (e >> 3)) & 1)) sc[u][e] = -INFINITY;
-              }
-          }
-#pragma unroll
-          for (int i = 0; i < kEarly; ++i) value(i);
+          mask(0, pos, shown);
           begin_weights();
+          if constexpr (NS == 2) {
 #pragma unroll
-          for (int i = 0; i < 8 * NS; ++i) weights(i);
-          // where the weights have grown too large, or are a row's first, its maximum moves and they are made again
-          bool large = sum > kAttendLimit<E> || m == -INFINITY;
-          if (__any(large)) {
-            large = __shfl_xor((int)large, 32, 64) || large;  // the two lanes of a row
-            float top = sc[0][0];
+            for (int i = 0; i < KQ; ++i) {
+              score(1, i);
 #pragma unroll
-            for (int u = 0; u < NS; ++u)
+              for (int e = i * 8 / KQ; e < (i + 1) * 8 / KQ; ++e) weights(0, e);
 #pragma unroll
-              for (int e = 0; e < 16; ++e) top = fmaxf(top, sc[u][e]);
-            top = fmaxf(top, __shfl_xor(top, 32, 64)) * c;
-            if (large && top > m) {
-              const float f = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m - top);
-              m = top;
-              l *= f;
-#pragma unroll
-              for (int k = 0; k < MT; ++k) o[k] *= f;
+              for (int e = i * H / KQ; e < (i + 1) * H / KQ; ++e) value(e);
+              __builtin_amdgcn_sched_barrier(0);
             }
+            settle(0);
+            mask(1, pos, shown);
             begin_weights();
 #pragma unroll
-            for (int i = 0; i < 8 * NS; ++i) weights(i);
+            for (int i = 0; i < H; ++i) {
+              gather(0, i);
+#pragma unroll
+              for (int e = i * 8 / H; e < (i + 1) * 8 / H; ++e) weights(1, e);
+              value(H + i);
+              __builtin_amdgcn_sched_barrier(0);
+            }
+          } else {
+#pragma unroll
+            for (int i = 0; i < kEarly; ++i) value(i);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) weights(0, e);
           }
-          l += sum;
-          __builtin_amdgcn_s_setprio(1);
+          settle(NS - 1);
           begin_convert(j + 1);  // beyond the last step: of codes that nothing reads
 #pragma unroll
-          for (int i = 0; i < FV; ++i) {
-            const int w = i / MT * 4;
-            o[i % MT] = mfma32(vf[i], __builtin_bit_cast(x8, u32x4{pw[w], pw[w + 1], pw[w + 2], pw[w + 3]}), o[i % MT]);
-            if (i + kEarly < FV) value(i + kEarly);
+          for (int i = 0; i < H; ++i) {
+            gather(NS - 1, i);
+            if (NS == 1 && i + kEarly < H) value(i + kEarly);
 #pragma unroll
-            for (int e = i * 2 * PARTS / FV; e < (i + 1) * 2 * PARTS / FV; ++e) convert(j + 1, e);
+            for (int e = i * 2 * PARTS / H; e < (i + 1) * 2 * PARTS / H; ++e) convert(j + 1, e);
             __builtin_amdgcn_sched_barrier(0);
           }
-          __builtin_amdgcn_s_setprio(0);
           if (__builtin_amdgcn_readfirstlane(poisoned.x | poisoned.y | poisoned.z | poisoned.w)) {
 #pragma unroll 1
             for (int w = 0; w < 4; ++w)
