@@ -530,7 +530,7 @@ Plan attend_plan(int64_t N, int kv_heads, int group, int D, int max_queries, int
   int64_t seen = window > 0 ? std::min(capacity, (int64_t)window + max_queries + kStep) : capacity;
   if (rows > kFewRows) {
     // as many parts as give the CUs the workgroups that their registers hold, each of at least 512 positions
-    const int64_t blocks = N * kv_heads * ((rows + 127) / 128), fit = D == 256 ? 256 : 512;
+    const int64_t blocks = N * kv_heads * ((rows + 127) / 128), fit = D == 256 ? 256 : D == 64 ? 768 : 512;
     if (window > 0) seen = std::min<int64_t>(capacity, (int64_t)window + 128 / group + 64);
     return {true, (int)std::max<int64_t>(1, std::min<int64_t>(seen / 512, fit / std::max<int64_t>(blocks, 1))), 0};
   }

@@ -70,7 +70,7 @@ __device__ __forceinline__ Piece<D> fetch(__amdgpu_buffer_rsrc_t page, int code,
 }
 
 template <class E, int D>
-__global__ __launch_bounds__(256, D == 256 ? 1 : 2) void tile_kernel(AttendArgs a, int tiles, int splits) {
+__global__ __launch_bounds__(256, D == 256 ? 1 : D == 64 ? 3 : 2) void tile_kernel(AttendArgs a, int tiles, int splits) {
   typedef typename Vec<E>::x8 x8;
   constexpr int TOK = kTokens<D>, VP = kPiece<D>, PV = D / VP, NS = TOK / 32, KQ = D / 16, MT = D / 32;
   constexpr int F = NS * KQ, FV = 2 * NS * MT;  // operands of a step: K's and V's
