@@ -18,7 +18,6 @@ namespace {
 constexpr int kWaves = 4;         // of a workgroup; they take its steps in turn
 constexpr int kStep = 64;         // positions of a wave's step
 constexpr int kMaxSplits = 512;
-constexpr int kBlocks = 1024;     // workgroups of a decode launch, 4 a CU
 // Rows of a request and key head above which its positions are converted once for all of them (attn_tile.hip)
 // and not once for every 16: over 2000 positions of 64 requests 36 rows take 38 us here and 43 there, 64 rows 49
 // and 46, 128 rows 89 and 58.
@@ -534,17 +533,21 @@ Plan attend_plan(int64_t N, int kv_heads, int group, int D, int max_queries, int
     if (window > 0) seen = std::min<int64_t>(capacity, (int64_t)window + 128 / group + 64);
     return {true, (int)std::max<int64_t>(1, std::min<int64_t>(seen / 512, fit / std::max<int64_t>(blocks, 1))), 0};
   }
-  // parts of the same length, so that ragged requests load the CUs alike: a step a wave at the least, and as
-  // long as keep the launch within kBlocks workgroups, were every request to fill its table row
+  const int64_t resident = D == 256 ? 512 : D == 128 ? 768 : 1024;
   constexpr int64_t kLeast = kWaves * kStep;
-  const auto parts = [](int64_t positions, int64_t most, int64_t& times) {
+  // Parts of the same length, so that ragged requests load the CUs alike: a step a wave at the least, and as long
+  // as keep the launch within one and a half times the workgroups that are resident at once, were every request to
+  // fill its table row (five ragged documents of 65536 positions, D = 256: 768 workgroups 36 us, 1024 42, 512 42; 64
+  // requests of 8192, D = 128: 1024 46 us, 768 50, 2048 49); three steps a wave where every CU still has a workgroup
+  // (one request of 65536: 21 us, with one step 30)
+  const auto parts = [](int64_t positions, int64_t most, int64_t blocks, int64_t& times) {
     const int64_t least = (positions + kLeast - 1) / kLeast;
-    times = std::max<int64_t>(1, (least + most - 1) / most);
+    times = std::max({(int64_t)1, (least + most - 1) / most, std::min<int64_t>(3, least * blocks / 256)});
     return std::max<int64_t>(1, (least + times - 1) / times);
   };
   const int64_t blocks = std::max<int64_t>(1, N * kv_heads * ((rows + 15) / 16));
-  int64_t times, splits = parts(capacity, std::min<int64_t>(kMaxSplits, std::max<int64_t>(1, kBlocks / blocks)), times);
-  if (window > 0) splits = parts(seen, splits, times);
+  int64_t times, splits = parts(capacity, std::min<int64_t>(kMaxSplits, std::max<int64_t>(1, resident * 3 / 2 / blocks)), blocks, times);
+  if (window > 0) splits = parts(seen, splits, blocks, times);
   return {false, (int)splits, (int)(times * kWaves)};
 }
 
