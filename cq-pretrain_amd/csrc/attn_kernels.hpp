@@ -43,6 +43,7 @@ struct RotaryArgs {
   int axes;
   const uint64_t* turns;       // [rotary / 2] turns a position, in units of 2^-64 of a turn
   const int32_t* axis;         // [rotary / 2]
+  Divider by_heads{1}, by_pairs{1};  // set by the launch
 };
 void launch_rotary(const RotaryArgs& a, hipStream_t st);
 

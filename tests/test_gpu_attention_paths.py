@@ -7,7 +7,8 @@ import math
 import pytest
 import torch
 
-from test_gpu_attention import DEV, DTYPES, R, _attend_case, _attend_check, _pages_case, _pages_check, i32, ops  # noqa: F401
+from test_gpu_attention import (DEV, DTYPES, R, _attend_case, _attend_check, _pages_case, _pages_check,  # noqa: F401
+                                _rotary_case, _rotary_close, i32, ops)
 
 pytestmark = pytest.mark.gpu
 
@@ -128,6 +129,28 @@ def test_a_row_does_not_depend_on_the_rows_beside_it(ops):
 def test_step_pages_over_rounds(ops, n, context, most, page, spare, padding, in_place):
     cached, new, tables, free, count = _pages_case(n, context, most, page, spare, n, end=0.3)
     _pages_check(ops, cached, new, tables, free, count, page, int(new.clamp(min=0).sum()) + padding, in_place)
+
+
+@pytest.mark.parametrize("case", [  # T, Hq, Hk, D, rotary, sections, mixed, adjacent, type, far
+    (3, 2, 1, 1030, 514, (100, 100, 57), True, False, "fp32", 5),    # more units than a workgroup has threads
+    (2, 1, 1, 1030, 1030, (515,), False, True, "bf16", 0),
+    (2, 1, 2, 8448, 8448, (4224,), False, False, "bf16", 3),         # more pairs than its LDS holds
+    (2, 1, 1, 8448, 8448, (2000, 2224), False, True, "fp16", 70),
+    (1500, 5, 3, 128, 128, (64,), False, True, "bf16", 11),          # ragged numbers of items, a last workgroup short
+    (2051, 1, 1, 64, 16, (2, 3, 3), True, False, "fp32", 0),
+    (19, 64, 1, 256, 256, (128,), False, False, "fp16", 0),
+], ids=str)
+def test_rotate_sizes(ops, case):
+    p, q, k, pos, freq, axis = _rotary_case(ops, case)
+    r, adjacent, dtype = case[4], case[7], case[8]
+    y, z = ops.rotary.rotate(q.to(DEV), k.to(DEV), pos.to(DEV), p)
+    _rotary_close(y, q, R.rotate_ref(q, pos, freq, axis, adjacent), r, adjacent, dtype)
+    _rotary_close(z, k, R.rotate_ref(k, pos, freq, axis, adjacent), r, adjacent, dtype)
+    none = torch.empty(case[0], 0, case[3], dtype=q.dtype, device=DEV)  # one of the two may have no heads
+    a, b = ops.rotary.rotate(q.to(DEV), none, pos.to(DEV), p)
+    assert torch.equal(a, y) and b.shape == none.shape
+    a, b = ops.rotary.rotate(none, k.to(DEV), pos.to(DEV), p)
+    assert torch.equal(b, z) and a.shape == none.shape
 
 
 def test_rotate_gradients_of_one_input_and_of_gradients(ops):
