@@ -202,3 +202,22 @@ def test_rotate_gradient_in_a_graph(ops):
         graph.replay()
         torch.cuda.synchronize()
         assert all(torch.equal(a, b) for a, b in zip(held, want))
+
+
+@pytest.mark.parametrize("T,heads,D,dtype", [(2101, 16, 128, "bf16"), (1100, 16, 256, "fp16"), (9001, 8, 64, "bf16")])
+def test_write_and_read_of_many_rows(ops, T, heads, D, dtype):
+    """Sizes where a thread takes several rows; skipped slots among them, tokens in no order."""
+    g = torch.Generator().manual_seed(T)
+    t, page = DTYPES[dtype], 32
+    pages = -(-T // page) + 2
+    cache = ops.kv.KVCache.empty(pages, heads, page=page, head_dim=D, dtype=t, device=DEV)
+    rows = (torch.randn(T, 2 * heads, D, generator=g) * torch.exp2(torch.randint(-5, 5, (T, 1, 1), generator=g))).to(t).to(DEV)
+    slots = torch.randperm(pages * page, generator=g)[:T].int()
+    slots[::11] = -1
+    k, v = rows[:, :heads], rows[:, heads:]
+    ops.kv.write(cache, k, v, slots.to(DEV))
+    real = (slots >= 0).to(DEV)[:, None, None]
+    for got, x in zip(ops.kv.read(cache, slots.to(DEV)), (k, v)):
+        assert torch.equal(got.cpu().double(), torch.where(real.cpu(), R.encode_ref(x.cpu()), 0.0))
+    unwritten = torch.tensor(sorted(set(range(pages * page)) - set(slots.tolist())), dtype=torch.int32, device=DEV)
+    assert not any(bool(x.any()) for x in ops.kv.read(cache, unwritten))
