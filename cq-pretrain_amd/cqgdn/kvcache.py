@@ -102,7 +102,7 @@ def read(cache, slots):
 def attend(q, cache, tables, starts, visible, *, window=None, scale=None, max_queries=None, return_lse=False):
     """Attention of the rows q [T, Hq, D] over the cached positions of their requests.
 
-    Rows starts[r] .. starts[r + 1] - 1 are request r's, whose pages are ``tables[r]``; row t sees the
+    Rows starts[r] .. starts[r + 1] - 1 (from 0 on) are request r's, whose pages are ``tables[r]``; row t sees the
     first ``visible[t]`` positions, or the last ``window`` of those.  Query head h reads key head
     h // (Hq // heads).  ``scale`` defaults to D^-0.5.  Rows that see nothing, and rows behind
     ``starts[-1]``, are zero.  Positions whose table entry names no page are not seen.

@@ -444,7 +444,7 @@ int cqgdn_kv4_read(const void* data, int64_t pages, int page, int kv_heads, int 
                    int64_t T, int dtype, void* k, void* v, void* stream);
 
 /*
- * Attention over the 4-bit pages: row t of request r (starts[r] <= t < starts[r+1]) sees the positions
+ * Attention over the 4-bit pages: row t of request r (starts[r] <= t < starts[r+1], starts[0] being 0) sees the positions
  * [max(0, visible[t] - window), visible[t]) of its request (window 0: from 0), whose pages are
  * tables[r][position / page].  out[t][h] = sum_j p_j v_j / sum_j p_j, p_j = exp(scale q k_j), query head h
  * reading key head h / (heads / kv_heads); rows that see nothing, and rows behind starts[N], are zero.
