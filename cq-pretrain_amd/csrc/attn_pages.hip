@@ -7,8 +7,8 @@
 //   it is not admitted (and, its need being counted, neither is a later one that needs pages).
 // One workgroup scans the requests, so the state (pool, tables, counts) has one writer and the result
 // does not depend on timing.  A prefix sum gives every page that moves, and every row, its request by a binary
-// search, so that all 1024 threads move them whatever the requests' sizes (64 requests, three of which return their
-// 100 pages: 15 us a page after the other, 6.6 like this): what is left is the latency of some six dependent rounds
+// search, so that all 1024 threads move them whatever the requests' sizes (64 requests, some of which return a
+// hundred pages: 15 us one after the other, 6.6 like this): what is left is the latency of some six dependent rounds
 // of memory and of the scans.  1000 requests: 10.6 us, and 4.6 for 28 thousand rows.
 #include <hip/hip_runtime.h>
 
