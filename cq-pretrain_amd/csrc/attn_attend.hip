@@ -202,7 +202,7 @@ __global__ __launch_bounds__(64 * kWaves, D == 256 ? 2 : 3) void attend_kernel(A
     f32x4 o[MT];
 #pragma unroll
     for (int i = 0; i < MT; ++i) o[i] = zero4();
-    float m = -INFINITY, l = 0.f;
+    float m = hi > 0 ? -INFINITY : 0.f, l = 0.f;
     uint32_t nan = 0;  // blocks of 32 dimensions in which the row sees a NaN value
     E* const vw = vt[wave];
 
@@ -404,7 +404,7 @@ __global__ __launch_bounds__(64 * kWaves, D == 256 ? 2 : 3) void attend_kernel(A
             y += f[w] * *reinterpret_cast<const f32x4*>(reinterpret_cast<float*>(vt[w]) + row * DC + 4 * (col ^ row));
           if (splits == 1)
             st4(static_cast<E*>(a.out) + at * D + DC * x + 4 * col, L == 0.f ? zero4() : y * (1.f / L));
-          else if (M != -INFINITY || L != 0.f)  // the join reads no part that saw nothing
+          else if (L != 0.f)  // the join reads no part that saw nothing
             *reinterpret_cast<f32x4*>(a.ws + (at * splits + s) * D + DC * x + 4 * col) = y;
         }
       }
@@ -413,7 +413,7 @@ __global__ __launch_bounds__(64 * kWaves, D == 256 ? 2 : 3) void attend_kernel(A
     if (n < rows && (late & 15) == 0) {
       if (splits > 1) {
         float* ml = a.ws + a.T * a.heads * splits * D + (at * splits + s) * 2;
-        ml[0] = M;
+        ml[0] = L == 0.f ? -INFINITY : M;
         ml[1] = L;
       } else if (a.lse) {
         a.lse[at] = (M - kAttendBias<E> + log2f(L)) * 0.693147180559945309f;
