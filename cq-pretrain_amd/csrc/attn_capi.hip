@@ -38,6 +38,13 @@ int check_rows(const char* what, int64_t T, int kv_heads, int D) {
   return CQGDN_OK;
 }
 
+// the rows of one request that a launch is made for: the caller's bound, and no fewer than the requests have on
+// average, so that a bound far too small costs neither workspace (parts of many rows) nor time
+int row_bound(int64_t T, int N, int max_queries) {
+  const int64_t bound = max_queries < T ? max_queries : T, average = N > 0 ? T / N : 1;
+  return (int)(bound > average ? bound : average);
+}
+
 }  // namespace
 
 extern "C" {
@@ -126,7 +133,7 @@ size_t cqgdn_kv4_attend_workspace_size(int64_t T, int N, int heads, int kv_heads
   if (T <= 0 || N < 0 || kv_heads <= 0 || heads <= 0 || heads % kv_heads || !dim_ok(head_dim) || max_queries <= 0 ||
       columns < 0 || !page_ok(page))
     return 0;
-  return attend_workspace_bytes(T, N, heads, kv_heads, head_dim, max_queries, (int64_t)columns * page);
+  return attend_workspace_bytes(T, N, heads, kv_heads, head_dim, row_bound(T, N, max_queries), (int64_t)columns * page);
 }
 
 int cqgdn_kv4_attend(const void* q, int64_t q_token, int64_t q_head, int dtype, int64_t T, int heads, int head_dim,
@@ -149,7 +156,7 @@ int cqgdn_kv4_attend(const void* q, int64_t q_token, int64_t q_head, int dtype, 
       q_token % 8 || q_head % 8)
     return fail(CQGDN_EINVAL, "q and out (16-byte aligned, strides multiples of 8 elements), tables, starts and "
                 "visible must be non-null");
-  const int most = (int)(max_queries < T ? max_queries : T);
+  const int most = row_bound(T, N, max_queries);
   const size_t need = attend_workspace_bytes(T, N, heads, kv_heads, head_dim, most, (int64_t)columns * page);
   if (need > 0 && (!workspace || !aligned(workspace, 256) || workspace_bytes < need))
     return fail(CQGDN_EINVAL, "workspace must be 256-byte aligned and >= cqgdn_kv4_attend_workspace_size");

@@ -452,7 +452,7 @@ int cqgdn_kv4_read(const void* data, int64_t pages, int page, int kv_heads, int 
  *   q, out      : bf16 or fp16 (dtype) [T][heads][head_dim]; q with strides in elements, multiples of 8
  *   lse         : NULL, or fp32 [T][heads]: log sum_j exp(scale q k_j), -inf for rows that see nothing
  *   max_queries : bound of the rows of one request; it sets the launch, and a larger request is served too
- *   workspace   : >= cqgdn_kv4_attend_workspace_size() bytes (with min(max_queries, T)), 256-byte aligned
+ *   workspace   : >= cqgdn_kv4_attend_workspace_size() bytes (of the same arguments), 256-byte aligned
  */
 size_t cqgdn_kv4_attend_workspace_size(int64_t T, int N, int heads, int kv_heads, int head_dim, int max_queries,
                                        int columns, int page);
