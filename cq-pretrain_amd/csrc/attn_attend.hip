@@ -545,9 +545,15 @@ Plan attend_plan(int64_t N, int kv_heads, int group, int D, int max_queries, int
   // as keep the launch within one and a half times the workgroups that are resident at once, were every request to
   // fill its table row (five ragged documents of 65536 positions, D = 256: 768 workgroups 36 us, 1024 42, 512 42; 64
   // requests of 8192, D = 128: 1024 46 us, 768 50, 2048 49); three steps a wave where every CU still has a workgroup
-  // (one request of 65536: 21 us, with one step 30)
-  const auto parts = [](int64_t positions, int64_t most, int64_t blocks, int64_t& times) {
+  // (one request of 65536: 21 us, with one step 30).  One part where it is short, because the join is a launch more:
+  // 8 requests of 450 positions 9.6 us, in two parts 13.1, of 1000 12.3 and 13.8; and where the workgroups fill the
+  // CUs already, 128 of 1700 22.6 and 26.7.
+  const auto parts = [D](int64_t positions, int64_t most, int64_t blocks, int64_t& times) {
     const int64_t least = (positions + kLeast - 1) / kLeast;
+    if (least <= (blocks >= 256 && D < 256 ? 8 : blocks >= 32 ? 5 : 3)) {
+      times = std::max<int64_t>(1, least);
+      return (int64_t)1;
+    }
     times = std::max({(int64_t)1, (least + most - 1) / most, std::min<int64_t>(3, least * blocks / 256)});
     return std::max<int64_t>(1, (least + times - 1) / times);
   };
