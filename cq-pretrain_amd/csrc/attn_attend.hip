@@ -24,6 +24,7 @@ namespace {
 constexpr int kWaves = 4;         // of a workgroup; they take its steps in turn
 constexpr int kStep = 64;         // positions of a wave's step
 constexpr int kMaxSplits = 512;
+constexpr int kPadding = 16;      // workgroups a key head for rows behind the requests'
 // Rows of a request and key head above which its positions are converted once for all of them (attn_tile.hip)
 // and not once for every 16: over 2000 positions of 64 requests 36 rows take 38 us here and 43 there, 64 rows 49
 // and 46, 128 rows 89 and 58.
@@ -129,7 +130,7 @@ __device__ __forceinline__ int max16(int x) {
   return __builtin_amdgcn_readfirstlane(max(x, turned<8>(x)));
 }
 
-// One workgroup: 16 rows of one request and key head, one of gridDim.z parts of the positions, `least` steps
+// One workgroup: 16 rows of one request and key head, one of `splits` parts of the positions, `least` steps
 // long (the last parts, which are empty where requests are shorter, come last).  The waves' steps interleave,
 // each with its own maximum, sum and O^T, and are joined at the end.  A step's codes are on their way from the
 // moment those before have been used, in registers.
@@ -144,11 +145,21 @@ __global__ __launch_bounds__(64 * kWaves, D == 256 ? 2 : 3) void attend_kernel(A
   static_assert(32 * LD * sizeof(E) >= 16 * DC * sizeof(float), "the waves' O^T pass through their value tiles");
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int r16 = lane & 15, q4 = lane >> 4;
-  const int s = blockIdx.z, splits = gridDim.z, h = blockIdx.y;
-  const int r = tiles == 1 ? blockIdx.x : blockIdx.x / tiles, tile0 = tiles == 1 ? 0 : blockIdx.x - r * tiles;
+  // The last slice of the launch is for the rows of padding behind the requests', "request N".  Were its workgroups
+  // between the others, those would meet every second XCD only where there is one request.
+  const int s = blockIdx.z, splits = gridDim.z - 1, h = blockIdx.y;
+  const bool padding = s == splits;
+  if (padding && blockIdx.x >= kPadding) return;
+  // Workgroups go to the XCDs in turn: where the requests are a multiple of some power of two, each would meet the
+  // same XCDs with all its heads and parts, the longest too.  Their low bits are turned within that power.
+  const int turn = (h + s) & (((int)gridDim.x & -(int)gridDim.x) - 1) & 7, x = padding ? blockIdx.x : blockIdx.x ^ turn;
+  const int r = padding ? a.N : tiles == 1 ? x : x / tiles;
+  const int tile0 = padding ? x : tiles == 1 ? 0 : x - r * tiles;
+  if (!padding && r >= a.N) return;
+  if (padding) tiles = min((int)gridDim.x, kPadding);
   const int T = (int)a.T, group = a.group.d;
   const int from = r == 0 ? 0 : min(max(a.starts[r], 0), T);
-  const int to = r == a.N ? T : min(max(a.starts[r + 1], from), T);  // request N: the padding behind the last
+  const int to = padding ? T : min(max(a.starts[r + 1], from), T);
   const int rows = (to - from) * group, size = 1 << a.page_shift;
   const int room = (int)min((int64_t)a.columns << a.page_shift, (int64_t)INT32_MAX - 1024);
   const uint8_t* const head_base = a.data + (int64_t)h * kv4_page_bytes(size, D);
@@ -190,12 +201,13 @@ __global__ __launch_bounds__(64 * kWaves, D == 256 ? 2 : 3) void attend_kernel(A
     // with a window the rows' limits may lie further apart than the launch was made for: longer parts then
     const int per = max(least, ((steps + splits - 1) / splits + kWaves - 1) & ~(kWaves - 1));
     const int stop = min(steps, (s + 1) * per);
-    if (s > 0 && s * per >= steps) {  // nothing of it here: only the join hears of this part
-      if (tid < 16 && real) {
-        float* ml = a.ws + a.T * a.heads * splits * D + (((int64_t)t * a.heads + head) * splits + s) * 2;
-        ml[0] = -INFINITY;
-        ml[1] = 0.f;
-      }
+    if (padding ? splits > 1 : s > 0 && s * per >= steps) {  // nothing here: only the join hears of it
+      if (tid < 16 && real)
+        for (int part = padding ? 0 : s; part < (padding ? splits : s + 1); ++part) {
+          float* ml = a.ws + a.T * a.heads * splits * D + (((int64_t)t * a.heads + head) * splits + part) * 2;
+          ml[0] = -INFINITY;
+          ml[1] = 0.f;
+        }
       continue;
     }
 
@@ -573,7 +585,8 @@ void launch_dim(const AttendArgs& a, hipStream_t st) {
     const int64_t each = (int64_t)(a.N + 1) * a.kv_heads * p.splits;
     const int tiles = (int)std::max<int64_t>(1, std::min<int64_t>(((int64_t)a.max_queries * group + 15) / 16, (1 << 23) / each));
     // a workgroup takes every tiles-th tile: none is left out whatever the bound
-    attend_kernel<E, D><<<dim3((unsigned)((a.N + 1) * tiles), a.kv_heads, p.splits), 64 * kWaves, 0, st>>>(a, tiles, p.per);
+    const dim3 grid((unsigned)std::max<int64_t>(1, (int64_t)a.N * tiles), a.kv_heads, p.splits + 1);
+    attend_kernel<E, D><<<grid, 64 * kWaves, 0, st>>>(a, tiles, p.per);
   }
   if (p.splits > 1) {
     // 2048 rows of 33 MB in two parts: 60 us by the kernel for few rows; 32 rows in 36 parts: 4 us by it

@@ -89,17 +89,25 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : D == 64 ? 3 : 2) void tile_kern
   const int n32 = lane & 31, kg = lane >> 5;
   // Launch order: a request's last tiles, which see most, first; every other round of 256 workgroups (one a
   // CU) reversed, so that a CU's workgroups add up to the same
-  const int each = a.kv_heads * (a.N + 1) * splits;
+  // The rows of padding behind the requests', "request N", come last: among the others, their workgroups would
+  // leave some XCDs with less.
+  const int each = a.kv_heads * a.N * splits, real_blocks = each * tiles;
   int b = blockIdx.x;
-  if ((b >> 8 & 1) && (b | 255) < (int)gridDim.x) b ^= 255;
-  const int tile0 = tiles - 1 - b / each;
-  b %= each;
-  const int s = b % splits;
-  b /= splits;
-  const int h = b % a.kv_heads, r = b / a.kv_heads;
+  const bool padding = b >= real_blocks;
+  if (padding)
+    b -= real_blocks;
+  else if ((b >> 8 & 1) && (b | 255) < real_blocks)
+    b ^= 255;
+  const int heads_each = padding ? a.kv_heads : each;
+  const int tile0 = padding ? b / heads_each : tiles - 1 - b / heads_each;
+  b %= heads_each;
+  const int s = padding ? 0 : b % splits;
+  if (!padding) b /= splits;
+  const int h = b % a.kv_heads, r = padding ? a.N : b / a.kv_heads;
+  if (padding) tiles = (gridDim.x - real_blocks) / a.kv_heads;
   const int group = a.group.d, T = (int)a.T;
   const int from = r == 0 ? 0 : min(max(a.starts[r], 0), T);
-  const int to = r == a.N ? T : min(max(a.starts[r + 1], from), T);  // request N: the padding behind the last
+  const int to = padding ? T : min(max(a.starts[r + 1], from), T);
   const int rows = (to - from) * group, size = 1 << a.page_shift;
   const int room = (int)min((int64_t)a.columns << a.page_shift, (int64_t)INT32_MAX - 1024);
   const int token = tid / PV, piece = tid % PV;  // the thread's part of a step
@@ -402,9 +410,11 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : D == 64 ? 3 : 2) void tile_kern
       }
       if (kg == 0) {
         if (splits > 1) {
-          float* ml = a.ws + a.T * a.heads * splits * D + (at * splits + s) * 2;
-          ml[0] = l == 0.f ? -INFINITY : m;
-          ml[1] = l;
+          for (int part = s; part < (padding ? splits : s + 1); ++part) {
+            float* ml = a.ws + a.T * a.heads * splits * D + (at * splits + part) * 2;
+            ml[0] = l == 0.f ? -INFINITY : m;
+            ml[1] = l;
+          }
         } else if (a.lse) {
           a.lse[at] = (m - bias + log2f(l)) * 0.693147180559945309f;
         }
@@ -416,10 +426,11 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : D == 64 ? 3 : 2) void tile_kern
 
 template <class E, int D>
 void launch_dim(const AttendArgs& a, int splits, hipStream_t st) {
-  const int64_t each = (int64_t)(a.N + 1) * a.kv_heads * splits;
+  const int64_t each = std::max<int64_t>(1, (int64_t)a.N * a.kv_heads * splits);
   const int64_t wanted = ((int64_t)a.max_queries * (a.heads / a.kv_heads) + kRows - 1) / kRows;
   const int tiles = (int)std::max<int64_t>(1, std::min<int64_t>(wanted, (1 << 23) / each));
-  tile_kernel<E, D><<<(unsigned)(each * tiles), 256, 0, st>>>(a, tiles, splits);
+  const int64_t blocks = (int64_t)a.N * a.kv_heads * splits * tiles + (int64_t)a.kv_heads * std::min(tiles, 16);
+  tile_kernel<E, D><<<(unsigned)blocks, 256, 0, st>>>(a, tiles, splits);
 }
 
 template <class E>

@@ -108,6 +108,36 @@ def test_rows_that_begin_to_see_at_different_steps(ops, rows, D):
     assert torch.equal(out[sees][..., 32:], good[sees][..., 32:]) and bool(torch.isnan(out[sees][..., :32]).all())
 
 
+@pytest.mark.parametrize("lengths,news,pad,D", [
+    ([3000], [1], 11, 128),                # single tokens, positions in parts
+    ([300] * 8, [1] * 8, 1, 64),           # in one part
+    ([300] * 32, [1] * 32, 320, 64),       # more rows of padding than of requests
+    ([3000], [1], 500, 128),               # so many that the launch is for many rows
+    ([300, 20, 7], [1, 0, 1], 700, 256),
+    ([2100], [70], 300, 128),              # many rows, in parts
+    ([200] * 12, [64] * 12, 2000, 64),     # and in one
+    ([], [], 90, 128),                     # nothing but padding
+    ([], [], 1, 128),
+])
+def test_rows_behind_the_requests(ops, lengths, news, pad, D):
+    """Zero and -inf, and the requests' rows hold beside them."""
+    n, rows, hq, hk = len(lengths), sum(news), 8, 2
+    cache, tables, starts, q, k, v = _attend_case(ops, lengths or [16], news or [1], hq, hk, D, 16, "bf16", seed=pad)
+    tables, starts, q = (tables, starts, q) if n else (tables[:0], [0], q[:0])
+    more = torch.cat([q, torch.full((pad, hq, D), math.nan, dtype=q.dtype)]).to(DEV)
+    visible = i32(_causal(lengths, news) + [7] * pad)
+    junk = [torch.full(s, 3.0, dtype=t, device=DEV) for s, t in ((more.shape, q.dtype), (more.shape[:2], torch.float32))]
+    del junk  # what new tensors hold is nobody's zeros
+    out, lse = ops.kv.attend(more, cache, tables.to(DEV), i32(starts), visible, max_queries=max(news, default=1),
+                             return_lse=True)
+    assert bool((out[rows:] == 0).all()) and bool((lse[rows:] == -math.inf).all())
+    if n:
+        same, lse2 = ops.kv.attend(q.to(DEV), cache, tables.to(DEV), i32(starts), visible[:rows], max_queries=max(news),
+                                   return_lse=True)
+        _attend_check(out[:rows], lse[:rows], q, k, v, starts, _causal(lengths, news), D ** -0.5, 0)
+        _attend_check(same, lse2, q, k, v, starts, _causal(lengths, news), D ** -0.5, 0)
+
+
 def test_a_row_does_not_depend_on_the_rows_beside_it(ops):
     """The same row alone in its call and among others of its request, by the same kernel."""
     length = 900
