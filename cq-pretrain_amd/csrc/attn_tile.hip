@@ -7,7 +7,7 @@
 // (and its partner 32 lanes on) owns a row: limits, maximum and sum stay in its registers, and S^T's layout
 // is already an operand of O^T.
 //
-// 4096 rows over 8192 positions (16 heads of 128, 4 key heads): 214 us, 965 TFLOP/s; the library's largest products
+// 4096 rows over 8192 positions (16 heads of 128, 4 key heads): 216 us, 955 TFLOP/s; the library's largest products
 // reach 1486.  A step of 32 rows and 64 positions is 32 MFMAs (1024 cycles of the matrix core, each of which keeps the
 // SIMD's issue 16 cycles), some 195 VALU instructions, 32 of them exponentials of 8 cycles, and 270 cycles of LDS, which
 // eight waves of a CU share: no one of them fills the time, and left out of a copy each takes 7 to 17% with it.
@@ -90,7 +90,7 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : D == 64 ? 3 : 2) void tile_kern
   // Launch order: a request's last tiles, which see most, first; every other round of 256 workgroups (one a
   // CU) reversed, so that a CU's workgroups add up to the same
   // The rows of padding behind the requests', "request N", come last: among the others, their workgroups would
-  // leave some XCDs with less.
+  // leave some XCDs with less (prefill of one request 238 us against 229, seven ragged prompts 83 against 75).
   const int each = a.kv_heads * a.N * splits, real_blocks = each * tiles;
   int b = blockIdx.x;
   const bool padding = b >= real_blocks;
