@@ -25,8 +25,6 @@ from pathlib import Path
 
 import torch
 
-sys.path.insert(0, str(Path(__file__).resolve().parents[1] / "cq-pretrain_amd"))
-
 own = False  # True: run() calls the framework's operators
 
 DEV = "cuda"
@@ -438,6 +436,9 @@ def own_attend(s):
 def run(state):
     kind = state["case"]["kind"]
     if own:
+        package = str(Path(__file__).resolve().parents[1] / "cq-pretrain_amd")
+        if package not in sys.path:
+            sys.path.insert(0, package)
         return dict(rotary=own_rotary, pages=own_pages, write=own_write, attend=own_attend)[kind](state)
     return dict(rotary=plain_rotary, pages=plain_pages, write=plain_write, attend=plain_attend)[kind](state)
 
