@@ -23,7 +23,7 @@ namespace {
 
 constexpr int kWaves = 4;         // of a workgroup; they take its steps in turn
 constexpr int kStep = 64;         // positions of a wave's step
-constexpr int kMaxSplits = 512;
+constexpr int kMaxSplits = 512;   // parts of a call by either kernel, which the join holds the weights of
 constexpr int kPadding = 16;      // workgroups a key head for rows behind the requests'
 // Rows of a request and key head above which its positions are converted once for all of them (attn_tile.hip)
 // and not once for every 16: over 2000 positions of 64 requests 36 rows take 38 us here and 43 there, 64 rows 49
@@ -551,7 +551,8 @@ Plan attend_plan(int64_t N, int kv_heads, int group, int D, int max_queries, int
     // as many parts as give the CUs the workgroups that their registers hold, each of at least 512 positions
     const int64_t blocks = N * kv_heads * ((rows + 127) / 128), fit = D == 256 ? 256 : D == 64 ? 768 : 512;
     if (window > 0) seen = std::min<int64_t>(capacity, (int64_t)window + 128 / group + 64);
-    return {true, (int)std::max<int64_t>(1, std::min<int64_t>(seen / 512, fit / std::max<int64_t>(blocks, 1))), 0};
+    const int64_t most = std::min<int64_t>(kMaxSplits, fit / std::max<int64_t>(blocks, 1));
+    return {true, (int)std::max<int64_t>(1, std::min<int64_t>(seen / 512, most)), 0};
   }
   const int64_t resident = D == 256 ? 512 : D == 128 ? 768 : 1024;
   constexpr int64_t kLeast = kWaves * kStep;

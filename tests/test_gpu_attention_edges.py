@@ -1,0 +1,21 @@
+"""Where the attention over the 4-bit pages once gave a wrong answer, held against the plain 64-bit form.
+Tolerances are those of test_gpu_attention.py, from the roundings of the weights and of the result."""
+
+import pytest
+import torch
+
+from test_gpu_attention import DEV, _attend_case, _attend_check, i32, ops  # noqa: F401
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.mark.parametrize("D,length", [(64, 49152), (64, 40001), (128, 49152)])
+def test_many_rows_over_a_table_of_many_parts(ops, D, length):
+    """64 rows of one key head over a table of 393216 positions: no more parts than the join reads, all of which
+    hold positions that count."""
+    cache, tables, starts, q, k, v = _attend_case(ops, [length], [4], 16, 1, D, 16, "bf16", seed=D)
+    wide = torch.full((1, 24576), -1, dtype=torch.int32)
+    wide[:, :tables.shape[1]] = tables
+    visible = [length - 3 + i for i in range(4)]
+    out, lse = ops.kv.attend(q.to(DEV), cache, wide.to(DEV), i32(starts), i32(visible), max_queries=4, return_lse=True)
+    _attend_check(out, lse, q, k, v, starts, visible, D ** -0.5)
