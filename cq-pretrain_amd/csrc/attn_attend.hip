@@ -17,18 +17,12 @@
 
 #include "attn_kernels.hpp"
 #include "attn_kv4.hpp"
+#include "attn_plan.hpp"
 
 namespace cqgdn {
 namespace {
 
-constexpr int kWaves = 4;         // of a workgroup; they take its steps in turn
-constexpr int kStep = 64;         // positions of a wave's step
-constexpr int kMaxSplits = 512;   // parts of a call by either kernel, which the join holds the weights of
-constexpr int kPadding = 16;      // workgroups a key head for rows behind the requests'
-// Rows of a request and key head above which its positions are converted once for all of them (attn_tile.hip)
-// and not once for every 16: over 2000 positions of 64 requests 36 rows take 38 us here and 43 there, 64 rows 49
-// and 46, 128 rows 89 and 58.
-constexpr int kFewRows = 48;
+constexpr int kPadding = 16;  // workgroups a key head for rows behind the requests'
 
 // The pages of a step's four 16 positions, the same for all lanes.  An entry that names no page reads as zeros
 // (its buffer has no bytes), and its positions are hidden.
@@ -163,7 +157,7 @@ __global__ __launch_bounds__(64 * kWaves, D == 256 ? 2 : 3) void attend_kernel(A
   const int from = r == 0 ? 0 : min(max(a.starts[r], 0), T);
   const int to = padding ? T : min(max(a.starts[r + 1], from), T);
   const int rows = (to - from) * group, size = 1 << a.page_shift;
-  const int room = (int)min((int64_t)a.columns << a.page_shift, (int64_t)INT32_MAX - 1024);
+  const int room = (int)min((int64_t)a.columns << a.page_shift, (int64_t)kAttendRoom);
   const uint8_t* const head_base = a.data + (int64_t)h * kv4_page_bytes(size, D);
   const uint64_t stride = (uint64_t)a.kv_heads * kv4_page_bytes(size, D);
   // the exponent's factor, never 0: a masked score stays -infinity; its sign goes with Q
@@ -538,50 +532,10 @@ __global__ __launch_bounds__(256) void join_kernel(AttendArgs a, int splits) {
   if (a.lse && tid == 0 && d0 == 0) a.lse[at] = (M - kAttendBias<E> + log2f(L)) * 0.693147180559945309f;
 }
 
-// How a call runs: by which kernel, and in how many parts of the positions, of `per` steps each (decode).
-struct Plan {
-  bool tiles;
-  int splits, per;
-};
-// `capacity` positions a table row holds; with a window a row sees no more of them than it, and never more parts.
-Plan attend_plan(int64_t N, int kv_heads, int group, int D, int max_queries, int64_t capacity, int window) {
-  const int64_t rows = (int64_t)max_queries * group;
-  int64_t seen = window > 0 ? std::min(capacity, (int64_t)window + max_queries + kStep) : capacity;
-  if (rows > kFewRows) {
-    // as many parts as give the CUs the workgroups that their registers hold, each of at least 512 positions
-    const int64_t blocks = N * kv_heads * ((rows + 127) / 128), fit = D == 256 ? 256 : D == 64 ? 768 : 512;
-    if (window > 0) seen = std::min<int64_t>(capacity, (int64_t)window + 128 / group + 64);
-    const int64_t most = std::min<int64_t>(kMaxSplits, fit / std::max<int64_t>(blocks, 1));
-    return {true, (int)std::max<int64_t>(1, std::min<int64_t>(seen / 512, most)), 0};
-  }
-  const int64_t resident = D == 256 ? 512 : D == 128 ? 768 : 1024;
-  constexpr int64_t kLeast = kWaves * kStep;
-  // Parts of the same length, so that ragged requests load the CUs alike: a step a wave at the least, and as long
-  // as keep the launch within one and a half times the workgroups that are resident at once, were every request to
-  // fill its table row (five ragged documents of 65536 positions, D = 256: 768 workgroups 36 us, 1024 42, 512 42; 64
-  // requests of 8192, D = 128: 1024 46 us, 768 50, 2048 49); three steps a wave where every CU still has a workgroup
-  // (one request of 65536: 21 us, with one step 30).  One part where it is short, because the join is a launch more:
-  // 8 requests of 450 positions 9.6 us, in two parts 13.1, of 1000 12.3 and 13.8; and where the workgroups fill the
-  // CUs already, 128 of 1700 22.6 and 26.7.
-  const auto parts = [D](int64_t positions, int64_t most, int64_t blocks, int64_t& times) {
-    const int64_t least = (positions + kLeast - 1) / kLeast;
-    if (least <= (blocks >= 256 && D < 256 ? 8 : blocks >= 32 ? 5 : 3)) {
-      times = std::max<int64_t>(1, least);
-      return (int64_t)1;
-    }
-    times = std::max({(int64_t)1, (least + most - 1) / most, std::min<int64_t>(3, least * blocks / 256)});
-    return std::max<int64_t>(1, (least + times - 1) / times);
-  };
-  const int64_t blocks = std::max<int64_t>(1, N * kv_heads * ((rows + 15) / 16));
-  int64_t times, splits = parts(capacity, std::min<int64_t>(kMaxSplits, std::max<int64_t>(1, resident * 3 / 2 / blocks)), blocks, times);
-  if (window > 0) splits = parts(seen, splits, blocks, times);
-  return {false, (int)splits, (int)(times * kWaves)};
-}
-
 template <class E, int D>
 void launch_dim(const AttendArgs& a, hipStream_t st) {
   const int group = a.heads / a.kv_heads;
-  const Plan p = attend_plan(a.N, a.kv_heads, group, D, a.max_queries, (int64_t)a.columns << a.page_shift, a.window);
+  const AttendPlan p = attend_plan(a.N, a.kv_heads, group, D, a.max_queries, (int64_t)a.columns << a.page_shift, a.window);
   if (p.tiles) {
     launch_attend_tiles(a, p.splits, st);
   } else {

@@ -17,6 +17,7 @@
 
 #include "attn_kernels.hpp"
 #include "attn_kv4.hpp"
+#include "attn_plan.hpp"
 
 namespace cqgdn {
 namespace {
@@ -109,7 +110,7 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : D == 64 ? 3 : 2) void tile_kern
   const int from = r == 0 ? 0 : min(max(a.starts[r], 0), T);
   const int to = padding ? T : min(max(a.starts[r + 1], from), T);
   const int rows = (to - from) * group, size = 1 << a.page_shift;
-  const int room = (int)min((int64_t)a.columns << a.page_shift, (int64_t)INT32_MAX - 1024);
+  const int room = (int)min((int64_t)a.columns << a.page_shift, (int64_t)kAttendRoom);
   const int token = tid / PV, piece = tid % PV;  // the thread's part of a step
   const uint8_t* const head_base = a.data + (int64_t)h * kv4_page_bytes(size, D);
   const uint64_t stride = (uint64_t)a.kv_heads * kv4_page_bytes(size, D);

@@ -19,3 +19,15 @@ def test_many_rows_over_a_table_of_many_parts(ops, D, length):
     visible = [length - 3 + i for i in range(4)]
     out, lse = ops.kv.attend(q.to(DEV), cache, wide.to(DEV), i32(starts), i32(visible), max_queries=4, return_lse=True)
     _attend_check(out, lse, q, k, v, starts, visible, D ** -0.5)
+
+
+@pytest.mark.parametrize("heads,rows", [(2, 1), (2, 60)])
+def test_a_table_row_of_more_than_32_bits_of_positions(ops, heads, rows):
+    """40000 columns of pages of 65536 positions, of which a request uses two."""
+    length, page, D = 70000, 65536, 64
+    cache, tables, starts, q, k, v = _attend_case(ops, [length], [rows], heads, 1, D, page, "bf16")
+    wide = torch.full((1, 40000), -1, dtype=torch.int32)
+    wide[:, :tables.shape[1]] = tables
+    visible = [length - rows + 1 + i for i in range(rows)]
+    out, lse = ops.kv.attend(q.to(DEV), cache, wide.to(DEV), i32(starts), i32(visible), max_queries=rows, return_lse=True)
+    _attend_check(out, lse, q, k, v, starts, visible, D ** -0.5)
