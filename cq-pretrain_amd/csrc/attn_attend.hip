@@ -24,8 +24,8 @@ namespace {
 
 constexpr int kPadding = 16;  // workgroups a key head for rows behind the requests'
 
-// The pages of a step's four 16 positions, the same for all lanes.  An entry that names no page reads as zeros
-// (its buffer has no bytes), and its positions are hidden.
+// The pages of a step's four 16 positions, the same for all lanes.  An entry that names no page reads as zeros (its
+// buffer has no bytes, and takes no scalar offset: buf_rsrc's rule), and its positions are hidden.
 struct Pages {
   const uint8_t* base[4];
   int shown;  // a bit each
@@ -33,6 +33,8 @@ struct Pages {
   __device__ __forceinline__ __amdgpu_buffer_rsrc_t page(int g, int size) const {
     return buf_rsrc(base[g], shown >> g & 1 ? kv4_page_bytes(size, D) : 0);
   }
+  // the scalar offset of a place in page g
+  __device__ __forceinline__ int place(int g, int offset) const { return shown >> g & 1 ? offset : 0; }
 };
 
 // The codes of a step's keys and their scale bytes.  Lane (r16, q4) holds key r16 of each 16: 16 bytes from
@@ -50,7 +52,8 @@ __device__ __forceinline__ void load_keys(Keys<D>& c, const Pages& p, int pos, i
   const int r16 = lane & 15, q4 = lane >> 4;
 #pragma unroll
   for (int g = 0; g < 4; ++g) {
-    const int at = (pos + 16 * g) & (size - 1), codes = at * (D / 2), scales = size * D + at * (D / 32);
+    const int at = (pos + 16 * g) & (size - 1);
+    const int codes = p.place(g, at * (D / 2)), scales = p.place(g, size * D + at * (D / 32));
     const __amdgpu_buffer_rsrc_t rs = p.template page<D>(g, size);
 #pragma unroll
     for (int x = 0; x < Keys<D>::XK; ++x) {
@@ -85,7 +88,8 @@ __device__ __forceinline__ void load_values(Values<D>& c, const Pages& p, int po
 #pragma unroll
     for (int j = 0; j < V::J; ++j) {
       const int g = 2 * half + j, at = (pos + 16 * g) & (size - 1);
-      const int codes = size * (D / 2) + at * (D / 2), scales = size * D + size * (D / 32) + at * (D / 32);
+      const int codes = p.place(g, size * (D / 2) + at * (D / 2));
+      const int scales = p.place(g, size * D + size * (D / 32) + at * (D / 32));
 #pragma unroll
       for (int x = 0; x < D / V::DC; ++x) {
         if constexpr (D >= 128) {
@@ -94,13 +98,14 @@ __device__ __forceinline__ void load_values(Values<D>& c, const Pages& p, int po
         } else {
           // 32 positions a load, which two pages may hold: a lane's offset lies beyond the one that is not its own
           const int at1 = (pos + 16 * g + 16) & (size - 1), none = 1 << 30;
+          const int codes1 = p.place(g + 1, size * (D / 2) + at1 * (D / 2));
+          const int scales1 = p.place(g + 1, size * D + size * (D / 32) + at1 * (D / 32));
           const int lo = lane < 32 ? lane * 16 : none, hi = lane < 32 ? none : (lane - 32) * 16;
           const int slo = lane < 32 ? lane : none, shi = lane < 32 ? none : lane - 32;
           c.w[x][half][j] = buf_ld16<u32x4>(p.template page<D>(g, size), lo, codes) |
-                            buf_ld16<u32x4>(p.template page<D>(g + 1, size), hi, size * (D / 2) + at1 * (D / 2));
+                            buf_ld16<u32x4>(p.template page<D>(g + 1, size), hi, codes1);
           c.s[x][half][j] = __builtin_amdgcn_raw_buffer_load_b8(p.template page<D>(g, size), slo, scales, 0) |
-                            __builtin_amdgcn_raw_buffer_load_b8(p.template page<D>(g + 1, size), shi,
-                                                                size * D + size * (D / 32) + at1 * (D / 32), 0);
+                            __builtin_amdgcn_raw_buffer_load_b8(p.template page<D>(g + 1, size), shi, scales1, 0);
         }
       }
     }

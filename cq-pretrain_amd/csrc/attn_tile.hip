@@ -197,8 +197,9 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : D == 64 ? 3 : 2) void tile_kern
       const bool ok = page < a.page_count;
       const __amdgpu_buffer_rsrc_t rs = buf_rsrc(head_base + (ok ? page * stride : 0), ok ? kv4_page_bytes(size, D) : 0);
       const int at = (pos0 + j * TOK + wave * WAVE_POS) & (size - 1);
-      kn = fetch<D>(rs, code, at * (D / 2), scale, size * D + at * (D / 32));
-      vn = fetch<D>(rs, code, (size + at) * (D / 2), scale, size * D + (size + at) * (D / 32));
+      const auto place = [&](int offset) { return ok ? offset : 0; };  // scalar: buf_rsrc's rule
+      kn = fetch<D>(rs, code, place(at * (D / 2)), scale, place(size * D + at * (D / 32)));
+      vn = fetch<D>(rs, code, place((size + at) * (D / 2)), scale, place(size * D + (size + at) * (D / 32)));
       return (int)__ballot((uint32_t)table < a.page_count) & ((1 << GROUPS) - 1);
     };
     // those codes become step j's K and V tiles, PARTS parts of each.  Where the step reaches beyond what the

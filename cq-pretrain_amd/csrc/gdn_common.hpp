@@ -444,7 +444,9 @@ __device__ __forceinline__ __amdgpu_buffer_rsrc_t chunk_rows_rsrc(E* base, int s
   return __builtin_amdgcn_make_buffer_rsrc(base + ((size_t)start * H + h) * D, (short)0, (len - 1) * H * D * 2 + D * 2,
                                            0x00020000);
 }
-// a raw buffer resource over ``bytes`` bytes from ``base``
+// a raw buffer resource over ``bytes`` bytes from ``base``.  Its range check turns a lane away (loads give 0) where the
+// lane's offset >= bytes - scalar offset.  That difference wraps around below 0, so a scalar offset never passes the
+// size, and a resource of no bytes takes none.
 __device__ __forceinline__ __amdgpu_buffer_rsrc_t buf_rsrc(const void* base, int bytes) {
   return __builtin_amdgcn_make_buffer_rsrc(const_cast<void*>(base), (short)0, bytes, 0x00020000);
 }

@@ -31,3 +31,24 @@ def test_a_table_row_of_more_than_32_bits_of_positions(ops, heads, rows):
     visible = [length - rows + 1 + i for i in range(rows)]
     out, lse = ops.kv.attend(q.to(DEV), cache, wide.to(DEV), i32(starts), i32(visible), max_queries=rows, return_lse=True)
     _attend_check(out, lse, q, k, v, starts, visible, D ** -0.5)
+
+
+@pytest.mark.parametrize("D", [64, 128, 256])
+@pytest.mark.parametrize("rows", [1, 60])
+def test_entries_that_name_no_page_read_no_page(ops, rows, D):
+    """Hidden pages between the others, at a tile's ends and behind the limit, while the cache's first page (which no
+    table names) is NaN in every block: nothing of it arrives."""
+    cache, tables, starts, q, k, v = _attend_case(ops, [400], [rows], 4, 1, D, 16, "bf16", seed=rows + D)
+    data = torch.cat((torch.full_like(cache.data[:1], 255), cache.data))
+    cache = ops.kv.KVCache(data, page=16, head_dim=D)
+    tables = torch.where(tables >= 0, tables + 1, -1)
+    hidden = torch.zeros(1, 400, dtype=torch.bool)
+    for c, entry in ((0, -1), (1, cache.pages), (5, 2 ** 31 - 1), (7, -1), (8, -2 ** 31), (17, -1), (24, -1)):
+        tables[0, c] = entry
+        hidden[0, 16 * c:16 * c + 16] = True
+    for limit in (400, 393, 272, 96, 40, 32):
+        visible = [max(0, limit - i % 3) for i in range(rows)]
+        for window in (0, 90):
+            out, lse = ops.kv.attend(q.to(DEV), cache, tables.to(DEV), i32(starts), i32(visible), window=window or None,
+                                     max_queries=rows, return_lse=True)
+            _attend_check(out, lse, q, k, v, starts, visible, D ** -0.5, window, hidden)
