@@ -191,8 +191,8 @@ __global__ __launch_bounds__(64 * kWaves, D == 256 ? 2 : 3) void attend_kernel(A
     };
     // without a window the part's first positions, and with them its pages, are known before the rows' limits
     const int early = a.window <= 0 && r < a.N ? entries((s * least + wave) * kStep) : -1;
-    const int hi = real && r < a.N ? min(max(a.visible[t], 0), room) : 0;
-    const int lo = a.window > 0 ? max(0, hi - a.window) : 0;
+    int lo, hi;
+    attend_limits(real && r < a.N ? a.visible[t] : 0, a.window, room, lo, hi);
     // over the rows that see anything: from the first position any of them sees to the last, and the
     // range that all of them see, where nothing is masked
     const int first = min16(hi > 0 ? lo : INT32_MAX), last = max16(hi);

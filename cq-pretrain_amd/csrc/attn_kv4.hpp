@@ -43,6 +43,15 @@ constexpr float kAttendBias = std::is_same<E, f16>::value ? 7.f : 8.f;
 template <class E>
 constexpr float kAttendLimit = std::is_same<E, f16>::value ? 60000.f : 16777216.f;
 
+// The positions [lo, hi) that a row with the limit `visible` sees of the `room` that its table holds, [0, 0) for
+// none.  The window is counted from the limit, which may lie beyond the table.
+__device__ __forceinline__ void attend_limits(int visible, int window, int room, int& lo, int& hi) {
+  const int limit = max(visible, 0);
+  lo = window > 0 ? max(0, limit - window) : 0;
+  hi = min(limit, room);
+  if (lo >= hi) lo = hi = 0;
+}
+
 // The entry of the block table that holds position pos, -1 outside the table
 __device__ __forceinline__ int page_of(const AttendArgs& a, int r, int pos) {
   const int column = pos >> a.page_shift;

@@ -130,8 +130,7 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : D == 64 ? 3 : 2) void tile_kern
 
   for (int tile = tile0; tile * kRows < rows; tile += tiles) {
     const auto limits = [&](int rho, int& lo, int& hi) {
-      hi = rho < rows && r < a.N ? min(max(a.visible[from + a.group.of(rho)], 0), room) : 0;
-      lo = a.window > 0 ? max(0, hi - a.window) : 0;
+      attend_limits(rho < rows && r < a.N ? a.visible[from + a.group.of(rho)] : 0, a.window, room, lo, hi);
     };
     // what the workgroup's rows see together
     int first, last;

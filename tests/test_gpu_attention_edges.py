@@ -52,3 +52,21 @@ def test_entries_that_name_no_page_read_no_page(ops, rows, D):
             out, lse = ops.kv.attend(q.to(DEV), cache, tables.to(DEV), i32(starts), i32(visible), window=window or None,
                                      max_queries=rows, return_lse=True)
             _attend_check(out, lse, q, k, v, starts, visible, D ** -0.5, window, hidden)
+
+
+@pytest.mark.parametrize("rows", [1, 60])
+@pytest.mark.parametrize("window", [1, 20, 1000])
+def test_a_window_whose_limit_lies_beyond_the_table(ops, rows, window):
+    """A row sees the last `window` of its first `visible` positions; those beyond the table are among them and are
+    not seen, so the window's other end moves with the limit."""
+    length = 160
+    cache, tables, starts, q, k, v = _attend_case(ops, [length] * 6, [rows] * 6, 4, 2, 128, 16, "bf16", extra_columns=0)
+    hidden = torch.zeros(6, 2048, dtype=torch.bool)
+    hidden[:, length:] = True
+    more = torch.zeros(6, 2048, 2, 128, dtype=torch.float64)
+    kw, vw = more.clone(), more.clone()
+    kw[:, :length], vw[:, :length] = k, v
+    visible = [x for x in (length, length + 1, length + 7, length + 20, 2000, 2 ** 31 - 1) for _ in range(rows)]
+    out, lse = ops.kv.attend(q.to(DEV), cache, tables.to(DEV), i32(starts), i32(visible), window=window, max_queries=rows,
+                             return_lse=True)
+    _attend_check(out, lse, q, kw, vw, starts, visible, 128 ** -0.5, window, hidden)
