@@ -33,15 +33,16 @@ __device__ __forceinline__ f16x8 kv4_values<f16>(uint32_t code, float scale) {
 
 // ---- shared by the attention kernels ----------------------------------------------------------------
 // The maximum of a row's scores that its weights are taken against need not be the exact one.  It is taken from
-// the first positions that the row sees, and moves only where a lane's weights of a step sum to more than
-// kAttendLimit: with fp16 a weight may pass the largest number there (65504), with bf16 nothing is near its
-// end.  P is held 2^bias higher because v_exp_f32 drops results below 2^-126 and fp16 keeps 2^-24 at the least:
+// the first positions that the row sees, and moves only where a lane's 16 weights of a step sum to more than
+// kAttendLimit.  With fp16 a weight may pass the largest number there (65504).  With bf16 the limit bounds the sums
+// of n positions by n 2^12 times the largest value (n times it bounds any softmax's sum before the division), so
+// that values up to 2^100 meet no overflow over 2^16 positions, up to 2^84 over any number.
+// P is held 2^bias higher because v_exp_f32 drops results below 2^-126 and fp16 keeps 2^-24 at the least:
 // weights down to 2^-134 of the maximum count with bf16 (whose results reach 2^-126), down to 2^-31 with fp16.
-// Values up to 2^100 meet no overflow.
 template <class E>
 constexpr float kAttendBias = std::is_same<E, f16>::value ? 7.f : 8.f;
 template <class E>
-constexpr float kAttendLimit = std::is_same<E, f16>::value ? 60000.f : 16777216.f;
+constexpr float kAttendLimit = std::is_same<E, f16>::value ? 60000.f : 65536.f;
 
 // The positions [lo, hi) that a row with the limit `visible` sees of the `room` that its table holds, [0, 0) for
 // none.  The window is counted from the limit, which may lie beyond the table.

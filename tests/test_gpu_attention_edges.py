@@ -70,3 +70,29 @@ def test_a_window_whose_limit_lies_beyond_the_table(ops, rows, window):
     out, lse = ops.kv.attend(q.to(DEV), cache, tables.to(DEV), i32(starts), i32(visible), window=window, max_queries=rows,
                              return_lse=True)
     _attend_check(out, lse, q, kw, vw, starts, visible, 128 ** -0.5, window, hidden)
+
+
+@pytest.mark.parametrize("requests,rows", [(256, 1), (1, 64)])
+def test_large_values_under_scores_that_rise(ops, requests, rows):
+    """Values of 2^100, and scores that lie 2^10 in weight above the first positions': the running sums stay
+    finite, whatever maximum the weights are taken against."""
+    length, D = 2048, 128
+    cache, tables, _, _, k, v = _attend_case(ops, [length], [1], 1, 1, D, 64, "bf16", seed=3, extra_columns=0)
+    kr, vr = torch.zeros(length, 1, D), torch.full((length, 1, D), 2.0 ** 100)
+    kr[:, :, 0] = torch.where(torch.arange(length) % 512 < (256 if rows == 1 else 64), 0.0, 6.0)[:, None]
+    if rows == 1:  # each of a workgroup's four waves begins with 64 low positions
+        kr[512:, :, 0] = 6.0
+    vr[:, :, 1::2] *= -1
+    slots = (tables[0, :, None] * 64 + torch.arange(64)).flatten().int().to(DEV)
+    ops.kv.write(cache, kr.bfloat16().to(DEV), vr.bfloat16().to(DEV), slots)
+    kr, vr = (x.cpu().double() for x in ops.kv.read(cache, slots))
+    k[0], v[0] = kr, vr
+    q = torch.zeros(requests * rows, 1, D).bfloat16()
+    q[:, :, 0] = 1
+    starts = [rows * i for i in range(requests + 1)]
+    scale = 10 / 6 * 0.6931471805599453
+    out, lse = ops.kv.attend(q.to(DEV), cache, tables.expand(requests, -1).contiguous().to(DEV), i32(starts),
+                             i32([length] * (requests * rows)), scale=scale, max_queries=rows, return_lse=True)
+    assert bool(torch.isfinite(out.float()).all())
+    _attend_check(out[:rows], lse[:rows], q[:rows], k, v, [0, rows], [length] * rows, scale)
+    assert torch.equal(out, out[:1].expand(requests * rows, -1, -1)) and torch.equal(lse, lse[:1].expand_as(lse))
