@@ -4,7 +4,7 @@
 // contract checks run before any launch and, but for the last ("a ROCm GPU"), for tensors on any device.
 //
 // Schemas:
-//   rotary(q, k, positions, turns, axis, adjacent, backward) -> (q', k'), differentiable in q and k
+//   rotary(q, k, positions, turns, axis, adjacent, backward) -> (q', k'), differentiable in q and k (both modes)
 //       q [T,Hq,D], k [T,Hk,D] of one type; positions [A,T] int32 or int64
 //   step_pages(cached, new, tables!, free!, free_count, page, tokens, in_place)
 //       -> (starts, lengths, admitted, free_count, slots, positions, visible)
@@ -12,6 +12,7 @@
 //   kv4_attend(q, data, tables, starts, visible, page, window, scale, max_queries, want_lse) -> (out, lse)
 
 #include <ATen/ATen.h>
+#include <ATen/ops/_make_dual.h>
 #include <ATen/ops/as_strided_native.h>
 #include <c10/core/DeviceGuard.h>
 #include <c10/hip/HIPStream.h>
@@ -124,6 +125,15 @@ struct Rotate : torch::autograd::Function<Rotate> {
 };
 std::tuple<Tensor, Tensor> rotary_autograd(const Tensor& q, const Tensor& k, const Tensor& positions, const Tensor& turns,
                                            const Tensor& axis, bool adjacent, bool backward) {
+  // a turn is linear: its forward derivative is the turn of the tangents, of no heads where an input has none
+  if (q._fw_grad(0).defined() || k._fw_grad(0).defined()) {
+    static const auto op = Rotate::rotary_op();
+    const auto [y, z] = op.call(q._fw_primal(0), k._fw_primal(0), positions, turns, axis, adjacent, backward);
+    const Tensor tq = q._fw_grad(0), tk = k._fw_grad(0);
+    const auto [ty, tz] = op.call(tq.defined() ? tq : y.detach().narrow(1, 0, 0),
+                                  tk.defined() ? tk : z.detach().narrow(1, 0, 0), positions, turns, axis, adjacent, backward);
+    return {tq.defined() ? at::_make_dual(y, ty, 0) : y, tk.defined() ? at::_make_dual(z, tz, 0) : z};
+  }
   if (!at::GradMode::is_enabled() || !(q.requires_grad() || k.requires_grad())) {
     const at::AutoDispatchBelowADInplaceOrView below;
     static const auto op = Rotate::rotary_op();
