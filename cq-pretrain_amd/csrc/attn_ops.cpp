@@ -93,25 +93,40 @@ std::tuple<Tensor, Tensor> rotary(const Tensor& q, const Tensor& k, const Tensor
 }
 
 // The gradient of a turn is the turn back.  In C++ because a Python function and its engine call cost 40 us more
-// than the kernels of a small step.
+// than the kernels of a small step.  An output whose input needs no gradient needs none, and only gradients that are
+// there are turned: the other operand goes in without heads, and where its input wants a gradient all the same (its
+// output has no part in the loss), that is zeros.
 struct Rotate : torch::autograd::Function<Rotate> {
   static torch::autograd::variable_list forward(torch::autograd::AutogradContext* ctx, const Tensor& q, const Tensor& k,
                                                 const Tensor& positions, const Tensor& turns, const Tensor& axis,
                                                 bool adjacent, bool backward) {
     const at::AutoDispatchBelowADInplaceOrView below;
+    ctx->set_materialize_grads(false);
     ctx->save_for_backward({positions, turns, axis});
     ctx->saved_data["adjacent"] = adjacent;
     ctx->saved_data["backward"] = backward;
+    ctx->saved_data["q"] = q.sizes().vec();
+    ctx->saved_data["k"] = k.sizes().vec();
     static const auto op = rotary_op();
     const auto [y, z] = op.call(q, k, positions, turns, axis, adjacent, backward);
+    if (!q.requires_grad()) ctx->mark_non_differentiable({y});
+    if (!k.requires_grad()) ctx->mark_non_differentiable({z});
     return {y, z};
   }
   static torch::autograd::variable_list backward(torch::autograd::AutogradContext* ctx,
                                                  const torch::autograd::variable_list& grad) {
+    if (!grad[0].defined() && !grad[1].defined()) return {{}, {}, {}, {}, {}, {}, {}};
     static const auto op = rotary_op();
     const auto saved = ctx->get_saved_variables();
-    const auto [dq, dk] = op.call(grad[0], grad[1], saved[0], saved[1], saved[2], ctx->saved_data["adjacent"].toBool(),
-                                  !ctx->saved_data["backward"].toBool());
+    const Tensor& one = grad[0].defined() ? grad[0] : grad[1];
+    auto [dq, dk] = op.call(grad[0].defined() ? grad[0] : one.detach().narrow(1, 0, 0),
+                            grad[1].defined() ? grad[1] : one.detach().narrow(1, 0, 0), saved[0], saved[1], saved[2],
+                            ctx->saved_data["adjacent"].toBool(), !ctx->saved_data["backward"].toBool());
+    const auto missing = [&](int i, const char* name) {
+      return ctx->needs_input_grad(i) ? at::zeros(ctx->saved_data[name].toIntVector(), one.options()) : Tensor();
+    };
+    if (!grad[0].defined()) dq = missing(0, "q");
+    if (!grad[1].defined()) dk = missing(1, "k");
     return {dq, dk, {}, {}, {}, {}, {}};
   }
   static c10::TypedOperatorHandle<std::tuple<Tensor, Tensor>(const Tensor&, const Tensor&, const Tensor&, const Tensor&,

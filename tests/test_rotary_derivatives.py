@@ -1,5 +1,5 @@
-"""Derivatives of ``rotary.rotate`` in forward mode: that they are there, on tensors without storage (no launch), and
-their values on the GPU, where a turn's derivative is the turn of the tangents."""
+"""Derivatives of ``rotary.rotate``: that those in forward mode are there and which rows a gradient turns, on tensors
+without storage (no launch), and values on the GPU, where a turn's derivative is the turn of the tangents."""
 
 import pytest
 import torch
@@ -15,9 +15,14 @@ def meta():
     """The operator for tensors without storage, for these tests: what its outputs look like."""
     _lib.ops()
     lib = torch.library.Library("cqgdn", "IMPL")
-    lib.impl("rotary", lambda q, k, *a: (torch.empty(q.shape, dtype=q.dtype, device="meta"),
-                                         torch.empty(k.shape, dtype=k.dtype, device="meta")), "Meta")
-    yield
+    heads = []  # of each call's q and k
+
+    def rotary(q, k, *a):
+        heads.append((q.shape[1], k.shape[1]))
+        return torch.empty(q.shape, dtype=q.dtype, device="meta"), torch.empty(k.shape, dtype=k.dtype, device="meta")
+
+    lib.impl("rotary", rotary, "Meta")
+    yield heads
     lib._destroy()
 
 
@@ -55,6 +60,51 @@ def test_tangents_are_there(meta, reverse):
 
     y, dy = torch.func.jvp(f, (q.detach(),), (tq,))
     assert y.shape == dy.shape == q.shape and calls
+
+
+def test_a_gradient_turns_what_has_one(meta):
+    """The output of an input without a gradient needs none, and a backward call turns the gradients that came."""
+    p, q, k, _, _, pos = _inputs("meta")
+    q.requires_grad_()
+    y, z = rotary.rotate(q, k, pos, p)
+    assert y.requires_grad and not z.requires_grad
+    del meta[:]
+    torch.autograd.grad(y, q, torch.empty_like(y))
+    assert meta == [(2, 0)]
+    y, z = rotary.rotate(k, q, pos, p)
+    assert z.requires_grad and not y.requires_grad
+    del meta[:]
+    torch.autograd.grad(z, q, torch.empty_like(z))
+    assert meta == [(0, 2)]
+    k.requires_grad_()
+    y, z = rotary.rotate(q, k, pos, p)
+    del meta[:]
+    dq, dk = torch.autograd.grad(y, (q, k), torch.empty_like(y))  # z has no part in it
+    assert meta == [(2, 0)] and dq.shape == q.shape and dk.shape == k.shape
+    y, z = rotary.rotate(q, k, pos, p)
+    del meta[:]
+    torch.autograd.grad((y, z), (q, k), (torch.empty_like(y), torch.empty_like(z)))
+    assert meta == [(2, 1)]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("used", ["y", "z", "yz"])
+@pytest.mark.parametrize("wanted", ["q", "k", "qk"])
+def test_gradients_of_some_inputs_from_some_outputs(gdn, used, wanted):
+    """As with both: a gradient is the same whatever else is asked for, and zeros where nothing comes in."""
+    p, q, k, w, v, pos = _inputs(DEV)
+    a, b = q.clone().requires_grad_(), k.clone().requires_grad_()
+    want = dict(zip("qk", torch.autograd.grad(rotary.rotate(a, b, pos, p), (a, b), (w, v))))
+    q.requires_grad_("q" in wanted)
+    k.requires_grad_("k" in wanted)
+    out = dict(zip("yz", rotary.rotate(q, k, pos, p)))
+    assert out["y"].requires_grad == ("q" in wanted) and out["z"].requires_grad == ("k" in wanted)
+    pairs = [(out[n], g) for n, g in (("y", w), ("z", v)) if n in used and out[n].requires_grad]
+    if not pairs:
+        return
+    got = torch.autograd.grad([x for x, _ in pairs], [dict(q=q, k=k)[n] for n in wanted], [g for _, g in pairs])
+    for n, x in zip(wanted, got):
+        assert torch.equal(x, want[n] if dict(q="y", k="z")[n] in used else torch.zeros_like(x))
 
 
 @pytest.mark.gpu
