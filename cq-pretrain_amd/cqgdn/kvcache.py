@@ -80,7 +80,10 @@ def step_pages(cached, new, tables, free, free_count, *, page, tokens, in_place=
     one that the pool cannot serve none that needs pages is admitted.  With ``in_place`` the lengths and
     the pool's count are written back into ``cached`` and ``free_count``."""
     CALLS["cqgdn_step_pages"] += 1
-    return PageStep(*_lib.ops().step_pages(cached, new, tables, free, free_count, page, tokens, in_place))
+    if not in_place:
+        return PageStep(*_lib.ops().step_pages(cached, new, tables, free, free_count, page, tokens))
+    starts, admitted, *rows = _lib.ops().step_pages_(cached, new, tables, free, free_count, page, tokens)
+    return PageStep(starts, cached, admitted, free_count, *rows)
 
 
 def write(cache, k, v, slots):

@@ -6,8 +6,10 @@
 // Schemas:
 //   rotary(q, k, positions, turns, axis, adjacent, backward) -> (q', k'), differentiable in q and k (both modes)
 //       q [T,Hq,D], k [T,Hk,D] of one type; positions [A,T] int32 or int64
-//   step_pages(cached, new, tables!, free!, free_count, page, tokens, in_place)
+//   step_pages(cached, new, tables!, free!, free_count, page, tokens)
 //       -> (starts, lengths, admitted, free_count, slots, positions, visible)
+//   step_pages_(cached!, new, tables!, free!, free_count!, page, tokens)
+//       -> (starts, admitted, slots, positions, visible); lengths and the count are written in place
 //   kv4_write(data!, k, v, slots, page) -> (), kv4_read(data, slots, page, head_dim, fp16) -> (k, v)
 //   kv4_attend(q, data, tables, starts, visible, page, window, scale, max_queries, want_lse) -> (out, lse)
 
@@ -158,10 +160,12 @@ std::tuple<Tensor, Tensor> rotary_autograd(const Tensor& q, const Tensor& k, con
   return {out[0], out[1]};
 }
 
-std::tuple<Tensor, Tensor, Tensor, Tensor, Tensor, Tensor, Tensor> step_pages(const Tensor& cached, const Tensor& fresh,
-                                                                              Tensor& tables, Tensor& pool,
-                                                                              const Tensor& count, int64_t page,
-                                                                              int64_t tokens, bool in_place) {
+// what a step's pages come to; in place, lengths and left are the caller's own
+struct Step {
+  Tensor starts, lengths, admitted, left, slots, positions, visible;
+};
+Step pages_of_step(const Tensor& cached, const Tensor& fresh, const Tensor& tables, const Tensor& pool,
+                   const Tensor& count, int64_t page, int64_t tokens, bool in_place) {
   int32_vector(cached, "cached");
   int32_vector(fresh, "new");
   int32_vector(pool, "free");
@@ -197,6 +201,19 @@ std::tuple<Tensor, Tensor, Tensor, Tensor, Tensor, Tensor, Tensor> step_pages(co
                          stream_of(cached)),
         "cqgdn_step_pages");
   return {starts, lengths, admitted, left, slots, positions, visible};
+}
+std::tuple<Tensor, Tensor, Tensor, Tensor, Tensor, Tensor, Tensor> step_pages(const Tensor& cached, const Tensor& fresh,
+                                                                              Tensor& tables, Tensor& pool,
+                                                                              const Tensor& count, int64_t page,
+                                                                              int64_t tokens) {
+  const Step s = pages_of_step(cached, fresh, tables, pool, count, page, tokens, false);
+  return {s.starts, s.lengths, s.admitted, s.left, s.slots, s.positions, s.visible};
+}
+std::tuple<Tensor, Tensor, Tensor, Tensor, Tensor> step_pages_(Tensor& cached, const Tensor& fresh, Tensor& tables,
+                                                               Tensor& pool, Tensor& count, int64_t page,
+                                                               int64_t tokens) {
+  const Step s = pages_of_step(cached, fresh, tables, pool, count, page, tokens, true);
+  return {s.starts, s.admitted, s.slots, s.positions, s.visible};
 }
 
 void check_data(const Tensor& data, int64_t page, int64_t head_dim) {
@@ -284,7 +301,9 @@ TORCH_LIBRARY_FRAGMENT(cqgdn, m) {
   m.def("rotary(Tensor q, Tensor k, Tensor positions, Tensor turns, Tensor axis, bool adjacent, bool backward) "
         "-> (Tensor, Tensor)");
   m.def("step_pages(Tensor cached, Tensor new, Tensor(a!) tables, Tensor(b!) free, Tensor free_count, int page, "
-        "int tokens, bool in_place) -> (Tensor, Tensor, Tensor, Tensor, Tensor, Tensor, Tensor)");
+        "int tokens) -> (Tensor, Tensor, Tensor, Tensor, Tensor, Tensor, Tensor)");
+  m.def("step_pages_(Tensor(a!) cached, Tensor new, Tensor(b!) tables, Tensor(c!) free, Tensor(d!) free_count, int page, "
+        "int tokens) -> (Tensor, Tensor, Tensor, Tensor, Tensor)");
   m.def("kv4_write(Tensor(a!) data, Tensor k, Tensor v, Tensor slots, int page) -> ()");
   m.def("kv4_read(Tensor data, Tensor slots, int page, int head_dim, bool fp16) -> (Tensor, Tensor)");
   m.def("kv4_attend(Tensor q, Tensor data, Tensor tables, Tensor starts, Tensor visible, int page, int window, "
@@ -296,6 +315,7 @@ TORCH_LIBRARY_IMPL(cqgdn, Autograd, m) { m.impl("rotary", &rotary_autograd); }
 TORCH_LIBRARY_IMPL(cqgdn, CUDA, m) {
   m.impl("rotary", &rotary);
   m.impl("step_pages", &step_pages);
+  m.impl("step_pages_", &step_pages_);
   m.impl("kv4_write", &kv4_write);
   m.impl("kv4_read", &kv4_read);
   m.impl("kv4_attend", &kv4_attend);
@@ -305,6 +325,7 @@ TORCH_LIBRARY_IMPL(cqgdn, CUDA, m) {
 TORCH_LIBRARY_IMPL(cqgdn, CPU, m) {
   m.impl("rotary", &rotary);
   m.impl("step_pages", &step_pages);
+  m.impl("step_pages_", &step_pages_);
   m.impl("kv4_write", &kv4_write);
   m.impl("kv4_read", &kv4_read);
   m.impl("kv4_attend", &kv4_attend);
