@@ -24,12 +24,14 @@ class RotaryPlan:
 
     ``turns`` int64 [rotary_dim / 2]: how far a position turns pair i, in units of 2^-64 of a turn, so
     that the angle of any integer position is exact; ``axis`` int32 [rotary_dim / 2]: which of the
-    position's axes pair i goes by; ``adjacent``: pair i is (2i, 2i + 1), else (i, i + rotary_dim / 2).
+    position's axes pair i goes by; ``adjacent``: pair i is (2i, 2i + 1), else (i, i + rotary_dim / 2);
+    ``axes``: how many axes the pairs go by (None: not known on the host).
     """
 
     turns: torch.Tensor
     axis: torch.Tensor
     adjacent: bool = False
+    axes: int | None = None
 
 
 def plan(rotary_dim, *, theta=10000.0, sections=None, mixed=False, adjacent=False, device="cuda"):
@@ -60,18 +62,20 @@ def plan(rotary_dim, *, theta=10000.0, sections=None, mixed=False, adjacent=Fals
         step = Decimal(theta) ** (Decimal(-2) / Decimal(rotary_dim))
         turns = [int((step ** i / (2 * _PI) * 2 ** 64).to_integral_value()) for i in range(pairs)]
     return RotaryPlan(torch.tensor(turns, dtype=torch.int64).to(device), torch.tensor(axis, dtype=torch.int32).to(device),
-                      bool(adjacent))
+                      bool(adjacent), max(axis) + 1)
 
 
 def rotate(q, k, positions, plan):
     """q [T, Hq, D] and k [T, Hk, D] (bf16, fp16 or fp32, any strides; or [1, T, H, D]) turned by the
-    positions of their tokens: int32 or int64 [axes, T], or [T] for one axis.  Values of a head behind
-    the plan's rotary_dim pass unchanged.  Computed in fp32, rounded once; differentiable in q and k."""
+    positions of their tokens: int32 or int64 [axes, T], or [T] (or [1, T]) for text, whose axes are
+    alike.  Values of a head behind the plan's rotary_dim pass unchanged.  Computed in fp32, rounded once; differentiable in q and k."""
     packed = q.dim() == 4 and k.dim() == 4 and q.shape[0] == 1 and k.shape[0] == 1
     if packed:
         q, k = q[0], k[0]
     if positions.dim() == 1:
         positions = positions[None]
+    if plan.axes is not None and 1 < positions.shape[0] < plan.axes:
+        raise ValueError(f"positions have {positions.shape[0]} axes, the plan {plan.axes}")
     CALLS["cqgdn_rotary"] += 1
     q, k = _lib.ops().rotary(q, k, positions, plan.turns, plan.axis, plan.adjacent, False)
     return (q[None], k[None]) if packed else (q, k)

@@ -392,7 +392,8 @@ int cqgdn_chunk_local_cumsum(const float* g, float* out, int64_t T, int H, const
  *   positions : [axes][T], int32 (int64 with wide_positions), axes axis_stride elements apart
  *   turns     : [rotary_dim / 2], f_i / (2 pi) in units of 2^-64 turns a position, so that the angle of
  *               any integer position is exact to 2^-32 of a turn
- *   axis      : [rotary_dim / 2], the axis of pair i
+ *   axis      : [rotary_dim / 2], the axis of pair i (beyond the last one: the last, so that the positions of text,
+ *               one axis, serve any plan)
  */
 #define CQGDN_BF16 0
 #define CQGDN_F16 1
