@@ -21,7 +21,6 @@ LIB_PATH = Path(__file__).resolve().with_name("libcqgdn.so")
 OPS_PATH = LIB_PATH.with_name("libcqgdn_torch.so")
 
 OK, EINVAL, EUNSUPPORTED, EHIP = 0, 1, 2, 3
-BF16, F16, F32 = 0, 1, 2
 NORMALIZE, TRAINING, PRECISE, NO_OUTPUT, FP16 = 1, 2, 4, 8, 16
 STATIC_WORKSPACE_BYTES = 64 << 20  # CQGDN_STATIC_WORKSPACE_BYTES
 FWD_BUFFERS, BWD_BUFFERS = 9, 8

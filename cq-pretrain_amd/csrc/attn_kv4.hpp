@@ -53,10 +53,4 @@ __device__ __forceinline__ void attend_limits(int visible, int window, int room,
   if (lo >= hi) lo = hi = 0;
 }
 
-// The entry of the block table that holds position pos, -1 outside the table
-__device__ __forceinline__ int page_of(const AttendArgs& a, int r, int pos) {
-  const int column = pos >> a.page_shift;
-  return column < a.columns ? a.tables[r * a.table_stride + column] : -1;
-}
-
 }  // namespace cqgdn
