@@ -7,7 +7,7 @@ A serving step of an attention layer, beside ``events.layer_decode_step`` of the
 * ``attend``      the step's query rows over the pages, one new token a request or a prompt's thousands.
 
 Everything is enqueued on the current stream and sized on the host alone, so a step can be captured into
-a HIP graph; lengths, tables and pools stay on the device.
+a HIP graph; lengths, tables and pools stay on the device.  No gradient passes through the cache.
 """
 
 from __future__ import annotations

@@ -310,7 +310,13 @@ TORCH_LIBRARY_FRAGMENT(cqgdn, m) {
         "float scale, int max_queries, bool want_lse) -> (Tensor, Tensor)");
 }
 
-TORCH_LIBRARY_IMPL(cqgdn, Autograd, m) { m.impl("rotary", &rotary_autograd); }
+// The cache and what reads it are for serving: no gradient passes, and their outputs say so (by default they would
+// require one and give none).
+TORCH_LIBRARY_IMPL(cqgdn, Autograd, m) {
+  m.impl("rotary", &rotary_autograd);
+  for (const char* name : {"step_pages", "step_pages_", "kv4_write", "kv4_read", "kv4_attend"})
+    m.impl(name, torch::CppFunction::makeFallthrough());
+}
 
 TORCH_LIBRARY_IMPL(cqgdn, CUDA, m) {
   m.impl("rotary", &rotary);

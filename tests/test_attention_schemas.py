@@ -1,4 +1,5 @@
-"""What the attention layers' operators say they write: the tensors that a call changes, and no others (no launch)."""
+"""What the attention layers' operators say they write, the tensors that a call changes and no others, and that the
+cache's pass no gradient (no launch)."""
 
 import pytest
 import torch
@@ -40,3 +41,20 @@ def test_a_step_in_place_takes_the_operator_that_writes(monkeypatch, in_place):
     step = kvcache.step_pages(cached, i(2), i(2, 4), i(8), count, page=16, tokens=5, in_place=in_place)
     assert taken == [("step_pages_" if in_place else "step_pages", 7)]
     assert (step.lengths is cached) == (step.free_count is count) == in_place
+
+
+def test_no_gradient_passes_through_the_cache():
+    """The output of rows that require a gradient does not require one itself, so asking for it fails."""
+    _lib.ops()
+    lib = torch.library.Library("cqgdn", "IMPL")
+    lib.impl("kv4_attend", lambda q, *a: (torch.empty_like(q), torch.empty(0, device="meta")), "Meta")
+    try:
+        i = lambda *x: torch.zeros(*x, dtype=torch.int32, device="meta")  # noqa: E731
+        cache = kvcache.KVCache(torch.empty(3, 2, 16 * 68, dtype=torch.uint8, device="meta"), page=16, head_dim=64)
+        q = torch.empty(4, 4, 64, dtype=torch.bfloat16, device="meta", requires_grad=True)
+        out = kvcache.attend(q, cache, i(2, 3), i(3), i(4))
+        assert not out.requires_grad
+        with pytest.raises(RuntimeError, match="does not require grad"):
+            out.sum().backward()
+    finally:
+        lib._destroy()
