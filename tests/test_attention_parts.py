@@ -30,3 +30,13 @@ def test_long_tables_are_split():
     for D in (64, 128, 256):
         for rows in (16, 48, 64, 128):
             assert parts(rows, D, 1, 24576, 16) >= 256
+
+
+@pytest.mark.parametrize("rows", [1, 2, 5, 70])
+def test_a_launch_is_for_the_average_request_at_least(rows):
+    """Eight requests of `rows` rows each under a bound of one: as under their own bound, so that a bound far too
+    small does not multiply the parts of many rows."""
+    size = lambda most: _lib.lib().cqgdn_kv4_attend_workspace_size(8 * rows, 8, 16, 4, 128, most, 512, 16)  # noqa: E731
+    assert size(1) == size(rows)
+    n, rest = divmod(size(rows), 8 * rows * 16 * 130 * 4)
+    assert rest == 0 and n == {1: 11, 2: 11, 5: 11, 70: 5}[rows]  # three steps a wave; 512 workgroups over 96
