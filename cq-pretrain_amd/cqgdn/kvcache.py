@@ -108,7 +108,11 @@ def attend(q, cache, tables, starts, visible, *, window=None, scale=None, max_qu
     Rows starts[r] .. starts[r + 1] - 1 (from 0 on) are request r's, whose pages are ``tables[r]``; row t sees the
     first ``visible[t]`` positions, or the last ``window`` of those.  Query head h reads key head
     h // (Hq // heads).  ``scale`` defaults to D^-0.5.  Rows that see nothing, and rows behind
-    ``starts[-1]``, are zero.  Positions whose table entry names no page are not seen.
+    ``starts[-1]``, are zero.  Positions whose table entry names no page are not seen.  Rows need not be those
+    that the step has written: read-only rows take starts and limits of their own.
+
+    Scores, sums and results are held in fp32; each weight is rounded to the cache's type before the product
+    with v, which moves a result by up to half a step of the type times sum p |v| / sum p.
 
     ``max_queries`` bounds the rows of one request and sets the launch (default: T; a decode step should
     pass 1): a larger request is still served.  With ``return_lse`` also fp32 [T, Hq]:

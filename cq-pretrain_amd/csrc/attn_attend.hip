@@ -6,8 +6,12 @@
 // the columns of S^T = K Q^T, 16 at a time, so a lane owns one row: its limits, maximum and sum are the
 // lane's own, and S^T's layout is already the operand of O^T = V^T P^T.
 //
+// Scores, sums and O are fp32.  The weights are rounded once to the rows' type, as the operand of that product, which
+// moves a result by at most half a step of the type times sum_j p_j |v_j| / sum_j p_j, as much as rounding the result
+// itself; sums of weights take them as they were.  Two terms of the type for a weight would double V's MFMAs.
+//
 // Few rows read each code once and are bound by that, or by latency.  64 ragged requests of up to 8192 positions (169
-// MB): 36 us and 5 for the join, 4.6 TB/s; five of up to 65536, D = 256 (109 MB): 28 and 4; one of 9216: 8 and 4, of
+// MB): 37 us and 5 for the join, 4.6 TB/s; five of up to 65536, D = 256 (109 MB): 29 and 4; one of 9216: 8 and 4, of
 // which the codes are one.  What it took: the parts' equal length (one eighth of the time), pages found without a load
 // in the loop (each step waited for all that was under way), waits for keys apart from those for values, operands of V
 // read from LDS three MFMAs early, and nothing spilled (the 11 KB a wave that were cost a third).

@@ -10,8 +10,8 @@ constexpr int kWaves = 4;         // of a workgroup; they take its steps in turn
 constexpr int kStep = 64;         // positions of a wave's step
 constexpr int kMaxSplits = 512;   // parts of a call by either kernel, which the join holds the weights of
 // Rows of a request and key head above which its positions are converted once for all of them (attn_tile.hip)
-// and not once for every 16: over 2000 positions of 64 requests 36 rows take 38 us here and 43 there, 64 rows 49
-// and 46, 128 rows 89 and 58.
+// and not once for every 16: over up to 2000 positions of 64 requests (D = 128) 36 rows take 27 us here and 35 there, 64
+// rows 31 and 38, 128 rows 55 and 47; with D = 64 64 rows 26 and 27, 128 rows 39 and 36.
 constexpr int kFewRows = 48;
 // Positions of a request that can be seen: limits are 32-bit, and a step may begin behind the last position and ask
 // for the one after it.

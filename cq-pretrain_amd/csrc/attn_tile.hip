@@ -1,14 +1,16 @@
 // Attention of many query rows a request over the 4-bit pages: a prompt's rows share the values of a page.
 //
-// The mathematics is that of attn_attend.hip.  Here a workgroup takes 128 rows of one request and key head,
+// The mathematics, and the rounding of the weights, are those of attn_attend.hip.  Here a workgroup takes 128 rows of one request and key head,
 // 32 a wave, and kTokens positions a step.  Its threads convert the step's codes once into K and V tiles of E
 // in shared memory, two deep, so that the next step's codes are on their way and being converted while the
 // waves multiply.  S^T = K Q^T and O^T = V^T P^T run on 32 x 32 x 16 MFMAs with a row a column, so a lane
 // (and its partner 32 lanes on) owns a row: limits, maximum and sum stay in its registers, and S^T's layout
 // is already an operand of O^T.
 //
-// 4096 rows over 8192 positions (16 heads of 128, 4 key heads): 216 us, 955 TFLOP/s; the library's largest products
-// reach 1486.  A step of 32 rows and 64 positions is 32 MFMAs (1024 cycles of the matrix core, each of which keeps the
+// 4096 rows over 8192 positions (16 heads of 128, 4 key heads): 219 us, 941 TFLOP/s; the library's largest products
+// reach 1486.  2048 rows over 4096 reach 661, in two parts that the join adds up; with D = 64 636 and 513, whose steps
+// hold half of the MFMAs against the same exponentials, masks and barriers; with D = 256, where a SIMD holds one wave
+// and its exponentials stand by themselves, 649 and 529.  A step of 32 rows and 64 positions is 32 MFMAs (1024 cycles of the matrix core, each of which keeps the
 // SIMD's issue 16 cycles), some 195 VALU instructions, 32 of them exponentials of 8 cycles, and 270 cycles of LDS, which
 // eight waves of a CU share: no one of them fills the time, and left out of a copy each takes 7 to 17% with it.
 #include <hip/hip_runtime.h>

@@ -449,7 +449,11 @@ int cqgdn_kv4_read(const void* data, int64_t pages, int page, int kv_heads, int 
  * [max(0, visible[t] - window), visible[t]) of its request (window 0: from 0), whose pages are
  * tables[r][position / page].  out[t][h] = sum_j p_j v_j / sum_j p_j, p_j = exp(scale q k_j), query head h
  * reading key head h / (heads / kv_heads); rows that see nothing, and rows behind starts[N], are zero.
- * Positions beyond the table's columns, or whose entry names no page, are not seen.
+ * Positions beyond the table's columns, or whose entry names no page, are not seen.  Scores, sums and results
+ * are held in fp32; each weight is rounded to dtype before the product with v, so a result is off by up to half
+ * a step of dtype times sum_j p_j |v_j| / sum_j p_j beside its own rounding.  With bf16 a sum of n positions may
+ * reach n 2^12 max |v| before the division: values up to 2^100 overflow over no less than 2^16 positions, values
+ * up to 2^84 never.
  *   q, out      : bf16 or fp16 (dtype) [T][heads][head_dim]; q with strides in elements, multiples of 8
  *   lse         : NULL, or fp32 [T][heads]: log sum_j exp(scale q k_j), -inf for rows that see nothing
  *   max_queries : bound of the rows of one request; it sets the launch, and a larger request is served too
