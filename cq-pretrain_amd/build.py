@@ -1,5 +1,5 @@
 """Build libcqgdn.so (gfx950 HIP kernels + the C ABI of include/cqgdn.h) and its PyTorch-ROCm
-operator library libcqgdn_torch.so (csrc/torch_ops.cpp and csrc/attn_ops.cpp, TORCH_LIBRARY(cqgdn)) in-tree.
+operator library libcqgdn_torch.so (OPS_SOURCES of csrc/, TORCH_LIBRARY(cqgdn)) in-tree.
 
 Usage: python cq-pretrain_amd/build.py [--jobs N]
 
@@ -27,6 +27,7 @@ INCLUDE = ROOT / "include"
 OUT = PKG / "cqgdn" / "libcqgdn.so"
 OPS_OUT = PKG / "cqgdn" / "libcqgdn_torch.so"
 BUILD = PKG / "_build"
+OPS_SOURCES = ("torch_ops.cpp", "attn_ops.cpp", "attn_core_ops.cpp")
 
 ARCH = os.environ.get("CQGDN_ARCH", "gfx950")
 FLAGS = [
@@ -85,7 +86,7 @@ def build(jobs: int | None = None, extra: list[str] | None = None, verbose: bool
 
 
 def build_ops(verbose: bool = True) -> Path:
-    """csrc/torch_ops.cpp and csrc/attn_ops.cpp -> cqgdn/libcqgdn_torch.so, linked to libcqgdn.so (rpath $ORIGIN)."""
+    """OPS_SOURCES -> cqgdn/libcqgdn_torch.so, linked to libcqgdn.so (rpath $ORIGIN)."""
     import torch
     from torch.utils import cpp_extension
 
@@ -96,7 +97,7 @@ def build_ops(verbose: bool = True) -> Path:
     tmp = OPS_OUT.with_suffix(".so.tmp")
     cmd = [os.environ.get("CXX", "g++"), "-O2", "-std=c++17", "-shared", "-fPIC", f"-D_GLIBCXX_USE_CXX11_ABI={abi}",
            "-D__HIP_PLATFORM_AMD__=1", "-DUSE_ROCM=1", *(f"-I{p}" for p in includes),
-           str(CSRC / "torch_ops.cpp"), str(CSRC / "attn_ops.cpp"), "-o", str(tmp),
+           *(str(CSRC / name) for name in OPS_SOURCES), "-o", str(tmp),
            *(f"-L{p}" for p in cpp_extension.library_paths()), "-lc10", "-lc10_hip", "-ltorch_cpu",
            f"-L{OUT.parent}", "-lcqgdn", "-Wl,-rpath,$ORIGIN"]
     proc = subprocess.run(cmd, capture_output=True, text=True)

@@ -71,6 +71,17 @@ SIGNATURES = {
     "cqgdn_kv4_attend_workspace_size": (_SZ, [_I64, _I, _I, _I, _I, _I, _I, _I]),
     "cqgdn_kv4_attend": (_I, [_P, _I64, _I64, _I, _I64, _I, _I, _P, _I64, _I, _I, _P, _I64, _I, _P, _I, _P, _I, _F, _I,
                               _P, _P, _P, _SZ, _P]),
+    "cqgdn_kv16_append": (_I, [_P, _I64, _I64, _I, _P, _I64, _I64, _P, _I64, _I64, _I64, _I, _I, _I, _I, _I, _P, _I, _I64,
+                               _I, _P, _P, _P, _P, _P, _I64, _I, _P]),
+    "cqgdn_kv16_attend_workspace_size": (_SZ, [_I64, _I, _I, _I, _I, _I, _I, _I]),
+    "cqgdn_kv16_attend": (_I, [_P, _I64, _I64, _I, _I64, _I, _I, _P, _I64, _I, _I, _P, _I64, _I, _P, _I, _P, _I, _P, _F,
+                               _F, _P, _I, _P, _P, _P, _SZ, _P]),
+    "cqgdn_attend_fwd_workspace_size": (_SZ, [_I64, _I64, _I, _I, _I]),
+    "cqgdn_attend_fwd": (_I, [_P, _I64, _I64, _P, _I64, _I64, _P, _I64, _I64, _I, _I64, _I64, _I, _I, _I, _P, _P, _P, _F,
+                              _F, _P, _P, _P, _P, _SZ, _P]),
+    "cqgdn_attend_bwd_workspace_size": (_SZ, [_I64, _I64, _I, _I, _I]),
+    "cqgdn_attend_bwd": (_I, [_P, _I64, _I64, _P, _I64, _I64, _P, _I64, _I64, _P, _I64, _I64, _I, _I64, _I64, _I, _I, _I,
+                              _P, _P, _P, _F, _F, _P, _P, _P, _P, _P, _P, _P, _P, _SZ, _P]),
     "cqgdn_timer_arm": (_I, [ctypes.c_char_p, _I]),
     "cqgdn_timer_read": (_I, [_P, _I, _P]),
 }
@@ -113,7 +124,7 @@ def lib():
 
 
 def ops():
-    """``torch.ops.cqgdn`` (the operators of csrc/torch_ops.cpp and csrc/attn_ops.cpp), loaded once; raise if unbuilt."""
+    """``torch.ops.cqgdn`` (the operators of csrc/*_ops.cpp), loaded once; raise if unbuilt."""
     global _OPS
     if _OPS is None:
         lib()  # the operator library links libcqgdn.so: load it (and check it exists) first

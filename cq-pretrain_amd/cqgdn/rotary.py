@@ -65,6 +65,15 @@ def plan(rotary_dim, *, theta=10000.0, sections=None, mixed=False, adjacent=Fals
                       bool(adjacent), max(axis) + 1)
 
 
+def token_positions(positions, plan):
+    """Positions [axes, T] of a call's [axes, T], [T] or [1, T]; fewer axes than the plan's, but for one, are refused."""
+    if positions.dim() == 1:
+        positions = positions[None]
+    if plan.axes is not None and 1 < positions.shape[0] < plan.axes:
+        raise ValueError(f"positions have {positions.shape[0]} axes, the plan {plan.axes}")
+    return positions
+
+
 def rotate(q, k, positions, plan):
     """q [T, Hq, D] and k [T, Hk, D] (bf16, fp16 or fp32, any strides; or [1, T, H, D]) turned by the
     positions of their tokens: int32 or int64 [axes, T], or [T] (or [1, T]) for text, whose axes are
@@ -72,10 +81,7 @@ def rotate(q, k, positions, plan):
     packed = q.dim() == 4 and k.dim() == 4 and q.shape[0] == 1 and k.shape[0] == 1
     if packed:
         q, k = q[0], k[0]
-    if positions.dim() == 1:
-        positions = positions[None]
-    if plan.axes is not None and 1 < positions.shape[0] < plan.axes:
-        raise ValueError(f"positions have {positions.shape[0]} axes, the plan {plan.axes}")
+    positions = token_positions(positions, plan)
     CALLS["cqgdn_rotary"] += 1
     q, k = _lib.ops().rotary(q, k, positions, plan.turns, plan.axis, plan.adjacent, False)
     return (q[None], k[None]) if packed else (q, k)

@@ -542,6 +542,16 @@ __global__ __launch_bounds__(256) void join_kernel(AttendArgs a, int splits) {
 }
 
 template <class E, int D>
+void join(const AttendArgs& a, int splits, hipStream_t st) {
+  // 2048 rows of 33 MB in two parts: 60 us by the kernel for few rows; 32 rows in 36 parts: 4 us by it
+  const int64_t groups = (a.T * a.heads * D + 1023) / 1024;
+  if (groups >= 256)
+    join_rows_kernel<E, D><<<(unsigned)groups, 256, 0, st>>>(a, splits);
+  else
+    join_kernel<E, D><<<(unsigned)(a.T * a.heads * (D / 64)), 256, 0, st>>>(a, splits);
+}
+
+template <class E, int D>
 void launch_dim(const AttendArgs& a, hipStream_t st) {
   const int group = a.heads / a.kv_heads;
   const AttendPlan p = attend_plan(a.N, a.kv_heads, group, D, a.max_queries, (int64_t)a.columns << a.page_shift, a.window);
@@ -554,14 +564,7 @@ void launch_dim(const AttendArgs& a, hipStream_t st) {
     const dim3 grid((unsigned)std::max<int64_t>(1, (int64_t)a.N * tiles), a.kv_heads, p.splits + 1);
     attend_kernel<E, D><<<grid, 64 * kWaves, 0, st>>>(a, tiles, p.per);
   }
-  if (p.splits > 1) {
-    // 2048 rows of 33 MB in two parts: 60 us by the kernel for few rows; 32 rows in 36 parts: 4 us by it
-    const int64_t groups = (a.T * a.heads * D + 1023) / 1024;
-    if (groups >= 256)
-      join_rows_kernel<E, D><<<(unsigned)groups, 256, 0, st>>>(a, p.splits);
-    else
-      join_kernel<E, D><<<(unsigned)(a.T * a.heads * (D / 64)), 256, 0, st>>>(a, p.splits);
-  }
+  if (p.splits > 1) join<E, D>(a, p.splits, st);
 }
 
 template <class E>
@@ -579,6 +582,13 @@ void by_dim(const AttendArgs& a, hipStream_t st) {
 size_t attend_workspace_bytes(int64_t T, int64_t N, int heads, int kv_heads, int D, int max_queries, int64_t capacity) {
   const int splits = attend_plan(N, kv_heads, heads / kv_heads, D, max_queries, capacity, 0).splits;
   return splits > 1 ? (size_t)T * heads * splits * (D + 2) * sizeof(float) : 0;
+}
+
+void launch_attend_join(const AttendArgs& a, int splits, hipStream_t st) {
+  if (a.fp16)
+    a.D == 64 ? join<f16, 64>(a, splits, st) : a.D == 128 ? join<f16, 128>(a, splits, st) : join<f16, 256>(a, splits, st);
+  else
+    a.D == 64 ? join<bf16, 64>(a, splits, st) : a.D == 128 ? join<bf16, 128>(a, splits, st) : join<bf16, 256>(a, splits, st);
 }
 
 void launch_attend(const AttendArgs& a, hipStream_t st) {

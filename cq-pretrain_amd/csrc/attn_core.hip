@@ -1,0 +1,411 @@
+// Attention over 16-bit keys and values, many rows: packed documents in training, prompts over a paged cache.
+//
+// Row (t, query head) gets sum_j p_j v_j / sum_j p_j over the keys j that it sees, p_j = exp(u_j - m), u_j its capped
+// and biased score, in one pass with a running maximum m.  A workgroup takes 128 rows of one key head, 32 a wave (with
+// grouped heads a row is a token and one of the group's query heads, so that the group shares K and V), and kTokens
+// keys a step, whose K and V rows go from memory to shared memory without passing registers, two steps deep.  S^T =
+// K Q^T and O^T = V^T P^T: a lane owns a row, so limits, maximum, sum and the head's slope are the lane's own and S^T's
+// layout is already an operand of O^T.  Steps that all of a wave's rows see whole, most of them, have no masks.
+//
+// Scores, sums and O are fp32; a weight is rounded once to the rows' type for its product with V (half a step of
+// the type times sum p |v| / sum p in a result).
+#include <hip/hip_runtime.h>
+
+#include <algorithm>
+
+#include "attn_core.hpp"
+#include "attn_plan.hpp"
+
+namespace cqgdn {
+namespace {
+
+constexpr int kRows = 128;  // of a workgroup, 32 a wave
+constexpr int kEarly = 4;   // MFMA operands read from LDS ahead of their use
+
+template <int D>
+constexpr int kTokens = D == 256 ? 32 : 64;
+
+// PAGED: keys from the pages of a cache; BENT: scores are capped or biased
+template <class E, int D, bool PAGED, bool BENT>
+__global__ __launch_bounds__(256, D == 256 ? 1 : D == 64 ? 3 : 2) void core_kernel(CoreArgs a, int tiles, int splits) {
+  typedef typename Vec<E>::x8 x8;
+  constexpr int TOK = kTokens<D>, NS = TOK / 32, KQ = D / 16, MT = D / 32;
+  constexpr int F = NS * KQ, FV = 2 * NS * MT, H = FV / NS;  // operands of a step: K's, V's, V's for 32 keys
+  constexpr int LR = kLoadRows<D>, LOADS = TOK / 4 / LR;     // rows a load, loads a wave and step of K (and of V)
+  constexpr int GROUPS = TOK / 16;
+  __shared__ __align__(16) E kt[2][TOK * D];
+  __shared__ __align__(16) E vt[2][TOK * D];
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int n32 = lane & 31, kg = lane >> 5;
+  // Launch order: the last tiles, which see most, first; every other round of 256 workgroups reversed, so that
+  // a CU's workgroups add up to the same.  Rows behind the requests' ("request N") come last.
+  const int requests = PAGED ? a.N : 1, each = a.kv_heads * requests * splits, real_blocks = each * tiles;
+  int b = blockIdx.x;
+  const bool padding = PAGED && b >= real_blocks;
+  if (padding)
+    b -= real_blocks;
+  else if ((b >> 8 & 1) && (b | 255) < real_blocks)
+    b ^= 255;
+  const int heads_each = padding ? a.kv_heads : each;
+  const int tile0 = padding ? b / heads_each : tiles - 1 - b / heads_each;
+  b %= heads_each;
+  const int s = padding ? 0 : b % splits;
+  if (!padding) b /= splits;
+  const int h = b % a.kv_heads, r = padding ? a.N : b / a.kv_heads;
+  if (padding) tiles = (gridDim.x - real_blocks) / a.kv_heads;
+  const int group = a.group.d, T = (int)a.T;
+  int from = 0, to = T, room = a.S;
+  if constexpr (PAGED) {
+    from = r == 0 ? 0 : min(max(a.starts[r], 0), T);
+    to = padding ? T : min(max(a.starts[r + 1], from), T);
+    room = (int)min((int64_t)a.columns << a.page_shift, (int64_t)kAttendRoom);
+  }
+  const int rows = (to - from) * group, size = 1 << a.page_shift;
+  // the exponent's factor of the plain scores, never 0: a masked score stays -infinity
+  const float c = BENT ? 1.f : fmaxf(fabsf(a.scale) * 1.44269504088896341f, 1.17549435e-38f);
+  constexpr float bias = kAttendBias<E>;
+  const TileOperands<E, D> at_tile(lane);
+
+  for (int tile = tile0; tile * kRows < rows; tile += tiles) {
+    const auto limits = [&](int rho, int& lo, int& hi) {
+      const int t = from + a.group.of(rho < rows ? rho : 0);
+      if constexpr (PAGED) {
+        attend_limits(rho < rows && r < a.N ? a.visible[t] : 0, a.window, room, lo, hi);
+      } else {
+        lo = rho < rows && a.first ? max(a.first[t], 0) : 0;
+        hi = rho < rows ? min(a.visible[t], room) : 0;
+        if (lo >= hi) lo = hi = 0;
+      }
+    };
+    // what the workgroup's rows see together
+    int first, last;
+    {
+      int lo0, hi0, lo1, hi1;
+      limits(tile * kRows + lane, lo0, hi0);
+      limits(tile * kRows + 64 + lane, lo1, hi1);
+      first = min(hi0 > 0 ? lo0 : INT32_MAX, hi1 > 0 ? lo1 : INT32_MAX);
+      last = max(hi0, hi1);
+#pragma unroll
+      for (int o = 1; o < 64; o <<= 1) {
+        first = min(first, __shfl_xor(first, o, 64));
+        last = max(last, __shfl_xor(last, o, 64));
+      }
+      first = __builtin_amdgcn_readfirstlane(first);
+      last = __builtin_amdgcn_readfirstlane(last);
+    }
+    const int rho = tile * kRows + 32 * wave + n32;
+    const bool real = rho < rows;
+    int lo, hi;
+    limits(rho, lo, hi);
+    // what any of the wave's rows sees, and what all of them see, where nothing is masked
+    int some = hi > 0 ? lo : INT32_MAX, most = hi, low = lo, high = real ? hi : INT32_MAX;
+#pragma unroll
+    for (int i = 1; i < 32; i <<= 1) {
+      some = min(some, __shfl_xor(some, i, 64));
+      most = max(most, __shfl_xor(most, i, 64));
+      low = max(low, __shfl_xor(low, i, 64));
+      high = min(high, __shfl_xor(high, i, 64));
+    }
+    some = __builtin_amdgcn_readfirstlane(some);
+    most = __builtin_amdgcn_readfirstlane(most);
+    low = __builtin_amdgcn_readfirstlane(low);
+    high = __builtin_amdgcn_readfirstlane(high);
+    const int row_t = real ? a.group.of(rho) : 0, t = from + row_t, head = h * group + (real ? rho - row_t * group : 0);
+    x8 qf[KQ];  // lane (n32, kg): row n32, dimensions 16 i + 8 kg ..
+    {
+      const E* q = static_cast<const E*>(a.q) + t * a.q_token + head * a.q_head + 8 * kg;
+#pragma unroll
+      for (int i = 0; i < KQ; ++i) {
+        u32x4 w = real ? *reinterpret_cast<const u32x4*>(q + 16 * i) : u32x4{0, 0, 0, 0};
+        if (!BENT && a.scale < 0.f) w ^= 0x80008000u;
+        qf[i] = __builtin_bit_cast(x8, w);
+      }
+    }
+    const Bend bend(a.scale, BENT ? a.cap : 0.f, BENT ? a.slopes : nullptr, head);
+    const int stands = BENT && real && r < requests ? (a.positions ? a.positions[t] : a.visible[t] - 1) : 0;
+    f32x16 o[MT];
+#pragma unroll
+    for (int i = 0; i < MT; ++i) o[i] = f32x16{};
+    float m = hi > 0 ? -INFINITY : 0.f, l = 0.f;
+
+    const int begin = last > 0 ? (PAGED ? first & ~(TOK - 1) : first) : 0;
+    const int steps = (last - begin + TOK - 1) / TOK, per = (steps + splits - 1) / splits;
+    const int n = min(steps, (s + 1) * per) - s * per, pos0 = begin + s * per * TOK;
+
+    // the block table's entries for the 16 positions each of step j, one a lane
+    const auto entries = [&](int j) {
+      const int column = (pos0 + j * TOK + 16 * (lane & (GROUPS - 1))) >> a.page_shift;
+      return j < n && column < a.columns ? a.tables[r * a.table_stride + column] : -1;
+    };
+    // step j's rows of the wave on their way into the tiles.  Returns which of the step's 16 positions are shown.
+    const auto stage = [&](int table, int j) {
+      const int row0 = wave * (TOK / 4), pos = pos0 + j * TOK;
+      E* const kd = kt[j & 1] + row0 * D;
+      E* const vd = vt[j & 1] + row0 * D;
+      if constexpr (PAGED) {
+        const uint32_t page = __builtin_amdgcn_readlane(table, row0 / 16);
+        const int at = (pos + row0) & (size - 1);
+        const E* base = reinterpret_cast<const E*>(a.data) + ((int64_t)(page < a.page_count ? page : 0) * a.kv_heads + h) * 2 * size * D;
+#pragma unroll
+        for (int i = 0; i < LOADS; ++i) {
+          const int row = row0 + i * LR + load_row<D>(lane);
+          const int off = (at + row - row0) * D + 8 * load_chunk<D>(lane, row);
+          dma16(base + off, kd + i * LR * D);
+          dma16(base + size * D + off, vd + i * LR * D);
+        }
+        return (int)__ballot((uint32_t)table < a.page_count) & ((1 << GROUPS) - 1);
+      } else {
+        const E* kb = static_cast<const E*>(a.k) + h * a.k_head + pos * a.k_token;
+        const E* vb = static_cast<const E*>(a.v) + h * a.v_head + pos * a.v_token;
+        const int end = a.S - 1 - pos;  // rows behind the last key: that key once more
+#pragma unroll
+        for (int i = 0; i < LOADS; ++i) {
+          const int row = row0 + i * LR + load_row<D>(lane), at = min(row, end), chunk = 8 * load_chunk<D>(lane, row);
+          dma16(kb + (at * (int)a.k_token + chunk), kd + i * LR * D);
+          dma16(vb + (at * (int)a.v_token + chunk), vd + i * LR * D);
+        }
+        return (1 << GROUPS) - 1;
+      }
+    };
+    f32x16 sc[NS];
+    // the weights of 32 keys, two a part, in the order of their scores
+    uint32_t pw[NS][8];
+    float base, sum;
+    const auto begin_weights = [&]() {
+      base = bias - (m == -INFINITY ? 0.f : m);
+      sum = 0.f;
+    };
+    const auto weights = [&](int u, int i) {
+      typedef float f32x2 __attribute__((ext_vector_type(2)));
+      typedef E x2 __attribute__((ext_vector_type(2)));
+      f32x2 p;
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        p[e] = __builtin_amdgcn_exp2f(BENT ? sc[u][2 * i + e] + base : __builtin_fmaf(sc[u][2 * i + e], c, base));
+        sum += p[e];
+      }
+      pw[u][i] = __builtin_bit_cast(uint32_t, __builtin_convertvector(p, x2));
+    };
+    // the scores with cap and bias, in units of log2 e
+    const auto bent = [&](int u, int pos) {
+      if constexpr (BENT) {
+        if (a.cap > 0.f) {
+#pragma unroll
+          for (int e = 0; e < 16; ++e) sc[u][e] = bend.capped(sc[u][e]);
+        } else {
+#pragma unroll
+          for (int e = 0; e < 16; ++e) sc[u][e] *= bend.c;
+        }
+        if (a.slopes) {
+          const float far = (float)(stands - pos - 32 * u - 4 * kg);
+#pragma unroll
+          for (int e = 0; e < 16; ++e) sc[u][e] = __builtin_fmaf(-bend.slope, fabsf(far - (float)c_row(e)), sc[u][e]);
+        }
+      }
+    };
+    // where the weights have grown too large, or are a row's first, its maximum moves and they are made again
+    const auto settle = [&](int u) {
+      bool large = sum > kAttendLimit<E> || m == -INFINITY;
+      if (__any(large)) {
+        large = __shfl_xor((int)large, 32, 64) || large;  // the two lanes of a row
+        float top = sc[u][0];
+#pragma unroll
+        for (int e = 1; e < 16; ++e) top = fmaxf(top, sc[u][e]);
+        top = fmaxf(top, __shfl_xor(top, 32, 64)) * c;
+        if (large && top > m) {
+          const float f = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m - top);
+          m = top;
+          l *= f;
+#pragma unroll
+          for (int k = 0; k < MT; ++k) o[k] *= f;
+        }
+        begin_weights();
+#pragma unroll
+        for (int i = 0; i < 8; ++i) weights(u, i);
+      }
+      l += sum;
+    };
+    const auto weight8 = [&](int u, int w) {
+      return __builtin_bit_cast(x8, u32x4{pw[u][w], pw[u][w + 1], pw[u][w + 2], pw[u][w + 3]});
+    };
+    // a step that all of the wave's rows see whole
+    const auto whole_step = [&](const E* kp, const E* vp, int pos) {
+      x8 kf[F], vf[FV];
+      const auto key = [&](int i) { kf[i] = at_tile.rows(kp, i / KQ, i % KQ); };
+      const auto value = [&](int i) { vf[i] = at_tile.columns(vp, i / MT, i % MT); };
+#pragma unroll
+      for (int i = 0; i < 2 * kEarly && i < F; ++i) key(i);
+      const auto score = [&](int u, int i) {
+        if (i == 0) sc[u] = f32x16{};
+        sc[u] = mfma32(kf[u * KQ + i], qf[i], sc[u]);
+        if (u * KQ + i + 2 * kEarly < F) key(u * KQ + i + 2 * kEarly);
+      };
+      const auto gather = [&](int u, int i) { o[i % MT] = mfma32(vf[u * H + i], weight8(u, i / MT * 4), o[i % MT]); };
+      // An MFMA leaves the wave's issue free for about as long as two weights take.  So the first 32 keys' weights
+      // stand between the second's scores, the second's between the first's products with V.
+      __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+      for (int i = 0; i < KQ; ++i) {
+        score(0, i);
+        __builtin_amdgcn_sched_barrier(0);
+      }
+      bent(0, pos);
+      begin_weights();
+      if constexpr (NS == 2) {
+#pragma unroll
+        for (int i = 0; i < KQ; ++i) {
+          score(1, i);
+#pragma unroll
+          for (int e = i * 8 / KQ; e < (i + 1) * 8 / KQ; ++e) weights(0, e);
+#pragma unroll
+          for (int e = i * H / KQ; e < (i + 1) * H / KQ; ++e) value(e);
+          __builtin_amdgcn_sched_barrier(0);
+        }
+        settle(0);
+        bent(1, pos);
+        begin_weights();
+#pragma unroll
+        for (int i = 0; i < H; ++i) {
+          gather(0, i);
+#pragma unroll
+          for (int e = i * 8 / H; e < (i + 1) * 8 / H; ++e) weights(1, e);
+          value(H + i);
+          __builtin_amdgcn_sched_barrier(0);
+        }
+      } else {
+#pragma unroll
+        for (int i = 0; i < kEarly; ++i) value(i);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) weights(0, e);
+      }
+      settle(NS - 1);
+#pragma unroll
+      for (int i = 0; i < H; ++i) {
+        gather(NS - 1, i);
+        if (NS == 1 && i + kEarly < H) value(i + kEarly);
+        __builtin_amdgcn_sched_barrier(0);
+      }
+    };
+    // one that they do not: hidden keys leave the scores, and values that are not finite reach only rows that see them
+    const auto cut_step = [&](const E* kp, const E* vp, int pos, int shown) {
+      const int lo0 = lo - pos - 4 * kg, hi0 = hi - pos - 4 * kg;
+      const bool odd = tile_is_odd<E, D, GROUPS>(vp, lane);
+#pragma unroll
+      for (int u = 0; u < NS; ++u) {
+        sc[u] = f32x16{};
+#pragma unroll
+        for (int i = 0; i < KQ; ++i) sc[u] = mfma32(at_tile.rows(kp, u, i), qf[i], sc[u]);
+        bent(u, pos);
+#pragma unroll
+        for (int e = 0; e < 16; ++e) {
+          const int at = 32 * u + c_row(e);
+          if ((int)(at < lo0) | (int)(at >= hi0) | (int)!(shown >> (2 * u + (e >> 3)) & 1)) sc[u][e] = -INFINITY;
+        }
+        begin_weights();
+#pragma unroll
+        for (int e = 0; e < 8; ++e) weights(u, e);
+        settle(u);
+#pragma unroll
+        for (int i = 0; i < H; ++i) {
+          x8 v = at_tile.columns(vp, 2 * u + i / MT, i % MT);
+          if (odd) v = finite_values<E>(v);
+          o[i % MT] = mfma32(v, weight8(u, i / MT * 4), o[i % MT]);
+        }
+      }
+      if (odd)
+        add_odd<E, D, GROUPS>(vp, o, lane, [&](int i) { return pos + i >= lo && pos + i < hi && (shown >> (i >> 4) & 1); });
+    };
+
+    if (n > 0) {
+      int table = -1, table1 = -1, shown, shown1 = 0;
+      if constexpr (PAGED) {
+        table = entries(0);
+        table1 = entries(1);
+      }
+      shown = stage(table, 0);
+      __syncthreads();
+#pragma unroll 1
+      for (int j = 0; j < n; ++j) {
+        const int pos = pos0 + j * TOK;
+        if (j + 1 < n) shown1 = stage(table1, j + 1);
+        if constexpr (PAGED) table1 = entries(j + 2);
+        if (pos < most && pos + TOK > some) {
+          if (pos >= low && pos + TOK <= high && shown == (1 << GROUPS) - 1)
+            whole_step(kt[j & 1], vt[j & 1], pos);
+          else
+            cut_step(kt[j & 1], vt[j & 1], pos, shown);
+        }
+        shown = shown1;
+        __syncthreads();
+      }
+    }
+    l += __shfl_xor(l, 32, 64);
+    if (real) {
+      const int64_t at = (int64_t)t * a.heads + head;
+      const float inv = l == 0.f ? 0.f : 1.f / l;
+      if (splits == 1 || l != 0.f) {  // the join reads no part that saw nothing
+#pragma unroll
+        for (int k = 0; k < MT; ++k)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            f32x4 y{o[k][4 * e], o[k][4 * e + 1], o[k][4 * e + 2], o[k][4 * e + 3]};
+            const int d = 32 * k + 8 * e + 4 * kg;
+            if (splits == 1)
+              st4(static_cast<E*>(a.out) + at * D + d, l == 0.f ? zero4() : y * inv);
+            else
+              *reinterpret_cast<f32x4*>(a.ws + (at * splits + s) * D + d) = y;
+          }
+      }
+      if (kg == 0) {
+        if (splits > 1) {
+          for (int part = s; part < (padding ? splits : s + 1); ++part) {
+            float* ml = a.ws + a.T * a.heads * splits * D + (at * splits + part) * 2;
+            ml[0] = l == 0.f ? -INFINITY : m;
+            ml[1] = l;
+          }
+        } else if (a.lse) {
+          a.lse[at] = (m - bias + log2f(l)) * 0.693147180559945309f;
+        }
+      }
+    }
+  }
+}
+
+template <class E, int D, bool PAGED, bool BENT>
+void launch_core(const CoreArgs& a, int splits, hipStream_t st) {
+  const int64_t requests = PAGED ? a.N : 1, each = std::max<int64_t>(1, requests * a.kv_heads * splits);
+  const int64_t wanted = ((int64_t)(PAGED ? a.max_queries : a.T) * (a.heads / a.kv_heads) + kRows - 1) / kRows;
+  const int tiles = (int)std::max<int64_t>(1, std::min<int64_t>(wanted, (1 << 23) / each));
+  const int64_t blocks = requests * a.kv_heads * splits * tiles + (PAGED ? (int64_t)a.kv_heads * std::min(tiles, 16) : 0);
+  core_kernel<E, D, PAGED, BENT><<<(unsigned)blocks, 256, 0, st>>>(a, tiles, splits);
+}
+
+template <class E, int D>
+void by_kind(const CoreArgs& a, bool paged, int splits, hipStream_t st) {
+  const bool bent = a.cap > 0.f || a.slopes;
+  if (paged)
+    bent ? launch_core<E, D, true, true>(a, splits, st) : launch_core<E, D, true, false>(a, splits, st);
+  else
+    bent ? launch_core<E, D, false, true>(a, splits, st) : launch_core<E, D, false, false>(a, splits, st);
+}
+
+template <class E>
+void by_dim(const CoreArgs& a, bool paged, int splits, hipStream_t st) {
+  if (a.D == 64)
+    by_kind<E, 64>(a, paged, splits, st);
+  else if (a.D == 128)
+    by_kind<E, 128>(a, paged, splits, st);
+  else
+    by_kind<E, 256>(a, paged, splits, st);
+}
+
+}  // namespace
+
+void launch_core(const CoreArgs& a, bool paged, int splits, hipStream_t st) {
+  if (a.fp16)
+    by_dim<f16>(a, paged, splits, st);
+  else
+    by_dim<bf16>(a, paged, splits, st);
+}
+
+}  // namespace cqgdn

@@ -1,0 +1,568 @@
+// Gradients of the attention over packed rows.
+//
+// With p the softmax's weights of row t, dy its output's gradient and delta = dy.y (less the gradient of lse):
+//   dv_j = sum_t p_tj dy_t,  du_tj = p_tj (dy_t.v_j - delta_t),  dx = du times the cap's derivative,
+//   dq_t = scale sum_j dx_tj k_j,  dk_j = scale sum_t dx_tj q_t.
+// The weights come again from the scores and the rows' logarithms.  Two kernels, each of which owns what it sums, so
+// that nothing is added atomically and results do not depend on timing: one goes through the keys of 128 rows for dq
+// (S and dP once more than a kernel for all three would form them: 14 D operations a pair of row and key for 10), the
+// other through the rows that see 128 keys for dk and dv, 32 rows a step.
+//
+// The first leaves, for every 32 rows, the range of keys they see, their logarithms and deltas: the second finds its
+// steps in those ranges, 64 at a time.  Where its workgroups would not fill the CUs, each takes every n-th of the
+// steps, and fp32 parts are added up by a third kernel in their order.
+//
+// Scores, products, sums are fp32.  p and dx are rounded once to the rows' type for the second products.  In fp16, where
+// a dx may be too small or too large for the type, it goes in times a power of two that follows the largest so far (of
+// the row, or of the key), and p times 2^15.
+#include <hip/hip_runtime.h>
+
+#include <algorithm>
+
+#include "attn_core.hpp"
+
+namespace cqgdn {
+namespace {
+
+constexpr int kRows = 128;  // of a workgroup for dq, 32 a wave
+
+template <int D>
+constexpr int kTokens = D == 256 ? 32 : 64;
+
+template <class E>
+constexpr float kWeightBias = std::is_same<E, f16>::value ? 15.f : 0.f;
+
+// Two elements of the type from two floats
+template <class E>
+__device__ __forceinline__ uint32_t pack2(float x, float y) {
+  typedef float f32x2 __attribute__((ext_vector_type(2)));
+  typedef E x2 __attribute__((ext_vector_type(2)));
+  return __builtin_bit_cast(uint32_t, __builtin_convertvector(f32x2{x, y}, x2));
+}
+
+// The power of two that a lane's dx go with in fp16 (bf16: 1): the largest lies near 2^10 when it is set, and below
+// 2^15 always.  The two lanes of a column share it.
+template <class E>
+struct Range {
+  static constexpr bool on = std::is_same<E, f16>::value;
+  float f = on ? 0.f : 1.f;
+  // for 16 new dx; `acc`, the sums so far, move with it
+  template <int MT>
+  __device__ __forceinline__ void fit(const f32x16& x, f32x16 (&acc)[MT]) {
+    if constexpr (on) {
+      float top = fabsf(x[0]);
+#pragma unroll
+      for (int e = 1; e < 16; ++e) top = fmaxf(top, fabsf(x[e]));
+      bool move = top * f > 32768.f || (f == 0.f && top > 0.f);
+      if (__any(move)) {
+        move = __shfl_xor((int)move, 32, 64) || move;
+        top = fmaxf(top, __shfl_xor(top, 32, 64));
+        if (move) {
+          const int e = (int)(__builtin_bit_cast(uint32_t, top) >> 23) - 127;
+          const float g = __builtin_bit_cast(float, (uint32_t)(127 + min(max(10 - e, -126), 126)) << 23);
+          const float by = f == 0.f ? 0.f : g / f;
+#pragma unroll
+          for (int m = 0; m < MT; ++m) acc[m] *= by;
+          f = g;
+        }
+      }
+    }
+  }
+  // what the sums are to be multiplied with
+  __device__ __forceinline__ float back() const { return !on ? 1.f : f == 0.f ? 0.f : 1.f / f; }
+};
+
+template <class E, int D, bool BENT>
+__global__ __launch_bounds__(256, D == 256 ? 1 : 2) void dq_kernel(CoreGradArgs a, int tiles) {
+  typedef typename Vec<E>::x8 x8;
+  constexpr int TOK = kTokens<D>, NS = TOK / 32, KQ = D / 16, MT = D / 32, GROUPS = TOK / 16;
+  constexpr int LR = kLoadRows<D>, LOADS = TOK / 4 / LR;
+  __shared__ __align__(16) E kt[2][TOK * D];
+  __shared__ __align__(16) E vt[2][TOK * D];
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int n32 = lane & 31, kg = lane >> 5;
+  // launch order: as the forward pass's
+  const int real_blocks = a.kv_heads * tiles;
+  int b = blockIdx.x;
+  if ((b >> 8 & 1) && (b | 255) < real_blocks) b ^= 255;
+  const int tile = tiles - 1 - b / a.kv_heads, h = b % a.kv_heads;
+  const int group = a.group.d, T = (int)a.T, rows = T * group;
+  const TileOperands<E, D> at_tile(lane);
+
+  const auto limits = [&](int rho, int& lo, int& hi) {
+    const int t = a.group.of(rho < rows ? rho : 0);
+    lo = rho < rows && a.first ? max(a.first[t], 0) : 0;
+    hi = rho < rows ? min(a.visible[t], a.S) : 0;
+    if (lo >= hi) lo = hi = 0;
+  };
+  int first, last;
+  {
+    int lo0, hi0, lo1, hi1;
+    limits(tile * kRows + lane, lo0, hi0);
+    limits(tile * kRows + 64 + lane, lo1, hi1);
+    first = min(hi0 > 0 ? lo0 : INT32_MAX, hi1 > 0 ? lo1 : INT32_MAX);
+    last = max(hi0, hi1);
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) {
+      first = min(first, __shfl_xor(first, o, 64));
+      last = max(last, __shfl_xor(last, o, 64));
+    }
+    first = __builtin_amdgcn_readfirstlane(first);
+    last = __builtin_amdgcn_readfirstlane(last);
+  }
+  const int rho = tile * kRows + 32 * wave + n32;
+  const bool real = rho < rows;
+  int lo, hi;
+  limits(rho, lo, hi);
+  int some = hi > 0 ? lo : INT32_MAX, most = hi, low = lo, high = hi;
+#pragma unroll
+  for (int i = 1; i < 32; i <<= 1) {
+    some = min(some, __shfl_xor(some, i, 64));
+    most = max(most, __shfl_xor(most, i, 64));
+    low = max(low, __shfl_xor(low, i, 64));
+    high = min(high, __shfl_xor(high, i, 64));
+  }
+  some = __builtin_amdgcn_readfirstlane(some);
+  most = __builtin_amdgcn_readfirstlane(most);
+  low = __builtin_amdgcn_readfirstlane(low);
+  high = __builtin_amdgcn_readfirstlane(high);
+  const int block = tile * (kRows / 32) + wave;
+  if (h == 0 && lane == 0) static_cast<RowRange*>(a.ranges)[block] = RowRange{some, most, low, high};
+  const int row_t = real ? a.group.of(rho) : 0, head = h * group + (real ? rho - row_t * group : 0);
+  const int64_t at = (int64_t)row_t * a.heads + head;
+  const Bend bend(a.scale, BENT ? a.cap : 0.f, BENT ? a.slopes : nullptr, head);
+  const int stands = BENT && real ? (a.positions ? a.positions[row_t] : a.visible[row_t] - 1) : 0;
+
+  x8 qf[KQ], yf[KQ];  // lane (n32, kg): q and dy of row n32, dimensions 16 i + 8 kg ..
+  float delta = 0.f;
+  {
+    const E* q = static_cast<const E*>(a.q) + row_t * a.q_token + head * a.q_head + 8 * kg;
+    const E* dy = static_cast<const E*>(a.dy) + row_t * a.dy_token + head * a.dy_head + 8 * kg;
+    const E* y = static_cast<const E*>(a.y) + at * D + 8 * kg;
+    const u32x4 none{0, 0, 0, 0};
+#pragma unroll
+    for (int i = 0; i < KQ; ++i) {
+      qf[i] = __builtin_bit_cast(x8, real ? *reinterpret_cast<const u32x4*>(q + 16 * i) : none);
+      yf[i] = __builtin_bit_cast(x8, real ? *reinterpret_cast<const u32x4*>(dy + 16 * i) : none);
+      const f32x8 z = cvtf8(__builtin_bit_cast(x8, real ? *reinterpret_cast<const u32x4*>(y + 16 * i) : none)), w = cvtf8(yf[i]);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) delta = __builtin_fmaf(z[e], w[e], delta);
+    }
+    delta += __shfl_xor(delta, 32, 64);
+  }
+  if (a.dlse && real) delta -= a.dlse[at];
+  const float lse = real ? a.lse[at] * 1.44269504088896341f : 0.f;
+  {
+    RowBlock& x = static_cast<RowBlock*>(a.blocks)[(int64_t)h * tiles * (kRows / 32) + block];
+    if (kg == 0) {
+      x.lse[n32] = lse;
+      x.delta[n32] = delta;
+      x.lo[n32] = lo;
+      x.hi[n32] = hi;
+      if constexpr (BENT) {
+        x.stands[n32] = (float)stands;
+        x.slope[n32] = bend.slope;
+      }
+    }
+  }
+
+  f32x16 acc[MT];
+#pragma unroll
+  for (int i = 0; i < MT; ++i) acc[i] = f32x16{};
+  Range<E> range;
+  const float base = kWeightBias<E> - lse;
+
+  const auto stage = [&](int j) {
+    const int row0 = wave * (TOK / 4), pos = first + j * TOK;
+    E* const kd = kt[j & 1] + row0 * D;
+    E* const vd = vt[j & 1] + row0 * D;
+    const E* kb = static_cast<const E*>(a.k) + h * a.k_head + pos * a.k_token;
+    const E* vb = static_cast<const E*>(a.v) + h * a.v_head + pos * a.v_token;
+    const int end = a.S - 1 - pos;  // rows behind the last key: that key once more
+#pragma unroll
+    for (int i = 0; i < LOADS; ++i) {
+      const int row = row0 + i * LR + load_row<D>(lane), r = min(row, end), chunk = 8 * load_chunk<D>(lane, row);
+      dma16(kb + (r * (int)a.k_token + chunk), kd + i * LR * D);
+      dma16(vb + (r * (int)a.v_token + chunk), vd + i * LR * D);
+    }
+  };
+  const auto step = [&](const E* kp, const E* vp, int pos, auto whole) {
+    constexpr bool WHOLE = decltype(whole)::value;
+    const bool odd = !WHOLE && tile_is_odd<E, D, GROUPS>(kp, lane);
+    const int lo0 = lo - pos - 4 * kg, hi0 = hi - pos - 4 * kg;
+#pragma unroll
+    for (int u = 0; u < NS; ++u) {
+      f32x16 sc = f32x16{}, dp = f32x16{} - delta;
+#pragma unroll
+      for (int i = 0; i < KQ; ++i) {
+        sc = mfma32(at_tile.rows(kp, u, i), qf[i], sc);
+        dp = mfma32(at_tile.rows(vp, u, i), yf[i], dp);
+      }
+      const float far = (float)(stands - pos - 32 * u - 4 * kg);
+#pragma unroll
+      for (int e = 0; e < 16; ++e) {
+        float x = sc[e], rate = 1.f;
+        if constexpr (BENT) {
+          x = a.cap > 0.f ? bend.capped(x, rate) : x * bend.c;
+          x = __builtin_fmaf(-bend.slope, fabsf(far - (float)c_row(e)), x);
+          x = __builtin_amdgcn_exp2f(x + base);
+        } else {
+          x = __builtin_amdgcn_exp2f(__builtin_fmaf(x, bend.c, base));
+        }
+        x *= dp[e];
+        if constexpr (BENT) x *= rate;
+        const int at = 32 * u + c_row(e);
+        if (!WHOLE && ((int)(at < lo0) | (int)(at >= hi0))) x = 0.f;
+        dp[e] = x;
+      }
+      range.fit(dp, acc);
+#pragma unroll
+      for (int b = 0; b < 2; ++b) {
+        u32x4 w;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) w[e] = pack2<E>(dp[8 * b + 2 * e] * range.f, dp[8 * b + 2 * e + 1] * range.f);
+#pragma unroll
+        for (int m = 0; m < MT; ++m) {
+          x8 k = at_tile.columns(kp, 2 * u + b, m);
+          if (odd) k = finite_values<E>(k);
+          acc[m] = mfma32(k, __builtin_bit_cast(x8, w), acc[m]);
+        }
+      }
+    }
+    if (odd) add_odd<E, D, GROUPS>(kp, acc, lane, [&](int i) { return pos + i >= lo && pos + i < hi; });
+  };
+
+  const int n = last > 0 ? (last - first + TOK - 1) / TOK : 0;
+  if (n > 0) {
+    stage(0);
+    __syncthreads();
+#pragma unroll 1
+    for (int j = 0; j < n; ++j) {
+      const int pos = first + j * TOK;
+      if (j + 1 < n) stage(j + 1);
+      if (pos < most && pos + TOK > some) {
+        if (pos >= low && pos + TOK <= high)
+          step(kt[j & 1], vt[j & 1], pos, std::true_type{});
+        else
+          step(kt[j & 1], vt[j & 1], pos, std::false_type{});
+      }
+      __syncthreads();
+    }
+  }
+  if (real) {
+    const float f = a.scale * range.back() * (Range<E>::on ? 0x1p-15f : 1.f);
+#pragma unroll
+    for (int k = 0; k < MT; ++k)
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+        st4(static_cast<E*>(a.dq) + at * D + 32 * k + 8 * e + 4 * kg,
+            f32x4{acc[k][4 * e], acc[k][4 * e + 1], acc[k][4 * e + 2], acc[k][4 * e + 3]} * f);
+  }
+}
+
+// Keys of a workgroup for dk and dv, 32 a wave.  With D = 256 two waves share 32 keys, as one's sums would not fit its
+// registers: one forms S, the other dP, they exchange them through shared memory, and each sums half of the dimensions.
+template <int D>
+constexpr bool kPair = D == 256;
+template <int D>
+constexpr int kKeys = kPair<D> ? 64 : 128;
+
+// dk and dv of kKeys keys of a key head; part s of `splits` takes every splits-th block of 32 rows that sees any of them
+template <class E, int D, bool BENT>
+__global__ __launch_bounds__(256, 1) void dkv_kernel(CoreGradArgs a, int blocks, int splits) {
+  typedef typename Vec<E>::x8 x8;
+  constexpr bool PAIR = kPair<D>;
+  constexpr int KQ = D / 16, MT = D / 32 / (PAIR ? 2 : 1), LR = kLoadRows<D>, LOADS = 32 / 4 / LR;
+  constexpr int WORDS = sizeof(RowBlock) / 16;
+  __shared__ __align__(16) E qt[2][32 * D];
+  __shared__ __align__(16) E yt[2][32 * D];
+  __shared__ __align__(16) float swap[PAIR ? 4 : 1][PAIR ? 1024 : 4];
+  __shared__ __align__(16) RowBlock info[2];
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int n32 = lane & 31, kg = lane >> 5;
+  const int half = PAIR ? wave & 1 : 0;  // of the pair: 0 forms S and sums dimensions below D / 2, 1 dP and those above
+  // the first keys, which most rows see, first
+  const int h = blockIdx.x % a.kv_heads, s = blockIdx.x / a.kv_heads % splits;
+  const int k0 = blockIdx.x / (a.kv_heads * splits) * kKeys<D>;
+  const int group = a.group.d, rows = (int)a.T * group, mine = k0 + 32 * (PAIR ? wave >> 1 : wave);
+  const int key = mine + n32;
+  const bool real = key < a.S;
+  const TileOperands<E, D> at_tile(lane);
+  const Bend bend(a.scale, BENT ? a.cap : 0.f, nullptr, 0);
+
+  x8 kf[KQ], vf[PAIR ? 1 : KQ];  // lane (n32, kg): key n32, dimensions 16 i + 8 kg ..; of a pair, kf is V in the second
+  {
+    const E* k = static_cast<const E*>(a.k) + h * a.k_head + (real ? key : 0) * a.k_token + 8 * kg;
+    const E* v = static_cast<const E*>(a.v) + h * a.v_head + (real ? key : 0) * a.v_token + 8 * kg;
+    const u32x4 none{0, 0, 0, 0};
+#pragma unroll
+    for (int i = 0; i < KQ; ++i) {
+      kf[i] = __builtin_bit_cast(x8, real ? *reinterpret_cast<const u32x4*>((half ? v : k) + 16 * i) : none);
+      if constexpr (!PAIR) vf[i] = __builtin_bit_cast(x8, real ? *reinterpret_cast<const u32x4*>(v + 16 * i) : none);
+    }
+  }
+  f32x16 dk[MT], dv[MT];
+#pragma unroll
+  for (int i = 0; i < MT; ++i) dk[i] = dv[i] = f32x16{};
+  Range<E> range;
+
+  // The blocks of rows, 64 ranges at a time, a lane each: `left` are those of the present 64 that see any of the keys.
+  const RowRange* const ranges = static_cast<const RowRange*>(a.ranges);
+  int base = -64, turn = s;
+  RowRange mine64{};
+  uint64_t left = 0;
+  const auto next = [&](RowRange& x) -> int {  // the next block of this part, or -1
+    while (true) {
+      while (left) {
+        const int i = __builtin_ctzll(left);
+        left &= left - 1;
+        if (turn-- == 0) {
+          turn = splits - 1;
+          x.first = __builtin_amdgcn_readlane(mine64.first, i);
+          x.last = __builtin_amdgcn_readlane(mine64.last, i);
+          x.low = __builtin_amdgcn_readlane(mine64.low, i);
+          x.high = __builtin_amdgcn_readlane(mine64.high, i);
+          return base + i;
+        }
+      }
+      base += 64;
+      if (base >= blocks) return -1;
+      const bool there = base + lane < blocks;
+      mine64 = there ? ranges[base + lane] : RowRange{INT32_MAX, 0, 0, 0};
+      left = __ballot(there && mine64.last > k0 && mine64.first < k0 + kKeys<D>);
+    }
+  };
+  const auto stage = [&](int block, int buffer) {
+    const int row0 = wave * 8;
+    E* const qd = qt[buffer] + row0 * D;
+    E* const yd = yt[buffer] + row0 * D;
+#pragma unroll
+    for (int i = 0; i < LOADS; ++i) {
+      const int row = row0 + i * LR + load_row<D>(lane), rho = min(block * 32 + row, rows - 1);  // behind the last: that once more
+      const int t = a.group.of(rho), head = h * group + rho - t * group, chunk = 8 * load_chunk<D>(lane, row);
+      dma16(static_cast<const E*>(a.q) + t * a.q_token + head * a.q_head + chunk, qd + i * LR * D);
+      dma16(static_cast<const E*>(a.dy) + t * a.dy_token + head * a.dy_head + chunk, yd + i * LR * D);
+    }
+    if (wave == 0 && lane < (BENT ? WORDS : WORDS * 2 / 3))
+      dma16(reinterpret_cast<const char*>(static_cast<const RowBlock*>(a.blocks) + ((int64_t)h * blocks + block)) + 16 * lane, &info[buffer]);
+  };
+  f32x16 sc, dp;
+  const auto products = [&](const E* qp, const E* yp, const RowBlock& x) {
+    sc = f32x16{};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const f32x4 delta = *reinterpret_cast<const f32x4*>(x.delta + 8 * i + 4 * kg);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) dp[4 * i + e] = -delta[e];
+    }
+    if constexpr (PAIR) {
+      if (half) sc = dp;
+      const E* const p = half ? yp : qp;
+#pragma unroll
+      for (int i = 0; i < KQ; ++i) sc = mfma32(at_tile.rows(p, 0, i), kf[i], sc);
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        *reinterpret_cast<f32x4*>(swap[wave] + 256 * i + 4 * lane) = f32x4{sc[4 * i], sc[4 * i + 1], sc[4 * i + 2], sc[4 * i + 3]};
+    } else {
+#pragma unroll
+      for (int i = 0; i < KQ; ++i) {
+        sc = mfma32(at_tile.rows(qp, 0, i), kf[i], sc);
+        dp = mfma32(at_tile.rows(yp, 0, i), vf[i], dp);
+      }
+    }
+  };
+  const auto exchange = [&] {
+    if constexpr (PAIR) {
+      f32x16 other;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const f32x4 x = *reinterpret_cast<const f32x4*>(swap[wave ^ 1] + 256 * i + 4 * lane);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) other[4 * i + e] = x[e];
+      }
+      dp = half ? sc : other;
+      sc = half ? other : sc;
+    }
+  };
+  const auto sums = [&](const E* qp, const E* yp, const RowBlock& x, auto whole) {
+    constexpr bool WHOLE = decltype(whole)::value;
+    bool odd = false;
+    if constexpr (!WHOLE) odd = tile_is_odd<E, D, 2>(qp, lane) || tile_is_odd<E, D, 2>(yp, lane);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const f32x4 lse = *reinterpret_cast<const f32x4*>(x.lse + 8 * i + 4 * kg);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const int e = 4 * i + j, row = 8 * i + j + 4 * kg;
+        float p, rate = 1.f;
+        const float from = kWeightBias<E> - lse[j];
+        if constexpr (BENT) {
+          p = a.cap > 0.f ? bend.capped(sc[e], rate) : sc[e] * bend.c;
+          p = __builtin_fmaf(-x.slope[row], fabsf(x.stands[row] - (float)key), p);
+          p = __builtin_amdgcn_exp2f(p + from);
+        } else {
+          p = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[e], bend.c, from));
+        }
+        float dx = p * dp[e];
+        if constexpr (BENT) dx *= rate;
+        if constexpr (!WHOLE) {
+          const bool hidden = (int)(key < x.lo[row]) | (int)(key >= x.hi[row]);
+          if (hidden) p = dx = 0.f;
+        }
+        sc[e] = p;
+        dp[e] = dx;
+      }
+    }
+    range.fit(dp, dk);
+#pragma unroll
+    for (int b = 0; b < 2; ++b) {
+      u32x4 w, z;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        w[e] = pack2<E>(sc[8 * b + 2 * e], sc[8 * b + 2 * e + 1]);
+        z[e] = pack2<E>(dp[8 * b + 2 * e] * range.f, dp[8 * b + 2 * e + 1] * range.f);
+      }
+#pragma unroll
+      for (int m = 0; m < MT; ++m) {
+        x8 y = at_tile.columns(yp, b, half * MT + m), q = at_tile.columns(qp, b, half * MT + m);
+        if (odd) {
+          y = finite_values<E>(y);
+          q = finite_values<E>(q);
+        }
+        dv[m] = mfma32(y, __builtin_bit_cast(x8, w), dv[m]);
+        dk[m] = mfma32(q, __builtin_bit_cast(x8, z), dk[m]);
+      }
+    }
+    if (odd) {
+      const auto sees = [&](int i) { return key >= x.lo[i] && key < x.hi[i]; };
+      add_odd<E, D, 2>(qp, dk, lane, sees, half * MT);
+      add_odd<E, D, 2>(yp, dv, lane, sees, half * MT);
+    }
+  };
+
+  RowRange x, y;
+  int block = next(x), buffer = 0;
+  if (block >= 0) {
+    stage(block, 0);
+    __syncthreads();
+#pragma unroll 1
+    while (true) {
+      const int following = next(y);
+      if (following >= 0) stage(following, buffer ^ 1);
+      const bool any = x.last > mine && x.first < mine + 32;
+      if (any) products(qt[buffer], yt[buffer], info[buffer]);
+      if constexpr (PAIR) lds_barrier();
+      if (any) {
+        exchange();
+        if (x.low <= mine && mine + 32 <= x.high)
+          sums(qt[buffer], yt[buffer], info[buffer], std::true_type{});
+        else
+          sums(qt[buffer], yt[buffer], info[buffer], std::false_type{});
+      }
+      __syncthreads();
+      if (following < 0) break;
+      x = y;
+      buffer ^= 1;
+    }
+  }
+  if (real) {
+    const float f = a.scale * range.back() * (Range<E>::on ? 0x1p-15f : 1.f), g = Range<E>::on ? 0x1p-15f : 1.f;
+    const int64_t at = ((int64_t)key * a.kv_heads + h) * D + half * (D / 2);
+    float* const part = a.ws + (int64_t)s * 2 * a.S * a.kv_heads * D;
+#pragma unroll
+    for (int k = 0; k < MT; ++k)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const f32x4 u = f32x4{dk[k][4 * e], dk[k][4 * e + 1], dk[k][4 * e + 2], dk[k][4 * e + 3]} * f;
+        const f32x4 w = f32x4{dv[k][4 * e], dv[k][4 * e + 1], dv[k][4 * e + 2], dv[k][4 * e + 3]} * g;
+        const int d = 32 * k + 8 * e + 4 * kg;
+        if (splits == 1) {
+          st4(static_cast<E*>(a.dk) + at + d, u);
+          st4(static_cast<E*>(a.dv) + at + d, w);
+        } else {
+          *reinterpret_cast<f32x4*>(part + at + d) = u;
+          *reinterpret_cast<f32x4*>(part + (int64_t)a.S * a.kv_heads * D + at + d) = w;
+        }
+      }
+  }
+}
+
+// the parts of dk and dv, added up in their order, 4 values a thread
+template <class E>
+__global__ __launch_bounds__(256) void join_parts_kernel(const float* ws, int64_t size, int splits, E* dk, E* dv) {
+  const int64_t at = ((int64_t)blockIdx.x * 256 + threadIdx.x) * 4;
+  if (at >= 2 * size) return;
+  f32x4 y = *reinterpret_cast<const f32x4*>(ws + at);
+#pragma unroll 4
+  for (int s = 1; s < splits; ++s) y += *reinterpret_cast<const f32x4*>(ws + s * 2 * size + at);
+  st4(at < size ? dk + at : dv + (at - size), y);
+}
+
+int64_t row_blocks(int64_t T, int group) { return (T * group + kRows - 1) / kRows * (kRows / 32); }
+
+// parts of the keys' gradients: two rounds of workgroups at least
+int key_parts(int64_t T, int64_t S, int kv_heads, int group, int D) {
+  const int keys = D == 256 ? kKeys<256> : kKeys<128>;
+  const int64_t each = std::max<int64_t>(1, (S + keys - 1) / keys * kv_heads);
+  return (int)std::max<int64_t>(1, std::min<int64_t>({1024 / each, 16, row_blocks(T, group)}));
+}
+
+template <class E, int D, bool BENT>
+void launch_grad(const CoreGradArgs& a, hipStream_t st) {
+  const int group = a.heads / a.kv_heads, tiles = (int)(row_blocks(a.T, group) / (kRows / 32));
+  const int splits = key_parts(a.T, a.S, a.kv_heads, group, D);
+  if (tiles > 0) dq_kernel<E, D, BENT><<<tiles * a.kv_heads, 256, 0, st>>>(a, tiles);
+  if (a.S == 0 || !a.dk) return;
+  dkv_kernel<E, D, BENT><<<(unsigned)((a.S + kKeys<D> - 1) / kKeys<D> * a.kv_heads * splits), 256, 0, st>>>(a, tiles * (kRows / 32), splits);
+  if (splits > 1) {
+    const int64_t size = (int64_t)a.S * a.kv_heads * D;
+    join_parts_kernel<E><<<(unsigned)((2 * size + 1023) / 1024), 256, 0, st>>>(a.ws, size, splits, static_cast<E*>(a.dk), static_cast<E*>(a.dv));
+  }
+}
+
+template <class E, int D>
+void by_kind(const CoreGradArgs& a, hipStream_t st) {
+  a.cap > 0.f || a.slopes ? launch_grad<E, D, true>(a, st) : launch_grad<E, D, false>(a, st);
+}
+
+template <class E>
+void by_dim(const CoreGradArgs& a, hipStream_t st) {
+  if (a.D == 64)
+    by_kind<E, 64>(a, st);
+  else if (a.D == 128)
+    by_kind<E, 128>(a, st);
+  else
+    by_kind<E, 256>(a, st);
+}
+
+}  // namespace
+
+// the row blocks, their ranges, and the parts where there are several
+static size_t backward_layout(int64_t T, int64_t S, int heads, int kv_heads, int D, size_t& ranges, size_t& parts) {
+  const int group = heads / kv_heads;
+  const int64_t blocks = row_blocks(T, group);
+  const int splits = key_parts(T, S, kv_heads, group, D);
+  ranges = (size_t)blocks * kv_heads * sizeof(RowBlock);
+  parts = ((ranges + blocks * sizeof(RowRange)) + 255) / 256 * 256;
+  return parts + (splits > 1 ? (size_t)splits * 2 * S * kv_heads * D * sizeof(float) : 0);
+}
+size_t core_backward_bytes(int64_t T, int64_t S, int heads, int kv_heads, int D) {
+  size_t ranges, parts;
+  return backward_layout(T, S, heads, kv_heads, D, ranges, parts);
+}
+
+void launch_core_backward(const CoreGradArgs& args, hipStream_t st) {
+  CoreGradArgs a = args;
+  size_t ranges, parts;
+  backward_layout(a.T, a.S, a.heads, a.kv_heads, a.D, ranges, parts);
+  char* const ws = reinterpret_cast<char*>(args.ws);
+  a.blocks = ws;
+  a.ranges = ws + ranges;
+  a.ws = reinterpret_cast<float*>(ws + parts);
+  if (a.fp16)
+    by_dim<f16>(a, st);
+  else
+    by_dim<bf16>(a, st);
+}
+
+}  // namespace cqgdn

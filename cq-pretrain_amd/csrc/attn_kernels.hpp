@@ -47,6 +47,16 @@ struct RotaryArgs {
 };
 void launch_rotary(const RotaryArgs& a, hipStream_t st);
 
+// Rows put into the 16-bit pages: queries and keys turned, queries out as rotary has them.
+struct AppendArgs : RotaryArgs {
+  const void* v;
+  int64_t v_token, v_head;
+  const int32_t* slots;
+  void* data;                  // [pages][kv_heads][2][page][D]
+  int slot_count, page_shift;
+};
+void launch_append(const AppendArgs& a, hipStream_t st);
+
 struct PagesArgs {
   const int32_t *cached, *fresh;  // [N]
   int N;
@@ -102,5 +112,34 @@ size_t attend_workspace_bytes(int64_t T, int64_t N, int heads, int kv_heads, int
 void launch_attend(const AttendArgs& a, hipStream_t st);
 // the kernel for many rows a request (attn_tile.hip); with more than one split its parts are joined by the caller
 void launch_attend_tiles(const AttendArgs& a, int splits, hipStream_t st);
+// adds up the parts of a call
+void launch_attend_join(const AttendArgs& a, int splits, hipStream_t st);
+
+// Attention over 16-bit keys and values: rows of packed documents, or the pages of a 16-bit cache.  Row t sees the
+// keys [first[t], limit[t]) of the rows, or the positions [limit[t] - window, limit[t]) of its request's pages.
+struct CoreArgs : AttendArgs {
+  const void *k, *v;           // rows [S][kv_heads][D], or the pages [pages][kv_heads][2][page][D] in `data`
+  int64_t k_token, k_head, v_token, v_head;
+  int S;
+  const int32_t* first;        // or null: from 0
+  const int32_t* positions;    // where row t stands, for the bias; null: at its last key
+  float cap;                   // 0: none
+  const float* slopes;         // [heads], or null
+};
+// many rows, over packed rows or (paged) the pages; with more than one split its parts are joined by the caller
+void launch_core(const CoreArgs& a, bool paged, int splits, hipStream_t st);
+// few rows a request, over the pages, in `splits` parts of `per` steps of 64 positions
+void launch_core_few(const CoreArgs& a, int splits, int per, hipStream_t st);
+
+// Its gradients, over packed rows; `lse` is read, `ws` is core_backward_bytes() bytes.
+struct CoreGradArgs : CoreArgs {
+  const void *dy, *y;          // the output's gradient (strides in elements) and the output, dense
+  int64_t dy_token, dy_head;
+  const float* dlse;           // [T][heads], or null
+  void *dq, *dk, *dv;          // dense
+  void *ranges, *blocks;       // in the workspace: RowRange and RowBlock of each 32 rows
+};
+size_t core_backward_bytes(int64_t T, int64_t S, int heads, int kv_heads, int D);
+void launch_core_backward(const CoreGradArgs& a, hipStream_t st);
 
 }  // namespace cqgdn

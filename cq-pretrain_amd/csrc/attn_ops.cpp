@@ -16,48 +16,14 @@
 #include <ATen/ATen.h>
 #include <ATen/ops/_make_dual.h>
 #include <ATen/ops/as_strided_native.h>
-#include <c10/core/DeviceGuard.h>
-#include <c10/hip/HIPStream.h>
 #include <torch/csrc/autograd/custom_function.h>
 #include <torch/library.h>
 
-#include "cqgdn.h"
+#include "attn_ops.hpp"
 
 namespace {
 
 using at::Tensor;
-
-hipStream_t stream_of(const Tensor& t) { return c10::hip::getCurrentHIPStream(t.device().index()).stream(); }
-
-void check(int rc, const char* what) {
-  if (rc == CQGDN_OK) return;
-  TORCH_CHECK_VALUE(rc != CQGDN_EINVAL, what, ": ", cqgdn_last_error());
-  TORCH_CHECK_NOT_IMPLEMENTED(rc != CQGDN_EUNSUPPORTED, what, ": ", cqgdn_last_error());
-  TORCH_CHECK(false, what, ": ", cqgdn_last_error());
-}
-
-void on_one_gpu(std::initializer_list<const Tensor*> all) {
-  const auto device = (*all.begin())->device();
-  for (const Tensor* x : all) TORCH_CHECK_VALUE(x->device() == device, "tensors lie on different devices");
-  TORCH_CHECK_VALUE(device.is_cuda(), "the hip GDN backend requires tensors on a ROCm GPU");
-}
-
-int dtype_code(const Tensor& x, const char* name) {
-  const auto t = x.scalar_type();
-  TORCH_CHECK_VALUE(t == at::kBFloat16 || t == at::kHalf, name, " must be bf16 or fp16");
-  return t == at::kHalf ? CQGDN_F16 : CQGDN_BF16;
-}
-
-void int32_vector(const Tensor& x, const char* name) {
-  TORCH_CHECK_VALUE(x.dim() == 1 && x.scalar_type() == at::kInt, name, " must be an int32 vector");
-}
-
-// x as the kernels read rows of heads: unit stride within a head, 16-byte aligned rows
-Tensor head_rows(const Tensor& x) {
-  const bool fit = x.stride(2) == 1 && x.stride(0) % 8 == 0 && x.stride(1) % 8 == 0 &&
-                   reinterpret_cast<uintptr_t>(x.data_ptr()) % 16 == 0;
-  return fit ? x : x.clone(at::MemoryFormat::Contiguous);
-}
 
 // n elements of the vector x from `at` on: a view made without the dispatcher's overhead, which seven narrow()
 // would cost more of than the kernel takes

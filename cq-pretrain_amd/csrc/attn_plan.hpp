@@ -59,4 +59,11 @@ inline AttendPlan attend_plan(int64_t N, int kv_heads, int group, int D, int max
   return {false, (int)splits, (int)(times * kWaves)};
 }
 
+// Parts of the keys in a call over packed rows: as many as give the CUs the workgroups that they hold, each of at least
+// 512 keys.
+inline int core_parts(int64_t T, int64_t S, int heads, int kv_heads, int D) {
+  const int64_t blocks = (T * (heads / kv_heads) + 127) / 128 * kv_heads, fit = D == 256 ? 256 : D == 64 ? 768 : 512;
+  return (int)std::max<int64_t>(1, std::min<int64_t>({S / 512, kMaxSplits, fit / std::max<int64_t>(blocks, 1)}));
+}
+
 }  // namespace cqgdn

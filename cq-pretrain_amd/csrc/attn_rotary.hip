@@ -13,7 +13,7 @@
 
 #include <algorithm>
 
-#include "attn_kernels.hpp"
+#include "attn_turn.hpp"
 #include "cqgdn.h"
 
 namespace cqgdn {
@@ -23,51 +23,13 @@ constexpr int kThreads = 256;
 constexpr int kTogether = 4;      // items of a thread whose loads are under way at once
 constexpr int kMostPairs = 4096;  // of a workgroup's tokens: 32 KB of sines and cosines
 
-__device__ __forceinline__ void turn(uint64_t fraction, float& s, float& c) {
-  const int32_t hi = (int32_t)(fraction >> 32);
-  const uint32_t quadrant = ((uint32_t)hi + 0x20000000u) >> 30;
-  // the rest after whole quadrants, in +-1/8 turn
-  const float x = (float)(int32_t)((uint32_t)hi - (quadrant << 30)) * 1.46291807926715968e-9f;  // 2 pi / 2^32
-  const float z = x * x;
-  const float sp =
-      x + x * z * (-1.f / 6 + z * (1.f / 120 + z * (-1.f / 5040 + z * (1.f / 362880))));
-  const float cp = 1.f + z * (-0.5f + z * (1.f / 24 + z * (-1.f / 720 + z * (1.f / 40320 + z * (-1.f / 3628800)))));
-  const float a = (quadrant & 1) ? cp : sp, b = (quadrant & 1) ? sp : cp;
-  s = (quadrant & 2) ? -a : a;
-  c = ((quadrant + 1) & 2) ? -b : b;
-}
-
-// Two vectors of VEC values of one head, one of either half of the values that turn (or of those that pass): lanes
-// side by side read side by side in both.
-template <int VEC, bool ADJ>
-struct Place {
-  int at0, at1;
-  bool rot;
-  __device__ __forceinline__ Place(const RotaryArgs& a, int u, int turned) : rot(u < turned) {
-    at0 = rot ? u * (ADJ && VEC == 1 ? 2 : VEC) : a.rotary + (u - turned) * VEC;
-    at1 = at0 + (rot ? (ADJ && VEC == 1 ? 1 : a.rotary / 2) : (a.D - a.rotary) / 2);
-  }
-  // the first pair of the vectors' j-th run of RUN pairs
-  static constexpr int RUN = ADJ && VEC > 1 ? VEC / 2 : VEC;
-  static __device__ __forceinline__ int pair(const RotaryArgs& a, int u, int j) { return u * RUN + (j ? a.rotary / 4 : 0); }
-};
-
-__device__ __forceinline__ void angle(const RotaryArgs& a, int64_t t, int pair, float& s, float& c) {
-  const int ax = min(max(a.axis[pair], 0), a.axes - 1);
-  const int64_t at = ax * a.axis_stride + t;
-  const int64_t p = a.wide ? static_cast<const int64_t*>(a.positions)[at]
-                           : (int64_t)static_cast<const int32_t*>(a.positions)[at];
-  turn((uint64_t)p * a.turns[pair], s, c);
-  if (a.back) s = -s;
-}
-
 // A workgroup takes all heads of `tokens` tokens.  Their sines and cosines (some 40 operations each) are worked out
 // once, into LDS, while the first loads are under way; then its threads go through the tokens' rows in the order
 // of memory, kTogether items (a unit of a head) each at once.  `slots` items fit the workgroup.
 template <class T, int VEC, bool ADJ>
 __global__ __launch_bounds__(kThreads) void rotary_kernel(RotaryArgs a, int units, int turned, int tokens, int slots) {
   typedef T P __attribute__((ext_vector_type(VEC)));
-  typedef Place<VEC, ADJ> L;
+  typedef TurnPlace<VEC, ADJ> L;
   extern __shared__ __align__(16) float lds[];  // sines [tokens][rotary / 2], then cosines
   const int tid = threadIdx.x, pairs = a.rotary / 2, heads = a.heads[0] + a.heads[1];
   const int64_t t0 = (int64_t)blockIdx.x * tokens;
@@ -142,7 +104,7 @@ template <class T, bool ADJ>
 __global__ __launch_bounds__(kThreads) void rotary_any_kernel(RotaryArgs a, int units, int turned) {
   const int64_t t = blockIdx.x;
   for (int u = threadIdx.x; u < units; u += kThreads) {
-    const Place<1, ADJ> place(a, u, turned);
+    const TurnPlace<1, ADJ> place(a, u, turned);
     float s = 0.f, c = 1.f;
     if (place.rot) angle(a, t, u, s, c);
     for (int g = 0; g < a.heads[0] + a.heads[1]; ++g) {

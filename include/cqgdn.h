@@ -468,6 +468,62 @@ int cqgdn_kv4_attend(const void* q, int64_t q_token, int64_t q_head, int dtype, 
                      size_t workspace_bytes, void* stream);
 
 /*
+ * The 16-bit cache of keys and values: data [pages][kv_heads][2][page][head_dim], bf16 or fp16 (dtype), the keys of a
+ * page before its values.  head_dim is 64, 128 or 256, page a power of two from 16 to 65536.  cqgdn_kv16_append puts the
+ * rows k, v [T][kv_heads][head_dim] into the slots (page * page_size + offset; slots outside [0, pages * page) are
+ * skipped, and none may be given twice), k turned by the positions of its tokens as by cqgdn_rotary, and writes q
+ * [T][q_heads][head_dim], turned likewise, to q_out (dense).  With rotary_dim 0 rows go as they are, and positions,
+ * turns and axis may be null; with q_heads 0 there are no queries.
+ */
+int cqgdn_kv16_append(const void* q, int64_t q_token, int64_t q_head, int q_heads, const void* k, int64_t k_token,
+                      int64_t k_head, const void* v, int64_t v_token, int64_t v_head, int64_t T, int kv_heads,
+                      int head_dim, int rotary_dim, int adjacent, int dtype, const void* positions, int wide_positions,
+                      int64_t axis_stride, int axes, const uint64_t* turns, const int32_t* axis, const int32_t* slots,
+                      void* q_out, void* data, int64_t pages, int page, void* stream);
+
+/*
+ * Attention over the 16-bit pages: rows, requests, tables, limits and window as for cqgdn_kv4_attend, with scores
+ *   u_j = cap tanh(scale q k_j / cap) - slopes[h] |positions[t] - j|
+ * of query head h and position j, p_j = exp(u_j).  cap 0: not capped; slopes NULL: no bias; positions NULL: rows stand
+ * at visible[t] - 1.  A capped score is off by up to 2^-22 of the cap.  A value that is not finite reaches the rows that
+ * see it, with any weight, and no other.
+ */
+size_t cqgdn_kv16_attend_workspace_size(int64_t T, int N, int heads, int kv_heads, int head_dim, int max_queries,
+                                        int columns, int page);
+int cqgdn_kv16_attend(const void* q, int64_t q_token, int64_t q_head, int dtype, int64_t T, int heads, int head_dim,
+                      const void* data, int64_t pages, int page, int kv_heads, const int32_t* tables,
+                      int64_t table_stride, int columns, const int32_t* starts, int N, const int32_t* visible,
+                      int window, const int32_t* positions, float scale, float cap, const float* slopes,
+                      int max_queries, void* out, float* lse, void* workspace, size_t workspace_bytes, void* stream);
+
+/*
+ * Attention over packed rows, for training: row t sees the keys first[t] <= j < limit[t] (first NULL: from 0; beyond S
+ * there are none), and out[t][h] = sum_j p_j v_j / sum_j p_j with the scores above, distances counted from positions[t]
+ * (NULL: limit[t] - 1).  Query head h reads key head h / (heads / kv_heads); rows that see nothing are zero.  Scores,
+ * sums and results are held in fp32; each weight is rounded to dtype for its product with v.
+ *   q, out   : bf16 or fp16 (dtype) [T][heads][head_dim], out dense; k, v: [S][kv_heads][head_dim].  Strides in
+ *              elements, multiples of 8, below 2^24 from token to token; rows 16-byte aligned
+ *   lse      : fp32 [T][heads]: log sum_j exp(u_j), -inf for rows that see nothing; the backward pass reads it (or NULL)
+ *   workspace: >= cqgdn_attend_fwd_workspace_size() bytes (it may be 0), 256-byte aligned
+ * cqgdn_attend_bwd writes the gradients dq, dk, dv (dense, of dtype) of a loss whose gradients by out and lse are dy
+ * and dlse (NULL: 0); dk and dv may both be NULL.  Nothing is added atomically: the same inputs give the same bits.  Keys that no row sees, and rows
+ * that see none, get zero.
+ */
+size_t cqgdn_attend_fwd_workspace_size(int64_t T, int64_t S, int heads, int kv_heads, int head_dim);
+int cqgdn_attend_fwd(const void* q, int64_t q_token, int64_t q_head, const void* k, int64_t k_token, int64_t k_head,
+                     const void* v, int64_t v_token, int64_t v_head, int dtype, int64_t T, int64_t S, int heads,
+                     int kv_heads, int head_dim, const int32_t* first, const int32_t* limit, const int32_t* positions,
+                     float scale, float cap, const float* slopes, void* out, float* lse, void* workspace,
+                     size_t workspace_bytes, void* stream);
+size_t cqgdn_attend_bwd_workspace_size(int64_t T, int64_t S, int heads, int kv_heads, int head_dim);
+int cqgdn_attend_bwd(const void* q, int64_t q_token, int64_t q_head, const void* k, int64_t k_token, int64_t k_head,
+                     const void* v, int64_t v_token, int64_t v_head, const void* dy, int64_t dy_token, int64_t dy_head,
+                     int dtype, int64_t T, int64_t S, int heads, int kv_heads, int head_dim, const int32_t* first,
+                     const int32_t* limit, const int32_t* positions, float scale, float cap, const float* slopes,
+                     const void* out, const float* lse, const float* dlse, void* dq, void* dk, void* dv,
+                     void* workspace, size_t workspace_bytes, void* stream);
+
+/*
  * Instrumentation (no counterpart in the reference; used by the benchmark to
  * price one kernel against its roofline).  cqgdn_timer_arm(name, n) makes the
  * library bracket each of the next n launches of the named kernel with
