@@ -2,7 +2,7 @@
 //
 // Row (t, query head) gets sum_j p_j v_j / sum_j p_j over the keys j that it sees, p_j = exp(u_j - m), u_j its capped
 // and biased score, in one pass with a running maximum m.  A workgroup takes 128 rows of one key head, 32 a wave (with
-// grouped heads a row is a token and one of the group's query heads, so that the group shares K and V), and kTokens
+// grouped heads a row is a token and one of the group's query heads, so that the group shares K and V), and 64
 // keys a step, whose K and V rows go from memory to shared memory without passing registers, two steps deep.  S^T =
 // K Q^T and O^T = V^T P^T: a lane owns a row, so limits, maximum, sum and the head's slope are the lane's own and S^T's
 // layout is already an operand of O^T.  Steps that all of a wave's rows see whole, most of them, have no masks.
@@ -22,19 +22,16 @@ namespace {
 constexpr int kRows = 128;  // of a workgroup, 32 a wave
 constexpr int kEarly = 4;   // MFMA operands read from LDS ahead of their use
 
-template <int D>
-constexpr int kTokens = D == 256 ? 32 : 64;
-
 // PAGED: keys from the pages of a cache; BENT: scores are capped or biased
 template <class E, int D, bool PAGED, bool BENT>
 __global__ __launch_bounds__(256, D == 256 ? 1 : D == 64 ? 3 : 2) void core_kernel(CoreArgs a, int tiles, int splits) {
   typedef typename Vec<E>::x8 x8;
-  constexpr int TOK = kTokens<D>, NS = TOK / 32, KQ = D / 16, MT = D / 32;
-  constexpr int F = NS * KQ, FV = 2 * NS * MT, H = FV / NS;  // operands of a step: K's, V's, V's for 32 keys
-  constexpr int LR = kLoadRows<D>, LOADS = TOK / 4 / LR;     // rows a load, loads a wave and step of K (and of V)
+  constexpr int TOK = kTile, KQ = D / 16, MT = D / 32;
+  constexpr int F = 2 * KQ, H = 2 * MT;  // operands of a step: K's, and V's for 32 keys
+  constexpr int kFirst = H < 8 ? H : 8;  // V's that are read while the scores of the second 32 keys are formed
   constexpr int GROUPS = TOK / 16;
-  __shared__ __align__(16) E kt[2][TOK * D];
-  __shared__ __align__(16) E vt[2][TOK * D];
+  __shared__ __align__(16) E kt[2][kTileSize<D>];
+  __shared__ __align__(16) E vt[2][kTileSize<D>];
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int n32 = lane & 31, kg = lane >> 5;
   // Launch order: the last tiles, which see most, first; every other round of 256 workgroups reversed, so that
@@ -139,37 +136,26 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : D == 64 ? 3 : 2) void core_kern
     };
     // step j's rows of the wave on their way into the tiles.  Returns which of the step's 16 positions are shown.
     const auto stage = [&](int table, int j) {
-      const int row0 = wave * (TOK / 4), pos = pos0 + j * TOK;
-      E* const kd = kt[j & 1] + row0 * D;
-      E* const vd = vt[j & 1] + row0 * D;
+      const int pos = pos0 + j * TOK;
       if constexpr (PAGED) {
-        const uint32_t page = __builtin_amdgcn_readlane(table, row0 / 16);
-        const int at = (pos + row0) & (size - 1);
-        const E* base = reinterpret_cast<const E*>(a.data) + ((int64_t)(page < a.page_count ? page : 0) * a.kv_heads + h) * 2 * size * D;
-#pragma unroll
-        for (int i = 0; i < LOADS; ++i) {
-          const int row = row0 + i * LR + load_row<D>(lane);
-          const int off = (at + row - row0) * D + 8 * load_chunk<D>(lane, row);
-          dma16(base + off, kd + i * LR * D);
-          dma16(base + size * D + off, vd + i * LR * D);
-        }
+        const uint32_t page = __builtin_amdgcn_readlane(table, wave);
+        const int at = (pos + 16 * wave) & (size - 1);
+        const E* base = reinterpret_cast<const E*>(a.data) +
+                        (((int64_t)(page < a.page_count ? page : 0) * a.kv_heads + h) * 2 * size + at) * D;
+        load_rows16<E, D>(base, lane / 4 * D, kt[j & 1], wave, lane);
+        load_rows16<E, D>(base + size * D, lane / 4 * D, vt[j & 1], wave, lane);
         return (int)__ballot((uint32_t)table < a.page_count) & ((1 << GROUPS) - 1);
       } else {
-        const E* kb = static_cast<const E*>(a.k) + h * a.k_head + pos * a.k_token;
-        const E* vb = static_cast<const E*>(a.v) + h * a.v_head + pos * a.v_token;
-        const int end = a.S - 1 - pos;  // rows behind the last key: that key once more
-#pragma unroll
-        for (int i = 0; i < LOADS; ++i) {
-          const int row = row0 + i * LR + load_row<D>(lane), at = min(row, end), chunk = 8 * load_chunk<D>(lane, row);
-          dma16(kb + (at * (int)a.k_token + chunk), kd + i * LR * D);
-          dma16(vb + (at * (int)a.v_token + chunk), vd + i * LR * D);
-        }
+        // rows behind the last key: that key once more
+        const uint32_t row = min(16 * wave + lane / 4, a.S - 1 - pos);
+        load_rows16<E, D>(static_cast<const E*>(a.k) + h * a.k_head + pos * a.k_token, row * (uint32_t)a.k_token, kt[j & 1], wave, lane);
+        load_rows16<E, D>(static_cast<const E*>(a.v) + h * a.v_head + pos * a.v_token, row * (uint32_t)a.v_token, vt[j & 1], wave, lane);
         return (1 << GROUPS) - 1;
       }
     };
-    f32x16 sc[NS];
+    f32x16 sc[2];
     // the weights of 32 keys, two a part, in the order of their scores
-    uint32_t pw[NS][8];
+    uint32_t pw[2][8];
     float base, sum;
     const auto begin_weights = [&]() {
       base = bias - (m == -INFINITY ? 0.f : m);
@@ -197,9 +183,9 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : D == 64 ? 3 : 2) void core_kern
           for (int e = 0; e < 16; ++e) sc[u][e] *= bend.c;
         }
         if (a.slopes) {
-          const float far = (float)(stands - pos - 32 * u - 4 * kg);
+          const float far = (float)(stands - pos - 16 * kg);
 #pragma unroll
-          for (int e = 0; e < 16; ++e) sc[u][e] = __builtin_fmaf(-bend.slope, fabsf(far - (float)c_row(e)), sc[u][e]);
+          for (int e = 0; e < 16; ++e) sc[u][e] = __builtin_fmaf(-bend.slope, fabsf(far - (float)c_row(u, e)), sc[u][e]);
         }
       }
     };
@@ -230,9 +216,9 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : D == 64 ? 3 : 2) void core_kern
     };
     // a step that all of the wave's rows see whole
     const auto whole_step = [&](const E* kp, const E* vp, int pos) {
-      x8 kf[F], vf[FV];
+      x8 kf[F], vf[2][H];
       const auto key = [&](int i) { kf[i] = at_tile.rows(kp, i / KQ, i % KQ); };
-      const auto value = [&](int i) { vf[i] = at_tile.columns(vp, i / MT, i % MT); };
+      const auto value = [&](int u, int i) { vf[u][i] = at_tile.columns(vp, u, i / MT, i % MT); };
 #pragma unroll
       for (int i = 0; i < 2 * kEarly && i < F; ++i) key(i);
       const auto score = [&](int u, int i) {
@@ -240,7 +226,7 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : D == 64 ? 3 : 2) void core_kern
         sc[u] = mfma32(kf[u * KQ + i], qf[i], sc[u]);
         if (u * KQ + i + 2 * kEarly < F) key(u * KQ + i + 2 * kEarly);
       };
-      const auto gather = [&](int u, int i) { o[i % MT] = mfma32(vf[u * H + i], weight8(u, i / MT * 4), o[i % MT]); };
+      const auto gather = [&](int u, int i) { o[i % MT] = mfma32(vf[u][i], weight8(u, i / MT * 4), o[i % MT]); };
       // An MFMA leaves the wave's issue free for about as long as two weights take.  So the first 32 keys' weights
       // stand between the second's scores, the second's between the first's products with V.
       __builtin_amdgcn_sched_barrier(0);
@@ -251,55 +237,51 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : D == 64 ? 3 : 2) void core_kern
       }
       bent(0, pos);
       begin_weights();
-      if constexpr (NS == 2) {
 #pragma unroll
-        for (int i = 0; i < KQ; ++i) {
-          score(1, i);
+      for (int i = 0; i < KQ; ++i) {
+        score(1, i);
 #pragma unroll
-          for (int e = i * 8 / KQ; e < (i + 1) * 8 / KQ; ++e) weights(0, e);
+        for (int e = i * 8 / KQ; e < (i + 1) * 8 / KQ; ++e) weights(0, e);
 #pragma unroll
-          for (int e = i * H / KQ; e < (i + 1) * H / KQ; ++e) value(e);
-          __builtin_amdgcn_sched_barrier(0);
-        }
-        settle(0);
-        bent(1, pos);
-        begin_weights();
-#pragma unroll
-        for (int i = 0; i < H; ++i) {
-          gather(0, i);
-#pragma unroll
-          for (int e = i * 8 / H; e < (i + 1) * 8 / H; ++e) weights(1, e);
-          value(H + i);
-          __builtin_amdgcn_sched_barrier(0);
-        }
-      } else {
-#pragma unroll
-        for (int i = 0; i < kEarly; ++i) value(i);
-#pragma unroll
-        for (int e = 0; e < 8; ++e) weights(0, e);
+        for (int e = i * kFirst / KQ; e < (i + 1) * kFirst / KQ; ++e) value(0, e);
+        __builtin_amdgcn_sched_barrier(0);
       }
-      settle(NS - 1);
+      settle(0);
+      bent(1, pos);
+      begin_weights();
 #pragma unroll
       for (int i = 0; i < H; ++i) {
-        gather(NS - 1, i);
-        if (NS == 1 && i + kEarly < H) value(i + kEarly);
+        gather(0, i);
+#pragma unroll
+        for (int e = i * 8 / H; e < (i + 1) * 8 / H; ++e) weights(1, e);
+        if (i + kFirst < H)
+          value(0, i + kFirst);
+        else
+          value(1, i + kFirst - H);
+        __builtin_amdgcn_sched_barrier(0);
+      }
+      settle(1);
+#pragma unroll
+      for (int i = 0; i < H; ++i) {
+        gather(1, i);
+        if (i + kFirst < H) value(1, i + kFirst);
         __builtin_amdgcn_sched_barrier(0);
       }
     };
     // one that they do not: hidden keys leave the scores, and values that are not finite reach only rows that see them
     const auto cut_step = [&](const E* kp, const E* vp, int pos, int shown) {
-      const int lo0 = lo - pos - 4 * kg, hi0 = hi - pos - 4 * kg;
-      const bool odd = tile_is_odd<E, D, GROUPS>(vp, lane);
+      const int lo0 = lo - pos - 16 * kg, hi0 = hi - pos - 16 * kg;
+      const bool odd = tile_is_odd<E, D>(vp, lane);
 #pragma unroll
-      for (int u = 0; u < NS; ++u) {
+      for (int u = 0; u < 2; ++u) {
         sc[u] = f32x16{};
 #pragma unroll
         for (int i = 0; i < KQ; ++i) sc[u] = mfma32(at_tile.rows(kp, u, i), qf[i], sc[u]);
         bent(u, pos);
 #pragma unroll
         for (int e = 0; e < 16; ++e) {
-          const int at = 32 * u + c_row(e);
-          if ((int)(at < lo0) | (int)(at >= hi0) | (int)!(shown >> (2 * u + (e >> 3)) & 1)) sc[u][e] = -INFINITY;
+          const int at = c_row(u, e);
+          if ((int)(at < lo0) | (int)(at >= hi0) | (int)!(shown >> (2 * (e >> 2 & 1) + kg) & 1)) sc[u][e] = -INFINITY;
         }
         begin_weights();
 #pragma unroll
@@ -307,13 +289,13 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : D == 64 ? 3 : 2) void core_kern
         settle(u);
 #pragma unroll
         for (int i = 0; i < H; ++i) {
-          x8 v = at_tile.columns(vp, 2 * u + i / MT, i % MT);
+          x8 v = at_tile.columns(vp, u, i / MT, i % MT);
           if (odd) v = finite_values<E>(v);
           o[i % MT] = mfma32(v, weight8(u, i / MT * 4), o[i % MT]);
         }
       }
       if (odd)
-        add_odd<E, D, GROUPS>(vp, o, lane, [&](int i) { return pos + i >= lo && pos + i < hi && (shown >> (i >> 4) & 1); });
+        add_odd<E, D>(vp, o, lane, [&](int i) { return pos + i >= lo && pos + i < hi && (shown >> (i >> 4) & 1); });
     };
 
     if (n > 0) {
@@ -323,7 +305,7 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : D == 64 ? 3 : 2) void core_kern
         table1 = entries(1);
       }
       shown = stage(table, 0);
-      __syncthreads();
+      tiles_ready();
 #pragma unroll 1
       for (int j = 0; j < n; ++j) {
         const int pos = pos0 + j * TOK;
@@ -336,7 +318,7 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : D == 64 ? 3 : 2) void core_kern
             cut_step(kt[j & 1], vt[j & 1], pos, shown);
         }
         shown = shown1;
-        __syncthreads();
+        tiles_ready();
       }
     }
     l += __shfl_xor(l, 32, 64);

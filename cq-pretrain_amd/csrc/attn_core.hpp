@@ -5,7 +5,7 @@
 // 32 columns and two halves:
 //   A (32 x 16): row n32, k = 8 kg .. 8 kg + 7;  B (16 x 32): column n32, the same k;
 //   C (32 x 32): column n32, element e is row 8 (e >> 2) + 4 kg + (e & 3)
-// so that elements 8 i .. 8 i + 7 of a C are the B operand of a product over rows 16 i .. 16 i + 15, whose k runs
+// so that elements 8 b .. 8 b + 7 of a C are the B operand of a product over its rows 16 b .. 16 b + 15, whose k runs
 // 4 kg + {0 .. 3, 8 .. 11}: the A operand is read from a tile in that order, transposed.
 #pragma once
 #include "attn_kernels.hpp"
@@ -22,49 +22,77 @@ __device__ __forceinline__ f32x16 mfma32(bf16x8 a, bf16x8 b, f32x16 c) {
 __device__ __forceinline__ f32x16 mfma32(f16x8 a, f16x8 b, f32x16 c) {
   return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0);
 }
-// the row of a C's element, without the lane's 4 kg
-__host__ __device__ constexpr int c_row(int e) { return 8 * (e >> 2) + (e & 3); }
-
-// A tile of rows [n][D] in LDS, as global loads write it: 1024 bytes an instruction, side by side, so there is no
-// room between rows.  The 16-byte chunk c of a row lies at c ^ turn(row): 16 rows read at the same chunk, and 4 rows
-// at 4 neighbouring chunks (the transposed reads), then meet all 64 banks once.
+// A tile of 64 rows [D] in LDS, as asynchronous loads write it: 1024 bytes an instruction, side by side, the lanes anywhere
+// in memory.  Such a block holds 4 chunks (of 16 bytes) of 16 rows, a row's side by side and in their order: the memory
+// pipeline then takes a row's 64 bytes as one request (chunks put in another order are a request each, and cost the
+// forward pass of 9216 rows 447 us against 412).  Each 16 rows' blocks lie 16 bytes further than the last's.  The rows that an MFMA
+// takes as its 32 come from all four: row m of the u-th 32 is tile row 16 (m >> 2 & 3) + 8 u + 4 (m >> 4) + (m & 3).
+// 16 rows read at the same chunk, and 4 rows at 4 neighbouring chunks (the transposed reads), meet all 64 banks once, and
+// but for two offsets of the lane every place in the tile is a constant.
+constexpr int kTile = 64;  // rows
 template <int D>
-__device__ __forceinline__ int tile_turn(int row) {
-  return D == 64 ? (row >> 1 & 1) << 2 | (row >> 2 & 3) : (row & 3) << 2 | (row >> 2 & 3);
+constexpr int kTileRows16 = 16 * D + 8;  // elements from 16 rows to the next
+template <int D>
+constexpr int kTileSize = 4 * kTileRows16<D>;
+template <int D>
+__host__ __device__ constexpr int tile_at(int row, int chunk) {  // in elements
+  return row / 16 * kTileRows16<D> + chunk / 4 * 512 + (row & 15) * 32 + (chunk & 3) * 8;
 }
+// the tile row of element e of the u-th C, without the lane's 16 kg
+__host__ __device__ constexpr int c_row(int u, int e) { return 32 * (e >> 2 & 1) + 8 * u + 4 * (e >> 3) + (e & 3); }
+
 template <class E, int D>
 struct TileOperands {
   typedef typename Vec<E>::x8 x8;
-  int row[D / 16], col[2][D / 32];  // of the lane, in elements
+  int row, col;  // of the lane, in elements
   __device__ __forceinline__ TileOperands(int lane) {
-    const int n32 = lane & 31, kg = lane >> 5, j = lane & 15;
-#pragma unroll
-    for (int i = 0; i < D / 16; ++i) row[i] = n32 * D + 8 * ((2 * i) ^ kg ^ tile_turn<D>(n32));
-#pragma unroll
-    for (int s = 0; s < 2; ++s)
-#pragma unroll
-      for (int m = 0; m < D / 32; ++m) {
-        const int r = 4 * kg + 8 * s + (j >> 2);
-        col[s][m] = r * D + 8 * ((4 * m + 2 * (lane >> 4 & 1) + (j >> 1 & 1)) ^ tile_turn<D>(r)) + 4 * (j & 1);
-      }
+    const int m = lane & 31, kg = lane >> 5, j = lane & 15;
+    row = tile_at<D>(16 * (m >> 2 & 3) + 4 * (m >> 4) + (m & 3), kg);
+    col = tile_at<D>(16 * kg + (j >> 2), 2 * (lane >> 4 & 1) + (j >> 1 & 1)) + 4 * (j & 1);
   }
-  // rows 32 u + n32, dimensions 16 i + 8 kg ..
-  __device__ __forceinline__ x8 rows(const E* tile, int u, int i) const { return ld8(tile + 32 * u * D + row[i]); }
-  // dimension 32 m + n32 of the rows 16 b + 4 kg + {0 .. 3, 8 .. 11}
-  __device__ __forceinline__ x8 columns(const E* tile, int b, int m) const {
+  // the u-th 32 rows, dimensions 16 i + 8 kg ..
+  __device__ __forceinline__ x8 rows(const E* tile, int u, int i) const { return ld8(tile + row + tile_at<D>(8 * u, 2 * i)); }
+  // dimension 32 m + n32 of the rows of elements 8 b .. 8 b + 7 of the u-th C
+  __device__ __forceinline__ x8 columns(const E* tile, int u, int b, int m) const {
     typedef __attribute__((address_space(3))) i16x4 lds_i16x4;
-    const i16x4 x = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_i16x4*)(tile + 16 * b * D + col[0][m]));
-    const i16x4 y = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_i16x4*)(tile + 16 * b * D + col[1][m]));
+    const E* p = tile + col + tile_at<D>(8 * u + 4 * b, 4 * m);
+    const i16x4 x = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_i16x4*)p);
+    const i16x4 y = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_i16x4*)(p + 2 * kTileRows16<D>));
     return __builtin_bit_cast(x8, __builtin_shufflevector(x, y, 0, 1, 2, 3, 4, 5, 6, 7));
   }
 };
-// rows that one instruction of a wave loads, and the lane's row and chunk of those from row0 (a multiple of kLoadRows)
-template <int D>
-constexpr int kLoadRows = 512 / D;
-template <int D>
-__device__ __forceinline__ int load_row(int lane) { return lane / (D / 8); }
-template <int D>
-__device__ __forceinline__ int load_chunk(int lane, int row) { return (lane % (D / 8)) ^ tile_turn<D>(row); }
+
+// N blocks of a tile on their way: lane l's 16 bytes of `base` + `off` + 64 i (bytes) land at `lds` + 1024 i + 16 l.  In
+// assembly because the compiler, which does not tell the tiles of a pair from each other, puts a wait for all that is on
+// its way before every read of the other one (train_9216's forward pass spent 61% of its time in that wait); tiles_ready()
+// is the wait that is needed.  Nothing is returned in registers.  An instruction's offset moves both addresses.
+template <int N>
+__device__ __forceinline__ void load_blocks(const void* base, uint32_t off, void* lds) {
+  const uint32_t at = (uint32_t)(uintptr_t)(lds_void_ptr)lds;
+#define CQGDN_LOAD(m0, more) "s_mov_b32 m0, " m0 "\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, %1" more "\n\t"
+  static_assert(N == 1 || N == 2 || N == 4 || N == 8, "blocks a wave");
+  if constexpr (N == 1) {
+    asm volatile(CQGDN_LOAD("%2", "") ::"v"(off), "s"(base), "s"(at) : "memory");
+  } else if constexpr (N == 2) {
+    asm volatile(CQGDN_LOAD("%2", "") CQGDN_LOAD("%3", " offset:64") ::"v"(off), "s"(base), "s"(at), "s"(at + 960) : "memory");
+  } else {
+    asm volatile(CQGDN_LOAD("%2", "") CQGDN_LOAD("%3", " offset:64") CQGDN_LOAD("%4", " offset:128")
+                     CQGDN_LOAD("%5", " offset:192") ::"v"(off),
+                 "s"(base), "s"(at), "s"(at + 960), "s"(at + 1920), "s"(at + 2880)
+                 : "memory");
+    if constexpr (N == 8) load_blocks<4>(static_cast<const char*>(base) + 256, off, static_cast<char*>(lds) + 4096);
+  }
+#undef CQGDN_LOAD
+}
+// 16 rows of a tile, by one wave: row lane / 4 of `rows` (the wave's, from dimension 0 on), `offset` elements from there
+template <class E, int D>
+__device__ __forceinline__ void load_rows16(const E* rows, uint32_t offset, E* tile, int wave, int lane) {
+  load_blocks<D / 32>(rows, (offset + 8 * (lane & 3)) * sizeof(E), tile + wave * kTileRows16<D>);
+}
+// Everything that the workgroup's waves have asked for has arrived, and all have read what they wanted.
+__device__ __forceinline__ void tiles_ready() {
+  asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
+}
 
 // ---- values that are not finite -----------------------------------------------------------------------
 // 0 x infinity and 0 x NaN are NaN, so a value that a row does not see must not meet its weight 0 in an MFMA.  Where a
@@ -88,28 +116,30 @@ __device__ __forceinline__ X8 finite_values(X8 x) {
   for (int e = 0; e < 4; ++e) w[e] &= ~(((((w[e] & exponent) + one) & 0x80008000u) >> 15) * 0xFFFFu);
   return __builtin_bit_cast(X8, w);
 }
-// whether the tile's first 16 B rows hold one
-template <class E, int D, int B>
+// whether the tile holds one
+template <class E, int D>
 __device__ __forceinline__ bool tile_is_odd(const E* tile, int lane) {
   uint32_t any = 0;
 #pragma unroll
-  for (int i = 0; i < B * 16 * D / 512; ++i) any |= odd_values<E>(*reinterpret_cast<const u32x4*>(tile + 512 * i + 8 * lane));
+  for (int b = 0; b < 4; ++b)
+#pragma unroll
+    for (int i = 0; i < D / 32; ++i) any |= odd_values<E>(*reinterpret_cast<const u32x4*>(tile + b * kTileRows16<D> + 512 * i + 8 * lane));
   return __any(any != 0);
 }
-// acc (dimension 32 (m0 + m) + c_row(e) + 4 kg of the lane's column) += what the tile's first 16 B rows hold beyond finite
+// acc (dimension 32 (m0 + m) + 8 (e >> 2) + 4 kg + (e & 3) of the lane's column) += what the tile's rows hold beyond finite
 // values, of the rows that sees(row) allows the lane
-template <class E, int D, int B, int MT, class Sees>
+template <class E, int D, int MT, class Sees>
 __device__ __forceinline__ void add_odd(const E* tile, f32x16 (&acc)[MT], int lane, Sees sees, int m0 = 0) {
   const int kg = lane >> 5;
 #pragma unroll 1
-  for (int i = 0; i < 16 * B; ++i) {
+  for (int i = 0; i < kTile; ++i) {
     const bool seen = sees(i);
 #pragma unroll
     for (int m = 0; m < MT; ++m)
 #pragma unroll
       for (int e4 = 0; e4 < 4; ++e4) {
         const int d = 32 * (m0 + m) + 8 * e4 + 4 * kg;
-        const auto x = ld4(tile + i * D + 8 * ((d >> 3) ^ tile_turn<D>(i)) + (d & 7));
+        const auto x = ld4(tile + tile_at<D>(i, d >> 3) + (d & 7));
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
           const float f = (float)x[e];
@@ -142,13 +172,13 @@ struct Bend {
   }
 };
 
-// What the keys' gradients need of 32 rows of a key head, as the queries' gradients leave it.
+// What the keys' gradients need of 64 rows of a key head, as the queries' gradients leave it.
 struct RowBlock {
-  float lse[32], delta[32];     // log2 sum of exp2, and dy.out less the gradient of lse
-  int lo[32], hi[32];           // the keys that the row sees
-  float stands[32], slope[32];  // with a bias: the row's position, its head's slope times log2 e
+  float lse[64], delta[64];     // log2 sum of exp2, and dy.out less the gradient of lse
+  int lo[64], hi[64];           // the keys that the row sees
+  float stands[64], slope[64];  // with a bias: the row's position, its head's slope times log2 e
 };
-// The keys that any of 32 rows sees, [first, last) (first = INT32_MAX, last = 0 where none sees any), and those that
+// The keys that any of 64 rows sees, [first, last) (first = INT32_MAX, last = 0 where none sees any), and those that
 // all of them see, [low, high).
 struct RowRange {
   int first, last, low, high;

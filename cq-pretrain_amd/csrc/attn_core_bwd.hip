@@ -6,9 +6,9 @@
 // The weights come again from the scores and the rows' logarithms.  Two kernels, each of which owns what it sums, so
 // that nothing is added atomically and results do not depend on timing: one goes through the keys of 128 rows for dq
 // (S and dP once more than a kernel for all three would form them: 14 D operations a pair of row and key for 10), the
-// other through the rows that see 128 keys for dk and dv, 32 rows a step.
+// other through the rows that see 128 keys for dk and dv, 64 rows a step.
 //
-// The first leaves, for every 32 rows, the range of keys they see, their logarithms and deltas: the second finds its
+// The first leaves, for every 64 rows, the range of keys they see, their logarithms and deltas: the second finds its
 // steps in those ranges, 64 at a time.  Where its workgroups would not fill the CUs, each takes every n-th of the
 // steps, and fp32 parts are added up by a third kernel in their order.
 //
@@ -25,9 +25,6 @@ namespace cqgdn {
 namespace {
 
 constexpr int kRows = 128;  // of a workgroup for dq, 32 a wave
-
-template <int D>
-constexpr int kTokens = D == 256 ? 32 : 64;
 
 template <class E>
 constexpr float kWeightBias = std::is_same<E, f16>::value ? 15.f : 0.f;
@@ -75,10 +72,9 @@ struct Range {
 template <class E, int D, bool BENT>
 __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void dq_kernel(CoreGradArgs a, int tiles) {
   typedef typename Vec<E>::x8 x8;
-  constexpr int TOK = kTokens<D>, NS = TOK / 32, KQ = D / 16, MT = D / 32, GROUPS = TOK / 16;
-  constexpr int LR = kLoadRows<D>, LOADS = TOK / 4 / LR;
-  __shared__ __align__(16) E kt[2][TOK * D];
-  __shared__ __align__(16) E vt[2][TOK * D];
+  constexpr int TOK = kTile, KQ = D / 16, MT = D / 32;
+  __shared__ __align__(16) E kt[2][kTileSize<D>];
+  __shared__ __align__(16) E vt[2][kTileSize<D>];
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int n32 = lane & 31, kg = lane >> 5;
   // launch order: as the forward pass's
@@ -126,8 +122,20 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void dq_kernel(CoreGradArgs 
   most = __builtin_amdgcn_readfirstlane(most);
   low = __builtin_amdgcn_readfirstlane(low);
   high = __builtin_amdgcn_readfirstlane(high);
-  const int block = tile * (kRows / 32) + wave;
-  if (h == 0 && lane == 0) static_cast<RowRange*>(a.ranges)[block] = RowRange{some, most, low, high};
+  const int block = tile * (kRows / kTile) + wave / 2;
+  if (h == 0 && (wave & 1) == 0) {  // of 64 rows: a lane each
+    int lo1, hi1;
+    limits(tile * kRows + 32 * wave + lane, lo1, hi1);
+    RowRange x{hi1 > 0 ? lo1 : INT32_MAX, hi1, lo1, hi1};
+#pragma unroll
+    for (int i = 1; i < 64; i <<= 1) {
+      x.first = min(x.first, __shfl_xor(x.first, i, 64));
+      x.last = max(x.last, __shfl_xor(x.last, i, 64));
+      x.low = max(x.low, __shfl_xor(x.low, i, 64));
+      x.high = min(x.high, __shfl_xor(x.high, i, 64));
+    }
+    if (lane == 0) static_cast<RowRange*>(a.ranges)[block] = x;
+  }
   const int row_t = real ? a.group.of(rho) : 0, head = h * group + (real ? rho - row_t * group : 0);
   const int64_t at = (int64_t)row_t * a.heads + head;
   const Bend bend(a.scale, BENT ? a.cap : 0.f, BENT ? a.slopes : nullptr, head);
@@ -153,15 +161,16 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void dq_kernel(CoreGradArgs 
   if (a.dlse && real) delta -= a.dlse[at];
   const float lse = real ? a.lse[at] * 1.44269504088896341f : 0.f;
   {
-    RowBlock& x = static_cast<RowBlock*>(a.blocks)[(int64_t)h * tiles * (kRows / 32) + block];
+    RowBlock& x = static_cast<RowBlock*>(a.blocks)[(int64_t)h * tiles * (kRows / kTile) + block];
+    const int n = 32 * (wave & 1) + n32;
     if (kg == 0) {
-      x.lse[n32] = lse;
-      x.delta[n32] = delta;
-      x.lo[n32] = lo;
-      x.hi[n32] = hi;
+      x.lse[n] = lse;
+      x.delta[n] = delta;
+      x.lo[n] = lo;
+      x.hi[n] = hi;
       if constexpr (BENT) {
-        x.stands[n32] = (float)stands;
-        x.slope[n32] = bend.slope;
+        x.stands[n] = (float)stands;
+        x.slope[n] = bend.slope;
       }
     }
   }
@@ -173,45 +182,38 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void dq_kernel(CoreGradArgs 
   const float base = kWeightBias<E> - lse;
 
   const auto stage = [&](int j) {
-    const int row0 = wave * (TOK / 4), pos = first + j * TOK;
-    E* const kd = kt[j & 1] + row0 * D;
-    E* const vd = vt[j & 1] + row0 * D;
-    const E* kb = static_cast<const E*>(a.k) + h * a.k_head + pos * a.k_token;
-    const E* vb = static_cast<const E*>(a.v) + h * a.v_head + pos * a.v_token;
-    const int end = a.S - 1 - pos;  // rows behind the last key: that key once more
-#pragma unroll
-    for (int i = 0; i < LOADS; ++i) {
-      const int row = row0 + i * LR + load_row<D>(lane), r = min(row, end), chunk = 8 * load_chunk<D>(lane, row);
-      dma16(kb + (r * (int)a.k_token + chunk), kd + i * LR * D);
-      dma16(vb + (r * (int)a.v_token + chunk), vd + i * LR * D);
-    }
+    const int pos = first + j * TOK;
+    // rows behind the last key: that key once more
+    const uint32_t row = min(16 * wave + lane / 4, a.S - 1 - pos);
+    load_rows16<E, D>(static_cast<const E*>(a.k) + h * a.k_head + pos * a.k_token, row * (uint32_t)a.k_token, kt[j & 1], wave, lane);
+    load_rows16<E, D>(static_cast<const E*>(a.v) + h * a.v_head + pos * a.v_token, row * (uint32_t)a.v_token, vt[j & 1], wave, lane);
   };
   const auto step = [&](const E* kp, const E* vp, int pos, auto whole) {
     constexpr bool WHOLE = decltype(whole)::value;
-    const bool odd = !WHOLE && tile_is_odd<E, D, GROUPS>(kp, lane);
-    const int lo0 = lo - pos - 4 * kg, hi0 = hi - pos - 4 * kg;
+    const bool odd = !WHOLE && tile_is_odd<E, D>(kp, lane);
+    const int lo0 = lo - pos - 16 * kg, hi0 = hi - pos - 16 * kg;
+    const float far = (float)(stands - pos - 16 * kg);
 #pragma unroll
-    for (int u = 0; u < NS; ++u) {
+    for (int u = 0; u < 2; ++u) {
       f32x16 sc = f32x16{}, dp = f32x16{} - delta;
 #pragma unroll
       for (int i = 0; i < KQ; ++i) {
         sc = mfma32(at_tile.rows(kp, u, i), qf[i], sc);
         dp = mfma32(at_tile.rows(vp, u, i), yf[i], dp);
       }
-      const float far = (float)(stands - pos - 32 * u - 4 * kg);
 #pragma unroll
       for (int e = 0; e < 16; ++e) {
         float x = sc[e], rate = 1.f;
         if constexpr (BENT) {
           x = a.cap > 0.f ? bend.capped(x, rate) : x * bend.c;
-          x = __builtin_fmaf(-bend.slope, fabsf(far - (float)c_row(e)), x);
+          x = __builtin_fmaf(-bend.slope, fabsf(far - (float)c_row(u, e)), x);
           x = __builtin_amdgcn_exp2f(x + base);
         } else {
           x = __builtin_amdgcn_exp2f(__builtin_fmaf(x, bend.c, base));
         }
         x *= dp[e];
         if constexpr (BENT) x *= rate;
-        const int at = 32 * u + c_row(e);
+        const int at = c_row(u, e);
         if (!WHOLE && ((int)(at < lo0) | (int)(at >= hi0))) x = 0.f;
         dp[e] = x;
       }
@@ -223,19 +225,19 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void dq_kernel(CoreGradArgs 
         for (int e = 0; e < 4; ++e) w[e] = pack2<E>(dp[8 * b + 2 * e] * range.f, dp[8 * b + 2 * e + 1] * range.f);
 #pragma unroll
         for (int m = 0; m < MT; ++m) {
-          x8 k = at_tile.columns(kp, 2 * u + b, m);
+          x8 k = at_tile.columns(kp, u, b, m);
           if (odd) k = finite_values<E>(k);
           acc[m] = mfma32(k, __builtin_bit_cast(x8, w), acc[m]);
         }
       }
     }
-    if (odd) add_odd<E, D, GROUPS>(kp, acc, lane, [&](int i) { return pos + i >= lo && pos + i < hi; });
+    if (odd) add_odd<E, D>(kp, acc, lane, [&](int i) { return pos + i >= lo && pos + i < hi; });
   };
 
   const int n = last > 0 ? (last - first + TOK - 1) / TOK : 0;
   if (n > 0) {
     stage(0);
-    __syncthreads();
+    tiles_ready();
 #pragma unroll 1
     for (int j = 0; j < n; ++j) {
       const int pos = first + j * TOK;
@@ -246,7 +248,7 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void dq_kernel(CoreGradArgs 
         else
           step(kt[j & 1], vt[j & 1], pos, std::false_type{});
       }
-      __syncthreads();
+      tiles_ready();
     }
   }
   if (real) {
@@ -267,15 +269,15 @@ constexpr bool kPair = D == 256;
 template <int D>
 constexpr int kKeys = kPair<D> ? 64 : 128;
 
-// dk and dv of kKeys keys of a key head; part s of `splits` takes every splits-th block of 32 rows that sees any of them
+// dk and dv of kKeys keys of a key head; part s of `splits` takes every splits-th block of 64 rows that sees any of them
 template <class E, int D, bool BENT>
 __global__ __launch_bounds__(256, 1) void dkv_kernel(CoreGradArgs a, int blocks, int splits) {
   typedef typename Vec<E>::x8 x8;
   constexpr bool PAIR = kPair<D>;
-  constexpr int KQ = D / 16, MT = D / 32 / (PAIR ? 2 : 1), LR = kLoadRows<D>, LOADS = 32 / 4 / LR;
-  constexpr int WORDS = sizeof(RowBlock) / 16;
-  __shared__ __align__(16) E qt[2][32 * D];
-  __shared__ __align__(16) E yt[2][32 * D];
+  constexpr int KQ = D / 16, MT = D / 32 / (PAIR ? 2 : 1);
+  static_assert(offsetof(RowBlock, stands) == 1024 && sizeof(RowBlock) == 1536, "an instruction, and half of one");
+  __shared__ __align__(16) E qt[2][kTileSize<D>];
+  __shared__ __align__(16) E yt[2][kTileSize<D>];
   __shared__ __align__(16) float swap[PAIR ? 4 : 1][PAIR ? 1024 : 4];
   __shared__ __align__(16) RowBlock info[2];
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -333,25 +335,23 @@ __global__ __launch_bounds__(256, 1) void dkv_kernel(CoreGradArgs a, int blocks,
     }
   };
   const auto stage = [&](int block, int buffer) {
-    const int row0 = wave * 8;
-    E* const qd = qt[buffer] + row0 * D;
-    E* const yd = yt[buffer] + row0 * D;
-#pragma unroll
-    for (int i = 0; i < LOADS; ++i) {
-      const int row = row0 + i * LR + load_row<D>(lane), rho = min(block * 32 + row, rows - 1);  // behind the last: that once more
-      const int t = a.group.of(rho), head = h * group + rho - t * group, chunk = 8 * load_chunk<D>(lane, row);
-      dma16(static_cast<const E*>(a.q) + t * a.q_token + head * a.q_head + chunk, qd + i * LR * D);
-      dma16(static_cast<const E*>(a.dy) + t * a.dy_token + head * a.dy_head + chunk, yd + i * LR * D);
-    }
-    if (wave == 0 && lane < (BENT ? WORDS : WORDS * 2 / 3))
-      dma16(reinterpret_cast<const char*>(static_cast<const RowBlock*>(a.blocks) + ((int64_t)h * blocks + block)) + 16 * lane, &info[buffer]);
+    // offsets from the wave's first token; rows behind the last: that once more
+    const int r0 = min(block * kTile + 16 * wave, rows - 1), t0 = a.group.of(r0);
+    const int rho = min(r0 + lane / 4, rows - 1), t = a.group.of(rho), g = rho - t * group;
+    load_rows16<E, D>(static_cast<const E*>(a.q) + t0 * a.q_token + h * group * a.q_head,
+                      (t - t0) * (uint32_t)a.q_token + g * (uint32_t)a.q_head, qt[buffer], wave, lane);
+    load_rows16<E, D>(static_cast<const E*>(a.dy) + t0 * a.dy_token + h * group * a.dy_head,
+                      (t - t0) * (uint32_t)a.dy_token + g * (uint32_t)a.dy_head, yt[buffer], wave, lane);
+    const RowBlock* const from = static_cast<const RowBlock*>(a.blocks) + ((int64_t)h * blocks + block);
+    if (wave == 0) load_blocks<1>(from, 16 * lane, &info[buffer]);
+    if (BENT && wave == 1 && lane < 32) load_blocks<1>(from->stands, 16 * lane, info[buffer].stands);
   };
-  f32x16 sc, dp;
-  const auto products = [&](const E* qp, const E* yp, const RowBlock& x) {
+  // of the u-th 32 rows: S and dP - delta, with a pair's one of them
+  const auto products = [&](const E* qp, const E* yp, const RowBlock& x, int u, f32x16& sc, f32x16& dp) {
     sc = f32x16{};
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-      const f32x4 delta = *reinterpret_cast<const f32x4*>(x.delta + 8 * i + 4 * kg);
+      const f32x4 delta = *reinterpret_cast<const f32x4*>(x.delta + c_row(u, 4 * i) + 16 * kg);
 #pragma unroll
       for (int e = 0; e < 4; ++e) dp[4 * i + e] = -delta[e];
     }
@@ -359,41 +359,40 @@ __global__ __launch_bounds__(256, 1) void dkv_kernel(CoreGradArgs a, int blocks,
       if (half) sc = dp;
       const E* const p = half ? yp : qp;
 #pragma unroll
-      for (int i = 0; i < KQ; ++i) sc = mfma32(at_tile.rows(p, 0, i), kf[i], sc);
-#pragma unroll
-      for (int i = 0; i < 4; ++i)
-        *reinterpret_cast<f32x4*>(swap[wave] + 256 * i + 4 * lane) = f32x4{sc[4 * i], sc[4 * i + 1], sc[4 * i + 2], sc[4 * i + 3]};
+      for (int i = 0; i < KQ; ++i) sc = mfma32(at_tile.rows(p, u, i), kf[i], sc);
     } else {
 #pragma unroll
       for (int i = 0; i < KQ; ++i) {
-        sc = mfma32(at_tile.rows(qp, 0, i), kf[i], sc);
-        dp = mfma32(at_tile.rows(yp, 0, i), vf[i], dp);
+        sc = mfma32(at_tile.rows(qp, u, i), kf[i], sc);
+        dp = mfma32(at_tile.rows(yp, u, i), vf[i], dp);
       }
     }
   };
-  const auto exchange = [&] {
-    if constexpr (PAIR) {
-      f32x16 other;
+  const auto give = [&](const f32x16& sc) {
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const f32x4 x = *reinterpret_cast<const f32x4*>(swap[wave ^ 1] + 256 * i + 4 * lane);
-#pragma unroll
-        for (int e = 0; e < 4; ++e) other[4 * i + e] = x[e];
-      }
-      dp = half ? sc : other;
-      sc = half ? other : sc;
-    }
+    for (int i = 0; i < 4; ++i)
+      *reinterpret_cast<f32x4*>(swap[wave] + 256 * i + 4 * lane) = f32x4{sc[4 * i], sc[4 * i + 1], sc[4 * i + 2], sc[4 * i + 3]};
   };
-  const auto sums = [&](const E* qp, const E* yp, const RowBlock& x, auto whole) {
-    constexpr bool WHOLE = decltype(whole)::value;
-    bool odd = false;
-    if constexpr (!WHOLE) odd = tile_is_odd<E, D, 2>(qp, lane) || tile_is_odd<E, D, 2>(yp, lane);
+  const auto take = [&](f32x16& sc, f32x16& dp) {
+    f32x16 other;
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-      const f32x4 lse = *reinterpret_cast<const f32x4*>(x.lse + 8 * i + 4 * kg);
+      const f32x4 x = *reinterpret_cast<const f32x4*>(swap[wave ^ 1] + 256 * i + 4 * lane);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) other[4 * i + e] = x[e];
+    }
+    dp = half ? sc : other;
+    sc = half ? other : sc;
+  };
+  const auto sums = [&](const E* qp, const E* yp, const RowBlock& x, int u, f32x16& sc, f32x16& dp, bool odd, auto whole) {
+    constexpr bool WHOLE = decltype(whole)::value;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int row4 = c_row(u, 4 * i) + 16 * kg;
+      const f32x4 lse = *reinterpret_cast<const f32x4*>(x.lse + row4);
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
-        const int e = 4 * i + j, row = 8 * i + j + 4 * kg;
+        const int e = 4 * i + j, row = row4 + j;
         float p, rate = 1.f;
         const float from = kWeightBias<E> - lse[j];
         if constexpr (BENT) {
@@ -424,7 +423,7 @@ __global__ __launch_bounds__(256, 1) void dkv_kernel(CoreGradArgs a, int blocks,
       }
 #pragma unroll
       for (int m = 0; m < MT; ++m) {
-        x8 y = at_tile.columns(yp, b, half * MT + m), q = at_tile.columns(qp, b, half * MT + m);
+        x8 y = at_tile.columns(yp, u, b, half * MT + m), q = at_tile.columns(qp, u, b, half * MT + m);
         if (odd) {
           y = finite_values<E>(y);
           q = finite_values<E>(q);
@@ -433,10 +432,36 @@ __global__ __launch_bounds__(256, 1) void dkv_kernel(CoreGradArgs a, int blocks,
         dk[m] = mfma32(q, __builtin_bit_cast(x8, z), dk[m]);
       }
     }
+  };
+  const auto step = [&](const E* qp, const E* yp, const RowBlock& x, auto whole) {
+    constexpr bool WHOLE = decltype(whole)::value;
+    bool odd = false;
+    if constexpr (!WHOLE) odd = tile_is_odd<E, D>(qp, lane) || tile_is_odd<E, D>(yp, lane);
+    if constexpr (PAIR) {
+      f32x16 sc[2], dp[2];
+#pragma unroll
+      for (int u = 0; u < 2; ++u) products(qp, yp, x, u, sc[u], dp[u]);
+      give(sc[0]);
+      lds_barrier();
+      take(sc[0], dp[0]);
+      lds_barrier();
+      give(sc[1]);
+      lds_barrier();
+      take(sc[1], dp[1]);
+#pragma unroll
+      for (int u = 0; u < 2; ++u) sums(qp, yp, x, u, sc[u], dp[u], odd, whole);
+    } else {
+#pragma unroll
+      for (int u = 0; u < 2; ++u) {
+        f32x16 sc, dp;
+        products(qp, yp, x, u, sc, dp);
+        sums(qp, yp, x, u, sc, dp, odd, whole);
+      }
+    }
     if (odd) {
       const auto sees = [&](int i) { return key >= x.lo[i] && key < x.hi[i]; };
-      add_odd<E, D, 2>(qp, dk, lane, sees, half * MT);
-      add_odd<E, D, 2>(yp, dv, lane, sees, half * MT);
+      add_odd<E, D>(qp, dk, lane, sees, half * MT);
+      add_odd<E, D>(yp, dv, lane, sees, half * MT);
     }
   };
 
@@ -444,22 +469,20 @@ __global__ __launch_bounds__(256, 1) void dkv_kernel(CoreGradArgs a, int blocks,
   int block = next(x), buffer = 0;
   if (block >= 0) {
     stage(block, 0);
-    __syncthreads();
+    tiles_ready();
 #pragma unroll 1
     while (true) {
       const int following = next(y);
       if (following >= 0) stage(following, buffer ^ 1);
+      // a pair's waves meet within the step, so all of the workgroup's go through it, as far as any of them has to
       const bool any = x.last > mine && x.first < mine + 32;
-      if (any) products(qt[buffer], yt[buffer], info[buffer]);
-      if constexpr (PAIR) lds_barrier();
-      if (any) {
-        exchange();
+      if (PAIR || any) {
         if (x.low <= mine && mine + 32 <= x.high)
-          sums(qt[buffer], yt[buffer], info[buffer], std::true_type{});
+          step(qt[buffer], yt[buffer], info[buffer], std::true_type{});
         else
-          sums(qt[buffer], yt[buffer], info[buffer], std::false_type{});
+          step(qt[buffer], yt[buffer], info[buffer], std::false_type{});
       }
-      __syncthreads();
+      tiles_ready();
       if (following < 0) break;
       x = y;
       buffer ^= 1;
@@ -498,7 +521,8 @@ __global__ __launch_bounds__(256) void join_parts_kernel(const float* ws, int64_
   st4(at < size ? dk + at : dv + (at - size), y);
 }
 
-int64_t row_blocks(int64_t T, int group) { return (T * group + kRows - 1) / kRows * (kRows / 32); }
+// blocks of 64 rows, of whole workgroups for dq
+int64_t row_blocks(int64_t T, int group) { return (T * group + kRows - 1) / kRows * (kRows / kTile); }
 
 // parts of the keys' gradients: two rounds of workgroups at least
 int key_parts(int64_t T, int64_t S, int kv_heads, int group, int D) {
@@ -509,11 +533,11 @@ int key_parts(int64_t T, int64_t S, int kv_heads, int group, int D) {
 
 template <class E, int D, bool BENT>
 void launch_grad(const CoreGradArgs& a, hipStream_t st) {
-  const int group = a.heads / a.kv_heads, tiles = (int)(row_blocks(a.T, group) / (kRows / 32));
+  const int group = a.heads / a.kv_heads, tiles = (int)(row_blocks(a.T, group) / (kRows / kTile));
   const int splits = key_parts(a.T, a.S, a.kv_heads, group, D);
   if (tiles > 0) dq_kernel<E, D, BENT><<<tiles * a.kv_heads, 256, 0, st>>>(a, tiles);
   if (a.S == 0 || !a.dk) return;
-  dkv_kernel<E, D, BENT><<<(unsigned)((a.S + kKeys<D> - 1) / kKeys<D> * a.kv_heads * splits), 256, 0, st>>>(a, tiles * (kRows / 32), splits);
+  dkv_kernel<E, D, BENT><<<(unsigned)((a.S + kKeys<D> - 1) / kKeys<D> * a.kv_heads * splits), 256, 0, st>>>(a, tiles * (kRows / kTile), splits);
   if (splits > 1) {
     const int64_t size = (int64_t)a.S * a.kv_heads * D;
     join_parts_kernel<E><<<(unsigned)((2 * size + 1023) / 1024), 256, 0, st>>>(a.ws, size, splits, static_cast<E*>(a.dk), static_cast<E*>(a.dv));

@@ -20,9 +20,10 @@ bool page_ok(int page) { return page >= 16 && page <= 65536 && (page & (page - 1
 bool dim_ok(int D) { return D == 64 || D == 128 || D == 256; }
 bool type_ok(int dtype) { return dtype == CQGDN_BF16 || dtype == CQGDN_F16; }
 bool finite(float x) { return x - x == 0.f; }
-// rows as the kernels read them
-bool rows_ok(const void* p, int64_t token, int64_t head) {
-  return p && aligned(p, 16) && token % 8 == 0 && head % 8 == 0 && token > -(1 << 24) && token < 1 << 24;
+// rows as the kernels read them: the offsets of 64 tokens, and of a token's heads, fit 32 bits
+bool rows_ok(const void* p, int64_t token, int64_t head, int heads) {
+  return p && aligned(p, 16) && token % 8 == 0 && head % 8 == 0 && token >= 0 && token < 1 << 24 && head >= 0 &&
+         head < (1 << 29) / heads;
 }
 
 int check_cache16(const void* data, int64_t pages, int kv_heads, int D, int page) {
@@ -149,9 +150,9 @@ int cqgdn_attend_fwd(const void* q, int64_t q_token, int64_t q_head, const void*
   if (const int e = check_packed(T, S, heads, kv_heads, head_dim)) return e;
   if (const int e = check_scores(dtype, scale, cap)) return e;
   if (T == 0) return ok();
-  if (!rows_ok(q, q_token, q_head) || (S > 0 && (!rows_ok(k, k_token, k_head) || !rows_ok(v, v_token, v_head))) || !limit ||
+  if (!rows_ok(q, q_token, q_head, heads) || (S > 0 && (!rows_ok(k, k_token, k_head, kv_heads) || !rows_ok(v, v_token, v_head, kv_heads))) || !limit ||
       !out || !aligned(out, 16))
-    return fail(CQGDN_EINVAL, "q, k, v and out (16-byte aligned, strides multiples of 8 elements below 2^24) and limit "
+    return fail(CQGDN_EINVAL, "q, k, v and out (16-byte aligned, strides multiples of 8 elements, not negative, below 2^24 a token and 2^29 all heads) and limit "
                 "must be non-null");
   const int splits = core_parts(T, S, heads, kv_heads, head_dim);
   const size_t need = part_bytes(T, heads, head_dim, splits);
@@ -179,11 +180,11 @@ int cqgdn_attend_bwd(const void* q, int64_t q_token, int64_t q_head, const void*
   if (const int e = check_packed(T, S, heads, kv_heads, head_dim)) return e;
   if (const int e = check_scores(dtype, scale, cap)) return e;
   if (T == 0 && S == 0) return ok();
-  if ((T > 0 && (!rows_ok(q, q_token, q_head) || !rows_ok(dy, dy_token, dy_head) || !limit || !out || !aligned(out, 16) ||
+  if ((T > 0 && (!rows_ok(q, q_token, q_head, heads) || !rows_ok(dy, dy_token, dy_head, heads) || !limit || !out || !aligned(out, 16) ||
                  !lse || !dq || !aligned(dq, 16))) ||
-      (S > 0 && (!rows_ok(k, k_token, k_head) || !rows_ok(v, v_token, v_head) || !dk != !dv || !aligned(dk, 16) || !aligned(dv, 16))))
-    return fail(CQGDN_EINVAL, "q, k, v, dy, out and the gradients (16-byte aligned, strides multiples of 8 elements "
-                "below 2^24), limit and lse must be non-null");
+      (S > 0 && (!rows_ok(k, k_token, k_head, kv_heads) || !rows_ok(v, v_token, v_head, kv_heads) || !dk != !dv || !aligned(dk, 16) || !aligned(dv, 16))))
+    return fail(CQGDN_EINVAL, "q, k, v, dy, out and the gradients (16-byte aligned, strides multiples of 8 elements, "
+                "not negative, below 2^24 a token and 2^29 all heads), limit and lse must be non-null");
   const size_t need = core_backward_bytes(T, S, heads, kv_heads, head_dim);
   if (need > 0 && (!workspace || !aligned(workspace, 256) || workspace_bytes < need))
     return fail(CQGDN_EINVAL, "workspace must be 256-byte aligned and >= cqgdn_attend_bwd_workspace_size");

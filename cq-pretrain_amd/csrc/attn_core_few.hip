@@ -49,7 +49,7 @@ struct Rows {
 template <class E, int D, bool BENT>
 __global__ __launch_bounds__(64 * kWaves, D == 256 ? 1 : 2) void few_kernel(CoreArgs a, int tiles, int least) {
   typedef typename Vec<E>::x8 x8;
-  constexpr int KQ = D / 32, MT = D / 16, LR = kLoadRows<D>;
+  constexpr int KQ = D / 32, MT = D / 16, LR = 512 / D;  // LR rows of values a load
   constexpr int LD = D + 16;  // 8 banks further each row: the transposed reads of 8 rows meet no bank twice
   __shared__ __align__(16) E vt[kWaves][kHalf * LD];
   __shared__ float wm[kWaves][16], wl[kWaves][16];

@@ -19,9 +19,9 @@ typedef std::optional<Tensor> Maybe;
 
 const Tensor* given(const Maybe& x) { return x.has_value() && x->defined() ? &*x : nullptr; }
 
-// rows as the kernels read them; strides from token to token fit 32 bits within a tile
+// rows as the kernels read them: the offsets of a tile's tokens and heads fit 32 bits
 Tensor core_rows(const Tensor& x) {
-  return std::abs(x.stride(0)) < 1 << 24 || x.size(0) <= 1 ? head_rows(x) : x.clone(at::MemoryFormat::Contiguous);
+  return x.stride(0) < 1 << 24 && x.stride(1) * x.size(1) < 1 << 29 ? head_rows(x) : x.clone(at::MemoryFormat::Contiguous);
 }
 
 // an int32 value a row, dense, or none

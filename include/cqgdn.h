@@ -502,7 +502,8 @@ int cqgdn_kv16_attend(const void* q, int64_t q_token, int64_t q_head, int dtype,
  * (NULL: limit[t] - 1).  Query head h reads key head h / (heads / kv_heads); rows that see nothing are zero.  Scores,
  * sums and results are held in fp32; each weight is rounded to dtype for its product with v.
  *   q, out   : bf16 or fp16 (dtype) [T][heads][head_dim], out dense; k, v: [S][kv_heads][head_dim].  Strides in
- *              elements, multiples of 8, below 2^24 from token to token; rows 16-byte aligned
+ *              elements, multiples of 8, not negative, below 2^24 from token to token and 2^29 over all heads; rows
+ *              16-byte aligned
  *   lse      : fp32 [T][heads]: log sum_j exp(u_j), -inf for rows that see nothing; the backward pass reads it (or NULL)
  *   workspace: >= cqgdn_attend_fwd_workspace_size() bytes (it may be 0), 256-byte aligned
  * cqgdn_attend_bwd writes the gradients dq, dk, dv (dense, of dtype) of a loss whose gradients by out and lse are dy

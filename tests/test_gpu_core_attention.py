@@ -293,25 +293,20 @@ def test_same_inputs_same_bits(attention):
 
 
 def test_offsets_beyond_32_bits(attention):
-    """More than 2^31 values of q, and of k and v, in windows of 16: the last rows against a call of those alone."""
-    T, hq, D = 70000, 256, 128
+    """More than 2^31 values of q, and of k and v, in windows of 16: the last rows and keys against the form for those alone
+    (rows and keys whose windows lie within the last 100)."""
+    T, hq, D, n, w = 70000, 256, 128, 100, 16
     assert T * hq * D > 2 ** 31
-    q, k, v, dy = (torch.randn(T, hq, D, device=DEV, dtype=torch.bfloat16) for _ in range(4))
+    g = torch.Generator(device=DEV).manual_seed(21)
+    q, k, v, dy = (torch.randn(T, hq, D, generator=g, device=DEV, dtype=torch.bfloat16) for _ in range(4))
     row = torch.arange(T, device=DEV)
-    first, limit = (row + 1 - 16).clamp(min=0).int(), (row + 1).int()
+    first, limit = (row + 1 - w).clamp(min=0).int(), (row + 1).int()
     got = run(attention, q, k, v, limit, dy, first=first)
-    n = 500
-    at = slice(T - n, T)
-    want = run(attention, q[at], k[at], v[at], (limit[at] - (T - n)), dy[at], first=(first[at] - (T - n)).clamp(min=0))
-    for name in want:
-        # rows whose window lies within the part
-        assert torch.equal(got[name][T - n + 128:].float(), want[name][128:].float()) or torch.allclose(
-            got[name][T - n + 128:].float(), want[name][128:].float(), atol=2 ** -6, rtol=2 ** -7), name
-    ref = {x: got[x][T - 60:] for x in ("out", "lse", "dq")}
-    w, tol = R.attend_ref(q[T - 60:, :4], k[T - 100:, :4], v[T - 100:, :4], first[T - 60:] - (T - 100), limit[T - 60:] - (T - 100),
-                          scale=D ** -0.5, dy=dy[T - 60:, :4])
-    for x in ref:
-        R.check(ref[x][:, :4], w[x], tol[x], x, q.dtype)
+    for heads in (slice(0, 2), slice(hq - 2, hq)):
+        part = [x[T - n:, heads] for x in (q, k, v)]
+        want, tol = R.attend_ref(*part, first[T - n:] - (T - n), limit[T - n:] - (T - n), scale=D ** -0.5, dy=dy[T - n:, heads])
+        for x in want:
+            R.check(got[x][T - n + w:, heads], want[x][w:], tol[x][w:], x, q.dtype)
 
 
 def test_another_stream_and_a_graph(attention):
