@@ -19,55 +19,10 @@
 
 #include <algorithm>
 
-#include "attn_core.hpp"
+#include "attn_core_grad.hpp"
 
 namespace cqgdn {
 namespace {
-
-constexpr int kRows = 128;  // of a workgroup for dq, 32 a wave
-
-template <class E>
-constexpr float kWeightBias = std::is_same<E, f16>::value ? 15.f : 0.f;
-
-// Two elements of the type from two floats
-template <class E>
-__device__ __forceinline__ uint32_t pack2(float x, float y) {
-  typedef float f32x2 __attribute__((ext_vector_type(2)));
-  typedef E x2 __attribute__((ext_vector_type(2)));
-  return __builtin_bit_cast(uint32_t, __builtin_convertvector(f32x2{x, y}, x2));
-}
-
-// The power of two that a lane's dx go with in fp16 (bf16: 1): the largest lies near 2^10 when it is set, and below
-// 2^15 always.  The two lanes of a column share it.
-template <class E>
-struct Range {
-  static constexpr bool on = std::is_same<E, f16>::value;
-  float f = on ? 0.f : 1.f;
-  // for 16 new dx; `acc`, the sums so far, move with it
-  template <int MT>
-  __device__ __forceinline__ void fit(const f32x16& x, f32x16 (&acc)[MT]) {
-    if constexpr (on) {
-      float top = fabsf(x[0]);
-#pragma unroll
-      for (int e = 1; e < 16; ++e) top = fmaxf(top, fabsf(x[e]));
-      bool move = top * f > 32768.f || (f == 0.f && top > 0.f);
-      if (__any(move)) {
-        move = __shfl_xor((int)move, 32, 64) || move;
-        top = fmaxf(top, __shfl_xor(top, 32, 64));
-        if (move) {
-          const int e = (int)(__builtin_bit_cast(uint32_t, top) >> 23) - 127;
-          const float g = __builtin_bit_cast(float, (uint32_t)(127 + min(max(10 - e, -126), 126)) << 23);
-          const float by = f == 0.f ? 0.f : g / f;
-#pragma unroll
-          for (int m = 0; m < MT; ++m) acc[m] *= by;
-          f = g;
-        }
-      }
-    }
-  }
-  // what the sums are to be multiplied with
-  __device__ __forceinline__ float back() const { return !on ? 1.f : f == 0.f ? 0.f : 1.f / f; }
-};
 
 template <class E, int D, bool BENT>
 __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void dq_kernel(CoreGradArgs a, int tiles) {
@@ -94,8 +49,8 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void dq_kernel(CoreGradArgs 
   int first, last;
   {
     int lo0, hi0, lo1, hi1;
-    limits(tile * kRows + lane, lo0, hi0);
-    limits(tile * kRows + 64 + lane, lo1, hi1);
+    limits(tile * kGradRows + lane, lo0, hi0);
+    limits(tile * kGradRows + 64 + lane, lo1, hi1);
     first = min(hi0 > 0 ? lo0 : INT32_MAX, hi1 > 0 ? lo1 : INT32_MAX);
     last = max(hi0, hi1);
 #pragma unroll
@@ -106,7 +61,7 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void dq_kernel(CoreGradArgs 
     first = __builtin_amdgcn_readfirstlane(first);
     last = __builtin_amdgcn_readfirstlane(last);
   }
-  const int rho = tile * kRows + 32 * wave + n32;
+  const int rho = tile * kGradRows + 32 * wave + n32;
   const bool real = rho < rows;
   int lo, hi;
   limits(rho, lo, hi);
@@ -122,10 +77,10 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void dq_kernel(CoreGradArgs 
   most = __builtin_amdgcn_readfirstlane(most);
   low = __builtin_amdgcn_readfirstlane(low);
   high = __builtin_amdgcn_readfirstlane(high);
-  const int block = tile * (kRows / kTile) + wave / 2;
+  const int block = tile * (kGradRows / kTile) + wave / 2;
   if (h == 0 && (wave & 1) == 0) {  // of 64 rows: a lane each
     int lo1, hi1;
-    limits(tile * kRows + 32 * wave + lane, lo1, hi1);
+    limits(tile * kGradRows + 32 * wave + lane, lo1, hi1);
     RowRange x{hi1 > 0 ? lo1 : INT32_MAX, hi1, lo1, hi1};
 #pragma unroll
     for (int i = 1; i < 64; i <<= 1) {
@@ -161,7 +116,7 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void dq_kernel(CoreGradArgs 
   if (a.dlse && real) delta -= a.dlse[at];
   const float lse = real ? a.lse[at] * 1.44269504088896341f : 0.f;
   {
-    RowBlock& x = static_cast<RowBlock*>(a.blocks)[(int64_t)h * tiles * (kRows / kTile) + block];
+    RowBlock& x = static_cast<RowBlock*>(a.blocks)[(int64_t)h * tiles * (kGradRows / kTile) + block];
     const int n = 32 * (wave & 1) + n32;
     if (kg == 0) {
       x.lse[n] = lse;
@@ -262,254 +217,6 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void dq_kernel(CoreGradArgs 
   }
 }
 
-// Keys of a workgroup for dk and dv, 32 a wave.  With D = 256 two waves share 32 keys, as one's sums would not fit its
-// registers: one forms S, the other dP, they exchange them through shared memory, and each sums half of the dimensions.
-template <int D>
-constexpr bool kPair = D == 256;
-template <int D>
-constexpr int kKeys = kPair<D> ? 64 : 128;
-
-// dk and dv of kKeys keys of a key head; part s of `splits` takes every splits-th block of 64 rows that sees any of them
-template <class E, int D, bool BENT>
-__global__ __launch_bounds__(256, 1) void dkv_kernel(CoreGradArgs a, int blocks, int splits) {
-  typedef typename Vec<E>::x8 x8;
-  constexpr bool PAIR = kPair<D>;
-  constexpr int KQ = D / 16, MT = D / 32 / (PAIR ? 2 : 1);
-  static_assert(offsetof(RowBlock, stands) == 1024 && sizeof(RowBlock) == 1536, "an instruction, and half of one");
-  __shared__ __align__(16) E qt[2][kTileSize<D>];
-  __shared__ __align__(16) E yt[2][kTileSize<D>];
-  __shared__ __align__(16) float swap[PAIR ? 4 : 1][PAIR ? 1024 : 4];
-  __shared__ __align__(16) RowBlock info[2];
-  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const int n32 = lane & 31, kg = lane >> 5;
-  const int half = PAIR ? wave & 1 : 0;  // of the pair: 0 forms S and sums dimensions below D / 2, 1 dP and those above
-  // the first keys, which most rows see, first
-  const int h = blockIdx.x % a.kv_heads, s = blockIdx.x / a.kv_heads % splits;
-  const int k0 = blockIdx.x / (a.kv_heads * splits) * kKeys<D>;
-  const int group = a.group.d, rows = (int)a.T * group, mine = k0 + 32 * (PAIR ? wave >> 1 : wave);
-  const int key = mine + n32;
-  const bool real = key < a.S;
-  const TileOperands<E, D> at_tile(lane);
-  const Bend bend(a.scale, BENT ? a.cap : 0.f, nullptr, 0);
-
-  x8 kf[KQ], vf[PAIR ? 1 : KQ];  // lane (n32, kg): key n32, dimensions 16 i + 8 kg ..; of a pair, kf is V in the second
-  {
-    const E* k = static_cast<const E*>(a.k) + h * a.k_head + (real ? key : 0) * a.k_token + 8 * kg;
-    const E* v = static_cast<const E*>(a.v) + h * a.v_head + (real ? key : 0) * a.v_token + 8 * kg;
-    const u32x4 none{0, 0, 0, 0};
-#pragma unroll
-    for (int i = 0; i < KQ; ++i) {
-      kf[i] = __builtin_bit_cast(x8, real ? *reinterpret_cast<const u32x4*>((half ? v : k) + 16 * i) : none);
-      if constexpr (!PAIR) vf[i] = __builtin_bit_cast(x8, real ? *reinterpret_cast<const u32x4*>(v + 16 * i) : none);
-    }
-  }
-  f32x16 dk[MT], dv[MT];
-#pragma unroll
-  for (int i = 0; i < MT; ++i) dk[i] = dv[i] = f32x16{};
-  Range<E> range;
-
-  // The blocks of rows, 64 ranges at a time, a lane each: `left` are those of the present 64 that see any of the keys.
-  const RowRange* const ranges = static_cast<const RowRange*>(a.ranges);
-  int base = -64, turn = s;
-  RowRange mine64{};
-  uint64_t left = 0;
-  const auto next = [&](RowRange& x) -> int {  // the next block of this part, or -1
-    while (true) {
-      while (left) {
-        const int i = __builtin_ctzll(left);
-        left &= left - 1;
-        if (turn-- == 0) {
-          turn = splits - 1;
-          x.first = __builtin_amdgcn_readlane(mine64.first, i);
-          x.last = __builtin_amdgcn_readlane(mine64.last, i);
-          x.low = __builtin_amdgcn_readlane(mine64.low, i);
-          x.high = __builtin_amdgcn_readlane(mine64.high, i);
-          return base + i;
-        }
-      }
-      base += 64;
-      if (base >= blocks) return -1;
-      const bool there = base + lane < blocks;
-      mine64 = there ? ranges[base + lane] : RowRange{INT32_MAX, 0, 0, 0};
-      left = __ballot(there && mine64.last > k0 && mine64.first < k0 + kKeys<D>);
-    }
-  };
-  const auto stage = [&](int block, int buffer) {
-    // offsets from the wave's first token; rows behind the last: that once more
-    const int r0 = min(block * kTile + 16 * wave, rows - 1), t0 = a.group.of(r0);
-    const int rho = min(r0 + lane / 4, rows - 1), t = a.group.of(rho), g = rho - t * group;
-    load_rows16<E, D>(static_cast<const E*>(a.q) + t0 * a.q_token + h * group * a.q_head,
-                      (t - t0) * (uint32_t)a.q_token + g * (uint32_t)a.q_head, qt[buffer], wave, lane);
-    load_rows16<E, D>(static_cast<const E*>(a.dy) + t0 * a.dy_token + h * group * a.dy_head,
-                      (t - t0) * (uint32_t)a.dy_token + g * (uint32_t)a.dy_head, yt[buffer], wave, lane);
-    const RowBlock* const from = static_cast<const RowBlock*>(a.blocks) + ((int64_t)h * blocks + block);
-    if (wave == 0) load_blocks<1>(from, 16 * lane, &info[buffer]);
-    if (BENT && wave == 1 && lane < 32) load_blocks<1>(from->stands, 16 * lane, info[buffer].stands);
-  };
-  // of the u-th 32 rows: S and dP - delta, with a pair's one of them
-  const auto products = [&](const E* qp, const E* yp, const RowBlock& x, int u, f32x16& sc, f32x16& dp) {
-    sc = f32x16{};
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const f32x4 delta = *reinterpret_cast<const f32x4*>(x.delta + c_row(u, 4 * i) + 16 * kg);
-#pragma unroll
-      for (int e = 0; e < 4; ++e) dp[4 * i + e] = -delta[e];
-    }
-    if constexpr (PAIR) {
-      if (half) sc = dp;
-      const E* const p = half ? yp : qp;
-#pragma unroll
-      for (int i = 0; i < KQ; ++i) sc = mfma32(at_tile.rows(p, u, i), kf[i], sc);
-    } else {
-#pragma unroll
-      for (int i = 0; i < KQ; ++i) {
-        sc = mfma32(at_tile.rows(qp, u, i), kf[i], sc);
-        dp = mfma32(at_tile.rows(yp, u, i), vf[i], dp);
-      }
-    }
-  };
-  const auto give = [&](const f32x16& sc) {
-#pragma unroll
-    for (int i = 0; i < 4; ++i)
-      *reinterpret_cast<f32x4*>(swap[wave] + 256 * i + 4 * lane) = f32x4{sc[4 * i], sc[4 * i + 1], sc[4 * i + 2], sc[4 * i + 3]};
-  };
-  const auto take = [&](f32x16& sc, f32x16& dp) {
-    f32x16 other;
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const f32x4 x = *reinterpret_cast<const f32x4*>(swap[wave ^ 1] + 256 * i + 4 * lane);
-#pragma unroll
-      for (int e = 0; e < 4; ++e) other[4 * i + e] = x[e];
-    }
-    dp = half ? sc : other;
-    sc = half ? other : sc;
-  };
-  const auto sums = [&](const E* qp, const E* yp, const RowBlock& x, int u, f32x16& sc, f32x16& dp, bool odd, auto whole) {
-    constexpr bool WHOLE = decltype(whole)::value;
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const int row4 = c_row(u, 4 * i) + 16 * kg;
-      const f32x4 lse = *reinterpret_cast<const f32x4*>(x.lse + row4);
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const int e = 4 * i + j, row = row4 + j;
-        float p, rate = 1.f;
-        const float from = kWeightBias<E> - lse[j];
-        if constexpr (BENT) {
-          p = a.cap > 0.f ? bend.capped(sc[e], rate) : sc[e] * bend.c;
-          p = __builtin_fmaf(-x.slope[row], fabsf(x.stands[row] - (float)key), p);
-          p = __builtin_amdgcn_exp2f(p + from);
-        } else {
-          p = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[e], bend.c, from));
-        }
-        float dx = p * dp[e];
-        if constexpr (BENT) dx *= rate;
-        if constexpr (!WHOLE) {
-          const bool hidden = (int)(key < x.lo[row]) | (int)(key >= x.hi[row]);
-          if (hidden) p = dx = 0.f;
-        }
-        sc[e] = p;
-        dp[e] = dx;
-      }
-    }
-    range.fit(dp, dk);
-#pragma unroll
-    for (int b = 0; b < 2; ++b) {
-      u32x4 w, z;
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        w[e] = pack2<E>(sc[8 * b + 2 * e], sc[8 * b + 2 * e + 1]);
-        z[e] = pack2<E>(dp[8 * b + 2 * e] * range.f, dp[8 * b + 2 * e + 1] * range.f);
-      }
-#pragma unroll
-      for (int m = 0; m < MT; ++m) {
-        x8 y = at_tile.columns(yp, u, b, half * MT + m), q = at_tile.columns(qp, u, b, half * MT + m);
-        if (odd) {
-          y = finite_values<E>(y);
-          q = finite_values<E>(q);
-        }
-        dv[m] = mfma32(y, __builtin_bit_cast(x8, w), dv[m]);
-        dk[m] = mfma32(q, __builtin_bit_cast(x8, z), dk[m]);
-      }
-    }
-  };
-  const auto step = [&](const E* qp, const E* yp, const RowBlock& x, auto whole) {
-    constexpr bool WHOLE = decltype(whole)::value;
-    bool odd = false;
-    if constexpr (!WHOLE) odd = tile_is_odd<E, D>(qp, lane) || tile_is_odd<E, D>(yp, lane);
-    if constexpr (PAIR) {
-      f32x16 sc[2], dp[2];
-#pragma unroll
-      for (int u = 0; u < 2; ++u) products(qp, yp, x, u, sc[u], dp[u]);
-      give(sc[0]);
-      lds_barrier();
-      take(sc[0], dp[0]);
-      lds_barrier();
-      give(sc[1]);
-      lds_barrier();
-      take(sc[1], dp[1]);
-#pragma unroll
-      for (int u = 0; u < 2; ++u) sums(qp, yp, x, u, sc[u], dp[u], odd, whole);
-    } else {
-#pragma unroll
-      for (int u = 0; u < 2; ++u) {
-        f32x16 sc, dp;
-        products(qp, yp, x, u, sc, dp);
-        sums(qp, yp, x, u, sc, dp, odd, whole);
-      }
-    }
-    if (odd) {
-      const auto sees = [&](int i) { return key >= x.lo[i] && key < x.hi[i]; };
-      add_odd<E, D>(qp, dk, lane, sees, half * MT);
-      add_odd<E, D>(yp, dv, lane, sees, half * MT);
-    }
-  };
-
-  RowRange x, y;
-  int block = next(x), buffer = 0;
-  if (block >= 0) {
-    stage(block, 0);
-    tiles_ready();
-#pragma unroll 1
-    while (true) {
-      const int following = next(y);
-      if (following >= 0) stage(following, buffer ^ 1);
-      // a pair's waves meet within the step, so all of the workgroup's go through it, as far as any of them has to
-      const bool any = x.last > mine && x.first < mine + 32;
-      if (PAIR || any) {
-        if (x.low <= mine && mine + 32 <= x.high)
-          step(qt[buffer], yt[buffer], info[buffer], std::true_type{});
-        else
-          step(qt[buffer], yt[buffer], info[buffer], std::false_type{});
-      }
-      tiles_ready();
-      if (following < 0) break;
-      x = y;
-      buffer ^= 1;
-    }
-  }
-  if (real) {
-    const float f = a.scale * range.back() * (Range<E>::on ? 0x1p-15f : 1.f), g = Range<E>::on ? 0x1p-15f : 1.f;
-    const int64_t at = ((int64_t)key * a.kv_heads + h) * D + half * (D / 2);
-    float* const part = a.ws + (int64_t)s * 2 * a.S * a.kv_heads * D;
-#pragma unroll
-    for (int k = 0; k < MT; ++k)
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        const f32x4 u = f32x4{dk[k][4 * e], dk[k][4 * e + 1], dk[k][4 * e + 2], dk[k][4 * e + 3]} * f;
-        const f32x4 w = f32x4{dv[k][4 * e], dv[k][4 * e + 1], dv[k][4 * e + 2], dv[k][4 * e + 3]} * g;
-        const int d = 32 * k + 8 * e + 4 * kg;
-        if (splits == 1) {
-          st4(static_cast<E*>(a.dk) + at + d, u);
-          st4(static_cast<E*>(a.dv) + at + d, w);
-        } else {
-          *reinterpret_cast<f32x4*>(part + at + d) = u;
-          *reinterpret_cast<f32x4*>(part + (int64_t)a.S * a.kv_heads * D + at + d) = w;
-        }
-      }
-  }
-}
-
 // the parts of dk and dv, added up in their order, 4 values a thread
 template <class E>
 __global__ __launch_bounds__(256) void join_parts_kernel(const float* ws, int64_t size, int splits, E* dk, E* dv) {
@@ -522,22 +229,22 @@ __global__ __launch_bounds__(256) void join_parts_kernel(const float* ws, int64_
 }
 
 // blocks of 64 rows, of whole workgroups for dq
-int64_t row_blocks(int64_t T, int group) { return (T * group + kRows - 1) / kRows * (kRows / kTile); }
+int64_t row_blocks(int64_t T, int group) { return (T * group + kGradRows - 1) / kGradRows * (kGradRows / kTile); }
 
 // parts of the keys' gradients: two rounds of workgroups at least
 int key_parts(int64_t T, int64_t S, int kv_heads, int group, int D) {
-  const int keys = D == 256 ? kKeys<256> : kKeys<128>;
+  const int keys = D == 256 ? kKeys<256> : D == 128 ? kKeys<128> : kKeys<64>;
   const int64_t each = std::max<int64_t>(1, (S + keys - 1) / keys * kv_heads);
   return (int)std::max<int64_t>(1, std::min<int64_t>({1024 / each, 16, row_blocks(T, group)}));
 }
 
 template <class E, int D, bool BENT>
 void launch_grad(const CoreGradArgs& a, hipStream_t st) {
-  const int group = a.heads / a.kv_heads, tiles = (int)(row_blocks(a.T, group) / (kRows / kTile));
+  const int group = a.heads / a.kv_heads, tiles = (int)(row_blocks(a.T, group) / (kGradRows / kTile));
   const int splits = key_parts(a.T, a.S, a.kv_heads, group, D);
   if (tiles > 0) dq_kernel<E, D, BENT><<<tiles * a.kv_heads, 256, 0, st>>>(a, tiles);
   if (a.S == 0 || !a.dk) return;
-  dkv_kernel<E, D, BENT><<<(unsigned)((a.S + kKeys<D> - 1) / kKeys<D> * a.kv_heads * splits), 256, 0, st>>>(a, tiles * (kRows / kTile), splits);
+  launch_dkv<E, D>(a, tiles * (kGradRows / kTile), splits, st);
   if (splits > 1) {
     const int64_t size = (int64_t)a.S * a.kv_heads * D;
     join_parts_kernel<E><<<(unsigned)((2 * size + 1023) / 1024), 256, 0, st>>>(a.ws, size, splits, static_cast<E*>(a.dk), static_cast<E*>(a.dv));

@@ -1,0 +1,550 @@
+// The keys' part of the attention's gradients: dv_j = sum_t p_tj dy_t, dk_j = scale sum_t dx_tj q_t (attn_core_bwd.hip has
+// the formulas).
+//
+// A workgroup owns 256 keys (128 where D is 256), 64 a wave (32), and goes through the blocks of 64 rows that see any of
+// them, two tiles of Q and dY deep.  S = Q K^T and dP = dY V^T: a lane owns a key, whose K and V stay in registers, and P
+// and dX are already operands of dV^T = dY^T P and dK^T = Q^T dX.  One wave a SIMD, whose 512 registers hold the sums (256)
+// and the keys (128): every operand read from shared memory then serves two MFMAs, where with 32 keys a wave the
+// reads alone take all of the time.  Nothing else fills an MFMA's shadow then, so the exponentials stand between dP's MFMAs
+// and the rest of dX between dV's.
+#include <hip/hip_runtime.h>
+
+#include <cstddef>
+
+#include "attn_core_grad.hpp"
+
+namespace cqgdn {
+namespace {
+
+constexpr int kEarly = 4;  // operands read from LDS ahead of their use
+
+template <class E, int D, bool BENT>
+__global__ __launch_bounds__(256, 1) void dkv_kernel(CoreGradArgs a, int blocks, int splits) {
+  typedef typename Vec<E>::x8 x8;
+  constexpr int NK = kKeyGroups<D>, KQ = D / 16, MT = D / 32;
+  static_assert(offsetof(RowBlock, stands) == 1024 && sizeof(RowBlock) == 1536, "an instruction, and half of one");
+  __shared__ __align__(16) E qt[2][kTileSize<D>];
+  __shared__ __align__(16) E yt[2][kTileSize<D>];
+  __shared__ __align__(16) RowBlock info[2];
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int n32 = lane & 31, kg = lane >> 5;
+  // the first keys, which most rows see, first
+  const int h = blockIdx.x % a.kv_heads, s = blockIdx.x / a.kv_heads % splits;
+  const int k0 = blockIdx.x / (a.kv_heads * splits) * kKeys<D>;
+  const int group = a.group.d, rows = (int)a.T * group, mine = k0 + 32 * NK * wave;
+  const TileOperands<E, D> at_tile(lane);
+  const Bend bend(a.scale, BENT ? a.cap : 0.f, nullptr, 0);
+
+  x8 kf[NK][KQ], vf[NK][KQ];  // lane (n32, kg): keys 32 n + n32, dimensions 16 i + 8 kg ..
+#pragma unroll
+  for (int n = 0; n < NK; ++n) {
+    const int key = mine + 32 * n + n32;
+    const bool real = key < a.S;
+    const E* k = static_cast<const E*>(a.k) + h * a.k_head + (real ? key : 0) * a.k_token + 8 * kg;
+    const E* v = static_cast<const E*>(a.v) + h * a.v_head + (real ? key : 0) * a.v_token + 8 * kg;
+    const u32x4 none{0, 0, 0, 0};
+#pragma unroll
+    for (int i = 0; i < KQ; ++i) {
+      kf[n][i] = __builtin_bit_cast(x8, real ? *reinterpret_cast<const u32x4*>(k + 16 * i) : none);
+      vf[n][i] = __builtin_bit_cast(x8, real ? *reinterpret_cast<const u32x4*>(v + 16 * i) : none);
+    }
+  }
+  f32x16 dk[NK][MT], dv[NK][MT];
+#pragma unroll
+  for (int n = 0; n < NK; ++n)
+#pragma unroll
+    for (int i = 0; i < MT; ++i) dk[n][i] = dv[n][i] = f32x16{};
+  Range<E> range[NK];
+
+  // The blocks of rows, 64 ranges at a time, a lane each: `left` are those of the present 64 that see any of the keys.
+  const RowRange* const ranges = static_cast<const RowRange*>(a.ranges);
+  int base = -64, turn = s;
+  RowRange mine64{};
+  uint64_t left = 0;
+  const auto next = [&](RowRange& x) -> int {  // the next block of this part, or -1
+    while (true) {
+      while (left) {
+        const int i = __builtin_ctzll(left);
+        left &= left - 1;
+        if (turn-- == 0) {
+          turn = splits - 1;
+          x.first = __builtin_amdgcn_readlane(mine64.first, i);
+          x.last = __builtin_amdgcn_readlane(mine64.last, i);
+          x.low = __builtin_amdgcn_readlane(mine64.low, i);
+          x.high = __builtin_amdgcn_readlane(mine64.high, i);
+          return base + i;
+        }
+      }
+      base += 64;
+      if (base >= blocks) return -1;
+      const bool there = base + lane < blocks;
+      mine64 = there ? ranges[base + lane] : RowRange{INT32_MAX, 0, 0, 0};
+      left = __ballot(there && mine64.last > k0 && mine64.first < k0 + kKeys<D>);
+    }
+  };
+  const auto stage = [&](int block, int buffer) {
+    // offsets from the wave's first token; rows behind the last: that once more
+    const int r0 = min(block * kTile + 16 * wave, rows - 1), t0 = a.group.of(r0);
+    const int rho = min(r0 + lane / 4, rows - 1), t = a.group.of(rho), g = rho - t * group;
+    load_rows16<E, D>(static_cast<const E*>(a.q) + t0 * a.q_token + h * group * a.q_head,
+                      (t - t0) * (uint32_t)a.q_token + g * (uint32_t)a.q_head, qt[buffer], wave, lane);
+    load_rows16<E, D>(static_cast<const E*>(a.dy) + t0 * a.dy_token + h * group * a.dy_head,
+                      (t - t0) * (uint32_t)a.dy_token + g * (uint32_t)a.dy_head, yt[buffer], wave, lane);
+    const RowBlock* const from = static_cast<const RowBlock*>(a.blocks) + ((int64_t)h * blocks + block);
+    if (wave == 0) load_blocks<1>(from, 16 * lane, &info[buffer]);
+    if (BENT && wave == 1 && lane < 32) load_blocks<1>(from->stands, 16 * lane, info[buffer].stands);
+  };
+  // A step of 64 rows.  WHOLE: all of them see all of the wave's keys; ODD: some value of the tiles is not finite.
+  const auto step = [&](const E* qp, const E* yp, const RowBlock& x, auto whole, auto odd) {
+    constexpr bool WHOLE = decltype(whole)::value, ODD = decltype(odd)::value;
+    const auto part = [&](int u) {
+      f32x16 sc[NK], dp[NK];
+      x8 q[KQ], y[KQ];
+      const auto query = [&](int i) { q[i] = at_tile.rows(qp, u, i); };
+      const auto dy = [&](int i) { y[i] = at_tile.rows(yp, u, i); };
+      const auto column = [&](const E* p, int i) {
+        const x8 c = at_tile.columns(p, u, i / MT, i % MT);
+        return ODD ? finite_values<E>(c) : c;
+      };
+      f32x4 lse[4], delta[4];
+#pragma unroll
+      for (int i = 0; i < kEarly; ++i) query(i);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        lse[i] = *reinterpret_cast<const f32x4*>(x.lse + c_row(u, 4 * i) + 16 * kg);
+        delta[i] = *reinterpret_cast<const f32x4*>(x.delta + c_row(u, 4 * i) + 16 * kg);
+      }
+      __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+      for (int i = 0; i < KQ; ++i) {
+        if (i + kEarly < KQ)
+          query(i + kEarly);
+        else
+          dy(i + kEarly - KQ);
+#pragma unroll
+        for (int n = 0; n < NK; ++n) sc[n] = mfma32(q[i], kf[n][i], i == 0 ? f32x16{} : sc[n]);
+        __builtin_amdgcn_sched_barrier(0);
+      }
+      // weights: element e of group n
+      float rate[BENT ? NK : 1][16];
+      const auto weight = [&](int n, int e) {
+        const float from = kWeightBias<E> - lse[e >> 2][e & 3];
+        float p;
+        if constexpr (BENT) {
+          const int row = c_row(u, e) + 16 * kg;
+          rate[n][e] = 1.f;
+          p = a.cap > 0.f ? bend.capped(sc[n][e], rate[n][e]) : sc[n][e] * bend.c;
+          p = __builtin_fmaf(-x.slope[row], fabsf(x.stands[row] - (float)(mine + 32 * n + n32)), p);
+          p = __builtin_amdgcn_exp2f(p + from);
+        } else {
+          p = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[n][e], bend.c, from));
+        }
+        sc[n][e] = p;
+      };
+      x8 yc[2 * MT], qc[2 * MT];
+#pragma unroll
+      for (int i = 0; i < KQ; ++i) {
+        if (i + kEarly < KQ)
+          dy(i + kEarly);
+        else
+          yc[i + kEarly - KQ] = column(yp, i + kEarly - KQ);
+#pragma unroll
+        for (int n = 0; n < NK; ++n) {
+          f32x16 none;
+          if (i == 0) {
+#pragma unroll
+            for (int e = 0; e < 16; ++e) none[e] = -delta[e >> 2][e & 3];
+          }
+          dp[n] = mfma32(y[i], vf[n][i], i == 0 ? none : dp[n]);
+#pragma unroll
+          for (int e = i * 16 / KQ; e < (i + 1) * 16 / KQ; ++e) weight(n, e);
+        }
+        __builtin_amdgcn_sched_barrier(0);
+      }
+      if constexpr (!WHOLE) {
+#pragma unroll
+        for (int n = 0; n < NK; ++n)
+#pragma unroll
+          for (int e = 0; e < 16; ++e) {
+            const int row = c_row(u, e) + 16 * kg, key = mine + 32 * n + n32;
+            if ((int)(key < x.lo[row]) | (int)(key >= x.hi[row])) sc[n][e] = dp[n][e] = 0.f;
+          }
+      }
+      const auto weight8 = [&](int n, int b) {
+        u32x4 w;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) w[e] = pack2<E>(sc[n][8 * b + 2 * e], sc[n][8 * b + 2 * e + 1]);
+        return __builtin_bit_cast(x8, w);
+      };
+      const auto change = [&](int n, int e) {
+        dp[n][e] *= sc[n][e];
+        if constexpr (BENT) dp[n][e] *= rate[n][e];
+      };
+#pragma unroll
+      for (int b = 0; b < 2; ++b) {
+        x8 w[NK];
+#pragma unroll
+        for (int n = 0; n < NK; ++n) w[n] = weight8(n, b);
+#pragma unroll
+        for (int m = 0; m < MT; ++m) {
+          const int i = b * MT + m;
+          if (i + kEarly < 2 * MT)
+            yc[i + kEarly] = column(yp, i + kEarly);
+          else
+            qc[i + kEarly - 2 * MT] = column(qp, i + kEarly - 2 * MT);
+#pragma unroll
+          for (int n = 0; n < NK; ++n) {
+            dv[n][m] = mfma32(yc[i], w[n], dv[n][m]);
+#pragma unroll
+            for (int e = m * 8 / MT; e < (m + 1) * 8 / MT; ++e) change(n, 8 * b + e);
+          }
+          __builtin_amdgcn_sched_barrier(0);
+        }
+      }
+#pragma unroll
+      for (int n = 0; n < NK; ++n) range[n].fit(dp[n], dk[n]);
+#pragma unroll
+      for (int b = 0; b < 2; ++b) {
+        x8 z[NK];
+#pragma unroll
+        for (int n = 0; n < NK; ++n) {
+          u32x4 w;
+#pragma unroll
+          for (int e = 0; e < 4; ++e) w[e] = pack2<E>(dp[n][8 * b + 2 * e] * range[n].f, dp[n][8 * b + 2 * e + 1] * range[n].f);
+          z[n] = __builtin_bit_cast(x8, w);
+        }
+#pragma unroll
+        for (int m = 0; m < MT; ++m) {
+          const int i = b * MT + m;
+          if (i + kEarly < 2 * MT) qc[i + kEarly] = column(qp, i + kEarly);
+#pragma unroll
+          for (int n = 0; n < NK; ++n) dk[n][m] = mfma32(qc[i], z[n], dk[n][m]);
+          __builtin_amdgcn_sched_barrier(0);
+        }
+      }
+    };
+    part(0);
+    part(1);
+    if constexpr (ODD) {
+#pragma unroll
+      for (int n = 0; n < NK; ++n) {
+        const int key = mine + 32 * n + n32;
+        const auto sees = [&](int i) { return key >= x.lo[i] && key < x.hi[i]; };
+        add_odd<E, D>(qp, dk[n], lane, sees);
+        add_odd<E, D>(yp, dv[n], lane, sees);
+      }
+    }
+  };
+
+  RowRange x, y;
+  int block = next(x), buffer = 0;
+  if (block >= 0) {
+    stage(block, 0);
+    tiles_ready();
+#pragma unroll 1
+    while (true) {
+      const int following = next(y);
+      if (following >= 0) stage(following, buffer ^ 1);
+      const E* const qp = qt[buffer];
+      const E* const yp = yt[buffer];
+      if (x.last > mine && x.first < mine + 32 * NK) {
+        if (x.low <= mine && mine + 32 * NK <= x.high)
+          step(qp, yp, info[buffer], std::true_type{}, std::false_type{});
+        else if (!(tile_is_odd<E, D>(qp, lane) || tile_is_odd<E, D>(yp, lane)))
+          step(qp, yp, info[buffer], std::false_type{}, std::false_type{});
+        else
+          step(qp, yp, info[buffer], std::false_type{}, std::true_type{});
+      }
+      tiles_ready();
+      if (following < 0) break;
+      x = y;
+      buffer ^= 1;
+    }
+  }
+#pragma unroll
+  for (int n = 0; n < NK; ++n) {
+    const int key = mine + 32 * n + n32;
+    if (key >= a.S) continue;
+    const float f = a.scale * range[n].back() * (Range<E>::on ? 0x1p-15f : 1.f), g = Range<E>::on ? 0x1p-15f : 1.f;
+    const int64_t at = ((int64_t)key * a.kv_heads + h) * D, size = (int64_t)a.S * a.kv_heads * D;
+    float* const part = a.ws + s * 2 * size;
+#pragma unroll
+    for (int k = 0; k < MT; ++k)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const f32x4 u = f32x4{dk[n][k][4 * e], dk[n][k][4 * e + 1], dk[n][k][4 * e + 2], dk[n][k][4 * e + 3]} * f;
+        const f32x4 w = f32x4{dv[n][k][4 * e], dv[n][k][4 * e + 1], dv[n][k][4 * e + 2], dv[n][k][4 * e + 3]} * g;
+        const int d = 32 * k + 8 * e + 4 * kg;
+        if (splits == 1) {
+          st4(static_cast<E*>(a.dk) + at + d, u);
+          st4(static_cast<E*>(a.dv) + at + d, w);
+        } else {
+          *reinterpret_cast<f32x4*>(part + at + d) = u;
+          *reinterpret_cast<f32x4*>(part + size + at + d) = w;
+        }
+      }
+  }
+}
+
+// dk and dv of kKeys keys of a key head; part s of `splits` takes every splits-th block of 64 rows that sees any of them
+template <class E, int D, bool BENT>
+__global__ __launch_bounds__(256, 1) void pair_kernel(CoreGradArgs a, int blocks, int splits) {
+  typedef typename Vec<E>::x8 x8;
+  constexpr bool PAIR = true;
+  constexpr int KQ = D / 16, MT = D / 32 / (PAIR ? 2 : 1);
+  static_assert(offsetof(RowBlock, stands) == 1024 && sizeof(RowBlock) == 1536, "an instruction, and half of one");
+  __shared__ __align__(16) E qt[2][kTileSize<D>];
+  __shared__ __align__(16) E yt[2][kTileSize<D>];
+  __shared__ __align__(16) float swap[PAIR ? 4 : 1][PAIR ? 1024 : 4];
+  __shared__ __align__(16) RowBlock info[2];
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int n32 = lane & 31, kg = lane >> 5;
+  const int half = PAIR ? wave & 1 : 0;  // of the pair: 0 forms S and sums dimensions below D / 2, 1 dP and those above
+  // the first keys, which most rows see, first
+  const int h = blockIdx.x % a.kv_heads, s = blockIdx.x / a.kv_heads % splits;
+  const int k0 = blockIdx.x / (a.kv_heads * splits) * kKeys<D>;
+  const int group = a.group.d, rows = (int)a.T * group, mine = k0 + 32 * (PAIR ? wave >> 1 : wave);
+  const int key = mine + n32;
+  const bool real = key < a.S;
+  const TileOperands<E, D> at_tile(lane);
+  const Bend bend(a.scale, BENT ? a.cap : 0.f, nullptr, 0);
+
+  x8 kf[KQ], vf[PAIR ? 1 : KQ];  // lane (n32, kg): key n32, dimensions 16 i + 8 kg ..; of a pair, kf is V in the second
+  {
+    const E* k = static_cast<const E*>(a.k) + h * a.k_head + (real ? key : 0) * a.k_token + 8 * kg;
+    const E* v = static_cast<const E*>(a.v) + h * a.v_head + (real ? key : 0) * a.v_token + 8 * kg;
+    const u32x4 none{0, 0, 0, 0};
+#pragma unroll
+    for (int i = 0; i < KQ; ++i) {
+      kf[i] = __builtin_bit_cast(x8, real ? *reinterpret_cast<const u32x4*>((half ? v : k) + 16 * i) : none);
+      if constexpr (!PAIR) vf[i] = __builtin_bit_cast(x8, real ? *reinterpret_cast<const u32x4*>(v + 16 * i) : none);
+    }
+  }
+  f32x16 dk[MT], dv[MT];
+#pragma unroll
+  for (int i = 0; i < MT; ++i) dk[i] = dv[i] = f32x16{};
+  Range<E> range;
+
+  // The blocks of rows, 64 ranges at a time, a lane each: `left` are those of the present 64 that see any of the keys.
+  const RowRange* const ranges = static_cast<const RowRange*>(a.ranges);
+  int base = -64, turn = s;
+  RowRange mine64{};
+  uint64_t left = 0;
+  const auto next = [&](RowRange& x) -> int {  // the next block of this part, or -1
+    while (true) {
+      while (left) {
+        const int i = __builtin_ctzll(left);
+        left &= left - 1;
+        if (turn-- == 0) {
+          turn = splits - 1;
+          x.first = __builtin_amdgcn_readlane(mine64.first, i);
+          x.last = __builtin_amdgcn_readlane(mine64.last, i);
+          x.low = __builtin_amdgcn_readlane(mine64.low, i);
+          x.high = __builtin_amdgcn_readlane(mine64.high, i);
+          return base + i;
+        }
+      }
+      base += 64;
+      if (base >= blocks) return -1;
+      const bool there = base + lane < blocks;
+      mine64 = there ? ranges[base + lane] : RowRange{INT32_MAX, 0, 0, 0};
+      left = __ballot(there && mine64.last > k0 && mine64.first < k0 + kKeys<D>);
+    }
+  };
+  const auto stage = [&](int block, int buffer) {
+    // offsets from the wave's first token; rows behind the last: that once more
+    const int r0 = min(block * kTile + 16 * wave, rows - 1), t0 = a.group.of(r0);
+    const int rho = min(r0 + lane / 4, rows - 1), t = a.group.of(rho), g = rho - t * group;
+    load_rows16<E, D>(static_cast<const E*>(a.q) + t0 * a.q_token + h * group * a.q_head,
+                      (t - t0) * (uint32_t)a.q_token + g * (uint32_t)a.q_head, qt[buffer], wave, lane);
+    load_rows16<E, D>(static_cast<const E*>(a.dy) + t0 * a.dy_token + h * group * a.dy_head,
+                      (t - t0) * (uint32_t)a.dy_token + g * (uint32_t)a.dy_head, yt[buffer], wave, lane);
+    const RowBlock* const from = static_cast<const RowBlock*>(a.blocks) + ((int64_t)h * blocks + block);
+    if (wave == 0) load_blocks<1>(from, 16 * lane, &info[buffer]);
+    if (BENT && wave == 1 && lane < 32) load_blocks<1>(from->stands, 16 * lane, info[buffer].stands);
+  };
+  // of the u-th 32 rows: S and dP - delta, with a pair's one of them
+  const auto products = [&](const E* qp, const E* yp, const RowBlock& x, int u, f32x16& sc, f32x16& dp) {
+    sc = f32x16{};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const f32x4 delta = *reinterpret_cast<const f32x4*>(x.delta + c_row(u, 4 * i) + 16 * kg);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) dp[4 * i + e] = -delta[e];
+    }
+    if constexpr (PAIR) {
+      if (half) sc = dp;
+      const E* const p = half ? yp : qp;
+#pragma unroll
+      for (int i = 0; i < KQ; ++i) sc = mfma32(at_tile.rows(p, u, i), kf[i], sc);
+    } else {
+#pragma unroll
+      for (int i = 0; i < KQ; ++i) {
+        sc = mfma32(at_tile.rows(qp, u, i), kf[i], sc);
+        dp = mfma32(at_tile.rows(yp, u, i), vf[i], dp);
+      }
+    }
+  };
+  const auto give = [&](const f32x16& sc) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      *reinterpret_cast<f32x4*>(swap[wave] + 256 * i + 4 * lane) = f32x4{sc[4 * i], sc[4 * i + 1], sc[4 * i + 2], sc[4 * i + 3]};
+  };
+  const auto take = [&](f32x16& sc, f32x16& dp) {
+    f32x16 other;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const f32x4 x = *reinterpret_cast<const f32x4*>(swap[wave ^ 1] + 256 * i + 4 * lane);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) other[4 * i + e] = x[e];
+    }
+    dp = half ? sc : other;
+    sc = half ? other : sc;
+  };
+  const auto sums = [&](const E* qp, const E* yp, const RowBlock& x, int u, f32x16& sc, f32x16& dp, bool odd, auto whole) {
+    constexpr bool WHOLE = decltype(whole)::value;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int row4 = c_row(u, 4 * i) + 16 * kg;
+      const f32x4 lse = *reinterpret_cast<const f32x4*>(x.lse + row4);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const int e = 4 * i + j, row = row4 + j;
+        float p, rate = 1.f;
+        const float from = kWeightBias<E> - lse[j];
+        if constexpr (BENT) {
+          p = a.cap > 0.f ? bend.capped(sc[e], rate) : sc[e] * bend.c;
+          p = __builtin_fmaf(-x.slope[row], fabsf(x.stands[row] - (float)key), p);
+          p = __builtin_amdgcn_exp2f(p + from);
+        } else {
+          p = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[e], bend.c, from));
+        }
+        float dx = p * dp[e];
+        if constexpr (BENT) dx *= rate;
+        if constexpr (!WHOLE) {
+          const bool hidden = (int)(key < x.lo[row]) | (int)(key >= x.hi[row]);
+          if (hidden) p = dx = 0.f;
+        }
+        sc[e] = p;
+        dp[e] = dx;
+      }
+    }
+    range.fit(dp, dk);
+#pragma unroll
+    for (int b = 0; b < 2; ++b) {
+      u32x4 w, z;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        w[e] = pack2<E>(sc[8 * b + 2 * e], sc[8 * b + 2 * e + 1]);
+        z[e] = pack2<E>(dp[8 * b + 2 * e] * range.f, dp[8 * b + 2 * e + 1] * range.f);
+      }
+#pragma unroll
+      for (int m = 0; m < MT; ++m) {
+        x8 y = at_tile.columns(yp, u, b, half * MT + m), q = at_tile.columns(qp, u, b, half * MT + m);
+        if (odd) {
+          y = finite_values<E>(y);
+          q = finite_values<E>(q);
+        }
+        dv[m] = mfma32(y, __builtin_bit_cast(x8, w), dv[m]);
+        dk[m] = mfma32(q, __builtin_bit_cast(x8, z), dk[m]);
+      }
+    }
+  };
+  const auto step = [&](const E* qp, const E* yp, const RowBlock& x, auto whole) {
+    constexpr bool WHOLE = decltype(whole)::value;
+    bool odd = false;
+    if constexpr (!WHOLE) odd = tile_is_odd<E, D>(qp, lane) || tile_is_odd<E, D>(yp, lane);
+    if constexpr (PAIR) {
+      f32x16 sc[2], dp[2];
+#pragma unroll
+      for (int u = 0; u < 2; ++u) products(qp, yp, x, u, sc[u], dp[u]);
+      give(sc[0]);
+      lds_barrier();
+      take(sc[0], dp[0]);
+      lds_barrier();
+      give(sc[1]);
+      lds_barrier();
+      take(sc[1], dp[1]);
+#pragma unroll
+      for (int u = 0; u < 2; ++u) sums(qp, yp, x, u, sc[u], dp[u], odd, whole);
+    } else {
+#pragma unroll
+      for (int u = 0; u < 2; ++u) {
+        f32x16 sc, dp;
+        products(qp, yp, x, u, sc, dp);
+        sums(qp, yp, x, u, sc, dp, odd, whole);
+      }
+    }
+    if (odd) {
+      const auto sees = [&](int i) { return key >= x.lo[i] && key < x.hi[i]; };
+      add_odd<E, D>(qp, dk, lane, sees, half * MT);
+      add_odd<E, D>(yp, dv, lane, sees, half * MT);
+    }
+  };
+
+  RowRange x, y;
+  int block = next(x), buffer = 0;
+  if (block >= 0) {
+    stage(block, 0);
+    tiles_ready();
+#pragma unroll 1
+    while (true) {
+      const int following = next(y);
+      if (following >= 0) stage(following, buffer ^ 1);
+      // a pair's waves meet within the step, so all of the workgroup's go through it, as far as any of them has to
+      const bool any = x.last > mine && x.first < mine + 32;
+      if (PAIR || any) {
+        if (x.low <= mine && mine + 32 <= x.high)
+          step(qt[buffer], yt[buffer], info[buffer], std::true_type{});
+        else
+          step(qt[buffer], yt[buffer], info[buffer], std::false_type{});
+      }
+      tiles_ready();
+      if (following < 0) break;
+      x = y;
+      buffer ^= 1;
+    }
+  }
+  if (real) {
+    const float f = a.scale * range.back() * (Range<E>::on ? 0x1p-15f : 1.f), g = Range<E>::on ? 0x1p-15f : 1.f;
+    const int64_t at = ((int64_t)key * a.kv_heads + h) * D + half * (D / 2);
+    float* const part = a.ws + (int64_t)s * 2 * a.S * a.kv_heads * D;
+#pragma unroll
+    for (int k = 0; k < MT; ++k)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const f32x4 u = f32x4{dk[k][4 * e], dk[k][4 * e + 1], dk[k][4 * e + 2], dk[k][4 * e + 3]} * f;
+        const f32x4 w = f32x4{dv[k][4 * e], dv[k][4 * e + 1], dv[k][4 * e + 2], dv[k][4 * e + 3]} * g;
+        const int d = 32 * k + 8 * e + 4 * kg;
+        if (splits == 1) {
+          st4(static_cast<E*>(a.dk) + at + d, u);
+          st4(static_cast<E*>(a.dv) + at + d, w);
+        } else {
+          *reinterpret_cast<f32x4*>(part + at + d) = u;
+          *reinterpret_cast<f32x4*>(part + (int64_t)a.S * a.kv_heads * D + at + d) = w;
+        }
+      }
+  }
+}
+
+}  // namespace
+
+template <class E, int D>
+void launch_dkv(const CoreGradArgs& a, int blocks, int splits, hipStream_t st) {
+  const unsigned grid = (unsigned)((a.S + kKeys<D> - 1) / kKeys<D> * a.kv_heads * splits);
+  const bool bent = a.cap > 0.f || a.slopes;
+  if constexpr (D == 256)
+    bent ? pair_kernel<E, D, true><<<grid, 256, 0, st>>>(a, blocks, splits)
+         : pair_kernel<E, D, false><<<grid, 256, 0, st>>>(a, blocks, splits);
+  else
+    bent ? dkv_kernel<E, D, true><<<grid, 256, 0, st>>>(a, blocks, splits)
+         : dkv_kernel<E, D, false><<<grid, 256, 0, st>>>(a, blocks, splits);
+}
+template void launch_dkv<bf16, 64>(const CoreGradArgs&, int, int, hipStream_t);
+template void launch_dkv<bf16, 128>(const CoreGradArgs&, int, int, hipStream_t);
+template void launch_dkv<bf16, 256>(const CoreGradArgs&, int, int, hipStream_t);
+template void launch_dkv<f16, 64>(const CoreGradArgs&, int, int, hipStream_t);
+template void launch_dkv<f16, 128>(const CoreGradArgs&, int, int, hipStream_t);
+template void launch_dkv<f16, 256>(const CoreGradArgs&, int, int, hipStream_t);
+
+}  // namespace cqgdn
