@@ -89,9 +89,12 @@ template <class E, int D>
 __device__ __forceinline__ void load_rows16(const E* rows, uint32_t offset, E* tile, int wave, int lane) {
   load_blocks<D / 32>(rows, (offset + 8 * (lane & 3)) * sizeof(E), tile + wave * kTileRows16<D>);
 }
-// Everything that the workgroup's waves have asked for has arrived, and all have read what they wanted.
+// What the workgroup's waves have asked for has arrived, but for the last LATER instructions of each, and all have read what
+// they wanted.  (Loads of the compiler's own behind those make it wait for more, never for less.)
+template <int LATER = 0>
 __device__ __forceinline__ void tiles_ready() {
-  asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
+  static_assert(LATER < 64, "vmcnt is 6 bits");
+  asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(LATER) : "memory");
 }
 
 // ---- values that are not finite -----------------------------------------------------------------------
@@ -174,7 +177,7 @@ struct Bend {
 
 // What the keys' gradients need of 64 rows of a key head, as the queries' gradients leave it.
 struct RowBlock {
-  float lse[64], delta[64];     // log2 sum of exp2, and dy.out less the gradient of lse
+  float lse[64], delta[64];     // less log2 sum of exp2, and less dy.out plus the gradient of lse: what is added
   int lo[64], hi[64];           // the keys that the row sees
   float stands[64], slope[64];  // with a bias: the row's position, its head's slope times log2 e
 };

@@ -115,12 +115,13 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void dq_kernel(CoreGradArgs 
   }
   if (a.dlse && real) delta -= a.dlse[at];
   const float lse = real ? a.lse[at] * 1.44269504088896341f : 0.f;
+  const float base = kWeightBias<E> - lse;
   {
     RowBlock& x = static_cast<RowBlock*>(a.blocks)[(int64_t)h * tiles * (kGradRows / kTile) + block];
     const int n = 32 * (wave & 1) + n32;
     if (kg == 0) {
-      x.lse[n] = lse;
-      x.delta[n] = delta;
+      x.lse[n] = base;
+      x.delta[n] = -delta;
       x.lo[n] = lo;
       x.hi[n] = hi;
       if constexpr (BENT) {
@@ -134,7 +135,6 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void dq_kernel(CoreGradArgs 
 #pragma unroll
   for (int i = 0; i < MT; ++i) acc[i] = f32x16{};
   Range<E> range;
-  const float base = kWeightBias<E> - lse;
 
   const auto stage = [&](int j) {
     const int pos = first + j * TOK;

@@ -17,15 +17,16 @@ namespace cqgdn {
 namespace {
 
 constexpr int kEarly = 4;  // operands read from LDS ahead of their use
+constexpr int kDepth = 4;  // tiles of Q and of dY, of which all but one are on their way
 
 template <class E, int D, bool BENT>
 __global__ __launch_bounds__(256, 1) void dkv_kernel(CoreGradArgs a, int blocks, int splits) {
   typedef typename Vec<E>::x8 x8;
-  constexpr int NK = kKeyGroups<D>, KQ = D / 16, MT = D / 32;
-  static_assert(offsetof(RowBlock, stands) == 1024 && sizeof(RowBlock) == 1536, "an instruction, and half of one");
-  __shared__ __align__(16) E qt[2][kTileSize<D>];
-  __shared__ __align__(16) E yt[2][kTileSize<D>];
-  __shared__ __align__(16) RowBlock info[2];
+  constexpr int NK = kKeyGroups<D>, KQ = D / 16, MT = D / 32, DEPTH = kDepth, LOADS = 2 * (D / 32) + 1;
+  static_assert(offsetof(RowBlock, stands) == 1024 && sizeof(RowBlock) == 1536, "a quarter a wave");
+  __shared__ __align__(16) E qt[DEPTH][kTileSize<D>];
+  __shared__ __align__(16) E yt[DEPTH][kTileSize<D>];
+  __shared__ __align__(16) RowBlock info[DEPTH];
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int n32 = lane & 31, kg = lane >> 5;
   // the first keys, which most rows see, first
@@ -90,9 +91,11 @@ __global__ __launch_bounds__(256, 1) void dkv_kernel(CoreGradArgs a, int blocks,
                       (t - t0) * (uint32_t)a.q_token + g * (uint32_t)a.q_head, qt[buffer], wave, lane);
     load_rows16<E, D>(static_cast<const E*>(a.dy) + t0 * a.dy_token + h * group * a.dy_head,
                       (t - t0) * (uint32_t)a.dy_token + g * (uint32_t)a.dy_head, yt[buffer], wave, lane);
+    // a quarter of the block's values, so that every wave has asked for as many instructions
+    constexpr int part = (BENT ? sizeof(RowBlock) : offsetof(RowBlock, stands)) / 4;
     const RowBlock* const from = static_cast<const RowBlock*>(a.blocks) + ((int64_t)h * blocks + block);
-    if (wave == 0) load_blocks<1>(from, 16 * lane, &info[buffer]);
-    if (BENT && wave == 1 && lane < 32) load_blocks<1>(from->stands, 16 * lane, info[buffer].stands);
+    if (lane < part / 16)
+      load_blocks<1>(reinterpret_cast<const char*>(from) + wave * part, 16 * lane, reinterpret_cast<char*>(&info[buffer]) + wave * part);
   };
   // A step of 64 rows.  WHOLE: all of them see all of the wave's keys; ODD: some value of the tiles is not finite.
   const auto step = [&](const E* qp, const E* yp, const RowBlock& x, auto whole, auto odd) {
@@ -107,13 +110,9 @@ __global__ __launch_bounds__(256, 1) void dkv_kernel(CoreGradArgs a, int blocks,
         return ODD ? finite_values<E>(c) : c;
       };
       f32x4 lse[4], delta[4];
+      const auto values = [&](const float* p, int i) { return *reinterpret_cast<const f32x4*>(p + c_row(u, 4 * i) + 16 * kg); };
 #pragma unroll
       for (int i = 0; i < kEarly; ++i) query(i);
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        lse[i] = *reinterpret_cast<const f32x4*>(x.lse + c_row(u, 4 * i) + 16 * kg);
-        delta[i] = *reinterpret_cast<const f32x4*>(x.delta + c_row(u, 4 * i) + 16 * kg);
-      }
       __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
       for (int i = 0; i < KQ; ++i) {
@@ -121,6 +120,8 @@ __global__ __launch_bounds__(256, 1) void dkv_kernel(CoreGradArgs a, int blocks,
           query(i + kEarly);
         else
           dy(i + kEarly - KQ);
+        if (i >= KQ - 4) delta[i - KQ + 4] = values(x.delta, i - KQ + 4);
+        if (i == KQ - 1) lse[0] = values(x.lse, 0);
 #pragma unroll
         for (int n = 0; n < NK; ++n) sc[n] = mfma32(q[i], kf[n][i], i == 0 ? f32x16{} : sc[n]);
         __builtin_amdgcn_sched_barrier(0);
@@ -128,7 +129,7 @@ __global__ __launch_bounds__(256, 1) void dkv_kernel(CoreGradArgs a, int blocks,
       // weights: element e of group n
       float rate[BENT ? NK : 1][16];
       const auto weight = [&](int n, int e) {
-        const float from = kWeightBias<E> - lse[e >> 2][e & 3];
+        const float from = lse[e >> 2][e & 3];
         float p;
         if constexpr (BENT) {
           const int row = c_row(u, e) + 16 * kg;
@@ -148,12 +149,13 @@ __global__ __launch_bounds__(256, 1) void dkv_kernel(CoreGradArgs a, int blocks,
           dy(i + kEarly);
         else
           yc[i + kEarly - KQ] = column(yp, i + kEarly - KQ);
+        if (i * 4 % KQ == 0 && i * 4 / KQ < 3) lse[i * 4 / KQ + 1] = values(x.lse, i * 4 / KQ + 1);
 #pragma unroll
         for (int n = 0; n < NK; ++n) {
           f32x16 none;
           if (i == 0) {
 #pragma unroll
-            for (int e = 0; e < 16; ++e) none[e] = -delta[e >> 2][e & 3];
+            for (int e = 0; e < 16; ++e) none[e] = delta[e >> 2][e & 3];
           }
           dp[n] = mfma32(y[i], vf[n][i], i == 0 ? none : dp[n]);
 #pragma unroll
@@ -236,30 +238,55 @@ __global__ __launch_bounds__(256, 1) void dkv_kernel(CoreGradArgs a, int blocks,
     }
   };
 
-  RowRange x, y;
-  int block = next(x), buffer = 0;
-  if (block >= 0) {
-    stage(block, 0);
-    tiles_ready();
-#pragma unroll 1
-    while (true) {
-      const int following = next(y);
-      if (following >= 0) stage(following, buffer ^ 1);
-      const E* const qp = qt[buffer];
-      const E* const yp = yt[buffer];
-      if (x.last > mine && x.first < mine + 32 * NK) {
-        if (x.low <= mine && mine + 32 * NK <= x.high)
-          step(qp, yp, info[buffer], std::true_type{}, std::false_type{});
-        else if (!(tile_is_odd<E, D>(qp, lane) || tile_is_odd<E, D>(yp, lane)))
-          step(qp, yp, info[buffer], std::false_type{}, std::false_type{});
-        else
-          step(qp, yp, info[buffer], std::false_type{}, std::true_type{});
-      }
+  // blocks and ranges of the present step and of those whose tiles are on their way
+  RowRange ranged[DEPTH];
+  int block[DEPTH], buffer = 0;
+  bool all = true;  // nothing has been left out behind the last step
+#pragma unroll
+  for (int i = 0; i < DEPTH - 1; ++i) {
+    block[i] = next(ranged[i]);
+    if (block[i] >= 0) stage(block[i], i);
+  }
+  tiles_ready();
+  const auto ask = [&] {
+    block[DEPTH - 1] = next(ranged[DEPTH - 1]);
+    all = block[DEPTH - 1] >= 0;
+    if (all) stage(block[DEPTH - 1], buffer == 0 ? DEPTH - 1 : buffer - 1);
+  };
+  const auto advance = [&] {
+    // the next step's tiles; those behind it, if all of them were asked for, may still be on their way
+    if (all)
+      tiles_ready<(DEPTH - 2) * LOADS>();
+    else
       tiles_ready();
-      if (following < 0) break;
-      x = y;
-      buffer ^= 1;
+#pragma unroll
+    for (int i = 0; i + 1 < DEPTH; ++i) {
+      block[i] = block[i + 1];
+      ranged[i] = ranged[i + 1];
     }
+    buffer = buffer == DEPTH - 1 ? 0 : buffer + 1;
+  };
+  const auto whole = [&] { return ranged[0].low <= mine && mine + 32 * NK <= ranged[0].high; };
+  // A loop for the whole steps by itself: in one for both kinds, the sums would be moved from the registers that one leaves
+  // them in to the other's, in every step.
+  while (block[0] >= 0) {
+#pragma unroll 1
+    while (block[0] >= 0 && whole()) {
+      ask();
+      step(qt[buffer], yt[buffer], info[buffer], std::true_type{}, std::false_type{});
+      advance();
+    }
+    if (block[0] < 0) break;
+    ask();
+    const E* const qp = qt[buffer];
+    const E* const yp = yt[buffer];
+    if (ranged[0].last > mine && ranged[0].first < mine + 32 * NK) {
+      if (!(tile_is_odd<E, D>(qp, lane) || tile_is_odd<E, D>(yp, lane)))
+        step(qp, yp, info[buffer], std::false_type{}, std::false_type{});
+      else
+        step(qp, yp, info[buffer], std::false_type{}, std::true_type{});
+    }
+    advance();
   }
 #pragma unroll
   for (int n = 0; n < NK; ++n) {
@@ -370,7 +397,7 @@ __global__ __launch_bounds__(256, 1) void pair_kernel(CoreGradArgs a, int blocks
     for (int i = 0; i < 4; ++i) {
       const f32x4 delta = *reinterpret_cast<const f32x4*>(x.delta + c_row(u, 4 * i) + 16 * kg);
 #pragma unroll
-      for (int e = 0; e < 4; ++e) dp[4 * i + e] = -delta[e];
+      for (int e = 0; e < 4; ++e) dp[4 * i + e] = delta[e];
     }
     if constexpr (PAIR) {
       if (half) sc = dp;
@@ -411,7 +438,7 @@ __global__ __launch_bounds__(256, 1) void pair_kernel(CoreGradArgs a, int blocks
       for (int j = 0; j < 4; ++j) {
         const int e = 4 * i + j, row = row4 + j;
         float p, rate = 1.f;
-        const float from = kWeightBias<E> - lse[j];
+        const float from = lse[j];
         if constexpr (BENT) {
           p = a.cap > 0.f ? bend.capped(sc[e], rate) : sc[e] * bend.c;
           p = __builtin_fmaf(-x.slope[row], fabsf(x.stands[row] - (float)key), p);
