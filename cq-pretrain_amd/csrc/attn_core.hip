@@ -22,10 +22,11 @@ namespace {
 constexpr int kRows = 128;  // of a workgroup, 32 a wave
 constexpr int kEarly = 4;   // MFMA operands read from LDS ahead of their use
 
-// PAGED: keys from the pages of a cache; BENT: scores are capped or biased
-template <class E, int D, bool PAGED, bool BENT>
+// PAGED: keys from the pages of a cache; CAP, BIAS: scores are capped, biased
+template <class E, int D, bool PAGED, bool CAP, bool BIAS>
 __global__ __launch_bounds__(256, D == 256 ? 1 : D == 64 ? 3 : 2) void core_kernel(CoreArgs a, int tiles, int splits) {
   typedef typename Vec<E>::x8 x8;
+  constexpr bool BENT = CAP || BIAS;
   constexpr int TOK = kTile, KQ = D / 16, MT = D / 32;
   constexpr int F = 2 * KQ, H = 2 * MT;  // operands of a step: K's, and V's for 32 keys
   constexpr int kFirst = H < 8 ? H : 8;  // V's that are read while the scores of the second 32 keys are formed
@@ -118,8 +119,8 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : D == 64 ? 3 : 2) void core_kern
         qf[i] = __builtin_bit_cast(x8, w);
       }
     }
-    const Bend bend(a.scale, BENT ? a.cap : 0.f, BENT ? a.slopes : nullptr, head);
-    const int stands = BENT && real && r < requests ? (a.positions ? a.positions[t] : a.visible[t] - 1) : 0;
+    const Bend bend(a.scale, CAP ? a.cap : 0.f, BIAS ? a.slopes : nullptr, head);
+    const int stands = BIAS && real && r < requests ? (a.positions ? a.positions[t] : a.visible[t] - 1) : 0;
     f32x16 o[MT];
 #pragma unroll
     for (int i = 0; i < MT; ++i) o[i] = f32x16{};
@@ -175,18 +176,13 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : D == 64 ? 3 : 2) void core_kern
     // the scores with cap and bias, in units of log2 e
     const auto bent = [&](int u, int pos) {
       if constexpr (BENT) {
-        if (a.cap > 0.f) {
 #pragma unroll
-          for (int e = 0; e < 16; ++e) sc[u][e] = bend.capped(sc[u][e]);
-        } else {
+        for (int e = 0; e < 16; ++e) sc[u][e] = CAP ? bend.capped(sc[u][e]) : sc[u][e] * bend.c;
+      }
+      if constexpr (BIAS) {
+        const float far = (float)(stands - pos - 16 * kg);
 #pragma unroll
-          for (int e = 0; e < 16; ++e) sc[u][e] *= bend.c;
-        }
-        if (a.slopes) {
-          const float far = (float)(stands - pos - 16 * kg);
-#pragma unroll
-          for (int e = 0; e < 16; ++e) sc[u][e] = __builtin_fmaf(-bend.slope, fabsf(far - (float)c_row(u, e)), sc[u][e]);
-        }
+        for (int e = 0; e < 16; ++e) sc[u][e] = __builtin_fmaf(-bend.slope, fabsf(far - (float)c_row(u, e)), sc[u][e]);
       }
     };
     // where the weights have grown too large, or are a row's first, its maximum moves and they are made again
@@ -306,19 +302,30 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : D == 64 ? 3 : 2) void core_kern
       }
       shown = stage(table, 0);
       tiles_ready();
-#pragma unroll 1
-      for (int j = 0; j < n; ++j) {
-        const int pos = pos0 + j * TOK;
+      int j = 0, pos = pos0;
+      const auto ask = [&] {
         if (j + 1 < n) shown1 = stage(table1, j + 1);
         if constexpr (PAGED) table1 = entries(j + 2);
-        if (pos < most && pos + TOK > some) {
-          if (pos >= low && pos + TOK <= high && shown == (1 << GROUPS) - 1)
-            whole_step(kt[j & 1], vt[j & 1], pos);
-          else
-            cut_step(kt[j & 1], vt[j & 1], pos, shown);
-        }
-        shown = shown1;
+      };
+      const auto advance = [&] {
         tiles_ready();
+        shown = shown1;
+        ++j;
+        pos += TOK;
+      };
+      // A loop for the whole steps by itself: in one for both kinds, the sums would be moved from the registers that
+      // one leaves them in to the other's, in every step.
+      while (j < n) {
+#pragma unroll 1
+        while (j < n && pos >= low && pos + TOK <= high && shown == (1 << GROUPS) - 1) {
+          ask();
+          whole_step(kt[j & 1], vt[j & 1], pos);
+          advance();
+        }
+        if (j == n) break;
+        ask();
+        if (pos < most && pos + TOK > some) cut_step(kt[j & 1], vt[j & 1], pos, shown);
+        advance();
       }
     }
     l += __shfl_xor(l, 32, 64);
@@ -353,22 +360,20 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : D == 64 ? 3 : 2) void core_kern
   }
 }
 
-template <class E, int D, bool PAGED, bool BENT>
-void launch_core(const CoreArgs& a, int splits, hipStream_t st) {
+template <class E, int D, bool PAGED>
+void launch(const CoreArgs& a, int splits, hipStream_t st) {
   const int64_t requests = PAGED ? a.N : 1, each = std::max<int64_t>(1, requests * a.kv_heads * splits);
   const int64_t wanted = ((int64_t)(PAGED ? a.max_queries : a.T) * (a.heads / a.kv_heads) + kRows - 1) / kRows;
   const int tiles = (int)std::max<int64_t>(1, std::min<int64_t>(wanted, (1 << 23) / each));
   const int64_t blocks = requests * a.kv_heads * splits * tiles + (PAGED ? (int64_t)a.kv_heads * std::min(tiles, 16) : 0);
-  core_kernel<E, D, PAGED, BENT><<<(unsigned)blocks, 256, 0, st>>>(a, tiles, splits);
+  by_scores(a, [&](auto cap, auto bias) {
+    core_kernel<E, D, PAGED, decltype(cap)::value, decltype(bias)::value><<<(unsigned)blocks, 256, 0, st>>>(a, tiles, splits);
+  });
 }
 
 template <class E, int D>
 void by_kind(const CoreArgs& a, bool paged, int splits, hipStream_t st) {
-  const bool bent = a.cap > 0.f || a.slopes;
-  if (paged)
-    bent ? launch_core<E, D, true, true>(a, splits, st) : launch_core<E, D, true, false>(a, splits, st);
-  else
-    bent ? launch_core<E, D, false, true>(a, splits, st) : launch_core<E, D, false, false>(a, splits, st);
+  paged ? launch<E, D, true>(a, splits, st) : launch<E, D, false>(a, splits, st);
 }
 
 template <class E>

@@ -175,6 +175,15 @@ struct Bend {
   }
 };
 
+// f with whether scores are capped and whether they are biased, as types
+template <class F>
+void by_scores(const CoreArgs& a, F f) {
+  if (a.cap > 0.f)
+    a.slopes ? f(std::true_type{}, std::true_type{}) : f(std::true_type{}, std::false_type{});
+  else
+    a.slopes ? f(std::false_type{}, std::true_type{}) : f(std::false_type{}, std::false_type{});
+}
+
 // What the keys' gradients need of 64 rows of a key head, as the queries' gradients leave it.
 struct RowBlock {
   float lse[64], delta[64];     // less log2 sum of exp2, and less dy.out plus the gradient of lse: what is added

@@ -24,7 +24,7 @@
 namespace cqgdn {
 namespace {
 
-template <class E, int D, bool BENT>
+template <class E, int D, bool CAP, bool BIAS>
 __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void dq_kernel(CoreGradArgs a, int tiles) {
   typedef typename Vec<E>::x8 x8;
   constexpr int TOK = kTile, KQ = D / 16, MT = D / 32;
@@ -93,8 +93,8 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void dq_kernel(CoreGradArgs 
   }
   const int row_t = real ? a.group.of(rho) : 0, head = h * group + (real ? rho - row_t * group : 0);
   const int64_t at = (int64_t)row_t * a.heads + head;
-  const Bend bend(a.scale, BENT ? a.cap : 0.f, BENT ? a.slopes : nullptr, head);
-  const int stands = BENT && real ? (a.positions ? a.positions[row_t] : a.visible[row_t] - 1) : 0;
+  const Bend bend(a.scale, CAP ? a.cap : 0.f, BIAS ? a.slopes : nullptr, head);
+  const int stands = BIAS && real ? (a.positions ? a.positions[row_t] : a.visible[row_t] - 1) : 0;
 
   x8 qf[KQ], yf[KQ];  // lane (n32, kg): q and dy of row n32, dimensions 16 i + 8 kg ..
   float delta = 0.f;
@@ -124,7 +124,7 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void dq_kernel(CoreGradArgs 
       x.delta[n] = -delta;
       x.lo[n] = lo;
       x.hi[n] = hi;
-      if constexpr (BENT) {
+      if constexpr (BIAS) {
         x.stands[n] = (float)stands;
         x.slope[n] = bend.slope;
       }
@@ -159,15 +159,10 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void dq_kernel(CoreGradArgs 
 #pragma unroll
       for (int e = 0; e < 16; ++e) {
         float x = sc[e], rate = 1.f;
-        if constexpr (BENT) {
-          x = a.cap > 0.f ? bend.capped(x, rate) : x * bend.c;
-          x = __builtin_fmaf(-bend.slope, fabsf(far - (float)c_row(u, e)), x);
-          x = __builtin_amdgcn_exp2f(x + base);
-        } else {
-          x = __builtin_amdgcn_exp2f(__builtin_fmaf(x, bend.c, base));
-        }
-        x *= dp[e];
-        if constexpr (BENT) x *= rate;
+        x = CAP ? bend.capped(x, rate) + base : __builtin_fmaf(x, bend.c, base);
+        if constexpr (BIAS) x = __builtin_fmaf(-bend.slope, fabsf(far - (float)c_row(u, e)), x);
+        x = __builtin_amdgcn_exp2f(x) * dp[e];
+        if constexpr (CAP) x *= rate;
         const int at = c_row(u, e);
         if (!WHOLE && ((int)(at < lo0) | (int)(at >= hi0))) x = 0.f;
         dp[e] = x;
@@ -193,17 +188,25 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void dq_kernel(CoreGradArgs 
   if (n > 0) {
     stage(0);
     tiles_ready();
-#pragma unroll 1
-    for (int j = 0; j < n; ++j) {
-      const int pos = first + j * TOK;
-      if (j + 1 < n) stage(j + 1);
-      if (pos < most && pos + TOK > some) {
-        if (pos >= low && pos + TOK <= high)
-          step(kt[j & 1], vt[j & 1], pos, std::true_type{});
-        else
-          step(kt[j & 1], vt[j & 1], pos, std::false_type{});
-      }
+    int j = 0, pos = first;
+    const auto advance = [&] {
       tiles_ready();
+      ++j;
+      pos += TOK;
+    };
+    // A loop for the whole steps by itself: in one for both kinds, the sums would be moved from the registers that one
+    // leaves them in to the other's, in every step.
+    while (j < n) {
+#pragma unroll 1
+      while (j < n && pos >= low && pos + TOK <= high) {
+        if (j + 1 < n) stage(j + 1);
+        step(kt[j & 1], vt[j & 1], pos, std::true_type{});
+        advance();
+      }
+      if (j == n) break;
+      if (j + 1 < n) stage(j + 1);
+      if (pos < most && pos + TOK > some) step(kt[j & 1], vt[j & 1], pos, std::false_type{});
+      advance();
     }
   }
   if (real) {
@@ -235,14 +238,17 @@ int64_t row_blocks(int64_t T, int group) { return (T * group + kGradRows - 1) / 
 int key_parts(int64_t T, int64_t S, int kv_heads, int group, int D) {
   const int keys = D == 256 ? kKeys<256> : D == 128 ? kKeys<128> : kKeys<64>;
   const int64_t each = std::max<int64_t>(1, (S + keys - 1) / keys * kv_heads);
-  return (int)std::max<int64_t>(1, std::min<int64_t>({1024 / each, 16, row_blocks(T, group)}));
+  return (int)std::max<int64_t>(1, std::min<int64_t>({512 / each, 16, row_blocks(T, group)}));
 }
 
-template <class E, int D, bool BENT>
+template <class E, int D>
 void launch_grad(const CoreGradArgs& a, hipStream_t st) {
   const int group = a.heads / a.kv_heads, tiles = (int)(row_blocks(a.T, group) / (kGradRows / kTile));
   const int splits = key_parts(a.T, a.S, a.kv_heads, group, D);
-  if (tiles > 0) dq_kernel<E, D, BENT><<<tiles * a.kv_heads, 256, 0, st>>>(a, tiles);
+  if (tiles > 0)
+    by_scores(a, [&](auto cap, auto bias) {
+      dq_kernel<E, D, decltype(cap)::value, decltype(bias)::value><<<tiles * a.kv_heads, 256, 0, st>>>(a, tiles);
+    });
   if (a.S == 0 || !a.dk) return;
   launch_dkv<E, D>(a, tiles * (kGradRows / kTile), splits, st);
   if (splits > 1) {
@@ -251,19 +257,14 @@ void launch_grad(const CoreGradArgs& a, hipStream_t st) {
   }
 }
 
-template <class E, int D>
-void by_kind(const CoreGradArgs& a, hipStream_t st) {
-  a.cap > 0.f || a.slopes ? launch_grad<E, D, true>(a, st) : launch_grad<E, D, false>(a, st);
-}
-
 template <class E>
 void by_dim(const CoreGradArgs& a, hipStream_t st) {
   if (a.D == 64)
-    by_kind<E, 64>(a, st);
+    launch_grad<E, 64>(a, st);
   else if (a.D == 128)
-    by_kind<E, 128>(a, st);
+    launch_grad<E, 128>(a, st);
   else
-    by_kind<E, 256>(a, st);
+    launch_grad<E, 256>(a, st);
 }
 
 }  // namespace

@@ -16,46 +16,46 @@
 namespace cqgdn {
 namespace {
 
-constexpr int kEarly = 4;  // operands read from LDS ahead of their use
-constexpr int kDepth = 4;  // tiles of Q and of dY, of which all but one are on their way
-
-template <class E, int D, bool BENT>
-__global__ __launch_bounds__(256, 1) void dkv_kernel(CoreGradArgs a, int blocks, int splits) {
+template <class E, int D, bool CAP, bool BIAS>
+__global__ __launch_bounds__(512, 2) void dkv_kernel(CoreGradArgs a, int blocks, int splits) {
   typedef typename Vec<E>::x8 x8;
-  constexpr int NK = kKeyGroups<D>, KQ = D / 16, MT = D / 32, DEPTH = kDepth, LOADS = 2 * (D / 32) + 1;
-  static_assert(offsetof(RowBlock, stands) == 1024 && sizeof(RowBlock) == 1536, "a quarter a wave");
-  __shared__ __align__(16) E qt[DEPTH][kTileSize<D>];
-  __shared__ __align__(16) E yt[DEPTH][kTileSize<D>];
-  __shared__ __align__(16) RowBlock info[DEPTH];
+  constexpr int KQ = D / 16, MT = D / 32;
+  static_assert(offsetof(RowBlock, stands) == 1024 && sizeof(RowBlock) == 1536, "an eighth a wave");
+  __shared__ __align__(16) E vt[4][kTileSize<D>];
+  __shared__ __align__(16) E qt[2][kTileSize<D>];
+  __shared__ __align__(16) E yt[2][kTileSize<D>];
+  __shared__ __align__(16) RowBlock info[2];
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int n32 = lane & 31, kg = lane >> 5;
   // the first keys, which most rows see, first
   const int h = blockIdx.x % a.kv_heads, s = blockIdx.x / a.kv_heads % splits;
   const int k0 = blockIdx.x / (a.kv_heads * splits) * kKeys<D>;
-  const int group = a.group.d, rows = (int)a.T * group, mine = k0 + 32 * NK * wave;
+  const int group = a.group.d, rows = (int)a.T * group, mine = k0 + 64 * (wave >> 1);
+  // the lane's key: as an MFMA takes the rows of a tile
+  const int part = wave & 1, key = mine + 16 * (n32 >> 2 & 3) + 8 * part + 4 * (n32 >> 4) + (n32 & 3);
   const TileOperands<E, D> at_tile(lane);
-  const Bend bend(a.scale, BENT ? a.cap : 0.f, nullptr, 0);
+  const Bend bend(a.scale, CAP ? a.cap : 0.f, nullptr, 0);
 
-  x8 kf[NK][KQ], vf[NK][KQ];  // lane (n32, kg): keys 32 n + n32, dimensions 16 i + 8 kg ..
-#pragma unroll
-  for (int n = 0; n < NK; ++n) {
-    const int key = mine + 32 * n + n32;
+  x8 kf[KQ];  // lane (n32, kg): its key, dimensions 16 i + 8 kg ..
+  {
     const bool real = key < a.S;
     const E* k = static_cast<const E*>(a.k) + h * a.k_head + (real ? key : 0) * a.k_token + 8 * kg;
-    const E* v = static_cast<const E*>(a.v) + h * a.v_head + (real ? key : 0) * a.v_token + 8 * kg;
-    const u32x4 none{0, 0, 0, 0};
 #pragma unroll
-    for (int i = 0; i < KQ; ++i) {
-      kf[n][i] = __builtin_bit_cast(x8, real ? *reinterpret_cast<const u32x4*>(k + 16 * i) : none);
-      vf[n][i] = __builtin_bit_cast(x8, real ? *reinterpret_cast<const u32x4*>(v + 16 * i) : none);
-    }
+    for (int i = 0; i < KQ; ++i)
+      kf[i] = __builtin_bit_cast(x8, real ? *reinterpret_cast<const u32x4*>(k + 16 * i) : u32x4{0, 0, 0, 0});
   }
-  f32x16 dk[NK][MT], dv[NK][MT];
+  // the values of all of the workgroup's keys, 32 keys a wave; behind the last key: that key once more
 #pragma unroll
-  for (int n = 0; n < NK; ++n)
+  for (int i = 0; i < 2; ++i) {
+    const int block = 2 * wave + i, first = min(k0 + 16 * block, a.S - 1);
+    const uint32_t row = min(lane / 4, a.S - 1 - first);
+    load_rows16<E, D>(static_cast<const E*>(a.v) + h * a.v_head + first * a.v_token, row * (uint32_t)a.v_token, vt[block / 4], block % 4, lane);
+  }
+  const E* const vp = vt[wave >> 1];
+  f32x16 dk[MT], dv[MT];
 #pragma unroll
-    for (int i = 0; i < MT; ++i) dk[n][i] = dv[n][i] = f32x16{};
-  Range<E> range[NK];
+  for (int i = 0; i < MT; ++i) dk[i] = dv[i] = f32x16{};
+  Range<E> range;
 
   // The blocks of rows, 64 ranges at a time, a lane each: `left` are those of the present 64 that see any of the keys.
   const RowRange* const ranges = static_cast<const RowRange*>(a.ranges);
@@ -84,109 +84,123 @@ __global__ __launch_bounds__(256, 1) void dkv_kernel(CoreGradArgs a, int blocks,
     }
   };
   const auto stage = [&](int block, int buffer) {
-    // offsets from the wave's first token; rows behind the last: that once more
-    const int r0 = min(block * kTile + 16 * wave, rows - 1), t0 = a.group.of(r0);
+    // the first four waves load Q's rows, the others dY's: offsets from the wave's first token; rows behind the last: that
+    // once more
+    const bool first = wave < 4;
+    const int r0 = min(block * kTile + 16 * (wave & 3), rows - 1), t0 = a.group.of(r0);
     const int rho = min(r0 + lane / 4, rows - 1), t = a.group.of(rho), g = rho - t * group;
-    load_rows16<E, D>(static_cast<const E*>(a.q) + t0 * a.q_token + h * group * a.q_head,
-                      (t - t0) * (uint32_t)a.q_token + g * (uint32_t)a.q_head, qt[buffer], wave, lane);
-    load_rows16<E, D>(static_cast<const E*>(a.dy) + t0 * a.dy_token + h * group * a.dy_head,
-                      (t - t0) * (uint32_t)a.dy_token + g * (uint32_t)a.dy_head, yt[buffer], wave, lane);
-    // a quarter of the block's values, so that every wave has asked for as many instructions
-    constexpr int part = (BENT ? sizeof(RowBlock) : offsetof(RowBlock, stands)) / 4;
+    const int64_t token = first ? a.q_token : a.dy_token, head = first ? a.q_head : a.dy_head;
+    load_rows16<E, D>(static_cast<const E*>(first ? a.q : a.dy) + t0 * token + h * group * head,
+                      (t - t0) * (uint32_t)token + g * (uint32_t)head, first ? qt[buffer] : yt[buffer], wave & 3, lane);
+    constexpr int size = (BIAS ? sizeof(RowBlock) : offsetof(RowBlock, stands)) / 8;
     const RowBlock* const from = static_cast<const RowBlock*>(a.blocks) + ((int64_t)h * blocks + block);
-    if (lane < part / 16)
-      load_blocks<1>(reinterpret_cast<const char*>(from) + wave * part, 16 * lane, reinterpret_cast<char*>(&info[buffer]) + wave * part);
+    if (lane < size / 16)
+      load_blocks<1>(reinterpret_cast<const char*>(from) + wave * size, 16 * lane, reinterpret_cast<char*>(&info[buffer]) + wave * size);
   };
   // A step of 64 rows.  WHOLE: all of them see all of the wave's keys; ODD: some value of the tiles is not finite.
   const auto step = [&](const E* qp, const E* yp, const RowBlock& x, auto whole, auto odd) {
     constexpr bool WHOLE = decltype(whole)::value, ODD = decltype(odd)::value;
-    const auto part = [&](int u) {
-      f32x16 sc[NK], dp[NK];
-      x8 q[KQ], y[KQ];
+    // operands read from LDS ahead of their use, of one and of two an MFMA: as many as leave nothing spilled
+    constexpr int kEarly = !WHOLE ? 1 : CAP ? 2 : 3, kEarlyPair = WHOLE && !CAP ? 2 : 1;
+    const auto half = [&](int u) {
+      f32x16 sc, dp;
+      x8 q[KQ], y[KQ], v[KQ];
       const auto query = [&](int i) { q[i] = at_tile.rows(qp, u, i); };
-      const auto dy = [&](int i) { y[i] = at_tile.rows(yp, u, i); };
+      const auto dy = [&](int i) {
+        y[i] = at_tile.rows(yp, u, i);
+        v[i] = at_tile.rows(vp, part, i);
+      };
       const auto column = [&](const E* p, int i) {
         const x8 c = at_tile.columns(p, u, i / MT, i % MT);
         return ODD ? finite_values<E>(c) : c;
       };
-      f32x4 lse[4], delta[4];
+      f32x4 lse[4];
       const auto values = [&](const float* p, int i) { return *reinterpret_cast<const f32x4*>(p + c_row(u, 4 * i) + 16 * kg); };
 #pragma unroll
       for (int i = 0; i < kEarly; ++i) query(i);
       __builtin_amdgcn_sched_barrier(0);
+      sc = f32x16{};
 #pragma unroll
       for (int i = 0; i < KQ; ++i) {
         if (i + kEarly < KQ)
           query(i + kEarly);
-        else
+        else if (i + kEarly - KQ < kEarlyPair)
           dy(i + kEarly - KQ);
-        if (i >= KQ - 4) delta[i - KQ + 4] = values(x.delta, i - KQ + 4);
-        if (i == KQ - 1) lse[0] = values(x.lse, 0);
+        if (i >= KQ - 4) {
+          const f32x4 d = values(x.delta, i - KQ + 4);
 #pragma unroll
-        for (int n = 0; n < NK; ++n) sc[n] = mfma32(q[i], kf[n][i], i == 0 ? f32x16{} : sc[n]);
+          for (int e = 0; e < 4; ++e) dp[4 * (i - KQ + 4) + e] = d[e];
+        }
+        if (i == KQ - 1) lse[0] = values(x.lse, 0);
+        sc = mfma32(q[i], kf[i], sc);
         __builtin_amdgcn_sched_barrier(0);
       }
-      // weights: element e of group n
-      float rate[BENT ? NK : 1][16];
-      const auto weight = [&](int n, int e) {
-        const float from = lse[e >> 2][e & 3];
-        float p;
-        if constexpr (BENT) {
-          const int row = c_row(u, e) + 16 * kg;
-          rate[n][e] = 1.f;
-          p = a.cap > 0.f ? bend.capped(sc[n][e], rate[n][e]) : sc[n][e] * bend.c;
-          p = __builtin_fmaf(-x.slope[row], fabsf(x.stands[row] - (float)(mine + 32 * n + n32)), p);
-          p = __builtin_amdgcn_exp2f(p + from);
-        } else {
-          p = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[n][e], bend.c, from));
+      // weights of elements 4 j .. 4 j + 3, from where they are read; with a cap, packed at once, and left times its derivative
+      uint32_t pw[8], hidden = 0;
+      const auto weights = [&](int j) {
+        f32x4 stands, slope;
+        u32x4 lo, hi;
+        const int row4 = c_row(u, 4 * j) + 16 * kg;
+        if constexpr (BIAS) {
+          stands = *reinterpret_cast<const f32x4*>(x.stands + row4);
+          slope = *reinterpret_cast<const f32x4*>(x.slope + row4);
         }
-        sc[n][e] = p;
+        if constexpr (!WHOLE) {
+          lo = *reinterpret_cast<const u32x4*>(x.lo + row4);
+          hi = *reinterpret_cast<const u32x4*>(x.hi + row4);
+        }
+        f32x4 p, rate;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const int e = 4 * j + i;
+          if constexpr (!CAP && !BIAS) {
+            p[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[e], bend.c, lse[j][i]));
+          } else {
+            float r = 1.f, y = lse[j][i];
+            if constexpr (CAP)
+              y += bend.capped(sc[e], r);
+            else
+              y = __builtin_fmaf(sc[e], bend.c, y);
+            if constexpr (BIAS) y = __builtin_fmaf(-slope[i], fabsf(stands[i] - (float)key), y);
+            rate[i] = r;
+            p[i] = __builtin_amdgcn_exp2f(y);
+          }
+          if constexpr (!WHOLE) {
+            if ((int)(key < (int)lo[i]) | (int)(key >= (int)hi[i])) {
+              p[i] = 0.f;
+              hidden |= 1u << e;
+            }
+          }
+        }
+        if constexpr (CAP) {
+          pw[2 * j] = pack2<E>(p[0], p[1]);
+          pw[2 * j + 1] = pack2<E>(p[2], p[3]);
+        }
+#pragma unroll
+        for (int i = 0; i < 4; ++i) sc[4 * j + i] = CAP ? p[i] * rate[i] : p[i];
       };
       x8 yc[2 * MT], qc[2 * MT];
 #pragma unroll
       for (int i = 0; i < KQ; ++i) {
-        if (i + kEarly < KQ)
-          dy(i + kEarly);
-        else
+        if (i + kEarlyPair < KQ)
+          dy(i + kEarlyPair);
+        if (i + kEarly >= KQ)
           yc[i + kEarly - KQ] = column(yp, i + kEarly - KQ);
         if (i * 4 % KQ == 0 && i * 4 / KQ < 3) lse[i * 4 / KQ + 1] = values(x.lse, i * 4 / KQ + 1);
+        dp = mfma32(y[i], v[i], dp);
 #pragma unroll
-        for (int n = 0; n < NK; ++n) {
-          f32x16 none;
-          if (i == 0) {
-#pragma unroll
-            for (int e = 0; e < 16; ++e) none[e] = delta[e >> 2][e & 3];
-          }
-          dp[n] = mfma32(y[i], vf[n][i], i == 0 ? none : dp[n]);
-#pragma unroll
-          for (int e = i * 16 / KQ; e < (i + 1) * 16 / KQ; ++e) weight(n, e);
-        }
+        for (int j = (i * 4 + KQ - 1) / KQ; j < ((i + 1) * 4 + KQ - 1) / KQ; ++j) weights(j);
         __builtin_amdgcn_sched_barrier(0);
       }
-      if constexpr (!WHOLE) {
-#pragma unroll
-        for (int n = 0; n < NK; ++n)
-#pragma unroll
-          for (int e = 0; e < 16; ++e) {
-            const int row = c_row(u, e) + 16 * kg, key = mine + 32 * n + n32;
-            if ((int)(key < x.lo[row]) | (int)(key >= x.hi[row])) sc[n][e] = dp[n][e] = 0.f;
-          }
-      }
-      const auto weight8 = [&](int n, int b) {
-        u32x4 w;
-#pragma unroll
-        for (int e = 0; e < 4; ++e) w[e] = pack2<E>(sc[n][8 * b + 2 * e], sc[n][8 * b + 2 * e + 1]);
-        return __builtin_bit_cast(x8, w);
-      };
-      const auto change = [&](int n, int e) {
-        dp[n][e] *= sc[n][e];
-        if constexpr (BENT) dp[n][e] *= rate[n][e];
+      const auto change = [&](int e) {
+        dp[e] *= sc[e];
+        if (!WHOLE && (hidden >> e & 1)) dp[e] = 0.f;  // dy may be no finite number there
       };
 #pragma unroll
       for (int b = 0; b < 2; ++b) {
-        x8 w[NK];
+        u32x4 w;
 #pragma unroll
-        for (int n = 0; n < NK; ++n) w[n] = weight8(n, b);
+        for (int e = 0; e < 4; ++e) w[e] = CAP ? pw[4 * b + e] : pack2<E>(sc[8 * b + 2 * e], sc[8 * b + 2 * e + 1]);
 #pragma unroll
         for (int m = 0; m < MT; ++m) {
           const int i = b * MT + m;
@@ -194,93 +208,65 @@ __global__ __launch_bounds__(256, 1) void dkv_kernel(CoreGradArgs a, int blocks,
             yc[i + kEarly] = column(yp, i + kEarly);
           else
             qc[i + kEarly - 2 * MT] = column(qp, i + kEarly - 2 * MT);
+          dv[m] = mfma32(yc[i], __builtin_bit_cast(x8, w), dv[m]);
 #pragma unroll
-          for (int n = 0; n < NK; ++n) {
-            dv[n][m] = mfma32(yc[i], w[n], dv[n][m]);
-#pragma unroll
-            for (int e = m * 8 / MT; e < (m + 1) * 8 / MT; ++e) change(n, 8 * b + e);
-          }
+          for (int e = m * 8 / MT; e < (m + 1) * 8 / MT; ++e) change(8 * b + e);
           __builtin_amdgcn_sched_barrier(0);
         }
       }
-#pragma unroll
-      for (int n = 0; n < NK; ++n) range[n].fit(dp[n], dk[n]);
+      range.fit(dp, dk);
 #pragma unroll
       for (int b = 0; b < 2; ++b) {
-        x8 z[NK];
+        u32x4 w;
 #pragma unroll
-        for (int n = 0; n < NK; ++n) {
-          u32x4 w;
-#pragma unroll
-          for (int e = 0; e < 4; ++e) w[e] = pack2<E>(dp[n][8 * b + 2 * e] * range[n].f, dp[n][8 * b + 2 * e + 1] * range[n].f);
-          z[n] = __builtin_bit_cast(x8, w);
-        }
+        for (int e = 0; e < 4; ++e) w[e] = pack2<E>(dp[8 * b + 2 * e] * range.f, dp[8 * b + 2 * e + 1] * range.f);
 #pragma unroll
         for (int m = 0; m < MT; ++m) {
           const int i = b * MT + m;
           if (i + kEarly < 2 * MT) qc[i + kEarly] = column(qp, i + kEarly);
-#pragma unroll
-          for (int n = 0; n < NK; ++n) dk[n][m] = mfma32(qc[i], z[n], dk[n][m]);
+          dk[m] = mfma32(qc[i], __builtin_bit_cast(x8, w), dk[m]);
           __builtin_amdgcn_sched_barrier(0);
         }
       }
     };
-    part(0);
-    part(1);
+    half(0);
+    half(1);
     if constexpr (ODD) {
-#pragma unroll
-      for (int n = 0; n < NK; ++n) {
-        const int key = mine + 32 * n + n32;
-        const auto sees = [&](int i) { return key >= x.lo[i] && key < x.hi[i]; };
-        add_odd<E, D>(qp, dk[n], lane, sees);
-        add_odd<E, D>(yp, dv[n], lane, sees);
-      }
+      const auto sees = [&](int i) { return key >= x.lo[i] && key < x.hi[i]; };
+      add_odd<E, D>(qp, dk, lane, sees);
+      add_odd<E, D>(yp, dv, lane, sees);
     }
   };
 
-  // blocks and ranges of the present step and of those whose tiles are on their way
-  RowRange ranged[DEPTH];
-  int block[DEPTH], buffer = 0;
-  bool all = true;  // nothing has been left out behind the last step
-#pragma unroll
-  for (int i = 0; i < DEPTH - 1; ++i) {
-    block[i] = next(ranged[i]);
-    if (block[i] >= 0) stage(block[i], i);
-  }
+  // the present step's block and range, and the next's, whose tiles are on their way
+  RowRange now, later;
+  int block = next(now), following = -1, buffer = 0;
+  if (block >= 0) stage(block, 0);
   tiles_ready();
   const auto ask = [&] {
-    block[DEPTH - 1] = next(ranged[DEPTH - 1]);
-    all = block[DEPTH - 1] >= 0;
-    if (all) stage(block[DEPTH - 1], buffer == 0 ? DEPTH - 1 : buffer - 1);
+    following = next(later);
+    if (following >= 0) stage(following, buffer ^ 1);
   };
   const auto advance = [&] {
-    // the next step's tiles; those behind it, if all of them were asked for, may still be on their way
-    if (all)
-      tiles_ready<(DEPTH - 2) * LOADS>();
-    else
-      tiles_ready();
-#pragma unroll
-    for (int i = 0; i + 1 < DEPTH; ++i) {
-      block[i] = block[i + 1];
-      ranged[i] = ranged[i + 1];
-    }
-    buffer = buffer == DEPTH - 1 ? 0 : buffer + 1;
+    tiles_ready();
+    block = following;
+    now = later;
+    buffer ^= 1;
   };
-  const auto whole = [&] { return ranged[0].low <= mine && mine + 32 * NK <= ranged[0].high; };
   // A loop for the whole steps by itself: in one for both kinds, the sums would be moved from the registers that one leaves
   // them in to the other's, in every step.
-  while (block[0] >= 0) {
+  while (block >= 0) {
 #pragma unroll 1
-    while (block[0] >= 0 && whole()) {
+    while (block >= 0 && now.low <= mine && mine + 64 <= now.high) {
       ask();
       step(qt[buffer], yt[buffer], info[buffer], std::true_type{}, std::false_type{});
       advance();
     }
-    if (block[0] < 0) break;
+    if (block < 0) break;
     ask();
     const E* const qp = qt[buffer];
     const E* const yp = yt[buffer];
-    if (ranged[0].last > mine && ranged[0].first < mine + 32 * NK) {
+    if (now.last > mine && now.first < mine + 64) {
       if (!(tile_is_odd<E, D>(qp, lane) || tile_is_odd<E, D>(yp, lane)))
         step(qp, yp, info[buffer], std::false_type{}, std::false_type{});
       else
@@ -288,19 +274,16 @@ __global__ __launch_bounds__(256, 1) void dkv_kernel(CoreGradArgs a, int blocks,
     }
     advance();
   }
-#pragma unroll
-  for (int n = 0; n < NK; ++n) {
-    const int key = mine + 32 * n + n32;
-    if (key >= a.S) continue;
-    const float f = a.scale * range[n].back() * (Range<E>::on ? 0x1p-15f : 1.f), g = Range<E>::on ? 0x1p-15f : 1.f;
+  if (key < a.S) {
+    const float f = a.scale * range.back() * (Range<E>::on ? 0x1p-15f : 1.f), g = Range<E>::on ? 0x1p-15f : 1.f;
     const int64_t at = ((int64_t)key * a.kv_heads + h) * D, size = (int64_t)a.S * a.kv_heads * D;
     float* const part = a.ws + s * 2 * size;
 #pragma unroll
     for (int k = 0; k < MT; ++k)
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
-        const f32x4 u = f32x4{dk[n][k][4 * e], dk[n][k][4 * e + 1], dk[n][k][4 * e + 2], dk[n][k][4 * e + 3]} * f;
-        const f32x4 w = f32x4{dv[n][k][4 * e], dv[n][k][4 * e + 1], dv[n][k][4 * e + 2], dv[n][k][4 * e + 3]} * g;
+        const f32x4 u = f32x4{dk[k][4 * e], dk[k][4 * e + 1], dk[k][4 * e + 2], dk[k][4 * e + 3]} * f;
+        const f32x4 w = f32x4{dv[k][4 * e], dv[k][4 * e + 1], dv[k][4 * e + 2], dv[k][4 * e + 3]} * g;
         const int d = 32 * k + 8 * e + 4 * kg;
         if (splits == 1) {
           st4(static_cast<E*>(a.dk) + at + d, u);
@@ -314,7 +297,7 @@ __global__ __launch_bounds__(256, 1) void dkv_kernel(CoreGradArgs a, int blocks,
 }
 
 // dk and dv of kKeys keys of a key head; part s of `splits` takes every splits-th block of 64 rows that sees any of them
-template <class E, int D, bool BENT>
+template <class E, int D, bool CAP, bool BIAS>
 __global__ __launch_bounds__(256, 1) void pair_kernel(CoreGradArgs a, int blocks, int splits) {
   typedef typename Vec<E>::x8 x8;
   constexpr bool PAIR = true;
@@ -334,7 +317,7 @@ __global__ __launch_bounds__(256, 1) void pair_kernel(CoreGradArgs a, int blocks
   const int key = mine + n32;
   const bool real = key < a.S;
   const TileOperands<E, D> at_tile(lane);
-  const Bend bend(a.scale, BENT ? a.cap : 0.f, nullptr, 0);
+  const Bend bend(a.scale, CAP ? a.cap : 0.f, nullptr, 0);
 
   x8 kf[KQ], vf[PAIR ? 1 : KQ];  // lane (n32, kg): key n32, dimensions 16 i + 8 kg ..; of a pair, kf is V in the second
   {
@@ -388,7 +371,7 @@ __global__ __launch_bounds__(256, 1) void pair_kernel(CoreGradArgs a, int blocks
                       (t - t0) * (uint32_t)a.dy_token + g * (uint32_t)a.dy_head, yt[buffer], wave, lane);
     const RowBlock* const from = static_cast<const RowBlock*>(a.blocks) + ((int64_t)h * blocks + block);
     if (wave == 0) load_blocks<1>(from, 16 * lane, &info[buffer]);
-    if (BENT && wave == 1 && lane < 32) load_blocks<1>(from->stands, 16 * lane, info[buffer].stands);
+    if (BIAS && wave == 1 && lane < 32) load_blocks<1>(from->stands, 16 * lane, info[buffer].stands);
   };
   // of the u-th 32 rows: S and dP - delta, with a pair's one of them
   const auto products = [&](const E* qp, const E* yp, const RowBlock& x, int u, f32x16& sc, f32x16& dp) {
@@ -439,15 +422,11 @@ __global__ __launch_bounds__(256, 1) void pair_kernel(CoreGradArgs a, int blocks
         const int e = 4 * i + j, row = row4 + j;
         float p, rate = 1.f;
         const float from = lse[j];
-        if constexpr (BENT) {
-          p = a.cap > 0.f ? bend.capped(sc[e], rate) : sc[e] * bend.c;
-          p = __builtin_fmaf(-x.slope[row], fabsf(x.stands[row] - (float)key), p);
-          p = __builtin_amdgcn_exp2f(p + from);
-        } else {
-          p = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[e], bend.c, from));
-        }
+        p = CAP ? bend.capped(sc[e], rate) + from : __builtin_fmaf(sc[e], bend.c, from);
+        if constexpr (BIAS) p = __builtin_fmaf(-x.slope[row], fabsf(x.stands[row] - (float)key), p);
+        p = __builtin_amdgcn_exp2f(p);
         float dx = p * dp[e];
-        if constexpr (BENT) dx *= rate;
+        if constexpr (CAP) dx *= rate;
         if constexpr (!WHOLE) {
           const bool hidden = (int)(key < x.lo[row]) | (int)(key >= x.hi[row]);
           if (hidden) p = dx = 0.f;
@@ -559,13 +538,13 @@ __global__ __launch_bounds__(256, 1) void pair_kernel(CoreGradArgs a, int blocks
 template <class E, int D>
 void launch_dkv(const CoreGradArgs& a, int blocks, int splits, hipStream_t st) {
   const unsigned grid = (unsigned)((a.S + kKeys<D> - 1) / kKeys<D> * a.kv_heads * splits);
-  const bool bent = a.cap > 0.f || a.slopes;
-  if constexpr (D == 256)
-    bent ? pair_kernel<E, D, true><<<grid, 256, 0, st>>>(a, blocks, splits)
-         : pair_kernel<E, D, false><<<grid, 256, 0, st>>>(a, blocks, splits);
-  else
-    bent ? dkv_kernel<E, D, true><<<grid, 256, 0, st>>>(a, blocks, splits)
-         : dkv_kernel<E, D, false><<<grid, 256, 0, st>>>(a, blocks, splits);
+  by_scores(a, [&](auto cap, auto bias) {
+    constexpr bool CAP = decltype(cap)::value, BIAS = decltype(bias)::value;
+    if constexpr (D == 256)
+      pair_kernel<E, D, CAP, BIAS><<<grid, 256, 0, st>>>(a, blocks, splits);
+    else
+      dkv_kernel<E, D, CAP, BIAS><<<grid, 512, 0, st>>>(a, blocks, splits);
+  });
 }
 template void launch_dkv<bf16, 64>(const CoreGradArgs&, int, int, hipStream_t);
 template void launch_dkv<bf16, 128>(const CoreGradArgs&, int, int, hipStream_t);

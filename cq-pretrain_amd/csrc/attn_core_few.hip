@@ -46,9 +46,10 @@ struct Rows {
   int shown;  // a bit for each 16 positions: a page holds them
 };
 
-template <class E, int D, bool BENT>
+template <class E, int D, bool CAP, bool BIAS>
 __global__ __launch_bounds__(64 * kWaves, D == 256 ? 1 : 2) void few_kernel(CoreArgs a, int tiles, int least) {
   typedef typename Vec<E>::x8 x8;
+  constexpr bool BENT = CAP || BIAS;
   constexpr int KQ = D / 32, MT = D / 16, LR = 512 / D;  // LR rows of values a load
   constexpr int LD = D + 16;  // 8 banks further each row: the transposed reads of 8 rows meet no bank twice
   __shared__ __align__(16) E vt[kWaves][kHalf * LD];
@@ -89,7 +90,7 @@ __global__ __launch_bounds__(64 * kWaves, D == 256 ? 1 : 2) void few_kernel(Core
         qf[k] = __builtin_bit_cast(x8, w);
       }
     }
-    const Bend bend(a.scale, BENT ? a.cap : 0.f, BENT ? a.slopes : nullptr, head);
+    const Bend bend(a.scale, CAP ? a.cap : 0.f, BIAS ? a.slopes : nullptr, head);
     // the block table's next 64 entries, an entry a lane, from position `at` on
     const auto entries = [&](int at) {
       const int column = (at >> a.page_shift) + lane;
@@ -99,7 +100,7 @@ __global__ __launch_bounds__(64 * kWaves, D == 256 ? 1 : 2) void few_kernel(Core
     const int early = a.window <= 0 && r < a.N ? entries((s * least + wave) * kStep) : -1;
     int lo, hi;
     attend_limits(real && r < a.N ? a.visible[t] : 0, a.window, room, lo, hi);
-    const int stands = BENT ? (real && r < a.N ? (a.positions ? a.positions[t] : a.visible[t] - 1) : 0) : 0;
+    const int stands = BIAS ? (real && r < a.N ? (a.positions ? a.positions[t] : a.visible[t] - 1) : 0) : 0;
     // over the rows that see anything: from the first position any of them sees to the last, and the
     // range that all of them see, where nothing is masked
     const int first = min16(hi > 0 ? lo : INT32_MAX), last = max16(hi);
@@ -178,8 +179,9 @@ __global__ __launch_bounds__(64 * kWaves, D == 256 ? 1 : 2) void few_kernel(Core
             for (int g = 0; g < 2; ++g)
 #pragma unroll
               for (int e = 0; e < 4; ++e) {
-                const float y = a.cap > 0.f ? bend.capped(sc[g][e]) : sc[g][e] * bend.c;
-                sc[g][e] = __builtin_fmaf(-bend.slope, fabsf((float)(stands - at - 16 * g - 4 * q4 - e)), y);
+                sc[g][e] = CAP ? bend.capped(sc[g][e]) : sc[g][e] * bend.c;
+                if constexpr (BIAS)
+                  sc[g][e] = __builtin_fmaf(-bend.slope, fabsf((float)(stands - at - 16 * g - 4 * q4 - e)), sc[g][e]);
               }
           }
           // where not every row sees every position, hidden ones leave the scores, and values that are not finite reach
@@ -321,10 +323,9 @@ void launch_dim(const CoreArgs& a, int splits, int per, hipStream_t st) {
   const int tiles = (int)std::max<int64_t>(1, std::min<int64_t>(((int64_t)a.max_queries * group + 15) / 16, (1 << 23) / each));
   // a workgroup takes every tiles-th tile: none is left out whatever the bound
   const dim3 grid((unsigned)std::max<int64_t>(1, (int64_t)a.N * tiles), a.kv_heads, splits + 1);
-  if (a.cap > 0.f || a.slopes)
-    few_kernel<E, D, true><<<grid, 64 * kWaves, 0, st>>>(a, tiles, per);
-  else
-    few_kernel<E, D, false><<<grid, 64 * kWaves, 0, st>>>(a, tiles, per);
+  by_scores(a, [&](auto cap, auto bias) {
+    few_kernel<E, D, decltype(cap)::value, decltype(bias)::value><<<grid, 64 * kWaves, 0, st>>>(a, tiles, per);
+  });
 }
 
 template <class E>

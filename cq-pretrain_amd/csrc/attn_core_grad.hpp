@@ -5,11 +5,9 @@
 namespace cqgdn {
 
 constexpr int kGradRows = 128;  // of a workgroup for dq, 32 a wave
-// keys of a wave for dk and dv, in groups of 32, and of a workgroup
+// keys of a workgroup for dk and dv
 template <int D>
-constexpr int kKeyGroups = D == 64 ? 2 : 1;
-template <int D>
-constexpr int kKeys = D == 256 ? 64 : 128 * kKeyGroups<D>;
+constexpr int kKeys = D == 256 ? 64 : 256;
 
 template <class E>
 constexpr float kWeightBias = std::is_same<E, f16>::value ? 15.f : 0.f;
