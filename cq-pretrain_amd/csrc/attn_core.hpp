@@ -62,13 +62,17 @@ struct TileOperands {
   }
 };
 
-// N blocks of a tile on their way: lane l's 16 bytes of `base` + `off` + 64 i (bytes) land at `lds` + 1024 i + 16 l.  In
+// N blocks of a tile on their way: lane l's 16 bytes of `from` + `off` + 64 i (bytes) land at `lds` + 1024 i + 16 l.  In
 // assembly because the compiler, which does not tell the tiles of a pair from each other, puts a wait for all that is on
 // its way before every read of the other one (train_9216's forward pass spent 61% of its time in that wait); tiles_ready()
 // is the wait that is needed.  Nothing is returned in registers.  An instruction's offset moves both addresses.
 template <int N>
-__device__ __forceinline__ void load_blocks(const void* base, uint32_t off, void* lds) {
-  const uint32_t at = (uint32_t)(uintptr_t)(lds_void_ptr)lds;
+__device__ __forceinline__ void load_blocks(const void* from, uint32_t off, void* lds) {
+  // the same for all lanes, in scalar registers
+  const uint32_t at = __builtin_amdgcn_readfirstlane((uint32_t)(uintptr_t)(lds_void_ptr)lds);
+  const uintptr_t x = reinterpret_cast<uintptr_t>(from);
+  const uintptr_t base = (uintptr_t)(uint32_t)__builtin_amdgcn_readfirstlane((uint32_t)(x >> 32)) << 32 |
+                         (uint32_t)__builtin_amdgcn_readfirstlane((uint32_t)x);
 #define CQGDN_LOAD(m0, more) "s_mov_b32 m0, " m0 "\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, %1" more "\n\t"
   static_assert(N == 1 || N == 2 || N == 4 || N == 8, "blocks a wave");
   if constexpr (N == 1) {
@@ -80,7 +84,7 @@ __device__ __forceinline__ void load_blocks(const void* base, uint32_t off, void
                      CQGDN_LOAD("%5", " offset:192") ::"v"(off),
                  "s"(base), "s"(at), "s"(at + 960), "s"(at + 1920), "s"(at + 2880)
                  : "memory");
-    if constexpr (N == 8) load_blocks<4>(static_cast<const char*>(base) + 256, off, static_cast<char*>(lds) + 4096);
+    if constexpr (N == 8) load_blocks<4>(static_cast<const char*>(from) + 256, off, static_cast<char*>(lds) + 4096);
   }
 #undef CQGDN_LOAD
 }
@@ -98,9 +102,19 @@ __device__ __forceinline__ void tiles_ready() {
 }
 
 // ---- values that are not finite -----------------------------------------------------------------------
-// 0 x infinity and 0 x NaN are NaN, so a value that a row does not see must not meet its weight 0 in an MFMA.  Where a
-// step's rows do not all see all of it, its operands are looked through; if one holds such a value, it goes in as 0
-// and is added afterwards, lane by lane, to those that see it.
+// 0 x infinity and 0 x NaN are NaN, so a value that a row does not see must not meet its weight 0 in an MFMA.  Looking
+// for such values in every step whose rows do not all see all of it would cost as much as the step.  Instead a workgroup
+// looks at its sums when it is done: if one is not finite it goes through its steps once more, carefully: there, values
+// that are not finite go in as 0 and are added afterwards, lane by lane, to those that see them.
+template <int N>
+__device__ __forceinline__ bool any_not_finite(const f32x16 (&x)[N]) {
+  float zero[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+  for (int i = 0; i < N; ++i)
+#pragma unroll
+    for (int e = 0; e < 16; ++e) zero[e & 3] = __builtin_fmaf(x[i][e], 0.f, zero[e & 3]);
+  return !((zero[0] + zero[1]) + (zero[2] + zero[3]) == 0.f);
+}
 template <class E>
 __device__ __forceinline__ uint32_t odd_values(u32x4 w) {
   constexpr uint32_t exponent = std::is_same<E, f16>::value ? 0x7C007C00u : 0x7F807F80u;

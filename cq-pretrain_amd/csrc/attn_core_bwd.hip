@@ -24,12 +24,17 @@
 namespace cqgdn {
 namespace {
 
-template <class E, int D, bool CAP, bool BIAS>
-__global__ __launch_bounds__(256, D == 256 ? 1 : 2) void dq_kernel(CoreGradArgs a, int tiles) {
+template <class E, int D>
+struct DqTiles {
+  E kt[2][kTileSize<D>], vt[2][kTileSize<D>];
+};
+// the workgroup's part of the work, in its shared memory; returns whether it has to be done once more, carefully
+template <class E, int D, bool CAP, bool BIAS, bool CAREFUL>
+__device__ __forceinline__ bool dq_rows(const CoreGradArgs& a, int tiles, DqTiles<E, D>& lds) {
   typedef typename Vec<E>::x8 x8;
   constexpr int TOK = kTile, KQ = D / 16, MT = D / 32;
-  __shared__ __align__(16) E kt[2][kTileSize<D>];
-  __shared__ __align__(16) E vt[2][kTileSize<D>];
+  auto& kt = lds.kt;
+  auto& vt = lds.vt;
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int n32 = lane & 31, kg = lane >> 5;
   // launch order: as the forward pass's
@@ -132,8 +137,6 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void dq_kernel(CoreGradArgs 
   }
 
   f32x16 acc[MT];
-#pragma unroll
-  for (int i = 0; i < MT; ++i) acc[i] = f32x16{};
   Range<E> range;
 
   const auto stage = [&](int j) {
@@ -144,11 +147,12 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void dq_kernel(CoreGradArgs 
     load_rows16<E, D>(static_cast<const E*>(a.v) + h * a.v_head + pos * a.v_token, row * (uint32_t)a.v_token, vt[j & 1], wave, lane);
   };
   const auto step = [&](const E* kp, const E* vp, int pos, auto whole) {
-    constexpr bool WHOLE = decltype(whole)::value;
-    const bool odd = !WHOLE && tile_is_odd<E, D>(kp, lane);
+    constexpr bool WHOLE = decltype(whole)::value, APART = CAREFUL && !WHOLE;
+    const bool odd = APART && tile_is_odd<E, D>(kp, lane);
     const int lo0 = lo - pos - 16 * kg, hi0 = hi - pos - 16 * kg;
     const float far = (float)(stands - pos - 16 * kg);
-#pragma unroll
+    // cut steps one half after the other: a short call's time is that of fetching this code once
+#pragma unroll(WHOLE ? 2 : 1)
     for (int u = 0; u < 2; ++u) {
       f32x16 sc = f32x16{}, dp = f32x16{} - delta;
 #pragma unroll
@@ -176,7 +180,7 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void dq_kernel(CoreGradArgs 
 #pragma unroll
         for (int m = 0; m < MT; ++m) {
           x8 k = at_tile.columns(kp, u, b, m);
-          if (odd) k = finite_values<E>(k);
+          if (APART) k = finite_values<E>(k);
           acc[m] = mfma32(k, __builtin_bit_cast(x8, w), acc[m]);
         }
       }
@@ -185,29 +189,34 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void dq_kernel(CoreGradArgs 
   };
 
   const int n = last > 0 ? (last - first + TOK - 1) / TOK : 0;
+#pragma unroll
+  for (int i = 0; i < MT; ++i) acc[i] = f32x16{};
   if (n > 0) {
     stage(0);
     tiles_ready();
-    int j = 0, pos = first;
-    const auto advance = [&] {
-      tiles_ready();
-      ++j;
-      pos += TOK;
-    };
-    // A loop for the whole steps by itself: in one for both kinds, the sums would be moved from the registers that one
-    // leaves them in to the other's, in every step.
-    while (j < n) {
+  }
+  int j = 0, pos = first;
+  const auto advance = [&] {
+    tiles_ready();
+    ++j;
+    pos += TOK;
+  };
+  // A loop for the whole steps by itself: in one for both kinds, the sums would be moved from the registers that one
+  // leaves them in to the other's, in every step.
+  while (j < n) {
 #pragma unroll 1
-      while (j < n && pos >= low && pos + TOK <= high) {
-        if (j + 1 < n) stage(j + 1);
-        step(kt[j & 1], vt[j & 1], pos, std::true_type{});
-        advance();
-      }
-      if (j == n) break;
+    while (j < n && pos >= low && pos + TOK <= high) {
       if (j + 1 < n) stage(j + 1);
-      if (pos < most && pos + TOK > some) step(kt[j & 1], vt[j & 1], pos, std::false_type{});
+      step(kt[j & 1], vt[j & 1], pos, std::true_type{});
       advance();
     }
+    if (j == n) break;
+    if (j + 1 < n) stage(j + 1);
+    if (pos < most && pos + TOK > some) step(kt[j & 1], vt[j & 1], pos, std::false_type{});
+    advance();
+  }
+  if constexpr (!CAREFUL) {
+    if (__builtin_amdgcn_readfirstlane(__syncthreads_or(any_not_finite(acc)))) return true;
   }
   if (real) {
     const float f = a.scale * range.back() * (Range<E>::on ? 0x1p-15f : 1.f);
@@ -218,6 +227,21 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void dq_kernel(CoreGradArgs 
         st4(static_cast<E*>(a.dq) + at * D + 32 * k + 8 * e + 4 * kg,
             f32x4{acc[k][4 * e], acc[k][4 * e + 1], acc[k][4 * e + 2], acc[k][4 * e + 3]} * f);
   }
+  return false;
+}
+
+// apart from the kernel, whose registers it would cost
+template <class E, int D, bool CAP, bool BIAS>
+__device__ __noinline__ void dq_again(CoreGradArgs a, int tiles, uint32_t lds) {
+  typedef __attribute__((address_space(3))) DqTiles<E, D>* Tiles;
+  dq_rows<E, D, CAP, BIAS, true>(a, tiles, *(DqTiles<E, D>*)(Tiles)lds);
+}
+
+template <class E, int D, bool CAP, bool BIAS>
+__global__ __launch_bounds__(256, D == 256 ? 1 : 2) void dq_kernel(CoreGradArgs a, int tiles) {
+  __shared__ __align__(16) DqTiles<E, D> lds;
+  if (dq_rows<E, D, CAP, BIAS, false>(a, tiles, lds))
+    dq_again<E, D, CAP, BIAS>(a, tiles, (uint32_t)(uintptr_t)(lds_void_ptr)&lds);
 }
 
 // the parts of dk and dv, added up in their order, 4 values a thread

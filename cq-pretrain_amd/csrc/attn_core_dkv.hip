@@ -16,15 +16,21 @@
 namespace cqgdn {
 namespace {
 
-template <class E, int D, bool CAP, bool BIAS>
-__global__ __launch_bounds__(512, 2) void dkv_kernel(CoreGradArgs a, int blocks, int splits) {
+// the workgroup's part of the work, in its shared memory; returns whether it has to be done once more, carefully
+template <class E, int D>
+struct DkvTiles {
+  E vt[4][kTileSize<D>], qt[2][kTileSize<D>], yt[2][kTileSize<D>];
+  RowBlock info[2];
+};
+template <class E, int D, bool CAP, bool BIAS, bool CAREFUL>
+__device__ __forceinline__ bool dkv_keys(const CoreGradArgs& a, int blocks, int splits, DkvTiles<E, D>& tiles) {
   typedef typename Vec<E>::x8 x8;
   constexpr int KQ = D / 16, MT = D / 32;
   static_assert(offsetof(RowBlock, stands) == 1024 && sizeof(RowBlock) == 1536, "an eighth a wave");
-  __shared__ __align__(16) E vt[4][kTileSize<D>];
-  __shared__ __align__(16) E qt[2][kTileSize<D>];
-  __shared__ __align__(16) E yt[2][kTileSize<D>];
-  __shared__ __align__(16) RowBlock info[2];
+  auto& vt = tiles.vt;
+  auto& qt = tiles.qt;
+  auto& yt = tiles.yt;
+  auto& info = tiles.info;
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int n32 = lane & 31, kg = lane >> 5;
   // the first keys, which most rows see, first
@@ -53,8 +59,6 @@ __global__ __launch_bounds__(512, 2) void dkv_kernel(CoreGradArgs a, int blocks,
   }
   const E* const vp = vt[wave >> 1];
   f32x16 dk[MT], dv[MT];
-#pragma unroll
-  for (int i = 0; i < MT; ++i) dk[i] = dv[i] = f32x16{};
   Range<E> range;
 
   // The blocks of rows, 64 ranges at a time, a lane each: `left` are those of the present 64 that see any of the keys.
@@ -97,9 +101,9 @@ __global__ __launch_bounds__(512, 2) void dkv_kernel(CoreGradArgs a, int blocks,
     if (lane < size / 16)
       load_blocks<1>(reinterpret_cast<const char*>(from) + wave * size, 16 * lane, reinterpret_cast<char*>(&info[buffer]) + wave * size);
   };
-  // A step of 64 rows.  WHOLE: all of them see all of the wave's keys; ODD: some value of the tiles is not finite.
-  const auto step = [&](const E* qp, const E* yp, const RowBlock& x, auto whole, auto odd) {
-    constexpr bool WHOLE = decltype(whole)::value, ODD = decltype(odd)::value;
+  // A step of 64 rows.  WHOLE: all of them see all of the wave's keys.
+  const auto step = [&](const E* qp, const E* yp, const RowBlock& x, auto whole) {
+    constexpr bool WHOLE = decltype(whole)::value, APART = CAREFUL && !WHOLE;
     // operands read from LDS ahead of their use, of one and of two an MFMA: as many as leave nothing spilled
     constexpr int kEarly = !WHOLE ? 1 : CAP ? 2 : 3, kEarlyPair = WHOLE && !CAP ? 2 : 1;
     const auto half = [&](int u) {
@@ -112,7 +116,7 @@ __global__ __launch_bounds__(512, 2) void dkv_kernel(CoreGradArgs a, int blocks,
       };
       const auto column = [&](const E* p, int i) {
         const x8 c = at_tile.columns(p, u, i / MT, i % MT);
-        return ODD ? finite_values<E>(c) : c;
+        return APART ? finite_values<E>(c) : c;
       };
       f32x4 lse[4];
       const auto values = [&](const float* p, int i) { return *reinterpret_cast<const f32x4*>(p + c_row(u, 4 * i) + 16 * kg); };
@@ -231,7 +235,7 @@ __global__ __launch_bounds__(512, 2) void dkv_kernel(CoreGradArgs a, int blocks,
     };
     half(0);
     half(1);
-    if constexpr (ODD) {
+    if (APART && (tile_is_odd<E, D>(qp, lane) || tile_is_odd<E, D>(yp, lane))) {
       const auto sees = [&](int i) { return key >= x.lo[i] && key < x.hi[i]; };
       add_odd<E, D>(qp, dk, lane, sees);
       add_odd<E, D>(yp, dv, lane, sees);
@@ -240,9 +244,7 @@ __global__ __launch_bounds__(512, 2) void dkv_kernel(CoreGradArgs a, int blocks,
 
   // the present step's block and range, and the next's, whose tiles are on their way
   RowRange now, later;
-  int block = next(now), following = -1, buffer = 0;
-  if (block >= 0) stage(block, 0);
-  tiles_ready();
+  int block, following, buffer;
   const auto ask = [&] {
     following = next(later);
     if (following >= 0) stage(following, buffer ^ 1);
@@ -253,26 +255,28 @@ __global__ __launch_bounds__(512, 2) void dkv_kernel(CoreGradArgs a, int blocks,
     now = later;
     buffer ^= 1;
   };
-  // A loop for the whole steps by itself: in one for both kinds, the sums would be moved from the registers that one leaves
-  // them in to the other's, in every step.
+#pragma unroll
+  for (int i = 0; i < MT; ++i) dk[i] = dv[i] = f32x16{};
+  buffer = 0;
+  block = next(now);
+  if (block >= 0) stage(block, 0);
+  tiles_ready();
+  // A loop for the whole steps by itself: in one for both kinds, the sums would be moved from the registers that one
+  // leaves them in to the other's, in every step.
   while (block >= 0) {
 #pragma unroll 1
     while (block >= 0 && now.low <= mine && mine + 64 <= now.high) {
       ask();
-      step(qt[buffer], yt[buffer], info[buffer], std::true_type{}, std::false_type{});
+      step(qt[buffer], yt[buffer], info[buffer], std::true_type{});
       advance();
     }
     if (block < 0) break;
     ask();
-    const E* const qp = qt[buffer];
-    const E* const yp = yt[buffer];
-    if (now.last > mine && now.first < mine + 64) {
-      if (!(tile_is_odd<E, D>(qp, lane) || tile_is_odd<E, D>(yp, lane)))
-        step(qp, yp, info[buffer], std::false_type{}, std::false_type{});
-      else
-        step(qp, yp, info[buffer], std::false_type{}, std::true_type{});
-    }
+    if (now.last > mine && now.first < mine + 64) step(qt[buffer], yt[buffer], info[buffer], std::false_type{});
     advance();
+  }
+  if constexpr (!CAREFUL) {
+    if (__builtin_amdgcn_readfirstlane(__syncthreads_or(any_not_finite(dk) || any_not_finite(dv)))) return true;
   }
   if (key < a.S) {
     const float f = a.scale * range.back() * (Range<E>::on ? 0x1p-15f : 1.f), g = Range<E>::on ? 0x1p-15f : 1.f;
@@ -294,6 +298,21 @@ __global__ __launch_bounds__(512, 2) void dkv_kernel(CoreGradArgs a, int blocks,
         }
       }
   }
+  return false;
+}
+
+// apart from the kernel, whose registers it would cost
+template <class E, int D, bool CAP, bool BIAS>
+__device__ __noinline__ void dkv_again(CoreGradArgs a, int blocks, int splits, uint32_t tiles) {
+  typedef __attribute__((address_space(3))) DkvTiles<E, D>* Tiles;
+  dkv_keys<E, D, CAP, BIAS, true>(a, blocks, splits, *(DkvTiles<E, D>*)(Tiles)tiles);
+}
+
+template <class E, int D, bool CAP, bool BIAS>
+__global__ __launch_bounds__(512, 2) void dkv_kernel(CoreGradArgs a, int blocks, int splits) {
+  __shared__ __align__(16) DkvTiles<E, D> tiles;
+  if (dkv_keys<E, D, CAP, BIAS, false>(a, blocks, splits, tiles))
+    dkv_again<E, D, CAP, BIAS>(a, blocks, splits, (uint32_t)(uintptr_t)(lds_void_ptr)&tiles);
 }
 
 // dk and dv of kKeys keys of a key head; part s of `splits` takes every splits-th block of 64 rows that sees any of them
