@@ -49,8 +49,11 @@ __device__ __forceinline__ void core_tile(const CoreArgs& a, const CorePlace pla
   const bool padding = place.padding;
   const int requests = PAGED ? a.N : 1, group = a.group.d, size = 1 << a.page_shift;
   const int room = PAGED ? (int)min((int64_t)a.columns << a.page_shift, (int64_t)kAttendRoom) : a.S;
-  // the exponent's factor of the plain scores, never 0: a masked score stays -infinity
-  const float c = BENT ? 1.f : fmaxf(fabsf(a.scale) * 1.44269504088896341f, 1.17549435e-38f);
+  // A score is c times what is held of it, plus `above`.  Plain: of q.k, the factor never 0, so that a masked score stays
+  // -infinity; capped: of the cap's -r.
+  constexpr bool LESS_R = CAP && !BIAS;
+  const float c = LESS_R ? 2.f * a.cap * 1.44269504088896341f : BENT ? 1.f : fmaxf(fabsf(a.scale) * 1.44269504088896341f, 1.17549435e-38f);
+  const float above = LESS_R ? a.cap * 1.44269504088896341f : 0.f;
   constexpr float bias = kAttendBias<E>;
   const TileOperands<E, D> at_tile(lane);
 
@@ -144,7 +147,7 @@ __device__ __forceinline__ void core_tile(const CoreArgs& a, const CorePlace pla
   // the weights of 32 keys, two a part, in the order of their scores
   float base, sum;
   const auto begin_weights = [&]() {
-    base = bias - (m == -INFINITY ? 0.f : m);
+    base = above + bias - (m == -INFINITY ? 0.f : m);
     sum = 0.f;
   };
   const auto weights = [&](const f32x16& s, uint32_t (&w)[8], int i) {
@@ -153,7 +156,7 @@ __device__ __forceinline__ void core_tile(const CoreArgs& a, const CorePlace pla
     f32x2 p;
 #pragma unroll
     for (int e = 0; e < 2; ++e) {
-      p[e] = __builtin_amdgcn_exp2f(BENT ? s[2 * i + e] + base : __builtin_fmaf(s[2 * i + e], c, base));
+      p[e] = __builtin_amdgcn_exp2f(BENT && !LESS_R ? s[2 * i + e] + base : __builtin_fmaf(s[2 * i + e], c, base));
       sum += p[e];
     }
     w[i] = __builtin_bit_cast(uint32_t, __builtin_convertvector(p, x2));
@@ -162,7 +165,7 @@ __device__ __forceinline__ void core_tile(const CoreArgs& a, const CorePlace pla
   const auto bent = [&](f32x16& s, int u, int pos) {
     if constexpr (BENT) {
 #pragma unroll
-      for (int e = 0; e < 16; ++e) s[e] = CAP ? bend.capped(s[e]) : s[e] * bend.c;
+      for (int e = 0; e < 16; ++e) s[e] = LESS_R ? bend.less_r(s[e]) : CAP ? bend.capped(s[e], bend.cap) : s[e] * bend.c;
     }
     if constexpr (BIAS) {
       const float far = (float)(stands - pos - 16 * kg);
@@ -178,7 +181,7 @@ __device__ __forceinline__ void core_tile(const CoreArgs& a, const CorePlace pla
       float top = s[0];
 #pragma unroll
       for (int e = 1; e < 16; ++e) top = fmaxf(top, s[e]);
-      top = fmaxf(top, __shfl_xor(top, 32, 64)) * c;
+      top = __builtin_fmaf(fmaxf(top, __shfl_xor(top, 32, 64)), c, above);
       if (large && top > m) {
         const float f = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m - top);
         m = top;

@@ -169,7 +169,7 @@ __device__ __forceinline__ void add_odd(const E* tile, f32x16 (&acc)[MT], int la
 // ---- scores -------------------------------------------------------------------------------------------
 // A score x = scale q.k becomes u = cap tanh(x / cap) - slope |distance|, in units of log2 e throughout.  With
 // r = 1 / (1 + e^(2 x / cap)) the tanh is 1 - 2 r (an exponential and a reciprocal; off by 2^-23 of the cap), and its
-// derivative 4 r (1 - r).
+// derivative 4 (r - r^2).
 struct Bend {
   float c, cap, slope;  // scale or 2 scale / cap, cap, slope, each times log2 e; cap 0: none
   __device__ __forceinline__ Bend(float scale, float cap_, const float* slopes, int head) {
@@ -178,14 +178,16 @@ struct Bend {
     cap = cap_ * log2e;
     slope = slopes ? slopes[head] * log2e : 0.f;
   }
-  __device__ __forceinline__ float capped(float x) const {
-    return __builtin_fmaf(-2.f * cap, __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(x * c)), cap);
+  // -r, which grows with x
+  __device__ __forceinline__ float less_r(float x) const {
+    return __builtin_amdgcn_rcpf(-1.f - __builtin_amdgcn_exp2f(x * c));
   }
-  // the capped score, and the derivative of it by the uncapped one
-  __device__ __forceinline__ float capped(float x, float& rate) const {
-    const float r = __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(x * c));
-    rate = 4.f * r * (1.f - r);
-    return __builtin_fmaf(-2.f * cap, r, cap);
+  // the capped score plus what is added to it less the cap, and a quarter of its derivative by the uncapped one
+  __device__ __forceinline__ float capped(float x, float more) const { return __builtin_fmaf(2.f * cap, less_r(x), more); }
+  __device__ __forceinline__ float capped(float x, float more, float& rate) const {
+    const float r = less_r(x);
+    rate = __builtin_fmaf(r, -r, -r);
+    return __builtin_fmaf(2.f * cap, r, more);
   }
 };
 
@@ -200,7 +202,7 @@ void by_scores(const CoreArgs& a, F f) {
 
 // What the keys' gradients need of 64 rows of a key head, as the queries' gradients leave it.
 struct RowBlock {
-  float lse[64], delta[64];     // less log2 sum of exp2, and less dy.out plus the gradient of lse: what is added
+  float lse[64], delta[64];     // cap less log2 sum of exp2, and less dy.out plus the gradient of lse: what is added
   int lo[64], hi[64];           // the keys that the row sees
   float stands[64], slope[64];  // with a bias: the row's position, its head's slope times log2 e
 };

@@ -120,7 +120,7 @@ __device__ __forceinline__ bool dq_rows(const CoreGradArgs& a, int tiles, DqTile
   }
   if (a.dlse && real) delta -= a.dlse[at];
   const float lse = real ? a.lse[at] * 1.44269504088896341f : 0.f;
-  const float base = kWeightBias<E> - lse;
+  const float base = kWeightBias<E> - lse + bend.cap;
   {
     RowBlock& x = static_cast<RowBlock*>(a.blocks)[(int64_t)h * tiles * (kGradRows / kTile) + block];
     const int n = 32 * (wave & 1) + n32;
@@ -163,7 +163,7 @@ __device__ __forceinline__ bool dq_rows(const CoreGradArgs& a, int tiles, DqTile
 #pragma unroll
       for (int e = 0; e < 16; ++e) {
         float x = sc[e], rate = 1.f;
-        x = CAP ? bend.capped(x, rate) + base : __builtin_fmaf(x, bend.c, base);
+        x = CAP ? bend.capped(x, base, rate) : __builtin_fmaf(x, bend.c, base);
         if constexpr (BIAS) x = __builtin_fmaf(-bend.slope, fabsf(far - (float)c_row(u, e)), x);
         x = __builtin_amdgcn_exp2f(x) * dp[e];
         if constexpr (CAP) x *= rate;
@@ -219,7 +219,7 @@ __device__ __forceinline__ bool dq_rows(const CoreGradArgs& a, int tiles, DqTile
     if (__builtin_amdgcn_readfirstlane(__syncthreads_or(any_not_finite(acc)))) return true;
   }
   if (real) {
-    const float f = a.scale * range.back() * (Range<E>::on ? 0x1p-15f : 1.f);
+    const float f = (CAP ? 4.f : 1.f) * a.scale * range.back() * (Range<E>::on ? 0x1p-15f : 1.f);
 #pragma unroll
     for (int k = 0; k < MT; ++k)
 #pragma unroll

@@ -162,7 +162,7 @@ __device__ __forceinline__ bool dkv_keys(const CoreGradArgs& a, int blocks, int 
           } else {
             float r = 1.f, y = lse[j][i];
             if constexpr (CAP)
-              y += bend.capped(sc[e], r);
+              y = bend.capped(sc[e], y, r);
             else
               y = __builtin_fmaf(sc[e], bend.c, y);
             if constexpr (BIAS) y = __builtin_fmaf(-slope[i], fabsf(stands[i] - (float)key), y);
@@ -279,7 +279,7 @@ __device__ __forceinline__ bool dkv_keys(const CoreGradArgs& a, int blocks, int 
     if (__builtin_amdgcn_readfirstlane(__syncthreads_or(any_not_finite(dk) || any_not_finite(dv)))) return true;
   }
   if (key < a.S) {
-    const float f = a.scale * range.back() * (Range<E>::on ? 0x1p-15f : 1.f), g = Range<E>::on ? 0x1p-15f : 1.f;
+    const float f = (CAP ? 4.f : 1.f) * a.scale * range.back() * (Range<E>::on ? 0x1p-15f : 1.f), g = Range<E>::on ? 0x1p-15f : 1.f;
     const int64_t at = ((int64_t)key * a.kv_heads + h) * D, size = (int64_t)a.S * a.kv_heads * D;
     float* const part = a.ws + s * 2 * size;
 #pragma unroll
@@ -441,7 +441,7 @@ __global__ __launch_bounds__(256, 1) void pair_kernel(CoreGradArgs a, int blocks
         const int e = 4 * i + j, row = row4 + j;
         float p, rate = 1.f;
         const float from = lse[j];
-        p = CAP ? bend.capped(sc[e], rate) + from : __builtin_fmaf(sc[e], bend.c, from);
+        p = CAP ? bend.capped(sc[e], from, rate) : __builtin_fmaf(sc[e], bend.c, from);
         if constexpr (BIAS) p = __builtin_fmaf(-x.slope[row], fabsf(x.stands[row] - (float)key), p);
         p = __builtin_amdgcn_exp2f(p);
         float dx = p * dp[e];
@@ -531,7 +531,7 @@ __global__ __launch_bounds__(256, 1) void pair_kernel(CoreGradArgs a, int blocks
     }
   }
   if (real) {
-    const float f = a.scale * range.back() * (Range<E>::on ? 0x1p-15f : 1.f), g = Range<E>::on ? 0x1p-15f : 1.f;
+    const float f = (CAP ? 4.f : 1.f) * a.scale * range.back() * (Range<E>::on ? 0x1p-15f : 1.f), g = Range<E>::on ? 0x1p-15f : 1.f;
     const int64_t at = ((int64_t)key * a.kv_heads + h) * D + half * (D / 2);
     float* const part = a.ws + (int64_t)s * 2 * a.S * a.kv_heads * D;
 #pragma unroll

@@ -179,7 +179,7 @@ __global__ __launch_bounds__(64 * kWaves, D == 256 ? 1 : 2) void few_kernel(Core
             for (int g = 0; g < 2; ++g)
 #pragma unroll
               for (int e = 0; e < 4; ++e) {
-                sc[g][e] = CAP ? bend.capped(sc[g][e]) : sc[g][e] * bend.c;
+                sc[g][e] = CAP ? bend.capped(sc[g][e], bend.cap) : sc[g][e] * bend.c;
                 if constexpr (BIAS)
                   sc[g][e] = __builtin_fmaf(-bend.slope, fabsf((float)(stands - at - 16 * g - 4 * q4 - e)), sc[g][e]);
               }
