@@ -35,7 +35,6 @@ struct CoreTiles {
 template <class E, int D, bool PAGED, bool CAP, bool BIAS>
 __device__ __forceinline__ void core_tile(const CoreArgs& a, const CorePlace place, int tile, CoreTiles<E, D>& lds) {
   typedef typename Vec<E>::x8 x8;
-  constexpr bool BENT = CAP || BIAS;
   constexpr int TOK = kTile, KQ = D / 16, MT = D / 32;
   constexpr int F = 2 * KQ, H = 2 * MT;  // operands of a step: K's, and V's for 32 keys
   // operands read from LDS ahead of their MFMA: K's, and V's while the scores of the second 32 keys are formed
@@ -49,11 +48,10 @@ __device__ __forceinline__ void core_tile(const CoreArgs& a, const CorePlace pla
   const bool padding = place.padding;
   const int requests = PAGED ? a.N : 1, group = a.group.d, size = 1 << a.page_shift;
   const int room = PAGED ? (int)min((int64_t)a.columns << a.page_shift, (int64_t)kAttendRoom) : a.S;
-  // A score is c times what is held of it, plus `above`.  Plain: of q.k, the factor never 0, so that a masked score stays
-  // -infinity; capped: of the cap's -r.
-  constexpr bool LESS_R = CAP && !BIAS;
-  const float c = LESS_R ? 2.f * a.cap * 1.44269504088896341f : BENT ? 1.f : fmaxf(fabsf(a.scale) * 1.44269504088896341f, 1.17549435e-38f);
-  const float above = LESS_R ? a.cap * 1.44269504088896341f : 0.f;
+  // A score is c times what is held of it, plus `above`, less the bias.  Held is q.k (the factor is never 0, so that a masked
+  // score stays -infinity; its sign goes with Q) or, of a capped score, -r.
+  const float c = CAP ? 2.f * a.cap * 1.44269504088896341f : fmaxf(fabsf(a.scale) * 1.44269504088896341f, 1.17549435e-38f);
+  const float above = CAP ? a.cap * 1.44269504088896341f : 0.f;
   constexpr float bias = kAttendBias<E>;
   const TileOperands<E, D> at_tile(lane);
 
@@ -107,7 +105,7 @@ __device__ __forceinline__ void core_tile(const CoreArgs& a, const CorePlace pla
 #pragma unroll
     for (int i = 0; i < KQ; ++i) {
       u32x4 w = real ? *reinterpret_cast<const u32x4*>(q + 16 * i) : u32x4{0, 0, 0, 0};
-      if (!BENT && a.scale < 0.f) w ^= 0x80008000u;
+      if (!CAP && a.scale < 0.f) w ^= 0x80008000u;
       qf[i] = __builtin_bit_cast(x8, w);
     }
   }
@@ -118,16 +116,21 @@ __device__ __forceinline__ void core_tile(const CoreArgs& a, const CorePlace pla
 
   const int begin = last > 0 ? (PAGED ? first & ~(TOK - 1) : first) : 0;
   const int steps = (last - begin + TOK - 1) / TOK, per = (steps + splits - 1) / splits;
-  const int n = min(steps, (s + 1) * per) - s * per, pos0 = begin + s * per * TOK;
+  const int n = min(steps, (s + 1) * per) - s * per;
+  // Steps go from the first key to the last; with a bias, which is least at a row's own position, the other way, so that a
+  // row's maximum is found early (steep slopes had it move in every step: seven documents with a window of 1024, heads of
+  // 64, 154 us, this way 106)
+  const int pos0 = begin + (s * per + (BIAS ? n - 1 : 0)) * TOK;
+  constexpr int FURTHER = BIAS ? -TOK : TOK;
 
   // the block table's entries for the 16 positions each of step j, one a lane
   const auto entries = [&](int j) {
-    const int column = (pos0 + j * TOK + 16 * (lane & (GROUPS - 1))) >> a.page_shift;
+    const int column = (pos0 + j * FURTHER + 16 * (lane & (GROUPS - 1))) >> a.page_shift;
     return j < n && column < a.columns ? a.tables[r * a.table_stride + column] : -1;
   };
   // step j's rows of the wave on their way into the tiles.  Returns which of the step's 16 positions are shown.
   const auto stage = [&](int table, int j) {
-    const int pos = pos0 + j * TOK;
+    const int pos = pos0 + j * FURTHER;
     if constexpr (PAGED) {
       const uint32_t page = __builtin_amdgcn_readlane(table, wave);
       const int at = (pos + 16 * wave) & (size - 1);
@@ -150,38 +153,37 @@ __device__ __forceinline__ void core_tile(const CoreArgs& a, const CorePlace pla
     base = above + bias - (m == -INFINITY ? 0.f : m);
     sum = 0.f;
   };
-  const auto weights = [&](const f32x16& s, uint32_t (&w)[8], int i) {
+  // of element e of the u-th scores of a step `far` from the row, with `more`
+  const auto scored = [&](const f32x16& s, int u, float far, int e, float more) {
+    if constexpr (BIAS) more = __builtin_fmaf(-bend.slope, fabsf(far - (float)c_row(u, e)), more);
+    return __builtin_fmaf(s[e], c, more);
+  };
+  const auto weights = [&](const f32x16& s, uint32_t (&w)[8], int u, float far, int i) {
     typedef float f32x2 __attribute__((ext_vector_type(2)));
     typedef E x2 __attribute__((ext_vector_type(2)));
     f32x2 p;
 #pragma unroll
     for (int e = 0; e < 2; ++e) {
-      p[e] = __builtin_amdgcn_exp2f(BENT && !LESS_R ? s[2 * i + e] + base : __builtin_fmaf(s[2 * i + e], c, base));
+      p[e] = __builtin_amdgcn_exp2f(scored(s, u, far, 2 * i + e, base));
       sum += p[e];
     }
     w[i] = __builtin_bit_cast(uint32_t, __builtin_convertvector(p, x2));
   };
-  // the scores with cap and bias, in units of log2 e
-  const auto bent = [&](f32x16& s, int u, int pos) {
-    if constexpr (BENT) {
+  const auto capped = [&](f32x16& s) {
+    if constexpr (CAP) {
 #pragma unroll
-      for (int e = 0; e < 16; ++e) s[e] = LESS_R ? bend.less_r(s[e]) : CAP ? bend.capped(s[e], bend.cap) : s[e] * bend.c;
-    }
-    if constexpr (BIAS) {
-      const float far = (float)(stands - pos - 16 * kg);
-#pragma unroll
-      for (int e = 0; e < 16; ++e) s[e] = __builtin_fmaf(-bend.slope, fabsf(far - (float)c_row(u, e)), s[e]);
+      for (int e = 0; e < 16; ++e) s[e] = bend.less_r(s[e]);
     }
   };
   // where the weights have grown too large, or are a row's first, its maximum moves and they are made again
-  const auto settle = [&](const f32x16& s, uint32_t (&w)[8]) {
+  const auto settle = [&](const f32x16& s, uint32_t (&w)[8], int u, float far) {
     bool large = sum > kAttendLimit<E> || m == -INFINITY;
     if (__any(large)) {
       large = __shfl_xor((int)large, 32, 64) || large;  // the two lanes of a row
-      float top = s[0];
+      float top = scored(s, u, far, 0, above);
 #pragma unroll
-      for (int e = 1; e < 16; ++e) top = fmaxf(top, s[e]);
-      top = __builtin_fmaf(fmaxf(top, __shfl_xor(top, 32, 64)), c, above);
+      for (int e = 1; e < 16; ++e) top = fmaxf(top, scored(s, u, far, e, above));
+      top = fmaxf(top, __shfl_xor(top, 32, 64));
       if (large && top > m) {
         const float f = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m - top);
         m = top;
@@ -191,7 +193,7 @@ __device__ __forceinline__ void core_tile(const CoreArgs& a, const CorePlace pla
       }
       begin_weights();
 #pragma unroll
-      for (int i = 0; i < 8; ++i) weights(s, w, i);
+      for (int i = 0; i < 8; ++i) weights(s, w, u, far, i);
     }
     l += sum;
   };
@@ -203,6 +205,7 @@ __device__ __forceinline__ void core_tile(const CoreArgs& a, const CorePlace pla
     x8 kf[F], vf[2][H];
     f32x16 sc[2];
     uint32_t pw[2][8];
+    const float far = (float)(stands - pos - 16 * kg);
     const auto key = [&](int i) { kf[i] = at_tile.rows(kp, i / KQ, i % KQ); };
     const auto value = [&](int u, int i) { vf[u][i] = at_tile.columns(vp, u, i / MT, i % MT); };
 #pragma unroll
@@ -221,32 +224,32 @@ __device__ __forceinline__ void core_tile(const CoreArgs& a, const CorePlace pla
       score(0, i);
       __builtin_amdgcn_sched_barrier(0);
     }
-    bent(sc[0], 0, pos);
+    capped(sc[0]);
     begin_weights();
 #pragma unroll
     for (int i = 0; i < KQ; ++i) {
       score(1, i);
 #pragma unroll
-      for (int e = i * 8 / KQ; e < (i + 1) * 8 / KQ; ++e) weights(sc[0], pw[0], e);
+      for (int e = i * 8 / KQ; e < (i + 1) * 8 / KQ; ++e) weights(sc[0], pw[0], 0, far, e);
 #pragma unroll
       for (int e = i * kFirst / KQ; e < (i + 1) * kFirst / KQ; ++e) value(0, e);
       __builtin_amdgcn_sched_barrier(0);
     }
-    settle(sc[0], pw[0]);
-    bent(sc[1], 1, pos);
+    settle(sc[0], pw[0], 0, far);
+    capped(sc[1]);
     begin_weights();
 #pragma unroll
     for (int i = 0; i < H; ++i) {
       gather(0, i);
 #pragma unroll
-      for (int e = i * 8 / H; e < (i + 1) * 8 / H; ++e) weights(sc[1], pw[1], e);
+      for (int e = i * 8 / H; e < (i + 1) * 8 / H; ++e) weights(sc[1], pw[1], 1, far, e);
       if (i + kFirst < H)
         value(0, i + kFirst);
       else
         value(1, i + kFirst - H);
       __builtin_amdgcn_sched_barrier(0);
     }
-    settle(sc[1], pw[1]);
+    settle(sc[1], pw[1], 1, far);
 #pragma unroll
     for (int i = 0; i < H; ++i) {
       gather(1, i);
@@ -258,6 +261,7 @@ __device__ __forceinline__ void core_tile(const CoreArgs& a, const CorePlace pla
   const auto cut_step = [&](const E* kp, const E* vp, int pos, int shown, auto careful) {
     constexpr bool CAREFUL = decltype(careful)::value;
     const int lo0 = lo - pos - 16 * kg, hi0 = hi - pos - 16 * kg;
+    const float far = (float)(stands - pos - 16 * kg);
     const bool odd = CAREFUL && tile_is_odd<E, D>(vp, lane);
     // one half after the other: a short call's time is that of fetching this code once
 #pragma unroll 1
@@ -266,7 +270,7 @@ __device__ __forceinline__ void core_tile(const CoreArgs& a, const CorePlace pla
       uint32_t pw[8];
 #pragma unroll
       for (int i = 0; i < KQ; ++i) sc = mfma32(at_tile.rows(kp, u, i), qf[i], sc);
-      bent(sc, u, pos);
+      capped(sc);
 #pragma unroll
       for (int e = 0; e < 16; ++e) {
         const int at = c_row(u, e);
@@ -274,8 +278,8 @@ __device__ __forceinline__ void core_tile(const CoreArgs& a, const CorePlace pla
       }
       begin_weights();
 #pragma unroll
-      for (int e = 0; e < 8; ++e) weights(sc, pw, e);
-      settle(sc, pw);
+      for (int e = 0; e < 8; ++e) weights(sc, pw, u, far, e);
+      settle(sc, pw, u, far);
 #pragma unroll
       for (int i = 0; i < H; ++i) {
         x8 v = at_tile.columns(vp, u, i / MT, i % MT);
@@ -305,7 +309,7 @@ __device__ __forceinline__ void core_tile(const CoreArgs& a, const CorePlace pla
       tiles_ready();
       shown = shown1;
       ++j;
-      pos += TOK;
+      pos += FURTHER;
     };
     // A loop for the whole steps by itself: in one for both kinds, the sums would be moved from the registers that one
     // leaves them in to the other's, in every step.

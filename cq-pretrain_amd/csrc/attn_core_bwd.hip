@@ -18,6 +18,7 @@
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
+#include <cmath>
 
 #include "attn_core_grad.hpp"
 
@@ -258,11 +259,15 @@ __global__ __launch_bounds__(256) void join_parts_kernel(const float* ws, int64_
 // blocks of 64 rows, of whole workgroups for dq
 int64_t row_blocks(int64_t T, int group) { return (T * group + kGradRows - 1) / kGradRows * (kGradRows / kTile); }
 
-// parts of the keys' gradients: two rounds of workgroups at least
+// Parts of the keys' gradients: no more than give two rounds of workgroups, one a CU, and no more than pay.  A step of 64
+// rows takes a workgroup that is alone some 2.5 us, a part's fp32 sums 16 bytes a value, written and read: b blocks of rows
+// over n parts 2.5 b / n + 3.3e-6 n S kv_heads D us, which is least at sqrt(750000 b / (S kv_heads D)) parts (2304 rows:
+// 10 parts 92 us with the join, 16 111; 317 rows: 30 either way).
 int key_parts(int64_t T, int64_t S, int kv_heads, int group, int D) {
   const int keys = D == 256 ? kKeys<256> : D == 128 ? kKeys<128> : kKeys<64>;
-  const int64_t each = std::max<int64_t>(1, (S + keys - 1) / keys * kv_heads);
-  return (int)std::max<int64_t>(1, std::min<int64_t>({512 / each, 16, row_blocks(T, group)}));
+  const int64_t each = std::max<int64_t>(1, (S + keys - 1) / keys * kv_heads), blocks = row_blocks(T, group);
+  const int64_t pays = (int64_t)std::lround(std::sqrt(750000. * blocks / std::max<int64_t>(1, S * kv_heads * D)));
+  return (int)std::max<int64_t>(1, std::min<int64_t>({512 / each, 16, blocks, pays}));
 }
 
 template <class E, int D>
