@@ -315,30 +315,36 @@ __global__ __launch_bounds__(512, 2) void dkv_kernel(CoreGradArgs a, int blocks,
     dkv_again<E, D, CAP, BIAS>(a, blocks, splits, (uint32_t)(uintptr_t)(lds_void_ptr)&tiles);
 }
 
-// dk and dv of kKeys keys of a key head; part s of `splits` takes every splits-th block of 64 rows that sees any of them
-template <class E, int D, bool CAP, bool BIAS>
-__global__ __launch_bounds__(256, 1) void pair_kernel(CoreGradArgs a, int blocks, int splits) {
+// With D = 256 the sums of 32 keys would fill a wave's registers.  Two waves share 32 keys: one forms S, the other dP, they
+// exchange them through shared memory, and each sums half of the dimensions; a workgroup takes 64 keys.
+template <class E, int D>
+struct PairTiles {
+  E qt[2][kTileSize<D>], yt[2][kTileSize<D>];
+  float swap[4][1024];
+  RowBlock info[2];
+};
+template <class E, int D, bool CAP, bool BIAS, bool CAREFUL>
+__device__ __forceinline__ bool pair_keys(const CoreGradArgs& a, int blocks, int splits, PairTiles<E, D>& tiles) {
   typedef typename Vec<E>::x8 x8;
-  constexpr bool PAIR = true;
-  constexpr int KQ = D / 16, MT = D / 32 / (PAIR ? 2 : 1);
+  constexpr int KQ = D / 16, MT = D / 64;
   static_assert(offsetof(RowBlock, stands) == 1024 && sizeof(RowBlock) == 1536, "an instruction, and half of one");
-  __shared__ __align__(16) E qt[2][kTileSize<D>];
-  __shared__ __align__(16) E yt[2][kTileSize<D>];
-  __shared__ __align__(16) float swap[PAIR ? 4 : 1][PAIR ? 1024 : 4];
-  __shared__ __align__(16) RowBlock info[2];
+  auto& qt = tiles.qt;
+  auto& yt = tiles.yt;
+  auto& swap = tiles.swap;
+  auto& info = tiles.info;
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int n32 = lane & 31, kg = lane >> 5;
-  const int half = PAIR ? wave & 1 : 0;  // of the pair: 0 forms S and sums dimensions below D / 2, 1 dP and those above
+  const int half = wave & 1;  // of the pair: 0 forms S and sums dimensions below D / 2, 1 dP and those above
   // the first keys, which most rows see, first
   const int h = blockIdx.x % a.kv_heads, s = blockIdx.x / a.kv_heads % splits;
   const int k0 = blockIdx.x / (a.kv_heads * splits) * kKeys<D>;
-  const int group = a.group.d, rows = (int)a.T * group, mine = k0 + 32 * (PAIR ? wave >> 1 : wave);
+  const int group = a.group.d, rows = (int)a.T * group, mine = k0 + 32 * (wave >> 1);
   const int key = mine + n32;
   const bool real = key < a.S;
   const TileOperands<E, D> at_tile(lane);
   const Bend bend(a.scale, CAP ? a.cap : 0.f, nullptr, 0);
 
-  x8 kf[KQ], vf[PAIR ? 1 : KQ];  // lane (n32, kg): key n32, dimensions 16 i + 8 kg ..; of a pair, kf is V in the second
+  x8 kf[KQ];  // lane (n32, kg): of key n32 K, in the second wave V, dimensions 16 i + 8 kg ..
   {
     const E* k = static_cast<const E*>(a.k) + h * a.k_head + (real ? key : 0) * a.k_token + 8 * kg;
     const E* v = static_cast<const E*>(a.v) + h * a.v_head + (real ? key : 0) * a.v_token + 8 * kg;
@@ -346,7 +352,6 @@ __global__ __launch_bounds__(256, 1) void pair_kernel(CoreGradArgs a, int blocks
 #pragma unroll
     for (int i = 0; i < KQ; ++i) {
       kf[i] = __builtin_bit_cast(x8, real ? *reinterpret_cast<const u32x4*>((half ? v : k) + 16 * i) : none);
-      if constexpr (!PAIR) vf[i] = __builtin_bit_cast(x8, real ? *reinterpret_cast<const u32x4*>(v + 16 * i) : none);
     }
   }
   f32x16 dk[MT], dv[MT];
@@ -392,7 +397,7 @@ __global__ __launch_bounds__(256, 1) void pair_kernel(CoreGradArgs a, int blocks
     if (wave == 0) load_blocks<1>(from, 16 * lane, &info[buffer]);
     if (BIAS && wave == 1 && lane < 32) load_blocks<1>(from->stands, 16 * lane, info[buffer].stands);
   };
-  // of the u-th 32 rows: S and dP - delta, with a pair's one of them
+  // of the u-th 32 rows: S or dP - delta
   const auto products = [&](const E* qp, const E* yp, const RowBlock& x, int u, f32x16& sc, f32x16& dp) {
     sc = f32x16{};
 #pragma unroll
@@ -401,18 +406,10 @@ __global__ __launch_bounds__(256, 1) void pair_kernel(CoreGradArgs a, int blocks
 #pragma unroll
       for (int e = 0; e < 4; ++e) dp[4 * i + e] = delta[e];
     }
-    if constexpr (PAIR) {
-      if (half) sc = dp;
-      const E* const p = half ? yp : qp;
+    if (half) sc = dp;
+    const E* const p = half ? yp : qp;
 #pragma unroll
-      for (int i = 0; i < KQ; ++i) sc = mfma32(at_tile.rows(p, u, i), kf[i], sc);
-    } else {
-#pragma unroll
-      for (int i = 0; i < KQ; ++i) {
-        sc = mfma32(at_tile.rows(qp, u, i), kf[i], sc);
-        dp = mfma32(at_tile.rows(yp, u, i), vf[i], dp);
-      }
-    }
+    for (int i = 0; i < KQ; ++i) sc = mfma32(at_tile.rows(p, u, i), kf[i], sc);
   };
   const auto give = [&](const f32x16& sc) {
 #pragma unroll
@@ -430,8 +427,8 @@ __global__ __launch_bounds__(256, 1) void pair_kernel(CoreGradArgs a, int blocks
     dp = half ? sc : other;
     sc = half ? other : sc;
   };
-  const auto sums = [&](const E* qp, const E* yp, const RowBlock& x, int u, f32x16& sc, f32x16& dp, bool odd, auto whole) {
-    constexpr bool WHOLE = decltype(whole)::value;
+  const auto sums = [&](const E* qp, const E* yp, const RowBlock& x, int u, f32x16& sc, f32x16& dp, auto whole) {
+    constexpr bool WHOLE = decltype(whole)::value, APART = CAREFUL && !WHOLE;
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       const int row4 = c_row(u, 4 * i) + 16 * kg;
@@ -466,7 +463,7 @@ __global__ __launch_bounds__(256, 1) void pair_kernel(CoreGradArgs a, int blocks
 #pragma unroll
       for (int m = 0; m < MT; ++m) {
         x8 y = at_tile.columns(yp, u, b, half * MT + m), q = at_tile.columns(qp, u, b, half * MT + m);
-        if (odd) {
+        if constexpr (APART) {
           y = finite_values<E>(y);
           q = finite_values<E>(q);
         }
@@ -476,59 +473,55 @@ __global__ __launch_bounds__(256, 1) void pair_kernel(CoreGradArgs a, int blocks
     }
   };
   const auto step = [&](const E* qp, const E* yp, const RowBlock& x, auto whole) {
-    constexpr bool WHOLE = decltype(whole)::value;
-    bool odd = false;
-    if constexpr (!WHOLE) odd = tile_is_odd<E, D>(qp, lane) || tile_is_odd<E, D>(yp, lane);
-    if constexpr (PAIR) {
-      f32x16 sc[2], dp[2];
+    constexpr bool WHOLE = decltype(whole)::value, APART = CAREFUL && !WHOLE;
+    f32x16 sc[2], dp[2];
 #pragma unroll
-      for (int u = 0; u < 2; ++u) products(qp, yp, x, u, sc[u], dp[u]);
-      give(sc[0]);
-      lds_barrier();
-      take(sc[0], dp[0]);
-      lds_barrier();
-      give(sc[1]);
-      lds_barrier();
-      take(sc[1], dp[1]);
+    for (int u = 0; u < 2; ++u) products(qp, yp, x, u, sc[u], dp[u]);
+    give(sc[0]);
+    lds_barrier();
+    take(sc[0], dp[0]);
+    lds_barrier();
+    give(sc[1]);
+    lds_barrier();
+    take(sc[1], dp[1]);
 #pragma unroll
-      for (int u = 0; u < 2; ++u) sums(qp, yp, x, u, sc[u], dp[u], odd, whole);
-    } else {
-#pragma unroll
-      for (int u = 0; u < 2; ++u) {
-        f32x16 sc, dp;
-        products(qp, yp, x, u, sc, dp);
-        sums(qp, yp, x, u, sc, dp, odd, whole);
-      }
-    }
-    if (odd) {
+    for (int u = 0; u < 2; ++u) sums(qp, yp, x, u, sc[u], dp[u], whole);
+    if (APART && (tile_is_odd<E, D>(qp, lane) || tile_is_odd<E, D>(yp, lane))) {
       const auto sees = [&](int i) { return key >= x.lo[i] && key < x.hi[i]; };
       add_odd<E, D>(qp, dk, lane, sees, half * MT);
       add_odd<E, D>(yp, dv, lane, sees, half * MT);
     }
   };
 
-  RowRange x, y;
-  int block = next(x), buffer = 0;
-  if (block >= 0) {
-    stage(block, 0);
+  RowRange now, later;
+  int buffer = 0, block = next(now), following = -1;
+  if (block >= 0) stage(block, 0);
+  tiles_ready();
+  const auto ask = [&] {
+    following = next(later);
+    if (following >= 0) stage(following, buffer ^ 1);
+  };
+  const auto advance = [&] {
     tiles_ready();
+    block = following;
+    now = later;
+    buffer ^= 1;
+  };
+  // The waves meet within a step, so all of them go through every step of the workgroup's, each in its own of the loops.
+  while (block >= 0) {
 #pragma unroll 1
-    while (true) {
-      const int following = next(y);
-      if (following >= 0) stage(following, buffer ^ 1);
-      // a pair's waves meet within the step, so all of the workgroup's go through it, as far as any of them has to
-      const bool any = x.last > mine && x.first < mine + 32;
-      if (PAIR || any) {
-        if (x.low <= mine && mine + 32 <= x.high)
-          step(qt[buffer], yt[buffer], info[buffer], std::true_type{});
-        else
-          step(qt[buffer], yt[buffer], info[buffer], std::false_type{});
-      }
-      tiles_ready();
-      if (following < 0) break;
-      x = y;
-      buffer ^= 1;
+    while (block >= 0 && now.low <= mine && mine + 32 <= now.high) {
+      ask();
+      step(qt[buffer], yt[buffer], info[buffer], std::true_type{});
+      advance();
     }
+    if (block < 0) break;
+    ask();
+    step(qt[buffer], yt[buffer], info[buffer], std::false_type{});
+    advance();
+  }
+  if constexpr (!CAREFUL) {
+    if (__builtin_amdgcn_readfirstlane(__syncthreads_or(any_not_finite(dk) || any_not_finite(dv)))) return true;
   }
   if (real) {
     const float f = (CAP ? 4.f : 1.f) * a.scale * range.back() * (Range<E>::on ? 0x1p-15f : 1.f), g = Range<E>::on ? 0x1p-15f : 1.f;
@@ -550,6 +543,20 @@ __global__ __launch_bounds__(256, 1) void pair_kernel(CoreGradArgs a, int blocks
         }
       }
   }
+  return false;
+}
+
+template <class E, int D, bool CAP, bool BIAS>
+__device__ __noinline__ void pair_again(CoreGradArgs a, int blocks, int splits, uint32_t tiles) {
+  typedef __attribute__((address_space(3))) PairTiles<E, D>* Tiles;
+  pair_keys<E, D, CAP, BIAS, true>(a, blocks, splits, *(PairTiles<E, D>*)(Tiles)tiles);
+}
+
+template <class E, int D, bool CAP, bool BIAS>
+__global__ __launch_bounds__(256, 1) void pair_kernel(CoreGradArgs a, int blocks, int splits) {
+  __shared__ __align__(16) PairTiles<E, D> tiles;
+  if (pair_keys<E, D, CAP, BIAS, false>(a, blocks, splits, tiles))
+    pair_again<E, D, CAP, BIAS>(a, blocks, splits, (uint32_t)(uintptr_t)(lds_void_ptr)&tiles);
 }
 
 }  // namespace
