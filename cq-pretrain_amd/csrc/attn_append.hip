@@ -4,6 +4,9 @@
 // into LDS, while the first rows are under way; then its threads go through the tokens' heads, queries, keys and
 // values, in the order of memory.  Keys and values go to the token's slot in its page, queries to their output, each
 // row written once: a token's keys are not written by one launch and read by another.
+//
+// Bound by memory: 8191 tokens of 16 + 4 + 4 heads of 256 (201 MB read and written) 39 us, 5.1 TB/s.  With two, four and
+// eight items' loads of a thread under way at once, and fewer waves a CU for their registers, it was 41, 52 and 63.
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
@@ -15,7 +18,7 @@ namespace cqgdn {
 namespace {
 
 constexpr int kThreads = 256;
-constexpr int kTogether = 4;      // items of a thread whose loads are under way at once
+constexpr int kItems = 4;         // of a thread, one after the other
 constexpr int kMostPairs = 4096;  // of a workgroup's tokens: 32 KB of sines and cosines
 
 template <class T, int VEC, bool ADJ>
@@ -31,75 +34,67 @@ __global__ __launch_bounds__(kThreads) void append_kernel(AppendArgs a, int unit
   const int slot = tid / units, u = tid - slot * units;
   const L place(a, u, turned);
   const bool working = slot < slots;
-  P p0[kTogether], p1[kTogether];
-  T* y[kTogether];  // null: not written
-  int token[kTogether];
-  bool turns[kTogether];
-  const auto fetch = [&](int first) {
-#pragma unroll
-    for (int i = 0; i < kTogether; ++i) {
-      const int item = min(first + i * slots, items - 1);  // the last once more rather than a branch between the loads
-      token[i] = a.by_heads.of(item);
-      const int g = item - token[i] * heads, w = g < a.heads[0] ? 0 : g < a.heads[0] + a.heads[1] ? 1 : 2;
-      const int h = w == 0 ? g : w == 1 ? g - a.heads[0] : g - a.heads[0] - a.heads[1];
-      const int64_t t = t0 + token[i];
-      const T* x = w == 2 ? static_cast<const T*>(a.v) + t * a.v_token + h * a.v_head
-                          : static_cast<const T*>(a.x[w]) + t * a.token[w] + h * a.head[w];
-      if (w == 0) {
-        y[i] = static_cast<T*>(a.y[0]) + (t * a.heads[0] + h) * a.D;
-      } else {
-        const int at = a.slots[t];
-        y[i] = at < 0 || at >= a.slot_count
-                   ? nullptr
-                   : static_cast<T*>(a.data) +
-                         ((((int64_t)(at >> a.page_shift) * a.heads[1] + h) * 2 + (w - 1)) * size + (at & (size - 1))) * a.D;
-      }
-      turns[i] = w < 2;
-      p0[i] = *reinterpret_cast<const P*>(x + place.at0);
-      p1[i] = *reinterpret_cast<const P*>(x + place.at1);
+  P p0, p1;
+  T* y;  // null: not written
+  int token;
+  bool turns;
+  const auto fetch = [&](int item) {
+    token = a.by_heads.of(item);
+    const int g = item - token * heads, w = g < a.heads[0] ? 0 : g < a.heads[0] + a.heads[1] ? 1 : 2;
+    const int h = w == 0 ? g : w == 1 ? g - a.heads[0] : g - a.heads[0] - a.heads[1];
+    const int64_t t = t0 + token;
+    const T* x = w == 2 ? static_cast<const T*>(a.v) + t * a.v_token + h * a.v_head
+                        : static_cast<const T*>(a.x[w]) + t * a.token[w] + h * a.head[w];
+    if (w == 0) {
+      y = static_cast<T*>(a.y[0]) + (t * a.heads[0] + h) * a.D;
+    } else {
+      const int at = a.slots[t];
+      y = at < 0 || at >= a.slot_count
+              ? nullptr
+              : static_cast<T*>(a.data) +
+                    ((((int64_t)(at >> a.page_shift) * a.heads[1] + h) * 2 + (w - 1)) * size + (at & (size - 1))) * a.D;
     }
+    turns = w < 2;
+    p0 = *reinterpret_cast<const P*>(x + place.at0);
+    p1 = *reinterpret_cast<const P*>(x + place.at1);
   };
-  if (working) fetch(slot);
+  if (working && slot < items) fetch(slot);
   for (int i = tid; i < n * pairs; i += kThreads) {
     const int token = a.by_pairs.of(i);
     angle(a, t0 + token, i - token * pairs, sines[i], cosines[i]);
   }
   __syncthreads();
   if (!working) return;
-  for (int first = slot; first < items; first += kTogether * slots) {
-    if (first != slot) fetch(first);
+  for (int item = slot; item < items; item += slots) {
+    if (item != slot) fetch(item);
+    if (!y) continue;
+    if (place.rot && turns) {
 #pragma unroll
-    for (int i = 0; i < kTogether; ++i) {
-      if (first + i * slots >= items) break;
-      if (!y[i]) continue;
-      if (place.rot && turns[i]) {
+      for (int j = 0; j < VEC / L::RUN; ++j) {
+        const int at = token * pairs + L::pair(a, u, j);
+        float s[L::RUN], c[L::RUN];
 #pragma unroll
-        for (int j = 0; j < VEC / L::RUN; ++j) {
-          const int at = token[i] * pairs + L::pair(a, u, j);
-          float s[L::RUN], c[L::RUN];
+        for (int e = 0; e < L::RUN; ++e) {
+          s[e] = sines[at + e];
+          c[e] = cosines[at + e];
+        }
 #pragma unroll
-          for (int e = 0; e < L::RUN; ++e) {
-            s[e] = sines[at + e];
-            c[e] = cosines[at + e];
-          }
-#pragma unroll
-          for (int e = 0; e < L::RUN; ++e) {
-            if constexpr (!ADJ || VEC == 1) {
-              const float l = (float)p0[i][e], r = (float)p1[i][e];
-              p0[i][e] = (T)(l * c[e] - r * s[e]);
-              p1[i][e] = (T)(r * c[e] + l * s[e]);
-            } else {
-              P& p = j ? p1[i] : p0[i];
-              const float l = (float)p[2 * e], r = (float)p[2 * e + 1];
-              p[2 * e] = (T)(l * c[e] - r * s[e]);
-              p[2 * e + 1] = (T)(r * c[e] + l * s[e]);
-            }
+        for (int e = 0; e < L::RUN; ++e) {
+          if constexpr (!ADJ || VEC == 1) {
+            const float l = (float)p0[e], r = (float)p1[e];
+            p0[e] = (T)(l * c[e] - r * s[e]);
+            p1[e] = (T)(r * c[e] + l * s[e]);
+          } else {
+            P& p = j ? p1 : p0;
+            const float l = (float)p[2 * e], r = (float)p[2 * e + 1];
+            p[2 * e] = (T)(l * c[e] - r * s[e]);
+            p[2 * e + 1] = (T)(r * c[e] + l * s[e]);
           }
         }
       }
-      *reinterpret_cast<P*>(y[i] + place.at0) = p0[i];
-      *reinterpret_cast<P*>(y[i] + place.at1) = p1[i];
     }
+    *reinterpret_cast<P*>(y + place.at0) = p0;
+    *reinterpret_cast<P*>(y + place.at1) = p1;
   }
 }
 
@@ -107,8 +102,8 @@ template <class T, int VEC>
 void launch(AppendArgs a, hipStream_t st) {
   const int units = a.D / (2 * VEC), turned = a.rotary / (2 * VEC), heads = a.heads[0] + 2 * a.heads[1];
   const int slots = kThreads / units;
-  // as many tokens as give a thread two rounds of kTogether items, but 1024 workgroups (4 a CU) first
-  int64_t tokens = std::max<int64_t>(1, (int64_t)slots * kTogether * 2 / heads);
+  // as many tokens as give a thread kItems, but 1024 workgroups (4 a CU) first
+  int64_t tokens = std::max<int64_t>(1, (int64_t)slots * kItems / heads);
   tokens = std::min<int64_t>({tokens, std::max<int64_t>(1, a.T / 1024), std::max(1, kMostPairs / std::max(1, a.rotary / 2))});
   a.by_heads = Divider(heads);
   a.by_pairs = Divider(std::max(1, a.rotary / 2));
