@@ -10,6 +10,7 @@
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
+#include <type_traits>
 
 #include "attn_turn.hpp"
 #include "cqgdn.h"
@@ -21,8 +22,31 @@ constexpr int kThreads = 256;
 constexpr int kItems = 4;         // of a thread, one after the other
 constexpr int kMostPairs = 4096;  // of a workgroup's tokens: 32 KB of sines and cosines
 
+// The product and sum rounded once, to T.  fp16 has an instruction for it, which the compiler takes in the rotary kernel
+// and takes or leaves here, so it is written out (the wait is for a register of which half is written).
+template <class T>
+__device__ __forceinline__ T rounded_fma(float a, float b, float c) {
+  if constexpr (std::is_same_v<T, _Float16>) {
+    uint32_t d;
+    asm("v_fma_mixlo_f16 %0, %1, %2, %3\n\ts_nop 1" : "=v"(d) : "v"(a), "v"(b), "v"(c));
+    return __builtin_bit_cast(_Float16, (uint16_t)d);
+  } else {
+    return (T)__builtin_fmaf(a, b, c);
+  }
+}
+
+// (l c - r s, r c + l s): which product of a sum is rounded first (l s if `left_first`) is left to no compiler, as rows
+// appended are those of the rotary kernel to the last bit.
+template <class T>
+__device__ __forceinline__ void turn_pair(T& left, T& right, float s, float c, bool left_first) {
+  const float l = (float)left, r = (float)right;
+  left = rounded_fma<T>(l, c, -(r * s));
+  right = left_first ? rounded_fma<T>(r, c, l * s) : rounded_fma<T>(l, s, r * c);
+}
+
 template <class T, int VEC, bool ADJ>
-__global__ __launch_bounds__(kThreads) void append_kernel(AppendArgs a, int units, int turned, int tokens, int slots) {
+__global__ __launch_bounds__(kThreads) void append_kernel(AppendArgs a, int units, int turned, int tokens, int slots,
+                                                             bool left_first) {
   typedef T P __attribute__((ext_vector_type(VEC)));
   typedef TurnPlace<VEC, ADJ> L;
   extern __shared__ __align__(16) float lds[];  // sines [tokens][rotary / 2], then cosines
@@ -81,14 +105,16 @@ __global__ __launch_bounds__(kThreads) void append_kernel(AppendArgs a, int unit
 #pragma unroll
         for (int e = 0; e < L::RUN; ++e) {
           if constexpr (!ADJ || VEC == 1) {
-            const float l = (float)p0[e], r = (float)p1[e];
-            p0[e] = (T)(l * c[e] - r * s[e]);
-            p1[e] = (T)(r * c[e] + l * s[e]);
+            T l = p0[e], r = p1[e];
+            turn_pair(l, r, s[e], c[e], VEC == 1 && left_first);
+            p0[e] = l;
+            p1[e] = r;
           } else {
             P& p = j ? p1 : p0;
-            const float l = (float)p[2 * e], r = (float)p[2 * e + 1];
-            p[2 * e] = (T)(l * c[e] - r * s[e]);
-            p[2 * e + 1] = (T)(r * c[e] + l * s[e]);
+            T l = p[2 * e], r = p[2 * e + 1];
+            turn_pair(l, r, s[e], c[e], true);
+            p[2 * e] = l;
+            p[2 * e + 1] = r;
           }
         }
       }
@@ -99,7 +125,7 @@ __global__ __launch_bounds__(kThreads) void append_kernel(AppendArgs a, int unit
 }
 
 template <class T, int VEC>
-void launch(AppendArgs a, hipStream_t st) {
+void launch(AppendArgs a, bool left_first, hipStream_t st) {
   const int units = a.D / (2 * VEC), turned = a.rotary / (2 * VEC), heads = a.heads[0] + 2 * a.heads[1];
   const int slots = kThreads / units;
   // as many tokens as give a thread kItems, but 1024 workgroups (4 a CU) first
@@ -109,9 +135,9 @@ void launch(AppendArgs a, hipStream_t st) {
   a.by_pairs = Divider(std::max(1, a.rotary / 2));
   const unsigned grid = (unsigned)((a.T + tokens - 1) / tokens), lds = (unsigned)(tokens * a.rotary * sizeof(float));
   if (a.adjacent)
-    append_kernel<T, VEC, true><<<grid, kThreads, lds, st>>>(a, units, turned, (int)tokens, slots);
+    append_kernel<T, VEC, true><<<grid, kThreads, lds, st>>>(a, units, turned, (int)tokens, slots, left_first);
   else
-    append_kernel<T, VEC, false><<<grid, kThreads, lds, st>>>(a, units, turned, (int)tokens, slots);
+    append_kernel<T, VEC, false><<<grid, kThreads, lds, st>>>(a, units, turned, (int)tokens, slots, left_first);
 }
 
 template <class T>
@@ -119,11 +145,13 @@ void by_alignment(const AppendArgs& a, hipStream_t st) {
   const auto fits = [](int64_t token, int64_t head, const void* p) {
     return token % 8 == 0 && head % 8 == 0 && (reinterpret_cast<uintptr_t>(p) & 15) == 0;
   };
-  if (a.rotary % 16 == 0 && fits(a.token[0], a.head[0], a.x[0]) && fits(a.token[1], a.head[1], a.x[1]) &&
-      fits(a.v_token, a.v_head, a.v) && (reinterpret_cast<uintptr_t>(a.y[0]) & 15) == 0)
-    launch<T, 8>(a, st);
+  const bool turns_wide = a.rotary % 16 == 0 && fits(a.token[0], a.head[0], a.x[0]) && fits(a.token[1], a.head[1], a.x[1]) &&
+                          (reinterpret_cast<uintptr_t>(a.y[0]) & 15) == 0;
+  const bool left_first = turns_wide && a.adjacent;  // as the rotary kernel's vectors of neighbours
+  if (turns_wide && fits(a.v_token, a.v_head, a.v))
+    launch<T, 8>(a, left_first, st);
   else
-    launch<T, 1>(a, st);
+    launch<T, 1>(a, left_first, st);
 }
 
 }  // namespace

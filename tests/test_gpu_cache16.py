@@ -68,6 +68,25 @@ def test_append_is_rotate_and_write(ops, T, hq, hk, D, rotary_dim, page, adjacen
         assert torch.equal(gk, torch.where(real, keys, 0)) and torch.equal(gv, torch.where(real, v, 0))
 
 
+@pytest.mark.parametrize("adjacent", [False, True])
+@pytest.mark.parametrize("dtype", ["bf16", "fp16"])
+@pytest.mark.parametrize("loose", [0, 1, 2])
+def test_append_with_one_operand_off_alignment(ops, loose, dtype, adjacent):
+    """One of q, k and v begins off 16 bytes: the turns are those of the rotary kernel, whichever way either goes."""
+    T, hq, hk, D = 201, 6, 2, 128
+    g = torch.Generator(device=DEV).manual_seed(loose)
+    rows = [torch.randn(T, h, D + 1, generator=g, device=DEV).to(DTYPES[dtype])[..., 1:] if i == loose else
+            torch.randn(T, h, D, generator=g, device=DEV).to(DTYPES[dtype]) for i, h in enumerate((hq, hk, hk))]
+    plan = ops.rotary.plan(64, theta=1e4, adjacent=adjacent, device=DEV)
+    pos = torch.randint(0, 2 ** 20, (T,), generator=g, device=DEV).int()
+    cache, two = (ops.kv.KVCache.empty(16, hk, page=16, head_dim=D, dtype=DTYPES[dtype], bits=16, device=DEV) for _ in range(2))
+    cache.data.zero_(), two.data.zero_()
+    slots = torch.randperm(256, generator=g, device=DEV)[:T].int()
+    turned, keys = ops.rotary.rotate(rows[0], rows[1], pos, plan)
+    ops.kv.write(two, keys, rows[2], slots)
+    assert torch.equal(ops.kv.append(cache, *rows, pos, plan, slots), turned) and torch.equal(cache.data, two.data)
+
+
 def test_write_changes_its_slots_alone(ops):
     cache = ops.kv.KVCache.empty(9, 3, page=16, head_dim=64, bits=16, device=DEV)
     cache.data.random_(0, 50)
