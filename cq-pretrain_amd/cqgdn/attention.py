@@ -43,8 +43,8 @@ def attend(q, k, v, limit, *, first=None, positions=None, scale=None, cap=None, 
 
     The score of key j is scale q k_j (``scale`` defaults to D^-0.5), capped to cap tanh(score / cap) with ``cap``, less
     ``slopes[h]`` |positions[t] - j| with ``slopes`` (fp32 [Hq], constants; ``positions`` int32 [T] is the key that row t
-    stands at, by default its last one, limit[t] - 1).  With ``return_lse`` also fp32 [T, Hq]: the logarithm of the sum of
-    exp(score), -inf for rows that see nothing.
+    stands at, by default limit[t] - 1; beyond 2^24 either way it counts as that, and S may be 2^24 at most).  With
+    ``return_lse`` also fp32 [T, Hq]: the logarithm of the sum of exp(score), -inf for rows that see nothing.
 
     Scores, sums and results are held in fp32, and each weight, and in the backward pass each score's gradient, is
     rounded once to the rows' type for its product.  A capped score is off by up to 2^-22 of the cap.  Differentiable in

@@ -7,6 +7,11 @@
 // K Q^T and O^T = V^T P^T: a lane owns a row, so limits, maximum, sum and the head's slope are the lane's own and S^T's
 // layout is already an operand of O^T.  Steps that all of a wave's rows see whole, most of them, have no masks.
 //
+// Bound by the MFMAs and, at about as many cycles, the operations on scores that stand between them: 8192 causal tokens and
+// 1024 queries, 16 heads of 128, 361 us, 881 TFLOP/s of the products that the mask leaves; with a cap, three transcendental
+// operations a score, by those (13 documents of up to 4096 tokens, 16 key heads: 750 us), as with heads of 64 (seven
+// documents with a window of 1024: 106 us).
+//
 // Scores, sums and O are fp32; a weight is rounded once to the rows' type for its product with V (half a step of
 // the type times sum p |v| / sum p in a result).
 #include <hip/hip_runtime.h>
@@ -110,7 +115,8 @@ __device__ __forceinline__ void core_tile(const CoreArgs& a, const CorePlace pla
     }
   }
   const Bend bend(a.scale, CAP ? a.cap : 0.f, BIAS ? a.slopes : nullptr, head);
-  const int stands = BIAS && real && r < requests ? (a.positions ? a.positions[t] : a.visible[t] - 1) : 0;
+  int stands = BIAS && real && r < requests ? (a.positions ? a.positions[t] : a.visible[t] - 1) : 0;
+  if (!PAGED) stands = within_reach(stands);
   f32x16 o[MT];
   float m, l;
 
@@ -205,7 +211,7 @@ __device__ __forceinline__ void core_tile(const CoreArgs& a, const CorePlace pla
     x8 kf[F], vf[2][H];
     f32x16 sc[2];
     uint32_t pw[2][8];
-    const float far = (float)(stands - pos - 16 * kg);
+    const float far = (float)__builtin_elementwise_sub_sat(stands, pos + 16 * kg);
     const auto key = [&](int i) { kf[i] = at_tile.rows(kp, i / KQ, i % KQ); };
     const auto value = [&](int u, int i) { vf[u][i] = at_tile.columns(vp, u, i / MT, i % MT); };
 #pragma unroll
@@ -261,7 +267,7 @@ __device__ __forceinline__ void core_tile(const CoreArgs& a, const CorePlace pla
   const auto cut_step = [&](const E* kp, const E* vp, int pos, int shown, auto careful) {
     constexpr bool CAREFUL = decltype(careful)::value;
     const int lo0 = lo - pos - 16 * kg, hi0 = hi - pos - 16 * kg;
-    const float far = (float)(stands - pos - 16 * kg);
+    const float far = (float)__builtin_elementwise_sub_sat(stands, pos + 16 * kg);
     const bool odd = CAREFUL && tile_is_odd<E, D>(vp, lane);
     // one half after the other: a short call's time is that of fetching this code once
 #pragma unroll 1

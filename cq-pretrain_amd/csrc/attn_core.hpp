@@ -64,7 +64,7 @@ struct TileOperands {
 
 // N blocks of a tile on their way: lane l's 16 bytes of `from` + `off` + 64 i (bytes) land at `lds` + 1024 i + 16 l.  In
 // assembly because the compiler, which does not tell the tiles of a pair from each other, puts a wait for all that is on
-// its way before every read of the other one (train_9216's forward pass spent 61% of its time in that wait); tiles_ready()
+// its way before every read of the other one (the forward pass of 9216 rows spent 61% of its time in that wait); tiles_ready()
 // is the wait that is needed.  Nothing is returned in registers.  An instruction's offset moves both addresses.
 template <int N>
 __device__ __forceinline__ void load_blocks(const void* from, uint32_t off, void* lds) {
@@ -93,12 +93,9 @@ template <class E, int D>
 __device__ __forceinline__ void load_rows16(const E* rows, uint32_t offset, E* tile, int wave, int lane) {
   load_blocks<D / 32>(rows, (offset + 8 * (lane & 3)) * sizeof(E), tile + wave * kTileRows16<D>);
 }
-// What the workgroup's waves have asked for has arrived, but for the last LATER instructions of each, and all have read what
-// they wanted.  (Loads of the compiler's own behind those make it wait for more, never for less.)
-template <int LATER = 0>
+// What the workgroup's waves have asked for has arrived, and all have read what they wanted.
 __device__ __forceinline__ void tiles_ready() {
-  static_assert(LATER < 64, "vmcnt is 6 bits");
-  asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(LATER) : "memory");
+  asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
 }
 
 // ---- values that are not finite -----------------------------------------------------------------------
@@ -190,6 +187,11 @@ struct Bend {
     return __builtin_fmaf(2.f * cap, r, more);
   }
 };
+
+// Distances of packed rows are counted in fp32: keys lie below 2^24, and a position beyond it counts as that, so that
+// every kernel has the same distance, not rounded.
+constexpr int kFarthest = 1 << 24;
+__device__ __forceinline__ int within_reach(int position) { return min(max(position, -kFarthest), kFarthest); }
 
 // f with whether scores are capped and whether they are biased, as types
 template <class F>

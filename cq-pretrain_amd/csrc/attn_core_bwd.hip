@@ -6,7 +6,11 @@
 // The weights come again from the scores and the rows' logarithms.  Two kernels, each of which owns what it sums, so
 // that nothing is added atomically and results do not depend on timing: one goes through the keys of 128 rows for dq
 // (S and dP once more than a kernel for all three would form them: 14 D operations a pair of row and key for 10), the
-// other through the rows that see 128 keys for dk and dv, 64 rows a step.
+// other through the rows that see 256 keys for dk and dv, 64 rows a step (attn_core_dkv.hip).
+//
+// The first is bound by the MFMAs and the exponentials that stand between them: 8192 causal tokens and 1024 queries, 16 heads
+// of 128, 486 us, 981 TFLOP/s of its products; with a cap by the operations on scores (13 documents of up to 4096 tokens, 16
+// key heads: 890 us); heads of 256, one wave a SIMD, by its waits (five documents of up to 1531 tokens, 8 heads: 130 us).
 //
 // The first leaves, for every 64 rows, the range of keys they see, their logarithms and deltas: the second finds its
 // steps in those ranges, 64 at a time.  Where its workgroups would not fill the CUs, each takes every n-th of the
@@ -100,7 +104,7 @@ __device__ __forceinline__ bool dq_rows(const CoreGradArgs& a, int tiles, DqTile
   const int row_t = real ? a.group.of(rho) : 0, head = h * group + (real ? rho - row_t * group : 0);
   const int64_t at = (int64_t)row_t * a.heads + head;
   const Bend bend(a.scale, CAP ? a.cap : 0.f, BIAS ? a.slopes : nullptr, head);
-  const int stands = BIAS && real ? (a.positions ? a.positions[row_t] : a.visible[row_t] - 1) : 0;
+  const int stands = BIAS && real ? within_reach(a.positions ? a.positions[row_t] : a.visible[row_t] - 1) : 0;
 
   x8 qf[KQ], yf[KQ];  // lane (n32, kg): q and dy of row n32, dimensions 16 i + 8 kg ..
   float delta = 0.f;

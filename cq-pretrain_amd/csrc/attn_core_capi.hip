@@ -38,8 +38,10 @@ int check_cache16(const void* data, int64_t pages, int kv_heads, int D, int page
 
 int check_scores(int dtype, float scale, float cap) {
   if (!type_ok(dtype)) return fail(CQGDN_EINVAL, "dtype=%d must be CQGDN_BF16 or CQGDN_F16", dtype);
-  if (!finite(scale) || !finite(cap) || cap < 0.f)
-    return fail(CQGDN_EINVAL, "scale=%g and cap=%g must be finite, the cap not negative", (double)scale, (double)cap);
+  // what the kernels hold of them: both, and their quotient, in units of log2 e
+  if (!finite(2.f * 1.45f * scale) || !finite(2.f * 1.45f * cap) || cap < 0.f || (cap > 0.f && !finite(2.f * scale / cap * 1.45f)))
+    return fail(CQGDN_EINVAL, "scale=%g and cap=%g must be finite, and so their quotient, the cap not negative", (double)scale,
+                (double)cap);
   return CQGDN_OK;
 }
 
@@ -54,13 +56,15 @@ size_t part_bytes(int64_t T, int heads, int D, int splits) {
 }
 
 // sizes of packed rows
-int check_packed(int64_t T, int64_t S, int heads, int kv_heads, int D) {
+int check_packed(int64_t T, int64_t S, int heads, int kv_heads, int D, const float* slopes) {
   if (!dim_ok(D)) return fail(CQGDN_EUNSUPPORTED, "head_dim=%d: attention takes 64, 128 and 256", D);
   if (T < 0 || S < 0 || heads <= 0 || kv_heads <= 0 || heads % kv_heads)
     return fail(CQGDN_EINVAL, "invalid sizes T=%lld S=%lld heads=%d kv_heads=%d", (long long)T, (long long)S, heads, kv_heads);
   if (T > (1 << 27) / heads || S > (1 << 27) / kv_heads || heads > 65535)
     return fail(CQGDN_EUNSUPPORTED, "T=%lld rows of %d heads, or S=%lld keys of %d, are too many", (long long)T, heads,
                 (long long)S, kv_heads);
+  if (slopes && S > 1 << 24)
+    return fail(CQGDN_EUNSUPPORTED, "S=%lld keys: distances are counted in fp32, over 2^24 keys at most", (long long)S);
   return CQGDN_OK;
 }
 
@@ -147,13 +151,14 @@ int cqgdn_attend_fwd(const void* q, int64_t q_token, int64_t q_head, const void*
                      int kv_heads, int head_dim, const int32_t* first, const int32_t* limit, const int32_t* positions,
                      float scale, float cap, const float* slopes, void* out, float* lse, void* workspace,
                      size_t workspace_bytes, void* stream) {
-  if (const int e = check_packed(T, S, heads, kv_heads, head_dim)) return e;
+  if (const int e = check_packed(T, S, heads, kv_heads, head_dim, slopes)) return e;
   if (const int e = check_scores(dtype, scale, cap)) return e;
   if (T == 0) return ok();
-  if (!rows_ok(q, q_token, q_head, heads) || (S > 0 && (!rows_ok(k, k_token, k_head, kv_heads) || !rows_ok(v, v_token, v_head, kv_heads))) || !limit ||
-      !out || !aligned(out, 16))
-    return fail(CQGDN_EINVAL, "q, k, v and out (16-byte aligned, strides multiples of 8 elements, not negative, below 2^24 a token and 2^29 all heads) and limit "
-                "must be non-null");
+  if (!rows_ok(q, q_token, q_head, heads) ||
+      (S > 0 && (!rows_ok(k, k_token, k_head, kv_heads) || !rows_ok(v, v_token, v_head, kv_heads))) || !limit || !out ||
+      !aligned(out, 16))
+    return fail(CQGDN_EINVAL, "q, k, v and out (16-byte aligned, strides multiples of 8 elements, not negative, below 2^24 "
+                "a token and 2^29 all heads) and limit must be non-null");
   const int splits = core_parts(T, S, heads, kv_heads, head_dim);
   const size_t need = part_bytes(T, heads, head_dim, splits);
   if (need > 0 && (!workspace || !aligned(workspace, 256) || workspace_bytes < need))
@@ -177,12 +182,13 @@ int cqgdn_attend_bwd(const void* q, int64_t q_token, int64_t q_head, const void*
                      const int32_t* limit, const int32_t* positions, float scale, float cap, const float* slopes,
                      const void* out, const float* lse, const float* dlse, void* dq, void* dk, void* dv,
                      void* workspace, size_t workspace_bytes, void* stream) {
-  if (const int e = check_packed(T, S, heads, kv_heads, head_dim)) return e;
+  if (const int e = check_packed(T, S, heads, kv_heads, head_dim, slopes)) return e;
   if (const int e = check_scores(dtype, scale, cap)) return e;
   if (T == 0 && S == 0) return ok();
-  if ((T > 0 && (!rows_ok(q, q_token, q_head, heads) || !rows_ok(dy, dy_token, dy_head, heads) || !limit || !out || !aligned(out, 16) ||
-                 !lse || !dq || !aligned(dq, 16))) ||
-      (S > 0 && (!rows_ok(k, k_token, k_head, kv_heads) || !rows_ok(v, v_token, v_head, kv_heads) || !dk != !dv || !aligned(dk, 16) || !aligned(dv, 16))))
+  if ((T > 0 && (!rows_ok(q, q_token, q_head, heads) || !rows_ok(dy, dy_token, dy_head, heads) || !limit || !out ||
+                 !aligned(out, 16) || !lse || !dq || !aligned(dq, 16))) ||
+      (S > 0 && (!rows_ok(k, k_token, k_head, kv_heads) || !rows_ok(v, v_token, v_head, kv_heads) || !dk != !dv ||
+                 !aligned(dk, 16) || !aligned(dv, 16))))
     return fail(CQGDN_EINVAL, "q, k, v, dy, out and the gradients (16-byte aligned, strides multiples of 8 elements, "
                 "not negative, below 2^24 a token and 2^29 all heads), limit and lse must be non-null");
   const size_t need = core_backward_bytes(T, S, heads, kv_heads, head_dim);

@@ -47,7 +47,7 @@ const float* floats(const Tensor& x) { return x.defined() ? x.data_ptr<float>() 
 
 void check_scores(double scale, double cap) {
   TORCH_CHECK_VALUE(std::isfinite((float)scale), "scale must be finite");
-  TORCH_CHECK_VALUE(std::isfinite((float)cap) && cap >= 0, "cap must be positive and finite");
+  TORCH_CHECK_VALUE(std::isfinite((float)cap) && cap >= 0 && (cap == 0 || (float)cap > 0), "cap must be positive and finite");
 }
 
 struct Packed {

@@ -499,16 +499,17 @@ int cqgdn_kv16_attend(const void* q, int64_t q_token, int64_t q_head, int dtype,
 /*
  * Attention over packed rows, for training: row t sees the keys first[t] <= j < limit[t] (first NULL: from 0; beyond S
  * there are none), and out[t][h] = sum_j p_j v_j / sum_j p_j with the scores above, distances counted from positions[t]
- * (NULL: limit[t] - 1).  Query head h reads key head h / (heads / kv_heads); rows that see nothing are zero.  Scores,
- * sums and results are held in fp32; each weight is rounded to dtype for its product with v.
+ * (NULL: limit[t] - 1; beyond 2^24 either way it counts as that, and with slopes S is 2^24 at most).  Query head h reads
+ * key head h / (heads / kv_heads); rows that see nothing are zero.  Scores, sums and results are held in fp32; each weight
+ * is rounded to dtype for its product with v.
  *   q, out   : bf16 or fp16 (dtype) [T][heads][head_dim], out dense; k, v: [S][kv_heads][head_dim].  Strides in
  *              elements, multiples of 8, not negative, below 2^24 from token to token and 2^29 over all heads; rows
  *              16-byte aligned
  *   lse      : fp32 [T][heads]: log sum_j exp(u_j), -inf for rows that see nothing; the backward pass reads it (or NULL)
  *   workspace: >= cqgdn_attend_fwd_workspace_size() bytes (it may be 0), 256-byte aligned
  * cqgdn_attend_bwd writes the gradients dq, dk, dv (dense, of dtype) of a loss whose gradients by out and lse are dy
- * and dlse (NULL: 0); dk and dv may both be NULL.  Nothing is added atomically: the same inputs give the same bits.  Keys that no row sees, and rows
- * that see none, get zero.
+ * and dlse (NULL: 0); dk and dv may both be NULL.  Nothing is added atomically: the same inputs give the same bits.  Keys
+ * that no row sees, and rows that see none, get zero.
  */
 size_t cqgdn_attend_fwd_workspace_size(int64_t T, int64_t S, int heads, int kv_heads, int head_dim);
 int cqgdn_attend_fwd(const void* q, int64_t q_token, int64_t q_head, const void* k, int64_t k_token, int64_t k_head,

@@ -47,6 +47,7 @@ def _attend(**kw):
     (dict(scale=1e300), "scale must be finite"),
     (dict(), DEVICE),
     (dict(q=torch.zeros(5, 4, 64, dtype=B, requires_grad=True)), DEVICE),
+    (dict(cap=1e-50), "cap must be positive"),  # 0 in fp32
 ])
 def test_attend_refusals(kw, match):
     with pytest.raises(ValueError, match=match):
@@ -170,20 +171,16 @@ def test_no_gradient_passes_through_the_16_bit_cache():
 
 # ---- the C ABI ---------------------------------------------------------------------------------------
 
-
-
-
-
 def test_workspaces_cover_the_parts():
     lib = _lib.lib()
     assert lib.cqgdn_attend_fwd_workspace_size(0, 5, 4, 2, 64) == lib.cqgdn_attend_fwd_workspace_size(5, 5, 4, 3, 64) == 0
     assert lib.cqgdn_attend_fwd_workspace_size(5, 5, 4, 2, 96) == 0
-    # 32 rows a block: 768 bytes for each key head, 16 for all; blocks by 128 rows
+    # 64 rows a block: 1536 bytes for each key head, 16 for all; blocks by 128 rows
     for T, S, hq, hk, D in ((1, 1, 1, 1, 64), (317, 253, 16, 4, 128), (5000, 700, 7, 1, 256), (40000, 40000, 16, 16, 128)):
-        blocks = -(-T * (hq // hk) // 128) * 4
+        blocks = -(-T * (hq // hk) // 128) * 2
         need = lib.cqgdn_attend_bwd_workspace_size(T, S, hq, hk, D)
-        assert need >= blocks * (768 * hk + 16)
-        rest = need - (blocks * (768 * hk + 16) + 255) // 256 * 256
+        assert need >= blocks * (1536 * hk + 16)
+        rest = need - (blocks * (1536 * hk + 16) + 255) // 256 * 256
         assert rest % (2 * S * hk * D * 4) == 0
     assert lib.cqgdn_kv16_attend_workspace_size(0, 1, 4, 2, 64, 1, 3, 16) == 0
 
@@ -241,3 +238,21 @@ def test_c_abi_refusals():
                    (dict(columns=1000, ts=1000), _lib.EINVAL),  # parts without a workspace
                    (dict(T=0), _lib.OK)):
         assert cached(**kw) == rc, (kw, lib.cqgdn_last_error())
+
+
+@pytest.mark.parametrize("kw,rc", [
+    (dict(cap=1e-39), _lib.EINVAL), (dict(cap=3e38), _lib.EINVAL), (dict(scale=3e38), _lib.EINVAL), (dict(scale=1e20, cap=1e-19), _lib.EINVAL),
+    (dict(S=(1 << 24) + 1, kv=1, slopes=True), _lib.EUNSUPPORTED),
+])
+def test_scores_that_fp32_does_not_hold(kw, rc):
+    lib = _lib.lib()
+    buf = (ctypes.c_char * 4096)()
+    p = (ctypes.addressof(buf) + 255) // 256 * 256
+    if kw.get("slopes"):
+        kw = kw | dict(slopes=p)
+    a = dict(q=p, qt=256, qh=64, k=p, kt=128, kh=64, v=p, vt=128, vh=64, dtype=0, T=2, S=3, heads=4, kv=2, D=64, first=None,
+             limit=p, positions=None, scale=1.0, cap=0.0, slopes=None, out=p, lse=p, ws=None, n=0, stream=None) | kw
+    assert lib.cqgdn_attend_fwd(*a.values()) == rc
+    back = dict(list(a.items())[:9]) | dict(dy=p, yt=256, yh=64) | dict(list(a.items())[9:21]) | dict(
+        out=p, lse=p, dlse=None, dq=p, dk=p, dv=p, ws=p, n=1, stream=None)
+    assert lib.cqgdn_attend_bwd(*back.values()) == rc

@@ -355,3 +355,73 @@ def test_derivatives_that_are_refused(attention):
     b.add_(1)
     with pytest.raises(RuntimeError, match="modified by an inplace operation"):
         torch.autograd.grad(out, a, dy)
+
+
+@pytest.mark.parametrize("D", [64, 256])
+def test_rows_that_stand_far_away(attention, D):
+    """Positions of any size: beyond 2^24 they count as that."""
+    T, S = 150, 130
+    q, k, v, dy = make(T, S, 2, 1, D, "bf16", seed=22)
+    limit = torch.randint(1, S + 1, (T,), generator=torch.Generator().manual_seed(4)).int().to(DEV)
+    where = torch.arange(T, device=DEV).int()
+    where[::3], where[1::7], where[2::11], where[5::13] = 2 ** 31 - 1, -2 ** 31, 2 ** 24 - 3, -2 ** 24 + 1
+    slopes = torch.tensor([2.0 ** -18, -2.0 ** -21], device=DEV)
+    got = run(attention, q, k, v, limit, dy, slopes=slopes, positions=where)
+    compare(got, q, k, v, None, limit, dy, slopes=slopes, positions=where.clamp(-2 ** 24, 2 ** 24))
+
+
+@pytest.mark.parametrize("adjacent", [False, True])
+def test_a_layer_with_rotary_positions(attention, adjacent):
+    """Rows turned, attended, and turned back in the backward pass: what the operators give one after the other, bit for bit,
+    and the attention's part against the plain form."""
+    from cqgdn import rotary
+
+    bounds = [0, 70, 71, 200]
+    first, limit = attention.documents(bounds, prefix=[10, 0, 40], device=DEV)
+    T, hq, hk, D = 200, 8, 2, 128
+    q, k, v, dy = make(T, T, hq, hk, D, "bf16", seed=23)
+    plan = rotary.plan(64, theta=1e5, adjacent=adjacent, device=DEV)
+    positions = torch.cat([torch.arange(b - a) for a, b in zip(bounds, bounds[1:])]).int().to(DEV)
+    a, b, c = (x.clone().requires_grad_() for x in (q, k, v))
+    out = attention.attend(*rotary.rotate(a, b, positions, plan), c, limit, first=first, cap=30.0)
+    grads = torch.autograd.grad(out, (a, b, c), dy)
+    x, y = q.clone().requires_grad_(), k.clone().requires_grad_()
+    turned = rotary.rotate(x, y, positions, plan)
+    part = run(attention, turned[0], turned[1], v, limit, dy, first=first, cap=30.0)
+    compare(part, turned[0].detach(), turned[1].detach(), v, first, limit, dy, cap=30.0)
+    dq, dk = torch.autograd.grad(turned, (x, y), (part["dq"], part["dk"]))
+    assert torch.equal(out, part["out"])
+    assert torch.equal(grads[0], dq) and torch.equal(grads[1], dk) and torch.equal(grads[2], part["dv"])
+
+
+def test_two_calls_at_once(attention):
+    """Calls on two streams that wait for nothing of each other's, in many parts each."""
+    args = []
+    for seed in (24, 25):
+        first, limit, _ = ranges([700, 90], 0, None, False)
+        args.append((make(len(limit), 790, 4, 2, 64, "fp16", seed=seed), first, limit))
+    want = [run(attention, *x[:3], limit, x[3], first=first) for x, first, limit in args]
+    streams = [torch.cuda.Stream() for _ in args]
+    torch.cuda.synchronize()
+    got = [[], []]
+    for _ in range(6):
+        for i, (stream, (x, first, limit)) in enumerate(zip(streams, args)):
+            with torch.cuda.stream(stream):
+                got[i].append(run(attention, *x[:3], limit, x[3], first=first))
+    torch.cuda.synchronize()
+    for w, all_of in zip(want, got):
+        assert all(torch.equal(g[n], w[n]) for g in all_of for n in w)
+
+
+def test_a_leaf_in_every_place(attention):
+    """Queries, keys and values are one tensor: its gradient is the sum of the three."""
+    x, _, _, dy = make(200, 200, 2, 2, 64, "bf16", seed=26)
+    limit = torch.arange(1, 201, dtype=torch.int32, device=DEV)
+    parts = run(attention, x, x, x, limit, dy)
+    compare(parts, x, x, x, None, limit, dy)
+    leaf = x.clone().requires_grad_()
+    attention.attend(leaf, leaf, leaf, limit).backward(dy)
+    total = sum(parts[n].double() for n in ("dq", "dk", "dv"))
+    # two sums in bf16, each rounded, of values no larger than the three magnitudes
+    size = sum(parts[n].double().abs() for n in ("dq", "dk", "dv"))
+    assert bool(((leaf.grad.double() - total).abs() <= 2 * 2 ** -8 * (1 + 2 ** -8) * size).all())
