@@ -123,6 +123,11 @@ __device__ __forceinline__ bool dq_rows(const CoreGradArgs& a, int tiles, DqTile
     }
     delta += __shfl_xor(delta, 32, 64);
   }
+  if (hi - lo == 1 && !a.dlse) {  // dx of an only key is 0: dy.v and delta are one sum, which two orders would not leave 0
+    delta *= 0.f;                 // NaN where they are not finite
+#pragma unroll
+    for (int i = 0; i < KQ; ++i) yf[i] = x8{};
+  }
   if (a.dlse && real) delta -= a.dlse[at];
   const float lse = real ? a.lse[at] * 1.44269504088896341f : 0.f;
   const float base = kWeightBias<E> - lse + bend.cap;

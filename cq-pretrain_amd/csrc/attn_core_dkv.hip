@@ -18,12 +18,23 @@
 namespace cqgdn {
 namespace {
 
-// the workgroup's part of the work, in its shared memory; returns whether it has to be done once more, carefully
+// A row's only key has the weight 1 whatever its score: dx is 0, which two orders of the sum dy.v would not leave.  The
+// kernel for dq has left such rows' delta as 0 (NaN, where it is not finite), unless lse has a gradient.  `dx`: of the lane's
+// key and the rows of the u-th C.
+__device__ __forceinline__ void only_keys(const RowBlock& x, int u, int kg, int key, f32x16& dx) {
+#pragma unroll
+  for (int e = 0; e < 16; ++e) {
+    const int row = c_row(u, e) + 16 * kg;
+    if (x.lo[row] == key && x.hi[row] == key + 1) dx[e] = x.delta[row];
+  }
+}
+
 template <class E, int D>
 struct DkvTiles {
   E vt[4][kTileSize<D>], qt[2][kTileSize<D>], yt[2][kTileSize<D>];
   RowBlock info[2];
 };
+// the workgroup's part of the work, in its shared memory; returns whether it has to be done once more, carefully
 template <class E, int D, bool CAP, bool BIAS, bool CAREFUL>
 __device__ __forceinline__ bool dkv_keys(const CoreGradArgs& a, int blocks, int splits, DkvTiles<E, D>& tiles) {
   typedef typename Vec<E>::x8 x8;
@@ -43,6 +54,8 @@ __device__ __forceinline__ bool dkv_keys(const CoreGradArgs& a, int blocks, int 
   const int part = wave & 1, key = mine + 16 * (n32 >> 2 & 3) + 8 * part + 4 * (n32 >> 4) + (n32 & 3);
   const TileOperands<E, D> at_tile(lane);
   const Bend bend(a.scale, CAP ? a.cap : 0.f, nullptr, 0);
+  // whether a block may have rows of one key: what such a row sees bounds what all see
+  const auto may_be_only = [&](const RowRange& x) { return !a.dlse && x.high - x.low <= 1; };
 
   x8 kf[KQ];  // lane (n32, kg): its key, dimensions 16 i + 8 kg ..
   {
@@ -104,7 +117,7 @@ __device__ __forceinline__ bool dkv_keys(const CoreGradArgs& a, int blocks, int 
       load_blocks<1>(reinterpret_cast<const char*>(from) + wave * size, 16 * lane, reinterpret_cast<char*>(&info[buffer]) + wave * size);
   };
   // A step of 64 rows.  WHOLE: all of them see all of the wave's keys.
-  const auto step = [&](const E* qp, const E* yp, const RowBlock& x, auto whole) {
+  const auto step = [&](const E* qp, const E* yp, const RowBlock& x, auto whole, bool only) {
     constexpr bool WHOLE = decltype(whole)::value, APART = CAREFUL && !WHOLE;
     // operands read from LDS ahead of their use, of one and of two an MFMA: as many as leave nothing spilled
     constexpr int kEarly = !WHOLE ? 1 : CAP ? 2 : 3, kEarlyPair = WHOLE && !CAP ? 2 : 1;
@@ -220,6 +233,7 @@ __device__ __forceinline__ bool dkv_keys(const CoreGradArgs& a, int blocks, int 
           __builtin_amdgcn_sched_barrier(0);
         }
       }
+      if (!WHOLE && only) only_keys(x, u, kg, key, dp);
       range.fit(dp, dk);
 #pragma unroll
       for (int b = 0; b < 2; ++b) {
@@ -269,12 +283,12 @@ __device__ __forceinline__ bool dkv_keys(const CoreGradArgs& a, int blocks, int 
 #pragma unroll 1
     while (block >= 0 && now.low <= mine && mine + 64 <= now.high) {
       ask();
-      step(qt[buffer], yt[buffer], info[buffer], std::true_type{});
+      step(qt[buffer], yt[buffer], info[buffer], std::true_type{}, false);
       advance();
     }
     if (block < 0) break;
     ask();
-    if (now.last > mine && now.first < mine + 64) step(qt[buffer], yt[buffer], info[buffer], std::false_type{});
+    if (now.last > mine && now.first < mine + 64) step(qt[buffer], yt[buffer], info[buffer], std::false_type{}, may_be_only(now));
     advance();
   }
   if constexpr (!CAREFUL) {
@@ -346,6 +360,8 @@ __device__ __forceinline__ bool pair_keys(const CoreGradArgs& a, int blocks, int
   const bool real = key < a.S;
   const TileOperands<E, D> at_tile(lane);
   const Bend bend(a.scale, CAP ? a.cap : 0.f, nullptr, 0);
+  // whether a block may have rows of one key: what such a row sees bounds what all see
+  const auto may_be_only = [&](const RowRange& x) { return !a.dlse && x.high - x.low <= 1; };
 
   x8 kf[KQ];  // lane (n32, kg): of key n32 K, in the second wave V, dimensions 16 i + 8 kg ..
   {
@@ -430,7 +446,8 @@ __device__ __forceinline__ bool pair_keys(const CoreGradArgs& a, int blocks, int
     dp = half ? sc : other;
     sc = half ? other : sc;
   };
-  const auto sums = [&](const E* qp, const E* yp, const RowBlock& x, int u, f32x16& sc, f32x16& dp, auto whole) {
+  const auto sums = [&](const E* qp, const E* yp, const RowBlock& x, int u, f32x16& sc, f32x16& dp, auto whole,
+                        bool only) {
     constexpr bool WHOLE = decltype(whole)::value, APART = CAREFUL && !WHOLE;
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
@@ -454,6 +471,7 @@ __device__ __forceinline__ bool pair_keys(const CoreGradArgs& a, int blocks, int
         dp[e] = dx;
       }
     }
+    if (!WHOLE && only) only_keys(x, u, kg, key, dp);
     range.fit(dp, dk);
 #pragma unroll
     for (int b = 0; b < 2; ++b) {
@@ -475,7 +493,7 @@ __device__ __forceinline__ bool pair_keys(const CoreGradArgs& a, int blocks, int
       }
     }
   };
-  const auto step = [&](const E* qp, const E* yp, const RowBlock& x, auto whole) {
+  const auto step = [&](const E* qp, const E* yp, const RowBlock& x, auto whole, bool only) {
     constexpr bool WHOLE = decltype(whole)::value, APART = CAREFUL && !WHOLE;
     f32x16 sc[2], dp[2];
 #pragma unroll
@@ -488,7 +506,7 @@ __device__ __forceinline__ bool pair_keys(const CoreGradArgs& a, int blocks, int
     lds_barrier();
     take(sc[1], dp[1]);
 #pragma unroll
-    for (int u = 0; u < 2; ++u) sums(qp, yp, x, u, sc[u], dp[u], whole);
+    for (int u = 0; u < 2; ++u) sums(qp, yp, x, u, sc[u], dp[u], whole, only);
     if (APART && (tile_is_odd<E, D>(qp, lane) || tile_is_odd<E, D>(yp, lane))) {
       const auto sees = [&](int i) { return key >= x.lo[i] && key < x.hi[i]; };
       add_odd<E, D>(qp, dk, lane, sees, half * MT);
@@ -515,12 +533,12 @@ __device__ __forceinline__ bool pair_keys(const CoreGradArgs& a, int blocks, int
 #pragma unroll 1
     while (block >= 0 && now.low <= mine && mine + 32 <= now.high) {
       ask();
-      step(qt[buffer], yt[buffer], info[buffer], std::true_type{});
+      step(qt[buffer], yt[buffer], info[buffer], std::true_type{}, false);
       advance();
     }
     if (block < 0) break;
     ask();
-    step(qt[buffer], yt[buffer], info[buffer], std::false_type{});
+    step(qt[buffer], yt[buffer], info[buffer], std::false_type{}, may_be_only(now));
     advance();
   }
   if constexpr (!CAREFUL) {

@@ -425,3 +425,22 @@ def test_a_leaf_in_every_place(attention):
     # two sums in bf16, each rounded, of values no larger than the three magnitudes
     size = sum(parts[n].double().abs() for n in ("dq", "dk", "dv"))
     assert bool(((leaf.grad.double() - total).abs() <= 2 * 2 ** -8 * (1 + 2 ** -8) * size).all())
+
+
+@pytest.mark.parametrize("D", [64, 128, 256])
+@pytest.mark.parametrize("dtype", ["bf16", "fp16"])
+def test_rows_of_one_key_move_no_score(attention, dtype, D):
+    """The weight of a row's only key is 1 whatever its score: the gradients of q and k are 0, or the gradient of the
+    logarithm's alone.  Values that are not finite still show."""
+    T = 90
+    q, k, v, dy = make(T, T, 4, 2, D, dtype, seed=27)
+    first = torch.arange(T, dtype=torch.int32, device=DEV)
+    got = run(attention, q, k, v, first + 1, dy, first=first, cap=20.0)
+    assert not bool(got["dq"].any()) and not bool(got["dk"].any()) and torch.equal(got["out"][:, ::2], v)
+    compare(got, q, k, v, first, first + 1, dy, cap=20.0)
+    dlse = torch.randn(T, 4, device=DEV)
+    compare(run(attention, q, k, v, first + 1, dy, dlse, first=first), q, k, v, first, first + 1, dy, dlse)
+    dy[7, 1, 3] = math.inf
+    got = run(attention, q, k, v, first + 1, dy, first=first)
+    assert bool(got["dq"][7, 1].isnan().all()) and bool(got["dk"][7, 0].isnan().all())
+    assert not bool(got["dq"][:7].any()) and not bool(got["dk"][8:].any()) and bool(got["dv"][8:].isfinite().all())
