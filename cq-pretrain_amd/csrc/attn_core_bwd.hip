@@ -16,7 +16,8 @@
 // steps in those ranges, 64 at a time.  Where its workgroups would not fill the CUs, each takes every n-th of the
 // steps, and fp32 parts are added up by a third kernel in their order.
 //
-// Scores, products, sums are fp32.  p and dx are rounded once to the rows' type for the second products.  In fp16, where
+// Scores, products, sums are fp32.  p and dx are rounded once to the rows' type for the second products (dx to two terms
+// where a mask cuts a step).  In fp16, where
 // a dx may be too small or too large for the type, it goes in times a power of two that follows the largest so far (of
 // the row, or of the key), and p times 2^15.
 #include <hip/hip_runtime.h>
@@ -184,14 +185,19 @@ __device__ __forceinline__ bool dq_rows(const CoreGradArgs& a, int tiles, DqTile
       range.fit(dp, acc);
 #pragma unroll
       for (int b = 0; b < 2; ++b) {
-        u32x4 w;
+        u32x4 w, rest;
 #pragma unroll
-        for (int e = 0; e < 4; ++e) w[e] = pack2<E>(dp[8 * b + 2 * e] * range.f, dp[8 * b + 2 * e + 1] * range.f);
+        for (int e = 0; e < 4; ++e) {
+          const float x = dp[8 * b + 2 * e] * range.f, y = dp[8 * b + 2 * e + 1] * range.f;
+          w[e] = pack2<E>(x, y);
+          if constexpr (kTwoTerms<E, WHOLE>) rest[e] = rest2<E>(x, y, w[e]);
+        }
 #pragma unroll
         for (int m = 0; m < MT; ++m) {
           x8 k = at_tile.columns(kp, u, b, m);
           if (APART) k = finite_values<E>(k);
           acc[m] = mfma32(k, __builtin_bit_cast(x8, w), acc[m]);
+          if constexpr (kTwoTerms<E, WHOLE>) acc[m] = mfma32(k, __builtin_bit_cast(x8, rest), acc[m]);
         }
       }
     }

@@ -237,14 +237,19 @@ __device__ __forceinline__ bool dkv_keys(const CoreGradArgs& a, int blocks, int 
       range.fit(dp, dk);
 #pragma unroll
       for (int b = 0; b < 2; ++b) {
-        u32x4 w;
+        u32x4 w, rest;
 #pragma unroll
-        for (int e = 0; e < 4; ++e) w[e] = pack2<E>(dp[8 * b + 2 * e] * range.f, dp[8 * b + 2 * e + 1] * range.f);
+        for (int e = 0; e < 4; ++e) {
+          const float x = dp[8 * b + 2 * e] * range.f, y = dp[8 * b + 2 * e + 1] * range.f;
+          w[e] = pack2<E>(x, y);
+          if constexpr (kTwoTerms<E, WHOLE>) rest[e] = rest2<E>(x, y, w[e]);
+        }
 #pragma unroll
         for (int m = 0; m < MT; ++m) {
           const int i = b * MT + m;
           if (i + kEarly < 2 * MT) qc[i + kEarly] = column(qp, i + kEarly);
           dk[m] = mfma32(qc[i], __builtin_bit_cast(x8, w), dk[m]);
+          if constexpr (kTwoTerms<E, WHOLE>) dk[m] = mfma32(qc[i], __builtin_bit_cast(x8, rest), dk[m]);
           __builtin_amdgcn_sched_barrier(0);
         }
       }
@@ -475,11 +480,13 @@ __device__ __forceinline__ bool pair_keys(const CoreGradArgs& a, int blocks, int
     range.fit(dp, dk);
 #pragma unroll
     for (int b = 0; b < 2; ++b) {
-      u32x4 w, z;
+      u32x4 w, z, rest;
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
+        const float one = dp[8 * b + 2 * e] * range.f, two = dp[8 * b + 2 * e + 1] * range.f;
         w[e] = pack2<E>(sc[8 * b + 2 * e], sc[8 * b + 2 * e + 1]);
-        z[e] = pack2<E>(dp[8 * b + 2 * e] * range.f, dp[8 * b + 2 * e + 1] * range.f);
+        z[e] = pack2<E>(one, two);
+        if constexpr (kTwoTerms<E, WHOLE>) rest[e] = rest2<E>(one, two, z[e]);
       }
 #pragma unroll
       for (int m = 0; m < MT; ++m) {
@@ -490,6 +497,7 @@ __device__ __forceinline__ bool pair_keys(const CoreGradArgs& a, int blocks, int
         }
         dv[m] = mfma32(y, __builtin_bit_cast(x8, w), dv[m]);
         dk[m] = mfma32(q, __builtin_bit_cast(x8, z), dk[m]);
+        if constexpr (kTwoTerms<E, WHOLE>) dk[m] = mfma32(q, __builtin_bit_cast(x8, rest), dk[m]);
       }
     }
   };

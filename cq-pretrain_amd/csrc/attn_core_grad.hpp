@@ -20,6 +20,18 @@ __device__ __forceinline__ uint32_t pack2(float x, float y) {
   return __builtin_bit_cast(uint32_t, __builtin_convertvector(f32x2{x, y}, x2));
 }
 
+// dx goes into its product in two bf16 terms, 2^-17 of it, where a mask cuts a step: there lie the rows that see few keys,
+// whose dx and gradients are many times those of the others (in 9216 causal rows 2^-9 of the first rows' dx is up to 0.45
+// times the root mean square of dq).  In fp16 one term is 2^-12.  (9216 rows: 2% of the gradients' time.)
+template <class E, bool WHOLE>
+constexpr bool kTwoTerms = !WHOLE && !std::is_same<E, f16>::value;
+// what pack2(x, y) = w leaves of x and y
+template <class E>
+__device__ __forceinline__ uint32_t rest2(float x, float y, uint32_t w) {
+  const float a = x - __builtin_bit_cast(float, w << 16), b = y - __builtin_bit_cast(float, w & 0xFFFF0000u);
+  return pack2<E>(a - a == 0.f ? a : 0.f, b - b == 0.f ? b : 0.f);
+}
+
 // The power of two that a lane's dx go with in fp16 (bf16: 1): the largest lies near 2^10 when it is set, and below
 // 2^15 always.  The two lanes of a column share it.
 template <class E>

@@ -9,7 +9,7 @@ The smallest weights are lost: bf16's, and fp32's, exponents end at 2^-126; in f
 2^-25, of weights held 2^7 times as large as the row's largest one's 1 (2^15 times in the backward pass), so a weight is
 off by that much (`floor`) beside.  A dx below 2^-126 is lost likewise.
 In the backward pass delta = dy.out takes the rounded out: off by at most E = sum |dy| u (A + |out|).  dx = p (dp - delta) is
-rounded once: off by u |dx| + p E + moved p (|dp| + |delta|).  A gradient is the sum of those, times |k| or |q|, and rounded."""
+rounded to one term (or `terms`): off by u |dx| (u^terms) + p E + moved p (|dp| + |delta|).  A gradient is the sum of those, times |k| or |q|, and rounded."""
 
 import math
 
@@ -33,7 +33,7 @@ def scores(q, k, scale, cap, slope, distance, seen):
     return x.masked_fill(~seen, -math.inf), rate, torch.where(seen, moved, 0.0)
 
 
-def attend_ref(q, k, v, first, limit, *, scale, cap=None, slopes=None, positions=None, dy=None, dlse=None, seen=None):
+def attend_ref(q, k, v, first, limit, *, scale, cap=None, slopes=None, positions=None, dy=None, dlse=None, seen=None, terms=1):
     """Attention and its gradients in float64, each with its tolerance (but for the results' own rounding)."""
     T, hq, D = q.shape
     S, hk, _ = k.shape
@@ -71,7 +71,7 @@ def attend_ref(q, k, v, first, limit, *, scale, cap=None, slopes=None, positions
         reach = torch.matmul(y.abs(), c.abs().t()) + (y * r["out"][:, h]).abs().sum(-1, keepdim=True)
         dx = p * (dp - delta + more) * rate
         # the fp32 sums dp and delta, and the cap's derivative, 4 r (1 - r), whose parts are off by 2^-22 each
-        dx_off = u * dx.abs() + there * 2 ** -126 * (1 + reach + abs(more)) + p * (around + (off + (2 * D + 8) * 2 ** -24) * (reach + abs(more)) +
+        dx_off = u ** terms * dx.abs() + there * 2 ** -126 * (1 + reach + abs(more)) + p * (around + (off + (2 * D + 8) * 2 ** -24) * (reach + abs(more)) +
                                      (2 ** -20 if cap else 0) * (dp - delta + more).abs())
         tiny = 2.0 ** -24 * (dx.abs().amax() if dx.numel() else 0)  # fp16: what its power of two leaves of the smallest
         dx_off = torch.where(seen, dx_off + tiny * 2 ** -8, 0.0) if q.dtype == torch.float16 else dx_off

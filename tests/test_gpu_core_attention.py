@@ -444,3 +444,14 @@ def test_rows_of_one_key_move_no_score(attention, dtype, D):
     got = run(attention, q, k, v, first + 1, dy, first=first)
     assert bool(got["dq"][7, 1].isnan().all()) and bool(got["dk"][7, 0].isnan().all())
     assert not bool(got["dq"][:7].any()) and not bool(got["dk"][8:].any()) and bool(got["dv"][8:].isfinite().all())
+
+
+@pytest.mark.parametrize("D", [64, 128, 256])
+@pytest.mark.parametrize("cap", [None, 20.0])
+def test_rows_of_few_keys_are_held_in_two_terms(attention, D, cap):
+    """Causal rows of 63 tokens, every step of which the mask cuts: no score's gradient is rounded to one bf16 term."""
+    docs = [63, 5, 2, 40]
+    first, limit, _ = ranges(docs, 0, None, False)
+    q, k, v, dy = make(sum(docs), sum(docs), 4, 2, D, "bf16", seed=28, size=1.5)
+    got = run(attention, q, k, v, limit, dy, first=first, cap=cap)
+    compare({n: got[n] for n in ("dq", "dk")}, q, k, v, first, limit, dy, cap=cap, terms=2)
