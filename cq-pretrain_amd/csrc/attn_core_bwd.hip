@@ -30,6 +30,8 @@
 namespace cqgdn {
 namespace {
 
+constexpr int kFewKeys = 64;  // rows that see no more have their delta made of the keys' own
+
 template <class E, int D>
 struct DqTiles {
   E kt[2][kTileSize<D>], vt[2][kTileSize<D>];
@@ -57,20 +59,28 @@ __device__ __forceinline__ bool dq_rows(const CoreGradArgs& a, int tiles, DqTile
     hi = rho < rows ? min(a.visible[t], a.S) : 0;
     if (lo >= hi) lo = hi = 0;
   };
-  int first, last;
+  // the keys that any of the workgroup's rows sees, and that any of its rows of few keys does
+  int first, last, few_first, few_last;
   {
     int lo0, hi0, lo1, hi1;
     limits(tile * kGradRows + lane, lo0, hi0);
     limits(tile * kGradRows + 64 + lane, lo1, hi1);
+    const bool few0 = hi0 > 0 && hi0 - lo0 <= kFewKeys, few1 = hi1 > 0 && hi1 - lo1 <= kFewKeys;
     first = min(hi0 > 0 ? lo0 : INT32_MAX, hi1 > 0 ? lo1 : INT32_MAX);
     last = max(hi0, hi1);
+    few_first = min(few0 ? lo0 : INT32_MAX, few1 ? lo1 : INT32_MAX);
+    few_last = max(few0 ? hi0 : 0, few1 ? hi1 : 0);
 #pragma unroll
     for (int o = 1; o < 64; o <<= 1) {
       first = min(first, __shfl_xor(first, o, 64));
       last = max(last, __shfl_xor(last, o, 64));
+      few_first = min(few_first, __shfl_xor(few_first, o, 64));
+      few_last = max(few_last, __shfl_xor(few_last, o, 64));
     }
     first = __builtin_amdgcn_readfirstlane(first);
     last = __builtin_amdgcn_readfirstlane(last);
+    few_first = __builtin_amdgcn_readfirstlane(few_first);
+    few_last = __builtin_amdgcn_readfirstlane(few_last);
   }
   const int rho = tile * kGradRows + 32 * wave + n32;
   const bool real = rho < rows;
@@ -124,14 +134,55 @@ __device__ __forceinline__ bool dq_rows(const CoreGradArgs& a, int tiles, DqTile
     }
     delta += __shfl_xor(delta, 32, 64);
   }
+  const float lse = real ? a.lse[at] * 1.44269504088896341f : 0.f;
+  const float base = kWeightBias<E> - lse + bend.cap;
+  const auto stage = [&](int j) {
+    const int pos = first + j * TOK;
+    // rows behind the last key: that key once more
+    const uint32_t row = min(16 * wave + lane / 4, a.S - 1 - pos);
+    load_rows16<E, D>(static_cast<const E*>(a.k) + h * a.k_head + pos * a.k_token, row * (uint32_t)a.k_token, kt[j & 1], wave, lane);
+    load_rows16<E, D>(static_cast<const E*>(a.v) + h * a.v_head + pos * a.v_token, row * (uint32_t)a.v_token, vt[j & 1], wave, lane);
+  };
+  // Rows of few keys: delta as sum_j p_j dy.v_j, which the rounding of out has no part in.  Their dx are large, and of a
+  // delta that is off every dx of the row is.
+  if (few_last > 0) {
+    float sum = 0.f;
+#pragma unroll 1
+    for (int j = (few_first - first) / TOK; first + j * TOK < few_last; ++j) {
+      stage(j);
+      tiles_ready();
+      const int pos = first + j * TOK;
+      if (pos < most && pos + TOK > some) {
+        const int lo0 = lo - pos - 16 * kg, hi0 = hi - pos - 16 * kg;
+        const float far = BIAS ? (float)(stands - pos - 16 * kg) : 0.f;
+#pragma unroll 1
+        for (int u = 0; u < 2; ++u) {
+          f32x16 sc = f32x16{}, dp = f32x16{};
+#pragma unroll
+          for (int i = 0; i < KQ; ++i) {
+            sc = mfma32(at_tile.rows(kt[j & 1], u, i), qf[i], sc);
+            dp = mfma32(at_tile.rows(vt[j & 1], u, i), yf[i], dp);
+          }
+#pragma unroll
+          for (int e = 0; e < 16; ++e) {
+            float x = CAP ? bend.capped(sc[e], bend.cap - lse) : __builtin_fmaf(sc[e], bend.c, -lse);
+            if constexpr (BIAS) x = __builtin_fmaf(-bend.slope, fabsf(far - (float)c_row(u, e)), x);
+            const int at = c_row(u, e);
+            if ((int)(at >= lo0) & (int)(at < hi0)) sum = __builtin_fmaf(__builtin_amdgcn_exp2f(x), dp[e], sum);
+          }
+        }
+      }
+      tiles_ready();
+    }
+    sum += __shfl_xor(sum, 32, 64);
+    if (hi - lo <= kFewKeys) delta = sum;
+  }
   if (hi - lo == 1 && !a.dlse) {  // dx of an only key is 0: dy.v and delta are one sum, which two orders would not leave 0
     delta *= 0.f;                 // NaN where they are not finite
 #pragma unroll
     for (int i = 0; i < KQ; ++i) yf[i] = x8{};
   }
   if (a.dlse && real) delta -= a.dlse[at];
-  const float lse = real ? a.lse[at] * 1.44269504088896341f : 0.f;
-  const float base = kWeightBias<E> - lse + bend.cap;
   {
     RowBlock& x = static_cast<RowBlock*>(a.blocks)[(int64_t)h * tiles * (kGradRows / kTile) + block];
     const int n = 32 * (wave & 1) + n32;
@@ -150,13 +201,6 @@ __device__ __forceinline__ bool dq_rows(const CoreGradArgs& a, int tiles, DqTile
   f32x16 acc[MT];
   Range<E> range;
 
-  const auto stage = [&](int j) {
-    const int pos = first + j * TOK;
-    // rows behind the last key: that key once more
-    const uint32_t row = min(16 * wave + lane / 4, a.S - 1 - pos);
-    load_rows16<E, D>(static_cast<const E*>(a.k) + h * a.k_head + pos * a.k_token, row * (uint32_t)a.k_token, kt[j & 1], wave, lane);
-    load_rows16<E, D>(static_cast<const E*>(a.v) + h * a.v_head + pos * a.v_token, row * (uint32_t)a.v_token, vt[j & 1], wave, lane);
-  };
   const auto step = [&](const E* kp, const E* vp, int pos, auto whole) {
     constexpr bool WHOLE = decltype(whole)::value, APART = CAREFUL && !WHOLE;
     const bool odd = APART && tile_is_odd<E, D>(kp, lane);
