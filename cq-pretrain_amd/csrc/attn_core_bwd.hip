@@ -9,8 +9,8 @@
 // other through the rows that see 256 keys for dk and dv, 64 rows a step (attn_core_dkv.hip).
 //
 // The first is bound by the MFMAs and the exponentials that stand between them: 8192 causal tokens and 1024 queries, 16 heads
-// of 128, 486 us, 981 TFLOP/s of its products; with a cap by the operations on scores (13 documents of up to 4096 tokens, 16
-// key heads: 890 us); heads of 256, one wave a SIMD, by its waits (five documents of up to 1531 tokens, 8 heads: 130 us).
+// of 128, 486 us before S and dP were formed twice; with a cap by the operations on scores (13 documents of up to 4096 tokens, 16
+// key heads: 890 us before); heads of 256, one wave a SIMD, by its waits (five documents of up to 1531 tokens, 8 heads: 130 us).
 //
 // The first leaves, for every 64 rows, the range of keys they see, their logarithms and deltas: the second finds its
 // steps in those ranges, 64 at a time.  Where its workgroups would not fill the CUs, each takes every n-th of the
@@ -29,8 +29,6 @@
 
 namespace cqgdn {
 namespace {
-
-constexpr int kFewKeys = 64;  // rows that see no more have their delta made of the keys' own
 
 template <class E, int D>
 struct DqTiles {
@@ -59,28 +57,20 @@ __device__ __forceinline__ bool dq_rows(const CoreGradArgs& a, int tiles, DqTile
     hi = rho < rows ? min(a.visible[t], a.S) : 0;
     if (lo >= hi) lo = hi = 0;
   };
-  // the keys that any of the workgroup's rows sees, and that any of its rows of few keys does
-  int first, last, few_first, few_last;
+  int first, last;  // the keys that any of the workgroup's rows sees
   {
     int lo0, hi0, lo1, hi1;
     limits(tile * kGradRows + lane, lo0, hi0);
     limits(tile * kGradRows + 64 + lane, lo1, hi1);
-    const bool few0 = hi0 > 0 && hi0 - lo0 <= kFewKeys, few1 = hi1 > 0 && hi1 - lo1 <= kFewKeys;
     first = min(hi0 > 0 ? lo0 : INT32_MAX, hi1 > 0 ? lo1 : INT32_MAX);
     last = max(hi0, hi1);
-    few_first = min(few0 ? lo0 : INT32_MAX, few1 ? lo1 : INT32_MAX);
-    few_last = max(few0 ? hi0 : 0, few1 ? hi1 : 0);
 #pragma unroll
     for (int o = 1; o < 64; o <<= 1) {
       first = min(first, __shfl_xor(first, o, 64));
       last = max(last, __shfl_xor(last, o, 64));
-      few_first = min(few_first, __shfl_xor(few_first, o, 64));
-      few_last = max(few_last, __shfl_xor(few_last, o, 64));
     }
     first = __builtin_amdgcn_readfirstlane(first);
     last = __builtin_amdgcn_readfirstlane(last);
-    few_first = __builtin_amdgcn_readfirstlane(few_first);
-    few_last = __builtin_amdgcn_readfirstlane(few_last);
   }
   const int rho = tile * kGradRows + 32 * wave + n32;
   const bool real = rho < rows;
@@ -143,12 +133,13 @@ __device__ __forceinline__ bool dq_rows(const CoreGradArgs& a, int tiles, DqTile
     load_rows16<E, D>(static_cast<const E*>(a.k) + h * a.k_head + pos * a.k_token, row * (uint32_t)a.k_token, kt[j & 1], wave, lane);
     load_rows16<E, D>(static_cast<const E*>(a.v) + h * a.v_head + pos * a.v_token, row * (uint32_t)a.v_token, vt[j & 1], wave, lane);
   };
-  // Rows of few keys: delta as sum_j p_j dy.v_j, which the rounding of out has no part in.  Their dx are large, and of a
-  // delta that is off every dx of the row is.
-  if (few_last > 0) {
+  // In bf16 delta is sum_j p_j dy.v_j, in which the rounding of out has no part: by a delta that is off every dx of the row is
+  // off alike, and keys that have something in common (a dimension far from 0) add that up (9216 rows of such keys: dq off
+  // by up to 0.45 times its root mean square with dy.out).  It costs S and dP once more: both passes 1350 -> 1800 us there.
+  if constexpr (!std::is_same<E, f16>::value) {
     float sum = 0.f;
 #pragma unroll 1
-    for (int j = (few_first - first) / TOK; first + j * TOK < few_last; ++j) {
+    for (int j = 0; first + (int64_t)j * TOK < last; ++j) {
       stage(j);
       tiles_ready();
       const int pos = first + j * TOK;
@@ -175,7 +166,7 @@ __device__ __forceinline__ bool dq_rows(const CoreGradArgs& a, int tiles, DqTile
       tiles_ready();
     }
     sum += __shfl_xor(sum, 32, 64);
-    if (hi - lo <= kFewKeys) delta = sum;
+    delta = sum;
   }
   if (hi - lo == 1 && !a.dlse) {  // dx of an only key is 0: dy.v and delta are one sum, which two orders would not leave 0
     delta *= 0.f;                 // NaN where they are not finite
