@@ -204,7 +204,7 @@ void by_scores(const CoreArgs& a, F f) {
 
 // What the keys' gradients need of 64 rows of a key head, as the queries' gradients leave it.
 struct RowBlock {
-  float lse[64], delta[64];     // cap less log2 sum of exp2, and less dy.out plus the gradient of lse: what is added
+  float lse[64], delta[64];     // cap less log2 sum of exp2, and the gradient of lse less sum p dy.v: what is added
   int lo[64], hi[64];           // the keys that the row sees
   float stands[64], slope[64];  // with a bias: the row's position, its head's slope times log2 e
 };

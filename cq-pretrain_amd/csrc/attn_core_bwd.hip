@@ -1,6 +1,6 @@
 // Gradients of the attention over packed rows.
 //
-// With p the softmax's weights of row t, dy its output's gradient and delta = dy.y (less the gradient of lse):
+// With p the softmax's weights of row t, dy its output's gradient and delta = sum_j p_j dy.v_j (less the gradient of lse):
 //   dv_j = sum_t p_tj dy_t,  du_tj = p_tj (dy_t.v_j - delta_t),  dx = du times the cap's derivative,
 //   dq_t = scale sum_j dx_tj k_j,  dk_j = scale sum_t dx_tj q_t.
 // The weights come again from the scores and the rows' logarithms.  Two kernels, each of which owns what it sums, so
@@ -108,21 +108,15 @@ __device__ __forceinline__ bool dq_rows(const CoreGradArgs& a, int tiles, DqTile
   const int stands = BIAS && real ? within_reach(a.positions ? a.positions[row_t] : a.visible[row_t] - 1) : 0;
 
   x8 qf[KQ], yf[KQ];  // lane (n32, kg): q and dy of row n32, dimensions 16 i + 8 kg ..
-  float delta = 0.f;
   {
     const E* q = static_cast<const E*>(a.q) + row_t * a.q_token + head * a.q_head + 8 * kg;
     const E* dy = static_cast<const E*>(a.dy) + row_t * a.dy_token + head * a.dy_head + 8 * kg;
-    const E* y = static_cast<const E*>(a.y) + at * D + 8 * kg;
     const u32x4 none{0, 0, 0, 0};
 #pragma unroll
     for (int i = 0; i < KQ; ++i) {
       qf[i] = __builtin_bit_cast(x8, real ? *reinterpret_cast<const u32x4*>(q + 16 * i) : none);
       yf[i] = __builtin_bit_cast(x8, real ? *reinterpret_cast<const u32x4*>(dy + 16 * i) : none);
-      const f32x8 z = cvtf8(__builtin_bit_cast(x8, real ? *reinterpret_cast<const u32x4*>(y + 16 * i) : none)), w = cvtf8(yf[i]);
-#pragma unroll
-      for (int e = 0; e < 8; ++e) delta = __builtin_fmaf(z[e], w[e], delta);
     }
-    delta += __shfl_xor(delta, 32, 64);
   }
   const float lse = real ? a.lse[at] * 1.44269504088896341f : 0.f;
   const float base = kWeightBias<E> - lse + bend.cap;
@@ -133,41 +127,39 @@ __device__ __forceinline__ bool dq_rows(const CoreGradArgs& a, int tiles, DqTile
     load_rows16<E, D>(static_cast<const E*>(a.k) + h * a.k_head + pos * a.k_token, row * (uint32_t)a.k_token, kt[j & 1], wave, lane);
     load_rows16<E, D>(static_cast<const E*>(a.v) + h * a.v_head + pos * a.v_token, row * (uint32_t)a.v_token, vt[j & 1], wave, lane);
   };
-  // In bf16 delta is sum_j p_j dy.v_j, in which the rounding of out has no part: by a delta that is off every dx of the row is
-  // off alike, and keys that have something in common (a dimension far from 0) add that up (9216 rows of such keys: dq off
-  // by up to 0.45 times its root mean square with dy.out).  It costs S and dP once more: both passes 1350 -> 1800 us there.
-  if constexpr (!std::is_same<E, f16>::value) {
-    float sum = 0.f;
+  // delta is formed from the keys and not as dy.out, in which out is rounded: by a delta that is off every dx of the row is
+  // off alike, and keys that have something in common (a dimension far from 0) add that up (9216 rows of such keys in bf16:
+  // dq off by up to 0.45 times its root mean square with dy.out; in fp16 by an eighth of it).  It costs S and dP once more:
+  // both passes 1350 -> 1800 us there.
+  float delta = 0.f;
 #pragma unroll 1
-    for (int j = 0; first + (int64_t)j * TOK < last; ++j) {
-      stage(j);
-      tiles_ready();
-      const int pos = first + j * TOK;
-      if (pos < most && pos + TOK > some) {
-        const int lo0 = lo - pos - 16 * kg, hi0 = hi - pos - 16 * kg;
-        const float far = BIAS ? (float)(stands - pos - 16 * kg) : 0.f;
+  for (int j = 0; first + (int64_t)j * TOK < last; ++j) {
+    stage(j);
+    tiles_ready();
+    const int pos = first + j * TOK;
+    if (pos < most && pos + TOK > some) {
+      const int lo0 = lo - pos - 16 * kg, hi0 = hi - pos - 16 * kg;
+      const float far = BIAS ? (float)(stands - pos - 16 * kg) : 0.f;
 #pragma unroll 1
-        for (int u = 0; u < 2; ++u) {
-          f32x16 sc = f32x16{}, dp = f32x16{};
+      for (int u = 0; u < 2; ++u) {
+        f32x16 sc = f32x16{}, dp = f32x16{};
 #pragma unroll
-          for (int i = 0; i < KQ; ++i) {
-            sc = mfma32(at_tile.rows(kt[j & 1], u, i), qf[i], sc);
-            dp = mfma32(at_tile.rows(vt[j & 1], u, i), yf[i], dp);
-          }
+        for (int i = 0; i < KQ; ++i) {
+          sc = mfma32(at_tile.rows(kt[j & 1], u, i), qf[i], sc);
+          dp = mfma32(at_tile.rows(vt[j & 1], u, i), yf[i], dp);
+        }
 #pragma unroll
-          for (int e = 0; e < 16; ++e) {
-            float x = CAP ? bend.capped(sc[e], bend.cap - lse) : __builtin_fmaf(sc[e], bend.c, -lse);
-            if constexpr (BIAS) x = __builtin_fmaf(-bend.slope, fabsf(far - (float)c_row(u, e)), x);
-            const int at = c_row(u, e);
-            if ((int)(at >= lo0) & (int)(at < hi0)) sum = __builtin_fmaf(__builtin_amdgcn_exp2f(x), dp[e], sum);
-          }
+        for (int e = 0; e < 16; ++e) {
+          float x = CAP ? bend.capped(sc[e], bend.cap - lse) : __builtin_fmaf(sc[e], bend.c, -lse);
+          if constexpr (BIAS) x = __builtin_fmaf(-bend.slope, fabsf(far - (float)c_row(u, e)), x);
+          const int at = c_row(u, e);
+          if ((int)(at >= lo0) & (int)(at < hi0)) delta = __builtin_fmaf(__builtin_amdgcn_exp2f(x), dp[e], delta);
         }
       }
-      tiles_ready();
     }
-    sum += __shfl_xor(sum, 32, 64);
-    delta = sum;
+    tiles_ready();
   }
+  delta += __shfl_xor(delta, 32, 64);
   if (hi - lo == 1 && !a.dlse) {  // dx of an only key is 0: dy.v and delta are one sum, which two orders would not leave 0
     delta *= 0.f;                 // NaN where they are not finite
 #pragma unroll

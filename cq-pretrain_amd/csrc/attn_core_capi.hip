@@ -198,7 +198,7 @@ int cqgdn_attend_bwd(const void* q, int64_t q_token, int64_t q_head, const void*
                          scale, dtype == CQGDN_F16, (int)T, nullptr, const_cast<float*>(lse), static_cast<float*>(workspace),
                          Divider(heads / kv_heads)},
                         k, v, k_token, k_head, v_token, v_head, (int)S, first, positions, cap, slopes},
-                       dy, out, dy_token, dy_head, dlse, dq, dk, dv, nullptr, nullptr};
+                       dy, dy_token, dy_head, dlse, dq, dk, dv, nullptr, nullptr};
   launch_core_backward(a, (hipStream_t)stream);
   return check_launch("cqgdn_attend_bwd");
 }

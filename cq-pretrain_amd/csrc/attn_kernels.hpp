@@ -133,7 +133,7 @@ void launch_core_few(const CoreArgs& a, int splits, int per, hipStream_t st);
 
 // Its gradients, over packed rows; `lse` is read, `ws` is core_backward_bytes() bytes.
 struct CoreGradArgs : CoreArgs {
-  const void *dy, *y;          // the output's gradient (strides in elements) and the output, dense
+  const void* dy;              // the output's gradient, strides in elements
   int64_t dy_token, dy_head;
   const float* dlse;           // [T][heads], or null
   void *dq, *dk, *dv;          // dense

@@ -508,7 +508,8 @@ int cqgdn_kv16_attend(const void* q, int64_t q_token, int64_t q_head, int dtype,
  *   lse      : fp32 [T][heads]: log sum_j exp(u_j), -inf for rows that see nothing; the backward pass reads it (or NULL)
  *   workspace: >= cqgdn_attend_fwd_workspace_size() bytes (it may be 0), 256-byte aligned
  * cqgdn_attend_bwd writes the gradients dq, dk, dv (dense, of dtype) of a loss whose gradients by out and lse are dy
- * and dlse (NULL: 0); dk and dv may both be NULL.  Nothing is added atomically: the same inputs give the same bits.  Keys
+ * and dlse (NULL: 0); dk and dv may both be NULL.  sum p dy.v is formed from the keys: out has to be given, but its values,
+ * which are rounded, are not read.  Nothing is added atomically: the same inputs give the same bits.  Keys
  * that no row sees, and rows that see none, get zero.
  */
 size_t cqgdn_attend_fwd_workspace_size(int64_t T, int64_t S, int heads, int kv_heads, int head_dim);

@@ -7,7 +7,7 @@ import rounding_testlib as L
 
 pytestmark = pytest.mark.gpu
 DEV = "cuda:0"
-TYPES = {"bf16": torch.bfloat16}
+TYPES = {"bf16": torch.bfloat16, "fp16": torch.float16}
 
 
 @pytest.fixture(scope="module")
