@@ -16,8 +16,9 @@ from .gated_delta_net import CALLS
 
 def documents(bounds, *, causal=True, window=None, prefix=None, device="cuda"):
     """(first, limit) int32 [T] for the rows of packed documents: row t of the document bounds[i] .. bounds[i + 1] - 1
-    sees its document's rows up to itself (all of them if not ``causal``), or the last ``window`` of those; rows of
-    the first ``prefix[i]`` tokens of document i see each other.  Made on the host, once for all layers of a step."""
+    sees its document's rows up to itself, or all of them if not ``causal``; with ``window`` those of them that lie less
+    than ``window`` rows away.  Rows of the first ``prefix[i]`` tokens of document i see the later ones of them too; rows
+    before the window stay unseen also there.  Made on the host, once for all layers of a step."""
     bounds = torch.as_tensor([int(b) for b in bounds])
     if bounds.numel() < 1 or int(bounds[0]) != 0 or bool((bounds.diff() < 0).any()):
         raise ValueError("bounds must begin with 0 and not fall")
@@ -28,7 +29,7 @@ def documents(bounds, *, causal=True, window=None, prefix=None, device="cuda"):
         raise ValueError("prefix must hold a value a document")
     row = torch.arange(int(bounds[-1]))
     start, end = bounds[:-1].repeat_interleave(lengths), bounds[1:].repeat_interleave(lengths)
-    limit = row + 1 if causal else end
+    limit = row + 1 if causal else end if window is None else torch.minimum(end, row + window)
     first = start if window is None else torch.maximum(start, row + 1 - window)
     if prefix is not None:
         ends = (bounds[:-1] + torch.as_tensor([int(p) for p in prefix])).repeat_interleave(lengths)
