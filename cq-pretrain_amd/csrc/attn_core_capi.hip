@@ -23,7 +23,7 @@ bool finite(float x) { return x - x == 0.f; }
 // rows as the kernels read them: the offsets of 64 tokens, and of a token's heads, fit 32 bits
 bool rows_ok(const void* p, int64_t token, int64_t head, int heads) {
   return p && aligned(p, 16) && token % 8 == 0 && head % 8 == 0 && token >= 0 && token < 1 << 24 && head >= 0 &&
-         head < (1 << 29) / heads;
+         head <= ((1 << 29) - 1) / heads;
 }
 
 int check_cache16(const void* data, int64_t pages, int kv_heads, int D, int page) {
