@@ -76,14 +76,15 @@ __device__ __forceinline__ void load_blocks(const void* from, uint32_t off, void
 #define CQGDN_LOAD(m0, more) "s_mov_b32 m0, " m0 "\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, %1" more "\n\t"
   static_assert(N == 1 || N == 2 || N == 4 || N == 8, "blocks a wave");
   if constexpr (N == 1) {
-    asm volatile(CQGDN_LOAD("%2", "") ::"v"(off), "s"(base), "s"(at) : "memory");
+    asm volatile(CQGDN_LOAD("%2", "") ::"v"(off), "s"(base), "s"(at) : "memory", "m0");
   } else if constexpr (N == 2) {
-    asm volatile(CQGDN_LOAD("%2", "") CQGDN_LOAD("%3", " offset:64") ::"v"(off), "s"(base), "s"(at), "s"(at + 960) : "memory");
+    asm volatile(CQGDN_LOAD("%2", "") CQGDN_LOAD("%3", " offset:64") ::"v"(off), "s"(base), "s"(at), "s"(at + 960)
+                 : "memory", "m0");
   } else {
     asm volatile(CQGDN_LOAD("%2", "") CQGDN_LOAD("%3", " offset:64") CQGDN_LOAD("%4", " offset:128")
                      CQGDN_LOAD("%5", " offset:192") ::"v"(off),
                  "s"(base), "s"(at), "s"(at + 960), "s"(at + 1920), "s"(at + 2880)
-                 : "memory");
+                 : "memory", "m0");
     if constexpr (N == 8) load_blocks<4>(static_cast<const char*>(from) + 256, off, static_cast<char*>(lds) + 4096);
   }
 #undef CQGDN_LOAD
