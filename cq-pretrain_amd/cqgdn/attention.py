@@ -40,7 +40,8 @@ def documents(bounds, *, causal=True, window=None, prefix=None, device="cuda"):
 def attend(q, k, v, limit, *, first=None, positions=None, scale=None, cap=None, slopes=None, return_lse=False):
     """Attention of the rows q [T, Hq, D] to the rows k, v [S, Hk, D] (bf16 or fp16, D = 64, 128 or 256, any strides;
     or [1, T, H, D]).  Row t sees the keys ``first[t]`` (default 0) .. ``limit[t]`` - 1 (int32 [T]; beyond S there are
-    none); a row that sees none is zero.  Query head h reads key head h // (Hq // Hk).
+    none); a row that sees none is zero, one that sees only scores of -infinity NaN.  Query head h reads key head
+    h // (Hq // Hk).
 
     The score of key j is scale q k_j (``scale`` defaults to D^-0.5), capped to cap tanh(score / cap) with ``cap``, less
     ``slopes[h]`` |positions[t] - j| with ``slopes`` (fp32 [Hq], constants; ``positions`` int32 [T] is the key that row t

@@ -158,7 +158,8 @@ def attend(q, cache, tables, starts, visible, *, window=None, scale=None, cap=No
 
     Over a 16-bit cache scores may be capped and biased as in ``attention.attend``: cap tanh(score / cap) with ``cap``, less
     ``slopes[h]`` |positions[t] - j| at position j with ``slopes`` (fp32 [Hq]; ``positions`` int32 [T], default
-    visible - 1, where the row's last position is).  A value that is not finite reaches only rows that see it.
+    visible - 1, where the row's last position is).  A value that is not finite reaches only rows that see it; a row that
+    sees only scores of -infinity is NaN.
 
     ``max_queries`` bounds the rows of one request and sets the launch (default: T; a decode step should
     pass 1): a larger request is still served.  With ``return_lse`` also fp32 [T, Hq]:

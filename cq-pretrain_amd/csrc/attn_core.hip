@@ -340,6 +340,11 @@ __device__ __forceinline__ void core_tile(const CoreArgs& a, const CorePlace pla
     careful = true;
   }
   l += __shfl_xor(l, 32, 64);
+  // No weight above 0: the row's keys are hidden here, or the scores of all are -infinity.
+  if (l == 0.f && hi > 0 && n > 0) {
+    const int from_key = max(lo, begin + s * per * TOK), to_key = min(hi, begin + min(steps, (s + 1) * per) * TOK);
+    if (PAGED ? pages_hold(a, r, from_key, to_key) : from_key < to_key) l = splits > 1 ? kNoWeight : __builtin_nanf("");
+  }
   if (real) {
     const int64_t at = (int64_t)t * a.heads + head;
     const float inv = l == 0.f ? 0.f : 1.f / l;

@@ -164,6 +164,17 @@ __device__ __forceinline__ void add_odd(const E* tile, f32x16 (&acc)[MT], int la
   }
 }
 
+// A row whose scores are all -infinity is NaN, as 0 / 0 is.  A part of it alone may be such a part of a row that is not:
+// it leaves the maximum -infinity and this as its sum, which the join multiplies with exp2(-infinity - the row's maximum):
+// 0 beside parts with finite scores, NaN where there is none.
+constexpr float kNoWeight = -1.f;
+// whether a page holds any of the positions [from, to) of request r
+__device__ __forceinline__ bool pages_hold(const CoreArgs& a, int r, int from, int to) {
+  for (int column = from >> a.page_shift; from < to && column <= (to - 1) >> a.page_shift; ++column)
+    if ((uint32_t)a.tables[r * a.table_stride + column] < a.page_count) return true;
+  return false;
+}
+
 // ---- scores -------------------------------------------------------------------------------------------
 // A score x = scale q.k becomes u = cap tanh(x / cap) - slope |distance|, in units of log2 e throughout.  With
 // r = 1 / (1 + e^(2 x / cap)) the tanh is 1 - 2 r (an exponential and a reciprocal; off by 2^-23 of the cap), and its

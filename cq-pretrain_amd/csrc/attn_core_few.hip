@@ -292,6 +292,10 @@ __global__ __launch_bounds__(64 * kWaves, D == 256 ? 1 : 2) void few_kernel(Core
       f[w] = wm[w][row] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(wm[w][row] - M);
       L += f[w] * wl[w][row];
     }
+    const int lo_n = __shfl(lo, row, 64), hi_n = __shfl(hi, row, 64);
+    // no weight above 0: the row's positions are hidden here, or the scores of all are -infinity
+    if (L == 0.f && hi_n > 0 && pages_hold(a, r, max(lo_n, begin + s * per * kStep), min(hi_n, begin + stop * kStep)))
+      L = splits > 1 ? kNoWeight : __builtin_nanf("");
     if (n < rows) {
 #pragma unroll
       for (int k = 0; k < D / 64; ++k) {

@@ -486,7 +486,7 @@ int cqgdn_kv16_append(const void* q, int64_t q_token, int64_t q_head, int q_head
  *   u_j = cap tanh(scale q k_j / cap) - slopes[h] |positions[t] - j|
  * of query head h and position j, p_j = exp(u_j).  cap 0: not capped; slopes NULL: no bias; positions NULL: rows stand
  * at visible[t] - 1.  A capped score is off by up to 2^-22 of the cap.  A value that is not finite reaches the rows that
- * see it, with any weight, and no other.
+ * see it, with any weight, and no other.  A row that sees only positions with scores of -infinity is NaN.
  */
 size_t cqgdn_kv16_attend_workspace_size(int64_t T, int N, int heads, int kv_heads, int head_dim, int max_queries,
                                         int columns, int page);
@@ -500,8 +500,8 @@ int cqgdn_kv16_attend(const void* q, int64_t q_token, int64_t q_head, int dtype,
  * Attention over packed rows, for training: row t sees the keys first[t] <= j < limit[t] (first NULL: from 0; beyond S
  * there are none), and out[t][h] = sum_j p_j v_j / sum_j p_j with the scores above, distances counted from positions[t]
  * (NULL: limit[t] - 1; beyond 2^24 either way it counts as that, and with slopes S is 2^24 at most).  Query head h reads
- * key head h / (heads / kv_heads); rows that see nothing are zero.  Scores, sums and results are held in fp32; each weight
- * is rounded to dtype for its product with v.
+ * key head h / (heads / kv_heads); rows that see nothing are zero, rows that see only scores of -infinity NaN.  Scores,
+ * sums and results are held in fp32; each weight is rounded to dtype for its product with v.
  *   q, out   : bf16 or fp16 (dtype) [T][heads][head_dim], out dense; k, v: [S][kv_heads][head_dim].  Strides in
  *              elements, multiples of 8, not negative, below 2^24 from token to token and 2^29 over all heads; rows
  *              16-byte aligned
