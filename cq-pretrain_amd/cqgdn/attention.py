@@ -49,9 +49,11 @@ def attend(q, k, v, limit, *, first=None, positions=None, scale=None, cap=None, 
     ``return_lse`` also fp32 [T, Hq]: the logarithm of the sum of exp(score), -inf for rows that see nothing.
 
     Scores, sums and results are held in fp32, and each weight, and in the backward pass each score's gradient, is
-    rounded once to the rows' type for its product.  A capped score is off by up to 2^-22 of the cap.  Differentiable in
-    q, k and v, once, through both results; the same inputs give the same bits.  A value that is not finite reaches the
-    rows that see it (a gradient's, the keys that are seen), and no other."""
+    rounded once to the rows' type for its product (in bf16 a score's gradient to two terms where a range cuts 64 keys).
+    The sum p dy.v of a row is formed in fp32 from its keys, not from the rounded result.  A capped score is off by up to
+    2^-22 of the cap.  Differentiable in q, k and v, once (a backward pass with ``create_graph`` is refused), through both
+    results; the same inputs give the same bits.  A value that is not finite reaches the rows that see it (a gradient's,
+    the keys that are seen), and no other."""
     packed = q.dim() == 4 and k.dim() == 4 and v.dim() == 4 and q.shape[0] == k.shape[0] == v.shape[0] == 1
     if packed:
         q, k, v = q[0], k[0], v[0]

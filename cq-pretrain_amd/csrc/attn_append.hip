@@ -23,7 +23,8 @@ constexpr int kItems = 4;         // of a thread, one after the other
 constexpr int kMostPairs = 4096;  // of a workgroup's tokens: 32 KB of sines and cosines
 
 // The product and sum rounded once, to T.  fp16 has an instruction for it, which the compiler takes in the rotary kernel
-// and takes or leaves here, so it is written out (the wait is for a register of which half is written).
+// and takes or leaves here, so it is written out (the wait is for a register of which half is written).  (Written out there
+// as well, the fp16 rotary kernel takes 2% longer.)
 template <class T>
 __device__ __forceinline__ T rounded_fma(float a, float b, float c) {
   if constexpr (std::is_same_v<T, _Float16>) {
@@ -35,8 +36,8 @@ __device__ __forceinline__ T rounded_fma(float a, float b, float c) {
   }
 }
 
-// (l c - r s, r c + l s): which product of a sum is rounded first (l s if `left_first`) is left to no compiler, as rows
-// appended are those of the rotary kernel to the last bit.
+// (l c - r s, r c + l s): which product of a sum is rounded first (l s if `left_first`) is not left to the compiler here: it is
+// the order that the compiler gives the rotary kernel, as rows appended are that kernel's to the last bit.
 template <class T>
 __device__ __forceinline__ void turn_pair(T& left, T& right, float s, float c, bool left_first) {
   const float l = (float)left, r = (float)right;

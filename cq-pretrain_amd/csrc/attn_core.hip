@@ -8,9 +8,11 @@
 // layout is already an operand of O^T.  Steps that all of a wave's rows see whole, most of them, have no masks.
 //
 // Bound by the MFMAs and, at about as many cycles, the operations on scores that stand between them: 8192 causal tokens and
-// 1024 queries, 16 heads of 128, 361 us, 881 TFLOP/s of the products that the mask leaves; with a cap, three transcendental
-// operations a score, by those (13 documents of up to 4096 tokens, 16 key heads: 750 us), as with heads of 64 (seven
-// documents with a window of 1024: 106 us).
+// 1024 queries, 16 heads of 128, 326 us, 975 TFLOP/s of the products that the mask leaves; the MFMAs are busy for half of it.
+// With a cap they are for 28%, and the VALU for 37% at four cycles an operation (its transcendental ones take more): neither
+// is full, as the cap's exponentials and reciprocals stand alone between the groups of MFMAs (13 documents of up to 4096
+// tokens, 16 key heads: 654 us).  With heads of 64 a score has half the MFMA work: 21% and 48% (seven documents with a window
+// of 1024: 97 us).
 //
 // Scores, sums and O are fp32; a weight is rounded once to the rows' type for its product with V (half a step of
 // the type times sum p |v| / sum p in a result).

@@ -4,22 +4,22 @@
 //   dv_j = sum_t p_tj dy_t,  du_tj = p_tj (dy_t.v_j - delta_t),  dx = du times the cap's derivative,
 //   dq_t = scale sum_j dx_tj k_j,  dk_j = scale sum_t dx_tj q_t.
 // The weights come again from the scores and the rows' logarithms.  Two kernels, each of which owns what it sums, so
-// that nothing is added atomically and results do not depend on timing: one goes through the keys of 128 rows for dq
-// (S and dP once more than a kernel for all three would form them: 14 D operations a pair of row and key for 10), the
-// other through the rows that see 256 keys for dk and dv, 64 rows a step (attn_core_dkv.hip).
+// that nothing is added atomically and results do not depend on timing: one goes through the keys of 128 rows twice, for
+// delta and for dq, the other through the rows that see 256 keys for dk and dv, 64 rows a step (attn_core_dkv.hip).  S and dP
+// are formed three times, 18 D operations a pair of row and key; a kernel for all, with delta known, would take 10 D.
 //
-// The first is bound by the MFMAs and the exponentials that stand between them: 8192 causal tokens and 1024 queries, 16 heads
-// of 128, 486 us before S and dP were formed twice; with a cap by the operations on scores (13 documents of up to 4096 tokens, 16
-// key heads: 890 us before); heads of 256, one wave a SIMD, by its waits (five documents of up to 1531 tokens, 8 heads: 130 us).
+// The first, of which the pass for delta is nearly half, is bound by its phases: MFMAs, exponentials and MFMAs follow each other,
+// in the pass for delta behind a wait for each step's keys.  8192 causal tokens and 1024 queries, 16 heads of 128: 812 us,
+// the MFMAs busy for 46% of it; 13 documents of up to 4096 tokens, 16 key heads, with a cap: 1559 us, 30%; heads of 256, one
+// workgroup a CU: five documents of up to 1531 tokens, 8 heads, 224 us, in which a SIMD has 0.4 waves on average.
 //
 // The first leaves, for every 64 rows, the range of keys they see, their logarithms and deltas: the second finds its
 // steps in those ranges, 64 at a time.  Where its workgroups would not fill the CUs, each takes every n-th of the
 // steps, and fp32 parts are added up by a third kernel in their order.
 //
-// Scores, products, sums are fp32.  p and dx are rounded once to the rows' type for the second products (dx to two terms
-// where a mask cuts a step).  In fp16, where
-// a dx may be too small or too large for the type, it goes in times a power of two that follows the largest so far (of
-// the row, or of the key), and p times 2^15.
+// Scores, products, sums are fp32.  p and dx are rounded once to the rows' type for the second products (in bf16 dx to two
+// terms where a mask cuts a step).  In fp16, where a dx may be too small or too large for the type, it goes in times a power
+// of two that follows the largest so far (of the row, or of the key), and p times 2^15.
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
@@ -130,7 +130,7 @@ __device__ __forceinline__ bool dq_rows(const CoreGradArgs& a, int tiles, DqTile
   // delta is formed from the keys and not as dy.out, in which out is rounded: by a delta that is off every dx of the row is
   // off alike, and keys that have something in common (a dimension far from 0) add that up (9216 rows of such keys in bf16:
   // dq off by up to 0.45 times its root mean square with dy.out; in fp16 by an eighth of it).  It costs S and dP once more:
-  // both passes 1350 -> 1800 us there.
+  // forward and backward 1350 -> 1710 us there, in fp16 1500 -> 1870.
   float delta = 0.f;
 #pragma unroll 1
   for (int j = 0; first + (int64_t)j * TOK < last; ++j) {

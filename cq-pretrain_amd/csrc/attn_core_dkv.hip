@@ -6,9 +6,10 @@
 // Two waves a SIMD with 256 registers each: the sums (128 with D = 128) and K stay in them, V's operands come from shared
 // memory, as do Q's and dY's.  The exponentials stand between dP's MFMAs and the rest of dX between dV's; what of an MFMA's
 // time and of the waits that leaves, the other wave takes.  (One wave a SIMD, with 64 keys and V in registers as well, reads
-// half as much from shared memory, but its waits are nobody's: 8192 causal tokens and 1024 queries, 16 heads of 128, 869 us;
-// this way 679, 937 TFLOP/s of the products that the mask leaves.)  Heads of 64 and capped scores are bound by the operations
-// on a score, three of them transcendental with a cap: 13 documents of up to 4096 tokens, 16 key heads, 1250 us.
+// half as much from shared memory, but its waits are nobody's: 8192 causal tokens and 1024 queries, 16 heads of 128, 869 us
+// where this way took 679.)  That case takes 579 us on a card at full clock, 1100 TFLOP/s of the products that the mask leaves,
+// the MFMAs busy for 52% of it; with a cap, three transcendental operations a score, they are for 33%: 13 documents of up to
+// 4096 tokens, 16 key heads, 1164 us.
 #include <hip/hip_runtime.h>
 
 #include <cstddef>
@@ -338,7 +339,8 @@ __global__ __launch_bounds__(512, 2) void dkv_kernel(CoreGradArgs a, int blocks,
 
 // With D = 256 the sums of 32 keys would fill a wave's registers.  Two waves share 32 keys: one forms S, the other dP, they
 // exchange them through shared memory, and each sums half of the dimensions; a workgroup takes 64 keys, one wave a SIMD.
-// Bound by its waits: five documents of up to 1531 tokens with prefixes and slopes, 8 heads, 176 us.
+// Bound by its waits, and by few workgroups: five documents of up to 1531 tokens with prefixes and slopes, 8 heads, 176 us, in
+// which a SIMD has 0.6 waves on average.
 template <class E, int D>
 struct PairTiles {
   E qt[2][kTileSize<D>], yt[2][kTileSize<D>];

@@ -6,7 +6,7 @@
 // shared memory, which turns them.  Four waves a workgroup take 32 positions each in turn, with a maximum, sum and O^T
 // of their own, and are joined at the end; a workgroup takes one of `splits` parts of the positions.
 //
-// Bound by memory: 64 requests of up to 8192 positions, 4 key heads of 128, 146 us, 4.4 TB/s (a large copy reaches 4.8); one
+// Bound by memory: 64 requests of up to 8192 positions, 4 key heads of 128, 144 us, 4.5 TB/s (a large copy reaches 4.8); one
 // request of 9216, in parts, 11 us, most of it the latency of one round of loads after another.
 //
 // Scores, sums and O are fp32, a weight is rounded once to the rows' type for its product with V.

@@ -137,7 +137,7 @@ struct CoreGradArgs : CoreArgs {
   int64_t dy_token, dy_head;
   const float* dlse;           // [T][heads], or null
   void *dq, *dk, *dv;          // dense
-  void *ranges, *blocks;       // in the workspace: RowRange and RowBlock of each 32 rows
+  void *ranges, *blocks;       // in the workspace: RowRange and RowBlock of each 64 rows
 };
 size_t core_backward_bytes(int64_t T, int64_t S, int heads, int kv_heads, int D);
 void launch_core_backward(const CoreGradArgs& a, hipStream_t st);
